@@ -452,6 +452,91 @@ int vt_gemm_i8_packed(const int8_t *A, const int8_t *Bp, const int32_t *D, int32
                       int64_t stride_c, int32_t k_split, void *stream);
 
 /*
+ * Scaled int8 operators.
+ *
+ * Linear layers and gated feed-forward products whose weights are int8 with a
+ * scale for each output channel and whose rows are int8 with a scale for each
+ * token, and their input gradients. The int8 products are vt_gemm_i8's; what
+ * follows the int32 sums (scales, bias, activation, product) is 32-bit
+ * floating point, rounded once to the output's type. The reference has no
+ * counterpart: its contract ends at the int32 sums.
+ *
+ *   quantise     top_i = max_k |x_ik|, t_i = top_i / 127,
+ *                q_ik = round(x_ik * (127 / top_i)), ties to even
+ *   linear       y_ij = t_i s_j sum_k q_ik W_kj + bias_j
+ *   gated        g, u as linear of two weights (no bias); h = act(g) * u
+ *   linear_grad  dx_ik = sum_j dy_ij s_j W_kj
+ *   gated_grad   dx_ik = sum_j dh_ij (u act'(g) sg_j Wg_kj + act(g) su_j Wu_kj),
+ *                g and u computed again from the int8 rows
+ *
+ * A row of zeros (or whose top_i is below 2^-120) has t_i = 0 and q_ik = 0. A
+ * row that holds NaN or an infinity has t_i = NaN, and NaN outputs. The
+ * gradients are those in x^ = q t (straight through the rounding); weights,
+ * scales and bias are constants. Gradient terms (dy s, or the factors of Wg and
+ * Wu above) are float16 with one power of two per row, in two halves (22 bits)
+ * when the gradients are float32; their products are summed in float32.
+ *
+ * Rows: X [M][ldx] of x_type; VT_TYPE_I8 rows come with their scales T [M].
+ * VT_TYPE_I8_PADDED rows also have ldx >= vt_quant_pitch(K), a multiple of 16,
+ * a 16-byte aligned base and zeros in columns K .. vt_quant_pitch(K) - 1, as
+ * vt_quant_rows writes them (then they are used in place). Outputs have any
+ * pitch and their elements' alignment; an output may not share memory with an
+ * input. M = 0 and empty outputs are no-ops, K = 0 sums are zero.
+ *
+ * Intermediate rows, sums and terms live in per-stream workspaces, as
+ * vt_gemm_i8's do (a call made once on a stream may be captured there).
+ */
+#define VT_TYPE_F32 1
+#define VT_TYPE_F16 2
+#define VT_TYPE_BF16 3
+#define VT_TYPE_I8 4
+#define VT_TYPE_I8_PADDED 5
+
+#define VT_ACT_SILU 0   /* g / (1 + exp(-g))                                  */
+#define VT_ACT_GELU 1   /* g (1 + tanh(sqrt(2 / pi) (g + 0.044715 g^3))) / 2  */
+
+/* Pitch in bytes of the rows vt_quant_rows writes: K rounded up to 64, from
+ * K = 1024 to 256. Negative: VT_E* (K < 0 or K >= 2^30). */
+int64_t vt_quant_pitch(int64_t K);
+
+/* Rows of floating X [M][ldx] -> int8 Q [M][ldq] (zeros past K up to
+ * vt_quant_pitch(K) <= ldq; ldq a multiple of 16, Q 16-byte aligned) and their
+ * scales T [M]. */
+int vt_quant_rows(const void *X, int32_t x_type, int64_t ldx, int8_t *Q, int64_t ldq,
+                  float *T, int64_t M, int64_t K, void *stream);
+
+/* Bytes of packed weights of K x N (pair: a gate and an up weight), and the
+ * floats of their scales; negative: VT_E*. No device call. */
+int64_t vt_scaled_size(int64_t K, int64_t N, int32_t pair, int64_t *meta_floats);
+
+/* Packs int8 weights W0 [K][ldw0] with channel scales s0 [N] and an optional
+ * bias [N] for vt_scaled_linear, or (s1 given) the gate W0, s0 and the up
+ * projection W1 [K][ldw1], s1 for vt_scaled_gated, into Bp and meta
+ * (vt_scaled_size), both 16-byte aligned. Any N, pitch and alignment. */
+int vt_scaled_pack(const int8_t *W0, const int8_t *W1, int64_t ldw0, int64_t ldw1,
+                   const float *s0, const float *s1, const float *bias, int64_t K, int64_t N,
+                   int8_t *Bp, float *meta, void *stream);
+
+int vt_scaled_linear(const void *X, int32_t x_type, int64_t ldx, const float *T, int64_t M,
+                     int64_t K, const int8_t *Bp, const float *meta, int64_t N, void *Y,
+                     int32_t y_type, int64_t ldy, void *stream);
+
+int vt_scaled_gated(const void *X, int32_t x_type, int64_t ldx, const float *T, int64_t M,
+                    int64_t K, const int8_t *Bp, const float *meta, int64_t N, int32_t act,
+                    void *Y, int32_t y_type, int64_t ldy, void *stream);
+
+/* dY [M][ldd] of N columns and dX [M][ldx] of K columns have one type. */
+int vt_scaled_linear_grad(const void *dY, int32_t type, int64_t ldd, int64_t M, int64_t K,
+                          const int8_t *Bp, const float *meta, int64_t N, void *dX, int64_t ldx,
+                          void *stream);
+
+/* Q, q_type, ldq, T: the int8 rows of the forward pass. */
+int vt_scaled_gated_grad(const void *dH, int32_t type, int64_t ldd, const int8_t *Q,
+                         int32_t q_type, int64_t ldq, const float *T, int64_t M, int64_t K,
+                         const int8_t *Bp, const float *meta, int64_t N, int32_t act, void *dX,
+                         int64_t ldx, void *stream);
+
+/*
  * Run-time compiled loop-nest kernels.
  *
  * The reference turns a loop nest (its `Stmt` JSON, README.md:456-503) into

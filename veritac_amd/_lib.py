@@ -40,7 +40,9 @@ VARIANTS = tuple(VARIANT_IDS)
 EXPORTS = ("vt_gemm_i8", "vt_gemm_i8_noalloc", "vt_gemm_check", "vt_gemm_route", "vt_gemm_select", "vt_variant_info", "vt_variant_name",
            "vt_last_error", "vt_sync", "vt_device_count", "vt_abi_version", "vt_replay_i8",
            "vt_device_query", "vt_packed_b_size", "vt_pack_b_i8", "vt_gemm_i8_packed",
-           "vt_rtc_compile", "vt_rtc_code_size", "vt_rtc_launch", "vt_rtc_release")
+           "vt_rtc_compile", "vt_rtc_code_size", "vt_rtc_launch", "vt_rtc_release",
+           "vt_quant_pitch", "vt_quant_rows", "vt_scaled_size", "vt_scaled_pack", "vt_scaled_linear",
+           "vt_scaled_gated", "vt_scaled_linear_grad", "vt_scaled_gated_grad")
 
 # Replay operation codes and status codes (VT_REPLAY_* in include/vt_hip_gemm.h).
 REPLAY_MVIN, REPLAY_LATCH_B, REPLAY_COMPUTE, REPLAY_MVOUT = 1, 2, 3, 4
@@ -132,6 +134,23 @@ def _declare(lib):
     lib.vt_rtc_compile.restype = ctypes.c_int
     lib.vt_rtc_code_size.argtypes = [p]
     lib.vt_rtc_code_size.restype = ctypes.c_int64
+    lib.vt_quant_pitch.argtypes = [i64]
+    lib.vt_quant_pitch.restype = ctypes.c_int64
+    lib.vt_quant_rows.argtypes = [p, i32, i64, p, i64, p, i64, i64, p]
+    lib.vt_quant_rows.restype = ctypes.c_int
+    lib.vt_scaled_size.argtypes = [i64, i64, i32, ctypes.POINTER(ctypes.c_int64)]
+    lib.vt_scaled_size.restype = ctypes.c_int64
+    lib.vt_scaled_pack.argtypes = [p, p, i64, i64, p, p, p, i64, i64, p, p, p]
+    lib.vt_scaled_pack.restype = ctypes.c_int
+    lib.vt_scaled_linear.argtypes = [p, i32, i64, p, i64, i64, p, p, i64, p, i32, i64, p]
+    lib.vt_scaled_linear.restype = ctypes.c_int
+    lib.vt_scaled_gated.argtypes = [p, i32, i64, p, i64, i64, p, p, i64, i32, p, i32, i64, p]
+    lib.vt_scaled_gated.restype = ctypes.c_int
+    lib.vt_scaled_linear_grad.argtypes = [p, i32, i64, i64, i64, p, p, i64, p, i64, p]
+    lib.vt_scaled_linear_grad.restype = ctypes.c_int
+    lib.vt_scaled_gated_grad.argtypes = [p, i32, i64, p, i32, i64, p, i64, i64, p, p, i64, i32, p,
+                                         i64, p]
+    lib.vt_scaled_gated_grad.restype = ctypes.c_int
     u32 = ctypes.c_uint32
     lib.vt_rtc_launch.argtypes = [p, u32, u32, u32, u32, u32, u32, ctypes.POINTER(p), p]
     lib.vt_rtc_launch.restype = ctypes.c_int
@@ -320,6 +339,28 @@ def gemm_packed_raw(A_ptr, Bp_ptr, D_ptr, C_ptr, M, N, K, lda, ldd, ldc, batch=1
     st = lib.vt_gemm_i8_packed(A_ptr, Bp_ptr, D_ptr, C_ptr, M, N, K, lda, ldd, ldc, batch,
                                stride_a, stride_bp, stride_d, stride_c, k_split, stream)
     return check(st, "vt_gemm_i8_packed")
+
+
+# VT_TYPE_* and VT_ACT_* of the scaled operators
+TYPE_F32, TYPE_F16, TYPE_BF16, TYPE_I8, TYPE_I8_PADDED = 1, 2, 3, 4, 5
+ACT_IDS = {"silu": 0, "gelu": 1}
+
+
+def quant_pitch(k):
+    """Pitch of the int8 rows vt_quant_rows writes for k columns."""
+    pitch = load_library().vt_quant_pitch(k)
+    if pitch < 0:
+        check(int(pitch), "vt_quant_pitch")
+    return pitch
+
+
+def scaled_size(k, n, pair):
+    """(bytes of packed weights, floats of their scales), vt_scaled_size."""
+    meta = ctypes.c_int64()
+    size = load_library().vt_scaled_size(k, n, int(pair), ctypes.byref(meta))
+    if size < 0:
+        check(int(size), "vt_scaled_size")
+    return size, meta.value
 
 
 class RtcProgram:

@@ -324,9 +324,9 @@ def artifact_paths():
              "header": os.path.join(build.INCLUDE, "vt_hip_gemm.h"),
              "build_recipe": os.path.abspath(build.__file__),
              "binding": os.path.abspath(_lib.__file__)}
-    for src in build.SOURCES:
+    for src in build.SOURCES + build.PARTS:
         paths["hip_source:" + os.path.basename(src)] = src
-    for mod in ("backend", "verify", "replay", "provenance"):
+    for mod in ("backend", "scaled", "verify", "replay", "provenance"):
         paths["module:" + mod] = os.path.join(PKG_DIR, mod + ".py")
     return paths
 
