@@ -495,7 +495,7 @@ int vt_gemm_i8_packed(const int8_t *A, const int8_t *Bp, const int32_t *D, int32
 #define VT_ACT_SILU 0   /* g / (1 + exp(-g))                                  */
 #define VT_ACT_GELU 1   /* g (1 + tanh(sqrt(2 / pi) (g + 0.044715 g^3))) / 2  */
 
-/* Pitch in bytes of the rows vt_quant_rows writes: K rounded up to 64, from
+/* Pitch in bytes of the rows vt_quant_rows writes: K rounded up to 128, from
  * K = 1024 to 256. Negative: VT_E* (K < 0 or K >= 2^30). */
 int64_t vt_quant_pitch(int64_t K);
 

@@ -147,6 +147,36 @@ def test_gated(dev, m, k, n, dtype, act):
     ref.check(h, want, bound, dtype, "gated " + act)
 
 
+# (m, k, packed columns): enough tiles of 256 x 256 or 256 x 128 for the persistent kernels, ragged ends
+LARGE = [(2100, 200, 8000), (1100, 1024, 3800), (260, 1500, 17000)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("m,k,cols", LARGE)
+def test_linear_on_whole_chip_tiles(dev, m, k, cols, dtype):
+    rng = np.random.default_rng(m + k)
+    x, x32 = rows(rng, m, k, dtype)
+    n = cols - 3
+    w, s = weights(rng, k, n)
+    bias = rng.normal(0, 0.3, n).astype(np.float32)
+    say("linear", m, k, n, dtype)
+    y = scaled.linear(x.to(dev), packed(dev, w, s, bias))
+    ref.check(y, *ref.linear(*ref.quantize(x32), w, s, bias), dtype, "linear")
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("m,k,cols", LARGE)
+def test_gated_on_whole_chip_tiles(dev, m, k, cols, dtype, act):
+    rng = np.random.default_rng(m + k)
+    x, x32 = rows(rng, m, k, dtype)
+    n = cols // 2 - 5
+    (wg, sg), (wu, su) = weights(rng, k, n), weights(rng, k, n)
+    say("gated", m, k, n, dtype, act)
+    h = scaled.gated(x.to(dev), packed_pair(dev, wg, sg, wu, su), act=act)
+    ref.check(h, *ref.gated(*ref.quantize(x32), wg, sg, wu, su, act), dtype, "gated")
+
+
 @pytest.mark.parametrize("m,k,n", [(1, 64, 40), (20, 100, 70), (70, 1024, 256), (300, 1300, 520)])
 def test_int8_rows_with_every_value(dev, m, k, n):
     """Rows that are int8 already: -128 among them, any pitch, scales that are zero or negative."""
@@ -312,6 +342,24 @@ def test_gated_grad(dev, m, k, n, dtype, act):
     # rows that are not padded give the same
     raw = scaled.QuantRows(up(q, dev), up(t, dev))
     assert torch.equal(dx, scaled.gated_grad(d.to(dev), raw, G, act=act))
+
+
+# tiles of 128 x 256 and 256 x 256 of the whole chip; one slice, few and many
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("m,k,n", [(2100, 2048, 20), (1990, 2300, 150), (4000, 4000, 140), (1025, 3900, 700)])
+def test_gradients_on_whole_chip_tiles(dev, m, k, n, dtype):
+    rng = np.random.default_rng(m + k + n)
+    d, d32 = gradients(rng, m, n, dtype)
+    w, s = weights(rng, k, n, -128)
+    say("linear_grad", m, k, n, dtype)
+    dx = scaled.linear_grad(d.to(dev), packed(dev, w, s))
+    ref.check(dx, *ref.linear_grad(d32, w, s, dtype != torch.float32), dtype, "linear_grad")
+    w2, s2 = weights(rng, k, n)
+    x, x32 = rows(rng, m, k, dtype)
+    q, t = ref.quantize(x32)
+    say("gated_grad", m, k, n, dtype)
+    dx = scaled.gated_grad(d.to(dev), scaled.quantize_rows(x.to(dev)), packed_pair(dev, w, s, w2, s2))
+    ref.check(dx, *ref.gated_grad(d32, q, t, w, s, w2, s2, "silu", dtype != torch.float32), dtype, "gated_grad")
 
 
 @pytest.mark.parametrize("act", ["silu", "gelu"])

@@ -292,8 +292,10 @@ struct GemmArgs {
 // 16 k of column l % 32 that its A operand also holds). Rows past K are zero
 // in the layout, so B needs no K-tail test; columns past N re-read the last
 // 16-column block and are masked at the store.
-template <int BM, int BN, int EDGE, bool HAS_D, bool SHORT, bool EARLY_D, bool PACKED_B = false>
-__global__ __launch_bounds__(256, 1) void gemm_mfma_kernel(GemmArgs p) {
+// OUT: nothing (the sums, plus D, are stored in C), or one type whose tile32
+// takes a wave's sums.
+template <int BM, int BN, int EDGE, bool HAS_D, bool SHORT, bool EARLY_D, bool PACKED_B = false, class... OUT>
+__global__ __launch_bounds__(256, 1) void gemm_mfma_kernel(GemmArgs p, OUT... out) {
   constexpr int BK = 64;
   constexpr int WTM = BM / 2, WTN = BN / 2;   // wave tile (2x2 waves)
   constexpr int MI = WTM / 32, NI = WTN / 32; // 32x32 blocks per wave
@@ -607,7 +609,10 @@ __global__ __launch_bounds__(256, 1) void gemm_mfma_kernel(GemmArgs p) {
     step(Last(), kt + 3, ra1, rb1);
   }
 
-  if constexpr (D_TILE) {
+  if constexpr (sizeof...(OUT) > 0) {
+    (out.template tile32<MI, NI>(acc, m0 + wm * WTM, n0 + wn * WTN, lane,
+                                 (LDS_AS int8_t *)smem + wave * 8192), ...);
+  } else if constexpr (D_TILE) {
     if constexpr (!D_EARLY)
       load_d_tile<MI, NI, (EDGE > 0)>(d_pre, p.D + bidx * p.sd, p.ldd, m0 + wm * WTM, n0 + wn * WTN,
                                       M, N, lane);
@@ -1184,8 +1189,13 @@ __device__ __forceinline__ void mfma16_in_place(v4i &acc, const v4i &a, const v4
 // RAGGED (with EDGE; the 256x256 form, row-major B): rows of C and D have
 // n_valid <= N columns at any 4-byte aligned address (A and B are padded
 // copies there).
-template <bool HAS_D, bool PACKED_B, bool EDGE, int BN, bool RAGGED>
-__device__ __forceinline__ void dma16_tiles(const GemmArgs &p) {
+// OUT: what happens to a tile's int32 sums; SumsOut stores them (plus D) in C.
+struct SumsOut {
+  static constexpr bool kScaled = false;
+};
+
+template <bool HAS_D, bool PACKED_B, bool EDGE, int BN, bool RAGGED, class OUT = SumsOut>
+__device__ __forceinline__ void dma16_tiles(const GemmArgs &p, const OUT &out = OUT()) {
   static_assert(!RAGGED || (EDGE && BN == 256 && !PACKED_B), "ragged rows: 256x256 edge tiles, row-major B");
   // BN = 128 (the 256x128 form) gives each wave a 128x64 block and half the
   // B slice; the rest is shared.
@@ -1429,7 +1439,8 @@ __device__ __forceinline__ void dma16_tiles(const GemmArgs &p) {
   // EDGE (moved-back tiles, masked stores): no early strips, so no store
   // branch enters the scheduled step; the 256x128 form stores every strip in
   // the epilogue.
-  using Early = std::integral_constant<bool, !HAS_D && !EDGE && BN == 256>;
+  constexpr bool PEEL = !HAS_D && !EDGE && BN == 256 && !OUT::kScaled;
+  using Early = std::integral_constant<bool, PEEL>;
 
   issue_slice(0);
   issue_slice(1);
@@ -1455,14 +1466,14 @@ __device__ __forceinline__ void dma16_tiles(const GemmArgs &p) {
     // the first EARLY_STRIPS strips of C (straight-line code: a branch over
     // steps that write the accumulators makes the register allocator
     // shuffle them).
-    const int KL = HAS_D || EDGE || BN != 256 ? KT : KT - 4;
+    const int KL = PEEL ? KT - 4 : KT;
     for (int kt = 0; kt < KL; kt += 4, gs += 4) {
       step(Plain(), 0, fb0, fb1);
       step(Plain(), 1, fb1, fb0);
       step(Plain(), 2, fb0, fb1);
       step(Plain(), 3, fb1, fb0);
     }
-    if constexpr (!HAS_D && !EDGE && BN == 256) {
+    if constexpr (PEEL) {
       step(Plain(), 0, fb0, fb1);
       step(Plain(), 1, fb1, fb0);
       step(Plain(), 2, fb0, fb1);
@@ -1474,7 +1485,10 @@ __device__ __forceinline__ void dma16_tiles(const GemmArgs &p) {
     fence_acc();
     // Rows [m0, mn) and columns [n0, nn) of a moved-back tile are its
     // neighbour's to store (0 unless EDGE).
-    if constexpr (BN == 256) {
+    if constexpr (OUT::kScaled) {
+      out.template tile16<MI, NI, EDGE>(acc, m0 + wm * WTM, n0 + wn * WTN, mn, nn, lane,
+                                        lds + STRIP0 + wave * 8192);
+    } else if constexpr (BN == 256) {
       store_tile16_lds<MI, NI, HAS_D, HAS_D || EDGE ? 0 : EARLY_STRIPS, EDGE, RAGGED>(
           acc, c_tile,
           HAS_D ? p.D + bidx * p.sd + (int64_t)(m0 + wm * WTM) * p.ldd + n0 + wn * WTN : nullptr,

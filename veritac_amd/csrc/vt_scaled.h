@@ -24,13 +24,13 @@ typedef __bf16 v4b __attribute__((ext_vector_type(4)));
 typedef __bf16 v8b __attribute__((ext_vector_type(8)));
 typedef float v4f __attribute__((ext_vector_type(4)));
 
-// K and N of the packed weights. K in whole 64-deep slices, from 1024 on in
-// the 256-deep groups that the 16x16x64 persistent kernels take (at most a
-// fifth more to read there; at small K it would be up to four times as much).
-// N in whole 64-column blocks: the gradient contracts over N in steps of 64,
-// and a gated product's 64 columns are 32 of the gate and 32 of the up weight.
+// K and N of the packed weights. K in whole pairs of 64-deep slices, from 1024
+// on in the 256-deep groups that the persistent kernels take (at most a fifth
+// more to read there; at small K it would be up to four times as much). N in
+// whole 64-column blocks: the gradient contracts over N in steps of 64, and a
+// gated product's 64 columns are 32 of the gate and 32 of the up weight.
 __host__ __device__ constexpr int64_t scaled_kp(int64_t K) {
-  return K < 1024 ? (K + 63) / 64 * 64 : (K + 255) / 256 * 256;
+  return K < 1024 ? (K + 127) / 128 * 128 : (K + 255) / 256 * 256;
 }
 constexpr int64_t scaled_np(int64_t N, bool pair) {
   return pair ? 2 * ((N + 31) / 32 * 32) : (N + 63) / 64 * 64;
@@ -340,50 +340,338 @@ __device__ __forceinline__ float normaliser(float bound) {
   return __uint_as_float((uint32_t)(max(-126, min(126, 14 - e)) + 127) << 23);
 }
 
-struct FinishArgs {
-  const int32_t *S;      // int32 sums [M][Np]
-  const float *t;        // row scales
-  const float *meta;     // channel scales and bias, packed order
-  const void *D;         // dh (terms)
-  const float *norm;     // row normalisers (terms)
-  void *Y;               // output [M][ldy], or terms [M][Np] (float16; low halves after them)
-  int64_t ldd, ldy;
-  int64_t lo;            // terms: elements from the high to the low half, 0 for none
-  int M, N, Np;
+// What becomes of the int32 sums. OP: the operator; E: bytes of the floating
+// type (2: float16 or bfloat16, by `type`; 4: float32).
+enum ScaledOp { kLinear = 0, kGated = 1, kTermsOp = 2, kGradOp = 3 };
+
+struct ScaledOut {
+  const float *t;      // row scales
+  const float *meta;   // channel scales [Np], bias [Np]
+  const void *D;       // kTermsOp: dh [M][ldd]
+  const float *norm;   // kTermsOp, kGradOp: row normalisers
+  void *Y;             // output [M][ldy]; kTermsOp: float16 terms [M][Np]
+  int64_t ldy, ldd;
+  int64_t lo;          // kTermsOp: elements from the high to the low halves, 0 for none
+  int M, N, Np;        // N: output columns (dh's for kTermsOp)
+  int act, type;
 };
 
-// OP 0 linear, 1 gated, 2 gradient terms of gated.
-template <int TYPE, int OP, int ACT>
-__global__ __launch_bounds__(256) void finish_kernel(FinishArgs p) {
-  typedef typename Elem<TYPE>::T T;
-  const int64_t row = blockIdx.y;
-  const int j = blockIdx.x * 256 + threadIdx.x;
-  const int64_t pg = OP ? pair_col(j, 0) : j, pu = pair_col(j, 1);
-  if (OP == 2 ? pu >= p.Np : j >= p.N) return;
-  const float t = p.t[row];
-  const int32_t *s = p.S + row * p.Np;
-  const float g = (float)s[pg] * t * p.meta[pg];
-  if constexpr (OP == 0) {
-    ((T *)p.Y)[row * p.ldy + j] = (T)(g + p.meta[p.Np + j]);
-  } else {
-    const float u = (float)s[pu] * t * p.meta[pu];
+// Two floats as 16-bit elements, the first in the low half.
+__device__ __forceinline__ uint32_t pack16(float a, float b, int type) {
+  typedef __bf16 v2b __attribute__((ext_vector_type(2)));
+  if (type == VT_TYPE_BF16) return __builtin_bit_cast(uint32_t, v2b{(__bf16)a, (__bf16)b});
+  return __builtin_bit_cast(uint32_t, v2h{(_Float16)a, (_Float16)b});
+}
+
+typedef float v4f_any __attribute__((ext_vector_type(4), aligned(4)));
+
+template <int OP, int E>
+struct ScaledTile : ScaledOut {
+  static constexpr bool kScaled = true;
+  // The type that is written: terms are float16 whatever dh's.
+  static constexpr int OE = OP == kTermsOp ? 2 : E;
+
+  __device__ __forceinline__ float act_value(float g, float &slope) const {
+    return act == VT_ACT_SILU ? act_of<VT_ACT_SILU>(g, slope) : act_of<VT_ACT_GELU>(g, slope);
+  }
+  __device__ __forceinline__ uint32_t pack(float a, float b) const {
+    return pack16(a, b, OP == kTermsOp ? VT_TYPE_F16 : type);
+  }
+  __device__ __forceinline__ void store1(int64_t i, float v) const {
+    if (OE == 4) ((float *)Y)[i] = v;
+    else ((uint16_t *)Y)[i] = (uint16_t)pack(v, 0.0f);
+  }
+  // g and u of a pair of sums -> h, or (kTermsOp) both terms.
+  __device__ __forceinline__ void pair(int32_t ag, int32_t au, float t_row, float sg, float su, float d,
+                                       float &first, float &second) const {
+    const float g = (float)ag * t_row * sg, u = (float)au * t_row * su;
     float slope;
-    const float a = act_of<ACT>(g, slope);
-    if constexpr (OP == 1) {
-      ((T *)p.Y)[row * p.ldy + j] = (T)(a * u);
+    const float a = act_value(g, slope);
+    if (OP == kGated) {
+      first = a * u;
     } else {
-      const float d = j < p.N ? (float)((const T *)p.D)[row * p.ldd + j] * p.norm[row] : 0.0f;
-      const float tg = d * u * slope * p.meta[pg], tu = d * a * p.meta[pu];
-      _Float16 *y = (_Float16 *)p.Y + row * p.Np;
-      const _Float16 hg = (_Float16)tg, hu = (_Float16)tu;
-      y[pg] = hg;
-      y[pu] = hu;
-      if (p.lo) {
-        y[p.lo + pg] = (_Float16)(tg - (float)hg);
-        y[p.lo + pu] = (_Float16)(tu - (float)hu);
+      first = d * u * slope * sg;
+      second = d * a * su;
+    }
+  }
+
+  // Rows [r0, r0 + ROWS) of `W` output columns from out0 leave the wave's LDS, in
+  // 16-byte pieces of whole rows (vector j of a lane: row (64 j + lane) / RC,
+  // chunk lane % RC). 16-byte chunk k of a row is at k ^ swz(row). Only rows in
+  // [row_min, row_max) and columns in [out_min, the last) are stored.
+  template <int ROWS, int W, class SWZ>
+  __device__ __forceinline__ void store_rows(LDS_AS int8_t *lds, SWZ swz, int r0, int out0, int64_t plane, int lane,
+                                             int row_min, int row_max, int out_min) const {
+    constexpr int PITCH = W * OE, RC = PITCH / 16, PER = 16 / OE;
+    const int out_n = OP == kTermsOp ? Np : N;
+    const int64_t ld = OP == kTermsOp ? Np : ldy;
+#pragma unroll
+    for (int j = 0; j < (ROWS * RC + 63) / 64; ++j) {
+      const int idx = 64 * j + lane, row = idx / RC, k = idx % RC;
+      if (ROWS * RC % 64 && row >= ROWS) break;
+      const v4i w = *(LDS_AS v4i *)(lds + row * PITCH + ((k ^ swz(row)) << 4));
+      const int col = out0 + k * PER;
+      if (r0 + row < row_min || r0 + row >= row_max || col < out_min) continue;
+      int8_t *y = (int8_t *)Y + ((int64_t)(r0 + row) * ld + plane + col) * OE;
+      if (col + PER <= out_n) {
+        __builtin_nontemporal_store(w, (v4i_any *)y);
+      } else {
+#pragma unroll
+        for (int e = 0; e < PER; ++e)
+          if (col + e < out_n) {
+            if constexpr (OE == 4) ((int32_t *)y)[e] = w[e];
+            else ((uint16_t *)y)[e] = (uint16_t)((uint32_t)w[e >> 1] >> (16 * (e & 1)));
+          }
       }
     }
   }
+
+  // Four elements of consecutive rows of one column into the wave's LDS.
+  template <int PITCH>
+  __device__ __forceinline__ void put4(LDS_AS int8_t *at, float a, float b, float c, float d) const {
+    if constexpr (OE == 4) {
+      *(LDS_AS float *)at = a;
+      *(LDS_AS float *)(at + PITCH) = b;
+      *(LDS_AS float *)(at + 2 * PITCH) = c;
+      *(LDS_AS float *)(at + 3 * PITCH) = d;
+    } else {
+      const uint32_t ab = pack(a, b), cd = pack(c, d);
+      *(LDS_AS uint16_t *)at = (uint16_t)ab;
+      *(LDS_AS uint16_t *)(at + PITCH) = (uint16_t)(ab >> 16);
+      *(LDS_AS uint16_t *)(at + 2 * PITCH) = (uint16_t)cd;
+      *(LDS_AS uint16_t *)(at + 3 * PITCH) = (uint16_t)(cd >> 16);
+    }
+  }
+
+  typedef typename std::conditional<E == 4, float, uint16_t>::type DBits;
+  __device__ __forceinline__ float d_value(DBits b) const {
+    if constexpr (E == 4) return b;
+    else return type == VT_TYPE_BF16 ? __uint_as_float((uint32_t)b << 16) : (float)__builtin_bit_cast(_Float16, b);
+  }
+
+  // Blocks of 16 x 16 sums (element e of lane l: row 4 (l / 16) + e, column
+  // l % 16) of 16 MI rows from row0 and 16 NI packed columns from col0. Each
+  // strip of 16 rows goes through the wave's LDS to whole 16-byte pieces of
+  // output rows, chunk k of strip row r at k ^ (OE * ((r / 4) % 4)): the writes
+  // of one instruction then fall on distinct banks, as in store_strip16_lds.
+  // Rows below row_min and packed columns below col_min are the neighbouring
+  // tile's. All loads are issued before the stores they would otherwise wait
+  // for (both count in vmcnt, in order): the scales first, a strip's dh one
+  // strip ahead.
+  template <int MI, int NI, bool EDGE>
+  __device__ __forceinline__ void tile16(const v4i (&acc)[MI][NI], int row0, int col0, int row_min, int col_min,
+                                         int lane, LDS_AS int8_t *lds) const {
+    constexpr int NB = OP == kGated ? NI / 2 : NI;   // blocks of output columns
+    constexpr int ND = OP == kTermsOp ? NI / 2 : 1;  // and of dh's
+    constexpr int W = NB * 16, PITCH = W * OE, RC = PITCH / 16;
+    const int g = lane >> 4, c = lane & 15;
+    float s[NI], bias[OP == kLinear ? NI : 1];
+    v4f tr[OP == kTermsOp ? 2 : MI], nr[2];
+    auto trow = [](int mi) { return OP == kTermsOp ? mi & 1 : mi; };
+#pragma unroll
+    for (int ni = 0; ni < NI; ++ni) {
+      s[ni] = meta[col0 + ni * 16 + c];
+      if constexpr (OP == kLinear) bias[ni] = meta[Np + col0 + ni * 16 + c];
+    }
+    if constexpr (OP != kTermsOp) {
+#pragma unroll
+      for (int mi = 0; mi < MI; ++mi) tr[mi] = *(const v4f_any *)(t + row0 + mi * 16 + 4 * g);
+    }
+    DBits d[2][ND][4];
+    auto load_strip = [&](int mi) {
+      if constexpr (OP == kTermsOp) {
+        tr[mi & 1] = *(const v4f_any *)(t + row0 + mi * 16 + 4 * g);
+        nr[mi & 1] = *(const v4f_any *)(norm + row0 + mi * 16 + 4 * g);
+#pragma unroll
+        for (int b = 0; b < ND; ++b) {
+          const int j = min(col0 / 2 + b * 16 + c, N - 1);
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            d[mi & 1][b][e] = ((const DBits *)D)[(int64_t)(row0 + mi * 16 + 4 * g + e) * ldd + j];
+        }
+      }
+    };
+    load_strip(0);
+    auto swz = [](int row) { return (((row >> 2) & 3) * OE) & (RC - 1); };
+    int wb[NB];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) wb[b] = 4 * g * PITCH + (((b * OE + (c * OE >> 4)) ^ swz(4 * g)) << 4) + (c * OE & 15);
+    auto flush = [&](const float (&v)[NB][4], int mi, int64_t plane) {
+#pragma unroll
+      for (int b = 0; b < NB; ++b) put4<PITCH>(lds + wb[b], v[b][0], v[b][1], v[b][2], v[b][3]);
+      store_rows<16, W>(lds, swz, row0 + mi * 16, OP == kGated ? col0 / 2 : col0, plane, lane, EDGE ? row_min : 0, M,
+                        OP == kGated ? col_min / 2 : col_min);
+    };
+#pragma unroll
+    for (int mi = 0; mi < MI; ++mi) {
+      float v[NB][4];
+      if (mi + 1 < MI) load_strip(mi + 1);
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (OP == kLinear) {
+#pragma unroll
+        for (int ni = 0; ni < NI; ++ni)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[ni][e] = (float)acc[mi][ni][e] * tr[trow(mi)][e] * s[ni] + bias[ni];
+      } else {
+#pragma unroll
+        for (int b = 0; b < NI / 2; ++b) {
+          const int ng = (b >> 1) * 4 + (b & 1);
+          const bool in = OP != kTermsOp || col0 / 2 + b * 16 + c < N;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            if constexpr (OP == kGated) {
+              float none;
+              pair(acc[mi][ng][e], acc[mi][ng + 2][e], tr[trow(mi)][e], s[ng], s[ng + 2], 0.0f, v[b][e], none);
+            } else {
+              const float de = in ? d_value(d[mi & 1][b][e]) * nr[mi & 1][e] : 0.0f;
+              pair(acc[mi][ng][e], acc[mi][ng + 2][e], tr[trow(mi)][e], s[ng], s[ng + 2], de, v[ng][e], v[ng + 2][e]);
+            }
+          }
+        }
+      }
+      flush(v, mi, 0);
+      if constexpr (OP == kTermsOp && E == 4) {
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[b][e] -= (float)(_Float16)v[b][e];
+        flush(v, mi, lo);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+
+  // The gradient's float32 sums, in tile16's layout, over the row's normaliser
+  // (a power of two: exact).
+  template <int MI, int NI>
+  __device__ __forceinline__ void grad16(const v4f (&acc)[MI][NI], int row0, int col0, int lane,
+                                         LDS_AS int8_t *lds) const {
+    constexpr int W = NI * 16, PITCH = W * OE, RC = PITCH / 16;
+    const int g = lane >> 4, c = lane & 15;
+    float un[MI][4];
+#pragma unroll
+    for (int mi = 0; mi < MI; ++mi)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) un[mi][e] = 1.0f / norm[min(row0 + mi * 16 + 4 * g + e, M - 1)];
+    auto swz = [](int row) { return (((row >> 2) & 3) * OE) & (RC - 1); };
+#pragma unroll
+    for (int mi = 0; mi < MI; ++mi) {
+#pragma unroll
+      for (int ni = 0; ni < NI; ++ni)
+        put4<PITCH>(lds + 4 * g * PITCH + (((ni * OE + (c * OE >> 4)) ^ swz(4 * g)) << 4) + (c * OE & 15),
+                    acc[mi][ni][0] * un[mi][0], acc[mi][ni][1] * un[mi][1], acc[mi][ni][2] * un[mi][2],
+                    acc[mi][ni][3] * un[mi][3]);
+      store_rows<16, W>(lds, swz, row0 + mi * 16, col0, 0, lane, 0, M, 0);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+
+  // One element: the sums of packed columns pc (and, of a pair, pc + 32) of a
+  // row, to output column j.
+  __device__ __forceinline__ void element(int32_t a0, int32_t a1, int row, int pc, int j, float t_row) const {
+    const float s0 = meta[pc];
+    if constexpr (OP == kLinear) {
+      if (j < N) store1((int64_t)row * ldy + j, (float)a0 * t_row * s0 + meta[Np + pc]);
+    } else {
+      float first, second = 0.0f;
+      const float d = OP == kTermsOp && j < N ? d_value(((const DBits *)D)[(int64_t)row * ldd + j]) * norm[row] : 0.0f;
+      pair(a0, a1, t_row, s0, meta[pc + 32], d, first, second);
+      if constexpr (OP == kGated) {
+        if (j < N) store1((int64_t)row * ldy + j, first);
+      } else {
+        const int64_t at = (int64_t)row * Np + pc;
+        store1(at, first);
+        store1(at + 32, second);
+        if constexpr (E == 4) {
+          store1(at + lo, first - (float)(_Float16)first);
+          store1(at + lo + 32, second - (float)(_Float16)second);
+        }
+      }
+    }
+  }
+
+  // Blocks of 32 x 32 sums (element e of lane l: row 8 (e / 4) + 4 (l / 32) +
+  // e % 4, column l % 32) of 32 MI rows from row0 and 64 packed columns from
+  // col0, one block row at a time through the wave's LDS (whose last reader was
+  // the k loop, before its last barrier): chunk k of row r at k ^ (2 OE * ((r /
+  // 4) % 2)), which puts an instruction's two rows on distinct banks.
+  template <int MI, int NI>
+  __device__ __forceinline__ void tile32(const v16i (&acc)[MI][NI], int row0, int col0, int lane,
+                                         LDS_AS int8_t *lds) const {
+    static_assert(NI == 2, "a gate and an up block");
+    constexpr int W = OP == kGated ? 32 : 64, PITCH = W * OE, RC = PITCH / 16;
+    if (col0 >= Np) return;
+    const int g = lane >> 5, c = lane & 31;
+    const float s0 = meta[col0 + c], s1 = meta[col0 + 32 + c];
+    const float b0 = OP == kLinear ? meta[Np + col0 + c] : 0.0f, b1 = OP == kLinear ? meta[Np + col0 + 32 + c] : 0.0f;
+    const int j = col0 / 2 + c;
+    float tr[MI][16], dr[OP == kTermsOp ? MI : 1][16];
+#pragma unroll
+    for (int mi = 0; mi < MI; ++mi)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int row = min(row0 + mi * 32 + (e >> 2) * 8 + g * 4 + (e & 3), M - 1);
+        tr[mi][e] = t[row];
+        if constexpr (OP == kTermsOp) {
+          const float x = d_value(((const DBits *)D)[(int64_t)row * ldd + min(j, N - 1)]) * norm[row];
+          dr[mi][e] = j < N ? x : 0.0f;
+        }
+      }
+    auto swz = [](int row) { return (((row >> 2) & 1) * 2 * OE) & (RC - 1); };
+    const int w0 = 4 * g * PITCH + (((c * OE >> 4) ^ swz(4 * g)) << 4) + (c * OE & 15);
+    const int w1 = 4 * g * PITCH + (((2 * OE + (c * OE >> 4)) ^ swz(4 * g)) << 4) + (c * OE & 15);
+    auto flush = [&](const float (&a)[16], const float (&b)[16], int mi, int64_t plane) {
+#pragma unroll
+      for (int e = 0; e < 16; e += 4) {
+        put4<PITCH>(lds + w0 + 2 * e * PITCH, a[e], a[e + 1], a[e + 2], a[e + 3]);
+        if constexpr (W == 64) put4<PITCH>(lds + w1 + 2 * e * PITCH, b[e], b[e + 1], b[e + 2], b[e + 3]);
+      }
+      store_rows<32, W>(lds, swz, row0 + mi * 32, OP == kGated ? col0 / 2 : col0, plane, lane, 0, M, 0);
+    };
+#pragma unroll
+    for (int mi = 0; mi < MI; ++mi) {
+      float a[16], b[16];
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        if constexpr (OP == kLinear) {
+          a[e] = (float)acc[mi][0][e] * tr[mi][e] * s0 + b0;
+          b[e] = (float)acc[mi][1][e] * tr[mi][e] * s1 + b1;
+        } else {
+          pair(acc[mi][0][e], acc[mi][1][e], tr[mi][e], s0, s1, OP == kTermsOp ? dr[mi][e] : 0.0f, a[e], b[e]);
+        }
+      }
+      flush(a, b, mi, 0);
+      if constexpr (OP == kTermsOp && E == 4) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          a[e] -= (float)(_Float16)a[e];
+          b[e] -= (float)(_Float16)b[e];
+        }
+        flush(a, b, mi, lo);
+      }
+    }
+  }
+};
+
+template <int OP, int E, int BN>
+__global__ __launch_bounds__(256, 1) void scaled_dma16_kernel(GemmArgs p, ScaledTile<OP, E> out) {
+  dma16_tiles<false, true, true, BN, false>(p, out);
+}
+
+// The same from int32 sums in memory: `slices` partial sums [M][Np] each.
+template <int OP, int E>
+__global__ __launch_bounds__(256) void finish_kernel(const int32_t *S, int slices, ScaledTile<OP, E> out) {
+  const int row = blockIdx.x, j = blockIdx.y * 256 + threadIdx.x;
+  const int pc = OP == kLinear ? j : (int)pair_col(j, 0);
+  if (pc >= out.Np) return;
+  const int32_t *s = S + (int64_t)row * out.Np + pc;
+  int32_t a0 = 0, a1 = 0;
+  for (int i = 0; i < slices; ++i) {
+    a0 = add_wrap(a0, s[0]);
+    if (OP != kLinear) a1 = add_wrap(a1, s[32]);
+    s += (int64_t)out.M * out.Np;
+  }
+  out.element(a0, a1, row, pc, j, out.t[row]);
 }
 
 struct TermArgs {
@@ -438,7 +726,8 @@ struct GradArgs {
   void *X;               // dx [M][ldx]
   int64_t ldx, lo;
   int M, K, Kp, Np;
-  int tiles_m, tiles_n;
+  int tiles_m, tiles_n, group_m;
+  int planes;            // 2: terms in two halves
 };
 
 // 8 int8 values as float16, exactly: a byte b = w + 128 below the exponent byte
@@ -457,6 +746,179 @@ __device__ __forceinline__ v8h bytes_to_half(v2i w) {
     r[4 * d + 3] = hi[1];
   }
   return r;
+}
+
+// v_mfma_f32_16x16x32_f16 accumulating in place in AGPRs (see mfma16_in_place:
+// the same register pressure and the same rules). Its B operand is written by
+// VALU instructions, of which two must lie between a write and the MFMA: the
+// conversions of a half step's operands end at least two slots before it
+// (tests/test_scaled_asm.py checks the compiled code).
+__device__ __forceinline__ void mfma16h_in_place(v4f &acc, const v4i &a, const v4i &b) {
+  asm volatile("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(acc) : "v"(a), "v"(b));
+}
+
+// f(0), f(1), .. f(N - 1) with compile-time arguments.
+template <class F, int... I>
+__device__ __forceinline__ void each(F &&f, std::integer_sequence<int, I...>) {
+  (f(std::integral_constant<int, I>()), ...);
+}
+
+// BM x 256 tiles of dx (BM 256: waves of 128 x 128; BM 128: of 128 x 64), one
+// tile per workgroup. A slice is 64 packed columns deep: the terms' rows (128
+// bytes, 16-byte chunk c of row r at c ^ (r % 8)) and 4 x 4 whole packed tiles,
+// both by DMA into three LDS stages, two slices ahead. A slice is multiplied in
+// two halves of 32; half (s, h) multiplies fragments read in the half before,
+// while it reads the next half's and turns its int8 values into float16:
+//   (s, 0)  reads half (s, 1) from stage s; DMAs of slice s + 2 begin. At its
+//           end slice s + 1 has landed (vmcnt: only slice s + 2's first DMAs
+//           remain), and the barrier publishes it.
+//   (s, 1)  reads half (s + 1, 0) from stage s + 1; the other DMAs of slice
+//           s + 2. Its MFMAs consume the last fragments of stage s, so after
+//           the barrier at its end stage s may be refilled (by slice s + 3).
+// `planes` 2: the terms' low halves are multiplied by the same weights in a
+// second pass over the slices.
+template <int E, int BM>
+__global__ __launch_bounds__(256, 1) void grad_dma_kernel(GradArgs p, ScaledTile<kGradOp, E> out) {
+  static_assert(BM == 256 || BM == 128, "256x256 or 128x256 tiles");
+  constexpr int WCOLS = BM == 256 ? 2 : 4, WTN = 256 / WCOLS, MI = 8, NI = WTN / 16;
+  constexpr int A_BYTES = BM * 128, B_BYTES = 64 * 256, NSTAGE = 3, B_REGION = NSTAGE * A_BYTES;
+  constexpr int DA = A_BYTES / 4096, DB = 4, DMAS = DA + DB, FIRST = DMAS / 2;
+  __shared__ __attribute__((aligned(1024))) int8_t smem[NSTAGE * (A_BYTES + B_BYTES)];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave / WCOLS, wn = wave % WCOLS;
+  const int g = lane >> 4, j = lane & 15;
+
+  const int total = gridDim.x, w = blockIdx.x;
+  const int q = total >> 3, r = total & 7, x = w & 7;
+  const int wl = x * q + (x < r ? x : r) + (w >> 3);
+  const int group = p.group_m * p.tiles_n, gid = wl / group, first_m = gid * p.group_m;
+  const int gm = min(p.tiles_m - first_m, p.group_m), within = wl - gid * group;
+  const int m0 = (first_m + within % gm) * BM, n0 = (within / gm) * 256;
+
+  const int kbt = p.Kp / 64;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(LDS_AS int8_t *)smem;
+  uint32_t a_lane[DA], b_lane[DB];
+#pragma unroll
+  for (int i = 0; i < DA; ++i) {
+    const int row = min(m0 + (wave * DA + i) * 8 + (lane >> 3), p.M - 1) - m0;
+    a_lane[i] = (uint32_t)(row * p.Np * 2 + ((lane & 7) ^ (lane >> 3)) * 16);
+  }
+#pragma unroll
+  for (int i = 0; i < DB; ++i)
+    b_lane[i] = (uint32_t)((wave * kbt + min(n0 / 64 + i, kbt - 1)) * 1024 + lane * 16);
+  const int8_t *const a_tile = (const int8_t *)(p.T + (int64_t)m0 * p.Np);
+  const int8_t *a_next = a_tile, *b_next = p.Bp;
+  const int per_plane = p.Np / 64, slices = per_plane * p.planes;
+  int left = per_plane, d_left = slices;   // slices left of the plane, and to fetch after the next one
+  const int64_t b_step = (int64_t)4 * kbt * 1024;
+  // The next slice's bases; past the last one it is fetched again (and not read).
+  auto next_slice = [&](const int8_t *&ab, const int8_t *&bb) {
+    ab = a_next;
+    bb = b_next;
+    if (--d_left > 0) {
+      if (--left == 0) {
+        left = per_plane;
+        a_next = a_tile + p.lo * 2;
+        b_next = p.Bp;
+      } else {
+        a_next += 128;
+        b_next += b_step;
+      }
+    }
+  };
+  auto dma = [&](int d, int stage, const int8_t *ab, const int8_t *bb) {
+    if (d < DA) dma_b128(ab, a_lane[d], lds0 + stage * A_BYTES + (wave * DA + d) * 1024);
+    else dma_b128(bb, b_lane[d - DA], lds0 + B_REGION + stage * B_BYTES + (wave * DB + d - DA) * 1024);
+  };
+
+  // Fragment addresses within a stage, less the blocks' constant parts.
+  const int a_row = (wm * 128 + j) * 128;
+  const int a_frag[2] = {a_row + ((g ^ (j & 7)) << 4), a_row + (((4 + g) ^ (j & 7)) << 4)};
+  const int b_frag = B_REGION + (g >> 1) * 4096 + wn * (WTN / 64) * 1024 + (8 * (g & 1) + (j >> 1)) * 16 + (j & 1) * 8;
+  v4f acc[MI][NI];
+  auto fence_acc = [&]() {
+#pragma unroll
+    for (int mi = 0; mi < MI; ++mi)
+#pragma unroll
+      for (int ni = 0; ni < NI; ++ni) asm volatile("" : "+a"(acc[mi][ni]));
+  };
+#pragma unroll
+  for (int mi = 0; mi < MI; ++mi)
+#pragma unroll
+    for (int ni = 0; ni < NI; ++ni) acc[mi][ni] = v4f{0, 0, 0, 0};
+  fence_acc();
+  asm volatile("s_nop 7\n\ts_nop 7" ::: "memory");
+
+  v4i fa[MI], fb0[NI], fb1[NI];
+  v2i raw[NI];
+  auto read_a = [&](int at, int mi) { fa[mi] = ld_lds_b128(smem, at + mi * 2048); };
+  auto read_b = [&](int at, int ni) { raw[ni] = ld_lds_tr8(smem, at + (ni >> 2) * 1024 + (ni & 3) * 256); };
+  const v2h off = {(_Float16)1152.0f, (_Float16)1152.0f};
+  // Operation o of a half step's 10 NI that turn its raw bytes into float16
+  // (bytes_to_half, one instruction at a time).
+  uint32_t biased = 0, pair = 0;
+  auto convert = [&](auto op, v4i *gb) __attribute__((always_inline)) {
+    constexpr int o = decltype(op)::value, ni = o / 10, d = o / 5 & 1;
+    if constexpr (o % 5 == 0) biased = (uint32_t)raw[ni][d] ^ 0x80808080u;
+    else if constexpr (o % 5 == 1) pair = __builtin_amdgcn_perm(0x64646464u, biased, 0x04010400u);
+    else if constexpr (o % 5 == 3) pair = __builtin_amdgcn_perm(0x64646464u, biased, 0x04030402u);
+    else gb[ni][2 * d + (o % 5 == 4)] = __builtin_bit_cast(int, __builtin_bit_cast(v2h, pair) - off);
+  };
+  constexpr int SLOTS = MI * NI, CONV0 = SLOTS / 4, DSTEP = SLOTS / (DMAS / 2 + 1);
+  static_assert(CONV0 + 5 * NI <= SLOTS - 2, "conversions end two slots before the half step does");
+  // One half step: MFMAs from fa and fb (odd rows right to left, so a row's
+  // first reuses the last B operand); the next half's fragments from at_a and
+  // at_b, B's converted into gb; DMAs d0 .. d1 - 1 of a slice into `stage`.
+  auto half = [&](v4i *fb, v4i *gb, int at_a, int at_b, auto first, auto last, int stage, const int8_t *ab,
+                  const int8_t *bb) __attribute__((always_inline)) {
+    constexpr int d0 = decltype(first)::value, d1 = decltype(last)::value;
+    each([&](auto at) __attribute__((always_inline)) {
+      constexpr int slot = decltype(at)::value, mi = slot / NI, pos = slot % NI, ni = (mi & 1) ? NI - 1 - pos : pos;
+      mfma16h_in_place(acc[mi][ni], fa[mi], fb[ni]);
+      if constexpr (slot < NI) read_b(at_b, slot);
+      if constexpr (pos == NI - 1) read_a(at_a, mi);
+      if constexpr (slot >= CONV0 && slot < CONV0 + 5 * NI) {
+        convert(std::integral_constant<int, 2 * (slot - CONV0)>(), gb);
+        convert(std::integral_constant<int, 2 * (slot - CONV0) + 1>(), gb);
+      }
+      if constexpr (slot % DSTEP == 2 && d0 + slot / DSTEP < d1) dma(d0 + slot / DSTEP, stage, ab, bb);
+      __builtin_amdgcn_sched_barrier(0);
+    }, std::make_integer_sequence<int, SLOTS>());
+  };
+  using Zero = std::integral_constant<int, 0>;
+  using First = std::integral_constant<int, FIRST>;
+  using All = std::integral_constant<int, DMAS>;
+
+  const int8_t *ab, *bb;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    next_slice(ab, bb);
+#pragma unroll
+    for (int d = 0; d < DMAS; ++d) dma(d, i, ab, bb);
+  }
+  asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" :: "n"(DMAS) : "memory");   // slice 0 landed
+#pragma unroll
+  for (int mi = 0; mi < MI; ++mi) read_a(a_frag[0], mi);
+#pragma unroll
+  for (int ni = 0; ni < NI; ++ni) read_b(b_frag, ni);
+  each([&](auto o) __attribute__((always_inline)) { convert(o, fb0); }, std::make_integer_sequence<int, 10 * NI>());
+  __builtin_amdgcn_s_waitcnt(0xC07F);   // lgkmcnt(0): no scalar load completes inside the loop
+  int st = 0;
+  for (int s = 0; s < slices; ++s) {
+    const int st1 = st == 2 ? 0 : st + 1, st2 = st == 0 ? 2 : st - 1;   // stages of slices s + 1, s + 2
+    next_slice(ab, bb);
+    half(fb0, fb1, a_frag[1] + st * A_BYTES, b_frag + 8192 + st * B_BYTES, Zero(), First(), st2, ab, bb);
+    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" :: "n"(FIRST) : "memory");
+    half(fb1, fb0, a_frag[0] + st1 * A_BYTES, b_frag + st1 * B_BYTES, First(), All(), st2, ab, bb);
+    asm volatile("s_barrier" ::: "memory");
+    st = st1;
+  }
+  // No DMA may write the LDS that the stores go through, and the last MFMAs'
+  // results must be there.
+  asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier\n\ts_nop 7\n\ts_nop 7" ::: "memory");
+  fence_acc();
+  out.template grad16<MI, NI>(acc, m0 + wm * 128, n0 + wn * WTN, lane, (LDS_AS int8_t *)smem + wave * 8192);
 }
 
 // 128 x 128 tiles of dx, 4 waves of 64 x 64. The contraction runs over packed
@@ -628,21 +1090,81 @@ int take_rows(const void *X, int type, int64_t ldx, const float *T, int64_t M, i
   return launch_quant(a, type, M, (hipStream_t)scr.stream);
 }
 
-template <int OP, int ACT>
-int launch_finish_typed(const FinishArgs &a, int type, hipStream_t s) {
-  const int cols = OP == 2 ? a.Np / 2 : a.N;
-  for (int r0 = 0; r0 < a.M; r0 += 65535) {
-    FinishArgs b = a;
-    b.S = a.S + (int64_t)r0 * a.Np;
-    b.t = a.t + r0;
-    b.D = a.D ? (const int8_t *)a.D + (int64_t)r0 * a.ldd * elem_size(type) : nullptr;
-    b.norm = a.norm ? a.norm + r0 : nullptr;
-    b.Y = (int8_t *)a.Y + (OP == 2 ? (int64_t)r0 * a.Np * 2 : (int64_t)r0 * a.ldy * elem_size(type));
-    const dim3 grid((unsigned)((cols + 255) / 256), (unsigned)std::min(a.M - r0, 65535));
-    switch (type) {
-      case VT_TYPE_F32: hipLaunchKernelGGL((finish_kernel<kF32, OP, ACT>), grid, dim3(256), 0, s, b); break;
-      case VT_TYPE_F16: hipLaunchKernelGGL((finish_kernel<kF16, OP, ACT>), grid, dim3(256), 0, s, b); break;
-      default: hipLaunchKernelGGL((finish_kernel<kBF16, OP, ACT>), grid, dim3(256), 0, s, b); break;
+GemmArgs scaled_args(const Rows &rows, const int8_t *Bp, int64_t M, int64_t Kp, int64_t Np, int bm, int bn) {
+  GemmArgs a = {};
+  a.A = rows.q;
+  a.B = Bp;
+  a.lda = rows.ld;
+  a.ldb = Kp / 64;
+  a.M = (int)M; a.N = (int)Np; a.K = (int)Kp;
+  a.tiles_m = (int)((M + bm - 1) / bm);
+  a.tiles_n = (int)((Np + bn - 1) / bn);
+  a.group_m = 4;
+  a.batch_count = 1;
+  a.k_last = a.K;
+  return a;
+}
+
+template <int OP, int E>
+int launch_finish(const int32_t *sums, int slices, const ScaledTile<OP, E> &out, hipStream_t s) {
+  const int cols = OP == kLinear ? out.Np : out.Np / 2;
+  const dim3 grid((unsigned)out.M, (unsigned)((cols + 255) / 256));
+  hipLaunchKernelGGL((finish_kernel<OP, E>), grid, dim3(256), 0, s, sums, slices, out);
+  VT_HIP_CHECK(hipGetLastError());
+  return VT_OK;
+}
+
+// The int8 product of rows and packed weights, and what follows it.
+template <int OP, int E>
+int launch_product(const Rows &rows, const int8_t *Bp, int64_t Kp, const ScaledTile<OP, E> &out, Scratch &scr) {
+  hipStream_t s = (hipStream_t)scr.stream;
+  const int cus = scr.st->num_cus;
+  const int64_t M = out.M, Np = out.Np;
+  const Problem q = {rows.q, Bp, nullptr, nullptr, M, Np, Kp, rows.ld, Kp / 64, 0, Np, 1, 0, 0, 0, 0};
+  void *w = nullptr;
+  if (Kp == 0) return launch_finish(nullptr, 0, out, s);
+  if (M <= kSkinnyMaxM || !packed_tiles_fit(q)) {
+    if (int rc = scr.take(kSums, (size_t)M * Np * sizeof(int32_t), &w)) return rc;
+    Problem r = q;
+    r.C = (int32_t *)w;
+    if (int rc = run_packed(r, 0, scr)) return rc;
+    return launch_finish((const int32_t *)w, 1, out, s);
+  }
+  const int64_t t256 = (M + 255) / 256 * ((Np + 255) / 256), t128 = (M + 255) / 256 * ((Np + 127) / 128);
+  const bool persistent = M >= 256 && Np >= 256 && Kp % 256 == 0 && 16 * 1024 * (Kp / 64) < (1ll << 32) - 4096;
+  if (persistent && (t256 >= 256 || (Kp >= 2048 && t256 > 128) || (Kp >= 1024 && t256 > 192))) {
+    const GemmArgs a = scaled_args(rows, Bp, M, Kp, Np, 256, 256);
+    hipLaunchKernelGGL((scaled_dma16_kernel<OP, E, 256>), dim3((unsigned)std::min<int64_t>(t256, cus)), dim3(256), 0, s, a, out);
+  } else if (persistent && Kp >= 1024 && t128 > 128 && t128 <= 256) {
+    const GemmArgs a = scaled_args(rows, Bp, M, Kp, Np, 256, 128);
+    hipLaunchKernelGGL((scaled_dma16_kernel<OP, E, 128>), dim3((unsigned)std::min<int64_t>(t128, cus)), dim3(256), 0, s, a, out);
+  } else {
+    const int ks = mfma_k_split<128, 128>(q);
+    if (ks > 1) {
+      if (int rc = scr.take(kPartials, (size_t)ks * M * Np * sizeof(int32_t), &w)) return rc;
+      const int64_t kc = Kp / ks;
+      Problem sl = q;
+      sl.K = kc;
+      sl.batch = ks;
+      sl.sa = kc;
+      sl.sb = kc / 64 * 1024;
+      sl.C = (int32_t *)w;
+      sl.ldc = Np;
+      sl.sc = M * Np;
+      if (int rc = launch_mfma_tiles<128, 128, true>(sl, s, cus)) return rc;
+      return launch_finish((const int32_t *)w, ks, out, s);
+    }
+    const int64_t half = (M + 63) / 64 * ((Np + 127) / 128), full = (M + 127) / 128 * ((Np + 127) / 128);
+    const bool short_k = Kp <= 128;
+    if (full > 0x7fffffff) return fail(VT_EUNSUPPORTED, "grid of %lld tiles too large", (long long)full);
+    if (half <= kHalfTileMaxWgs) {
+      const GemmArgs a = scaled_args(rows, Bp, M, Kp, Np, 64, 128);
+      if (short_k) hipLaunchKernelGGL((gemm_mfma_kernel<64, 128, 1, false, true, false, true, ScaledTile<OP, E>>), dim3((unsigned)half), dim3(256), 0, s, a, out);
+      else hipLaunchKernelGGL((gemm_mfma_kernel<64, 128, 1, false, false, false, true, ScaledTile<OP, E>>), dim3((unsigned)half), dim3(256), 0, s, a, out);
+    } else {
+      const GemmArgs a = scaled_args(rows, Bp, M, Kp, Np, 128, 128);
+      if (short_k) hipLaunchKernelGGL((gemm_mfma_kernel<128, 128, 1, false, true, false, true, ScaledTile<OP, E>>), dim3((unsigned)full), dim3(256), 0, s, a, out);
+      else hipLaunchKernelGGL((gemm_mfma_kernel<128, 128, 1, false, false, false, true, ScaledTile<OP, E>>), dim3((unsigned)full), dim3(256), 0, s, a, out);
     }
   }
   VT_HIP_CHECK(hipGetLastError());
@@ -650,18 +1172,15 @@ int launch_finish_typed(const FinishArgs &a, int type, hipStream_t s) {
 }
 
 template <int OP>
-int launch_finish(const FinishArgs &a, int type, int act, hipStream_t s) {
-  if (OP == 0 || act == VT_ACT_SILU) return launch_finish_typed<OP, VT_ACT_SILU>(a, type, s);
-  return launch_finish_typed<OP, VT_ACT_GELU>(a, type, s);
-}
-
-// int32 sums [M][Np] of rows and packed weights into a workspace.
-int take_sums(const Rows &rows, const int8_t *Bp, int64_t M, int64_t Kp, int64_t Np, Scratch &scr, int32_t **out) {
-  void *w = nullptr;
-  if (int rc = scr.take(kSums, (size_t)M * Np * sizeof(int32_t), &w)) return rc;
-  *out = (int32_t *)w;
-  const Problem q = {rows.q, Bp, nullptr, *out, M, Np, Kp, rows.ld, 0, 0, Np, 1, 0, 0, 0, 0};
-  return run_packed(q, 0, scr);
+int launch_scaled(const Rows &rows, const int8_t *Bp, int64_t Kp, const ScaledOut &o, Scratch &scr) {
+  if (o.type == VT_TYPE_F32) {
+    ScaledTile<OP, 4> t;
+    (ScaledOut &)t = o;
+    return launch_product(rows, Bp, Kp, t, scr);
+  }
+  ScaledTile<OP, 2> t;
+  (ScaledOut &)t = o;
+  return launch_product(rows, Bp, Kp, t, scr);
 }
 
 template <bool LINEAR>
@@ -676,13 +1195,30 @@ int launch_row_terms(const TermArgs &a, int type, hipStream_t s) {
   return VT_OK;
 }
 
-int launch_grad(GradArgs a, int type, hipStream_t s) {
+template <int E>
+int launch_grad_typed(GradArgs a, const ScaledOut &o, hipStream_t s, int cus) {
+  ScaledTile<kGradOp, E> out;
+  (ScaledOut &)out = o;
+  const int64_t cols = (a.Kp + 255) / 256;
+  const int64_t t256 = (a.M + 255) / 256 * cols, t128 = (a.M + 127) / 128 * cols;
+  a.group_m = 4;
+  if (a.Np > 0 && t128 >= 128 && 256ll * a.Np * 2 < (1ll << 31) && 4ll * a.Kp * 16 < (1ll << 31)) {
+    const int64_t r256 = (t256 + cus - 1) / cus * 2, r128 = (t128 + cus - 1) / cus;
+    const bool big = r256 <= r128;
+    a.tiles_m = (a.M + (big ? 255 : 127)) / (big ? 256 : 128);
+    a.tiles_n = (int)cols;
+    if (t128 > 0x7fffffff) return fail(VT_EUNSUPPORTED, "gradient grid too large");
+    if (big) hipLaunchKernelGGL((grad_dma_kernel<E, 256>), dim3((unsigned)t256), dim3(256), 0, s, a, out);
+    else hipLaunchKernelGGL((grad_dma_kernel<E, 128>), dim3((unsigned)t128), dim3(256), 0, s, a, out);
+    VT_HIP_CHECK(hipGetLastError());
+    return VT_OK;
+  }
   a.tiles_m = (a.M + 127) / 128;
   a.tiles_n = (a.Kp + 127) / 128;
   const int64_t tiles = (int64_t)a.tiles_m * a.tiles_n;
   if (tiles > 0x7fffffff) return fail(VT_EUNSUPPORTED, "gradient grid too large");
   const dim3 grid((unsigned)tiles);
-  switch (type) {
+  switch (o.type) {
     case VT_TYPE_F32: hipLaunchKernelGGL((grad_kernel<kF32, true>), grid, dim3(256), 0, s, a); break;
     case VT_TYPE_F16: hipLaunchKernelGGL((grad_kernel<kF16, false>), grid, dim3(256), 0, s, a); break;
     default: hipLaunchKernelGGL((grad_kernel<kBF16, false>), grid, dim3(256), 0, s, a); break;
@@ -758,13 +1294,6 @@ int open_scratch(void *stream, Scratch *scr) {
   return VT_OK;
 }
 
-// K == 0: the sums are zero. Cleared by a kernel (a captured memset is none of
-// the library's).
-__global__ __launch_bounds__(256) void zero_sums_kernel(int32_t *S, int64_t n) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i < n) S[i] = 0;
-}
-
 int forward(const ScaledCall &c, int act, void *stream) {
   bool empty = false;
   if (int rc = check_scaled(c, &empty)) return rc;
@@ -772,23 +1301,14 @@ int forward(const ScaledCall &c, int act, void *stream) {
   if (empty) return VT_OK;
   Scratch scr;
   if (int rc = open_scratch(stream, &scr)) return rc;
-  hipStream_t s = (hipStream_t)stream;
   const int64_t Kp = scaled_kp(c.K), Np = scaled_np(c.N, c.pair);
   Rows rows;
   if (int rc = take_rows(c.X, c.x_type, c.ldx, c.T, c.M, c.K, scr, &rows)) return rc;
-  int32_t *sums = nullptr;
-  if (c.K > 0) {
-    if (int rc = take_sums(rows, c.Bp, c.M, Kp, Np, scr, &sums)) return rc;
-  } else {
-    void *w = nullptr;
-    if (int rc = scr.take(kSums, (size_t)c.M * Np * sizeof(int32_t), &w)) return rc;
-    sums = (int32_t *)w;
-    const int64_t n = c.M * Np;
-    if (n > ((int64_t)1 << 38)) return fail(VT_EUNSUPPORTED, "%s: output too large", c.who);
-    hipLaunchKernelGGL(zero_sums_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, sums, n);
-  }
-  const FinishArgs f = {sums, rows.t, c.meta, nullptr, nullptr, c.Y, 0, c.ldy, 0, (int)c.M, (int)c.N, (int)Np};
-  return c.pair ? launch_finish<1>(f, c.y_type, act, s) : launch_finish<0>(f, c.y_type, act, s);
+  ScaledOut o = {};
+  o.t = rows.t; o.meta = c.meta; o.Y = c.Y; o.ldy = c.ldy;
+  o.M = (int)c.M; o.N = (int)c.N; o.Np = (int)Np;
+  o.act = act; o.type = c.y_type;
+  return c.pair ? launch_scaled<kGated>(rows, c.Bp, Kp, o, scr) : launch_scaled<kLinear>(rows, c.Bp, Kp, o, scr);
 }
 
 // The gradient in x^: D [M][ldd] of N columns, X the output [M][ldx] of K.
@@ -828,13 +1348,19 @@ int backward(const ScaledCall &c, const int8_t *Q, int q_type, int64_t ldq, cons
     if (int rc = launch_row_terms<false>(ta, c.x_type, s)) return rc;
     Rows rows;
     if (int rc = take_rows(Q, q_type, ldq, t, c.M, c.K, scr, &rows)) return rc;
-    int32_t *sums = nullptr;
-    if (int rc = take_sums(rows, c.Bp, c.M, Kp, Np, scr, &sums)) return rc;
-    const FinishArgs f = {sums, rows.t, c.meta, c.X, norm, terms, c.ldx, 0, lo, (int)c.M, (int)c.N, (int)Np};
-    if (int rc = launch_finish<2>(f, c.x_type, act, s)) return rc;
+    ScaledOut o = {};
+    o.t = rows.t; o.meta = c.meta; o.D = c.X; o.norm = norm; o.Y = terms;
+    o.ldd = c.ldx; o.lo = lo;
+    o.M = (int)c.M; o.N = (int)c.N; o.Np = (int)Np;
+    o.act = act; o.type = c.x_type;
+    if (int rc = launch_scaled<kTermsOp>(rows, c.Bp, Kp, o, scr)) return rc;
   }
-  const GradArgs g = {terms, c.Bp, norm, c.Y, c.ldy, lo, (int)c.M, (int)c.K, (int)Kp, (int)Np, 0, 0};
-  return launch_grad(g, c.y_type, s);
+  const GradArgs g = {terms, c.Bp, norm, c.Y, c.ldy, lo, (int)c.M, (int)c.K, (int)Kp, (int)Np, 0, 0, 0, split ? 2 : 1};
+  ScaledOut o = {};
+  o.norm = norm; o.Y = c.Y; o.ldy = c.ldy;
+  o.M = (int)c.M; o.N = (int)c.K;
+  o.type = c.y_type;
+  return split ? launch_grad_typed<4>(g, o, s, scr.st->num_cus) : launch_grad_typed<2>(g, o, s, scr.st->num_cus);
 }
 
 }  // namespace
