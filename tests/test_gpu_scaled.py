@@ -116,7 +116,9 @@ def test_quantize_weight_rounds_each_channel(dev):
 
 SHAPES = [(1, 1, 1), (1, 16, 16), (2, 64, 64), (5, 120, 72), (3, 63, 65), (16, 300, 31), (17, 256, 33), (33, 130, 200),
           (48, 1024, 96), (64, 1000, 130), (65, 333, 203), (100, 1023, 97), (130, 1024, 300), (257, 1025, 511),
-          (300, 2048, 1000), (512, 1024, 2048), (1, 4096, 1000), (4, 5000, 260), (1000, 320, 1300), (700, 4096, 520)]
+          (300, 2048, 1000), (512, 1024, 2048), (1, 4096, 1000), (4, 5000, 260), (1000, 320, 1300), (700, 4096, 520),
+          # few rows: rounded by the product itself or not, K in slices that finish in it or not
+          (1, 16384, 40), (3, 5000, 20), (16, 2048, 48), (9, 1700, 1000), (16, 1024, 500), (2, 131071, 17)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
@@ -197,6 +199,16 @@ def test_int8_rows_with_every_value(dev, m, k, n):
         ref.check(scaled.linear(r, W, out_dtype=torch.float32), want, bound, torch.float32, "linear")
         want, bound = ref.gated(q, t, w, s, w2, s2, "silu")
         ref.check(scaled.gated(r, G, out_dtype=torch.bfloat16), want, bound, torch.bfloat16, "gated")
+
+
+def test_the_longest_sums_stay_exact(dev):
+    """131071 products of -128 and -128: the largest sum that int32 holds."""
+    k = 131071
+    q, w = np.full((3, k), -128, np.int8), np.full((k, 5), -128, np.int8)
+    q[1], w[:, 2] = 127, 127
+    t, s = np.ones(3, np.float32), np.ones(5, np.float32)
+    y = scaled.linear(scaled.QuantRows(up(q, dev), up(t, dev)), packed(dev, w, s), out_dtype=torch.float32)
+    assert np.array_equal(y.cpu().numpy(), (q.astype(np.float64) @ w.astype(np.float64)).astype(np.float32))
 
 
 def test_rows_rounded_once_serve_several_products(dev):

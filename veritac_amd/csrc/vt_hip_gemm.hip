@@ -2360,8 +2360,8 @@ constexpr int kMaxSkinnyLds = 160 * 1024;
 
 // Scratch memory of one call: the K-split partial sums of the decode
 // kernels, the padded variant's operand copies, and the scaled operators'
-// int8 rows (kRows), int32 sums (kSums) and 16-bit gradient terms (kTerms).
-enum ScratchKind { kPartials = 0, kPadded = 1, kFinWords = 2, kRows = 3, kSums = 4, kTerms = 5, kScratchKinds = 6 };
+// int8 rows (kRows) and 16-bit gradient terms (kTerms).
+enum ScratchKind { kPartials = 0, kPadded = 1, kFinWords = 2, kRows = 3, kTerms = 4, kScratchKinds = 5 };
 
 struct Workspace {
   void *ptr = nullptr;
@@ -3491,34 +3491,6 @@ int launch_packed_rows(const Problem &q, int k_split, Scratch &scr, bool a_split
   return VT_OK;
 }
 
-// Any number of rows of a packed-B GEMM. Rows on the persistent DMA kernel
-// when there are enough whole 256-row tiles (all rows, unless the partial last
-// tile row would add a round), or all rows on its 256x128 form
-// (packed_dma128_fits); more than 64 remaining rows on 128x128 tiles; up to 64
-// rows, or tiles whose offsets do not fit 32 bits, in groups of up to 64 rows
-// on the decode kernel, each group streaming B once.
-int run_packed(const Problem &q, int k_split, Scratch &scr) {
-  hipStream_t stream = (hipStream_t)scr.stream;
-  if (packed_dma_rows(q) == 0 && packed_dma128_fits(q))
-    return launch_packed_dma128(q, stream, scr.st->num_cus);
-  int64_t r_first = 0;
-  if (const int64_t rows = packed_dma_rows(q)) {
-    if (int rc = launch_packed_dma(q, rows, stream, scr.st->num_cus)) return rc;
-    r_first = rows;
-  }
-  if (q.M - r_first > kSkinnyMaxM && packed_tiles_fit(q)) {
-    Problem g = rows_from(q, r_first);
-    g.ldb = packed_kbt(q.K);
-    return launch_mfma<128, 128, true>(g, scr);
-  }
-  for (int64_t r0 = r_first; r0 < q.M; r0 += kSkinnyMaxM) {
-    Problem g = rows_from(q, r0);
-    g.M = std::min<int64_t>(g.M, kSkinnyMaxM);
-    if (int rc = launch_packed_rows(g, k_split, scr)) return rc;
-  }
-  return VT_OK;
-}
-
 // ---------------------------------------------------------------------------
 // Padded path: any shape through the vector kernels
 // ---------------------------------------------------------------------------
@@ -4583,7 +4555,39 @@ int vt_gemm_i8_packed(const int8_t *A, const int8_t *Bp, const int32_t *D, int32
   scr.st = st;
   scr.stream = stream;
   if (K == 0) return launch_generic(q, (hipStream_t)stream);   // C = D (or 0)
-  return run_packed(q, k_split, scr);
+  // Rows on the persistent DMA kernel when there are enough whole 256-row
+  // tiles (all rows, unless the partial last tile row would add a round), or
+  // all rows on its 256x128 form (packed_dma128_fits);
+  // more than 64 remaining rows on 128x128 tiles; up to 64 rows, or tiles
+  // whose offsets do not fit 32 bits, in groups of up to 64 rows on the
+  // decode kernel, each group streaming B once.
+  if (packed_dma_rows(q) == 0 && packed_dma128_fits(q))
+    return launch_packed_dma128(q, (hipStream_t)stream, st->num_cus);
+  int64_t r_first = 0;
+  if (const int64_t rows = packed_dma_rows(q)) {
+    rc = launch_packed_dma(q, rows, (hipStream_t)stream, st->num_cus);
+    if (rc) return rc;
+    r_first = rows;
+  }
+  if (M - r_first > kSkinnyMaxM && packed_tiles_fit(q)) {
+    Problem g = q;
+    g.A = A + r_first * lda;
+    g.C = C + r_first * ldc;
+    g.D = D ? D + r_first * ldd : nullptr;
+    g.M = M - r_first;
+    g.ldb = packed_kbt(K);
+    return launch_mfma<128, 128, true>(g, scr);
+  }
+  for (int64_t r0 = r_first; r0 < M; r0 += kSkinnyMaxM) {
+    Problem g = q;
+    g.A = A + r0 * lda;
+    g.C = C + r0 * ldc;
+    g.D = D ? D + r0 * ldd : nullptr;
+    g.M = M - r0 < kSkinnyMaxM ? M - r0 : kSkinnyMaxM;
+    rc = launch_packed_rows(g, k_split, scr);
+    if (rc) return rc;
+  }
+  return VT_OK;
 }
 
 }  // extern "C"

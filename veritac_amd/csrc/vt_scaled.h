@@ -674,6 +674,301 @@ __global__ __launch_bounds__(256) void finish_kernel(const int32_t *S, int slice
   out.element(a0, a1, row, pc, j, out.t[row]);
 }
 
+// ---------------------------------------------------------------------------
+// Up to 64 rows
+// ---------------------------------------------------------------------------
+
+struct ScaledSkinnyArgs {
+  const void *X;      // int8 rows (XB 0), or the floating rows themselves
+  const int8_t *Bp;
+  float *t;           // XB > 0 with partial sums: the rows' scales for finish_kernel
+  int32_t *ws;        // [k_split][M][Np] partial sums, or null
+  uint64_t *fin;      // finishing words, or null
+  int64_t ldx;
+  int x_type, x_aligned;
+  int K, Kp, nbt;     // nbt: 16-column blocks of a projection
+  int hpw, groups, k_split, kb_per_split, fin_bits;
+};
+
+// Values of floating rows that a workgroup rounds to int8 itself: two pieces
+// of 16 for each of its 512 threads.
+constexpr int kFusedValues = 16384;
+
+// M <= 16 MB rows over packed weights, bound by reading the weights once: the
+// scheme of packed_skinny_kernel (a group of 8-column half blocks per
+// workgroup, its 8 waves taking 64-row blocks in turn, S of them in flight in
+// registers), for P projections whose column groups it takes together, and
+// with what follows the sums in its epilogue. XB > 0: X holds float32 (4) or
+// 16-bit (2) rows, at most kFusedValues with their padding; every workgroup
+// finds the rows' scales and keeps the rounded rows in LDS. Their loads are
+// issued before the first weights' and waited for behind them, so the stream
+// of weights starts no later.
+//
+// K slices finish through 64-bit words as in packed_skinny_kernel: the words'
+// two sums are two rows of a column (P = 1) or the two projections of one
+// element (P = 2).
+template <int OP, int NBW, int MB, int XB>
+__global__ __launch_bounds__(512) void scaled_skinny_kernel(ScaledSkinnyArgs p, ScaledOut o) {
+  constexpr int P = OP == kGated ? 2 : 1, NT = NBW * P, WAVES = 8, S = packed_stages(NT);
+  static_assert(XB == 0 || MB == 1, "rows are rounded here for M <= 16");
+  __shared__ v4i red[WAVES * NT * 64];
+  __shared__ __attribute__((aligned(16))) int8_t arows[XB ? kFusedValues + 16 * 32 : 16];
+  __shared__ uint32_t tops[16];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int G = gridDim.x, w = blockIdx.x;
+  const int q = G >> 3, r = G & 7, x = w & 7;
+  const int wl = x * q + (x < r ? x : r) + (w >> 3);
+  const int group = wl % p.groups, split = wl / p.groups;
+  const int h0 = group * p.hpw, h1 = min(h0 + p.hpw, 2 * p.nbt);   // half blocks [h0, h1) of a projection
+  const int nb0 = h0 >> 1, live = ((h1 - 1) >> 1) - nb0 + 1;
+  const int kbt = p.Kp / 64, kb_beg = split * p.kb_per_split, kb_end = min(kb_beg + p.kb_per_split, kbt);
+  const int acol = (lane >> 4) * 16, M = o.M;
+  auto col_lo = [&](int n) { return (n == 0 && (h0 & 1)) ? 8 : 0; };
+  auto col_hi = [&](int n) { return n >= live ? 0 : (n == live - 1 && (h1 & 1)) ? 8 : 16; };
+  // 16-column block nb of projection `which` among the packed ones
+  auto block = [&](int nb, int which) { return P == 1 ? nb : (nb >> 1) * 4 + (nb & 1) + 2 * which; };
+
+  // This thread's pieces of the floating rows.
+  uint32_t raw[XB ? 2 : 1][XB ? XB * 4 : 1];
+  const int per_row = p.Kp / 16;
+  if constexpr (XB > 0) {
+    if (tid < 16) tops[tid] = 0;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int idx = tid + 512 * i, row = idx / per_row, pos = (idx - row * per_row) * 16;
+#pragma unroll
+      for (int e = 0; e < XB * 4; ++e) raw[i][e] = 0;
+      if (row < M) {
+        const int8_t *src = (const int8_t *)p.X + ((int64_t)row * p.ldx + pos) * XB;
+        if (p.x_aligned && pos + 16 <= p.K) {
+#pragma unroll
+          for (int v = 0; v < XB; ++v) {
+            const v4i y = *(const v4i *)(src + v * 16);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) raw[i][v * 4 + e] = (uint32_t)y[e];
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            if (pos + e < p.K) {
+              if constexpr (XB == 4) raw[i][e] = ((const uint32_t *)src)[e];
+              else raw[i][e >> 1] |= (uint32_t)((const uint16_t *)src)[e] << (16 * (e & 1));
+            }
+        }
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  }
+
+  const bool dead_lo = (h0 & 1) && (lane & 15) < 8, dead_hi = (h1 & 1) && (lane & 15) >= 8;
+  const int8_t *b_tile[NT];
+  uint32_t b_lane[NBW];
+#pragma unroll
+  for (int n = 0; n < NBW; ++n) {
+    const bool dead = ((n == 0 || live == 1) && dead_lo) || (n >= live - 1 && dead_hi);
+    b_lane[n] = (uint32_t)(dead ? lane ^ 8 : lane) * 16;
+#pragma unroll
+    for (int i = 0; i < P; ++i)
+      b_tile[i * NBW + n] = p.Bp + (int64_t)block(nb0 + min(n, live - 1), i) * kbt * 1024;
+  }
+  const int8_t *a_src[MB];
+#pragma unroll
+  for (int mb = 0; mb < MB; ++mb) {
+    const int row = min(mb * 16 + (lane & 15), M - 1);
+    a_src[mb] = XB ? arows + row * (p.Kp + 32) + acol : (const int8_t *)p.X + (int64_t)row * p.ldx + acol;
+  }
+  v4i acc[MB][NT];
+#pragma unroll
+  for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+    for (int n = 0; n < NT; ++n) acc[mb][n] = v4i{0, 0, 0, 0};
+
+  const int first = kb_beg + wave;
+  const int steps = first < kb_end ? (kb_end - first + WAVES - 1) / WAVES : 0;
+  v4i a[S][MB], b[S][NT];
+  auto load_b = [&](int s, v4i (&bv)[NT]) {
+    const int kb = first + s * WAVES;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+      bv[n] = __builtin_nontemporal_load((const v4i *)(b_tile[n] + (int64_t)kb * 1024 + b_lane[n % NBW]));
+  };
+  auto load_a = [&](int s, v4i (&av)[MB]) {
+    const int kb = first + s * WAVES;
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb) {
+      if constexpr (XB > 0) av[mb] = *(const LDS_AS v4i *)((const LDS_AS int8_t *)a_src[mb] + kb * 64);
+      else av[mb] = *(const v4i *)(a_src[mb] + kb * 64);
+    }
+  };
+  auto load = [&](int s, v4i (&av)[MB], v4i (&bv)[NT]) {
+    load_b(s, bv);
+    load_a(s, av);
+  };
+  auto multiply = [&](const v4i (&av)[MB], const v4i (&bv)[NT]) {
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+        acc[mb][n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(av[mb], bv[n], acc[mb][n], 0, 0, 0);
+  };
+  // Rounds the rows, between the first weights' loads and their use.
+  auto round_rows = [&]() {
+    if constexpr (XB > 0) {
+      float v[2][16];
+      uint32_t top[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        top[i] = 0;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          if constexpr (XB == 4) {
+            v[i][e] = __uint_as_float(raw[i][e]);
+          } else {
+            const uint32_t h = raw[i][e >> 1] >> (16 * (e & 1));
+            v[i][e] = p.x_type == VT_TYPE_BF16 ? __uint_as_float(h << 16)
+                                               : (float)__builtin_bit_cast(_Float16, (uint16_t)h);
+          }
+          top[i] = max(top[i], magnitude(v[i][e]));
+        }
+        // the 8 threads of 128 columns share a row (Kp is a multiple of 128)
+#pragma unroll
+        for (int d = 4; d; d >>= 1) top[i] = max(top[i], (uint32_t)__shfl_xor((int)top[i], d));
+      }
+      lds_barrier();
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int row = (tid + 512 * i) / per_row;
+        if (row < M && (tid & 7) == 0) atomicMax(&tops[row], top[i]);
+      }
+      lds_barrier();
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int idx = tid + 512 * i, row = idx / per_row, pos = (idx - row * per_row) * 16;
+        if (row < M) {
+          const float inv = row_scale(tops[row]).inv;
+          v4i out;
+#pragma unroll
+          for (int d = 0; d < 4; ++d)
+            out[d] = inv == 0.0f ? 0
+                                 : pack_bytes(round_byte(v[i][4 * d], inv), round_byte(v[i][4 * d + 1], inv),
+                                              round_byte(v[i][4 * d + 2], inv), round_byte(v[i][4 * d + 3], inv));
+          st_lds_b128(arows, row * (p.Kp + 32) + pos, out);
+        }
+      }
+      lds_barrier();
+      if (p.ws && wl == 0 && tid < M) p.t[tid] = row_scale(tops[tid]).scale;
+    }
+  };
+  if (steps >= S) {
+#pragma unroll
+    for (int s = 0; s < S; ++s) load_b(s, b[s]);
+    if constexpr (XB > 0) __builtin_amdgcn_sched_barrier(0);
+    round_rows();
+#pragma unroll
+    for (int s = 0; s < S; ++s) load_a(s, a[s]);
+    int s0 = 0;
+    for (; s0 + 2 * S <= steps; s0 += S) {
+#pragma unroll
+      for (int s = 0; s < S; ++s) {
+        multiply(a[s], b[s]);
+        load(s0 + s + S, a[s], b[s]);
+      }
+    }
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      if (s0 + s < steps) multiply(a[s], b[s]);
+      if (s0 + s + S < steps) load(s0 + s + S, a[s], b[s]);
+    }
+#pragma unroll
+    for (int s = 0; s < S; ++s)
+      if (s0 + s + S < steps) multiply(a[s], b[s]);
+  } else {
+#pragma unroll
+    for (int s = 0; s < S; ++s)
+      if (s < steps) load_b(s, b[s]);
+    if constexpr (XB > 0) __builtin_amdgcn_sched_barrier(0);
+    round_rows();
+#pragma unroll
+    for (int s = 0; s < S; ++s)
+      if (s < steps) load_a(s, a[s]);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int s = 0; s < S; ++s)
+      if (s < steps) multiply(a[s], b[s]);
+  }
+
+  auto row_t = [&](int row) { return XB ? row_scale(tops[row]).scale : o.t[row]; };
+  auto finish = [&](int32_t a0, int32_t a1, int row, int col, float t_row) {
+    const int pc = P == 1 ? col : (int)pair_col(col, 0);
+    if (o.type == VT_TYPE_F32) {
+      ScaledTile<OP, 4> out;
+      (ScaledOut &)out = o;
+      out.element(a0, a1, row, pc, col, t_row);
+    } else {
+      ScaledTile<OP, 2> out;
+      (ScaledOut &)out = o;
+      out.element(a0, a1, row, pc, col, t_row);
+    }
+  };
+  // The sum over the waves of element e of source lane `src` of tile n.
+  auto sum = [&](int n, int src, int e) {
+    int32_t s = 0;
+#pragma unroll
+    for (int wv = 0; wv < WAVES; ++wv) s = add_wrap(s, ((const int32_t *)&red[(wv * NT + n) * 64 + src])[e]);
+    return s;
+  };
+  if (MB == 1 && p.fin) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n) red[(wave * NT + n) * 64 + lane] = acc[0][n];
+    __syncthreads();
+    const int fw = p.fin_bits;
+    const uint64_t field = (1ull << fw) - 1;
+    const int64_t bias = (int64_t)kFinBiasPerRow * p.kb_per_split * 64;
+    constexpr int PER_BLOCK = P == 1 ? 128 : 256;   // words of a column block
+    for (int t = tid; t < NBW * PER_BLOCK; t += 512) {
+      const int n = t / PER_BLOCK, rw = t % PER_BLOCK >> 4, c = t & 15;
+      const int row = P == 1 ? 2 * rw : rw, src = (row >> 2) * 16 + c, e = row & 3;
+      const int32_t s0 = sum(n, src, e), s1 = P == 1 ? sum(n, src, e + 1) : sum(n + NBW, src, e);
+      if (c < col_lo(n) || c >= col_hi(n) || row >= M) continue;
+      const int col = (nb0 + n) * 16 + c;
+      const uint64_t lo = (uint64_t)((int64_t)s0 + bias), hi = (uint64_t)((int64_t)s1 + bias);
+      uint64_t *word = p.fin + ((int64_t)rw * p.nbt * 16 + col);
+      const uint64_t old = __hip_atomic_fetch_add(word, (1ull << (2 * fw)) | (hi << fw) | lo, __ATOMIC_RELAXED,
+                                                  __HIP_MEMORY_SCOPE_AGENT);
+      if ((old >> (2 * fw)) != (uint64_t)(p.k_split - 1)) continue;
+      const int64_t all_bias = bias * p.k_split;
+      const int32_t v0 = (int32_t)((int64_t)((old & field) + lo) - all_bias);
+      const int32_t v1 = (int32_t)((int64_t)(((old >> fw) & field) + hi) - all_bias);
+      finish(v0, v1, row, col, row_t(row));
+      if (P == 1 && row + 1 < M) finish(v1, 0, row + 1, col, row_t(row + 1));
+      __hip_atomic_store(word, 0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    return;
+  }
+#pragma unroll
+  for (int mb = 0; mb < MB; ++mb) {
+    if (mb > 0) __syncthreads();
+#pragma unroll
+    for (int n = 0; n < NT; ++n) red[(wave * NT + n) * 64 + lane] = acc[mb][n];
+    __syncthreads();
+    for (int t = tid; t < NBW * 256; t += 512) {
+      const int n = t >> 8, r16 = (t >> 4) & 15, c = t & 15;
+      const int src = (r16 >> 2) * 16 + c, e = r16 & 3, row = mb * 16 + r16;
+      if (row >= M || c < col_lo(n) || c >= col_hi(n)) continue;
+      const int32_t s0 = sum(n, src, e), s1 = P == 1 ? 0 : sum(n + NBW, src, e);
+      const int col = (nb0 + n) * 16 + c;
+      if (!p.ws) {
+        finish(s0, s1, row, col, row_t(row));
+      } else {
+        int32_t *ws = p.ws + ((int64_t)split * M + row) * o.Np;
+        ws[P == 1 ? col : pair_col(col, 0)] = s0;
+        if (P == 2) ws[pair_col(col, 1)] = s1;
+      }
+    }
+  }
+}
+
 struct TermArgs {
   const void *D;
   const float *t;      // gated: row scales
@@ -1032,6 +1327,10 @@ __global__ __launch_bounds__(256) void grad_kernel(GradArgs p) {
 bool float_type(int type) { return type == VT_TYPE_F32 || type == VT_TYPE_F16 || type == VT_TYPE_BF16; }
 
 constexpr int64_t kScaledMax = (int64_t)1 << 30;
+// The longest sums: 131071 products of -128 and -128 stay below 2^31.
+constexpr int64_t kScaledMaxK = 131071;
+// Pitch of int8 rows from which on they are copied before the products.
+constexpr int64_t kFarRows = (int64_t)1 << 23;
 
 template <int TYPE, bool ALIGNED>
 void launch_quant_typed(const QuantArgs &a, int64_t M, hipStream_t s) {
@@ -1063,10 +1362,11 @@ struct Rows {
 };
 
 // X (any type) -> rows of Kp int8 values: int8 rows that are already so are
-// used where they are, others are copied (int8) or rounded to a workspace.
+// used where they are (unless they lie too far apart for the tile kernels'
+// 32-bit offsets), others are copied (int8) or rounded to a workspace.
 int take_rows(const void *X, int type, int64_t ldx, const float *T, int64_t M, int64_t K, Scratch &scr, Rows *out) {
   const int64_t Kp = scaled_kp(K);
-  if ((type == VT_TYPE_I8 && K == Kp && ldx % 16 == 0 && aligned16(X)) || type == VT_TYPE_I8_PADDED) {
+  if (ldx <= kFarRows && ((type == VT_TYPE_I8 && K == Kp && ldx % 16 == 0 && aligned16(X)) || type == VT_TYPE_I8_PADDED)) {
     *out = Rows{(const int8_t *)X, T, ldx};
     return VT_OK;
   }
@@ -1074,8 +1374,8 @@ int take_rows(const void *X, int type, int64_t ldx, const float *T, int64_t M, i
   const size_t q_bytes = (size_t)M * Kp;
   if (int rc = scr.take(kRows, q_bytes + (size_t)M * sizeof(float), &w)) return rc;
   QuantArgs a = {X, (int8_t *)w, (float *)((int8_t *)w + q_bytes), ldx, Kp, K, Kp};
-  *out = Rows{a.Q, type == VT_TYPE_I8 ? T : a.T, Kp};
-  if (type == VT_TYPE_I8) {
+  *out = Rows{a.Q, float_type(type) ? a.T : T, Kp};
+  if (!float_type(type)) {
     for (int64_t r0 = 0; r0 < M; r0 += 65535) {
       QuantArgs b = a;
       b.X = (const int8_t *)X + r0 * ldx;
@@ -1114,7 +1414,7 @@ int launch_finish(const int32_t *sums, int slices, const ScaledTile<OP, E> &out,
   return VT_OK;
 }
 
-// The int8 product of rows and packed weights, and what follows it.
+// The int8 product of rows and packed weights, and what follows it, on tiles.
 template <int OP, int E>
 int launch_product(const Rows &rows, const int8_t *Bp, int64_t Kp, const ScaledTile<OP, E> &out, Scratch &scr) {
   hipStream_t s = (hipStream_t)scr.stream;
@@ -1123,13 +1423,6 @@ int launch_product(const Rows &rows, const int8_t *Bp, int64_t Kp, const ScaledT
   const Problem q = {rows.q, Bp, nullptr, nullptr, M, Np, Kp, rows.ld, Kp / 64, 0, Np, 1, 0, 0, 0, 0};
   void *w = nullptr;
   if (Kp == 0) return launch_finish(nullptr, 0, out, s);
-  if (M <= kSkinnyMaxM || !packed_tiles_fit(q)) {
-    if (int rc = scr.take(kSums, (size_t)M * Np * sizeof(int32_t), &w)) return rc;
-    Problem r = q;
-    r.C = (int32_t *)w;
-    if (int rc = run_packed(r, 0, scr)) return rc;
-    return launch_finish((const int32_t *)w, 1, out, s);
-  }
   const int64_t t256 = (M + 255) / 256 * ((Np + 255) / 256), t128 = (M + 255) / 256 * ((Np + 127) / 128);
   const bool persistent = M >= 256 && Np >= 256 && Kp % 256 == 0 && 16 * 1024 * (Kp / 64) < (1ll << 32) - 4096;
   if (persistent && (t256 >= 256 || (Kp >= 2048 && t256 > 128) || (Kp >= 1024 && t256 > 192))) {
@@ -1169,6 +1462,123 @@ int launch_product(const Rows &rows, const int8_t *Bp, int64_t Kp, const ScaledT
   }
   VT_HIP_CHECK(hipGetLastError());
   return VT_OK;
+}
+
+// Column groups and K slices for up to 64 rows: packed_geometry's rules, for
+// groups that hold both projections' columns.
+struct ScaledGeom {
+  int hpw, groups, ks;
+};
+
+template <int P>
+ScaledGeom skinny_geom(int64_t M, int64_t nbt, int64_t Kp, int cus) {
+  const int64_t units = 2 * nbt, most = 2 * kPackedNBW / P, kbt = Kp / 64;
+  auto halves = [&](int64_t ks) {
+    if ((units + most - 1) / most * ks >= 192) return most;
+    return std::max<int64_t>(1, std::min(most, (units * ks + cus - 1) / cus));
+  };
+  int64_t hpw = halves(1), ks = 1;
+  const int64_t groups = (units + hpw - 1) / hpw;
+  if (groups < 192) {
+    ks = std::max<int64_t>(1, std::min({(224 + groups - 1) / groups, (kbt + kPackedWaves - 1) / kPackedWaves, (int64_t)64}));
+  } else if (hpw < most) {
+    // narrow groups read A for longer than a split takes to sum (packed_a_split)
+    int64_t least = 0;
+    for (int64_t k = 1; k <= 4 && (k == 1 || kbt >= k * kPackedWaves); k *= 2) {
+      const int64_t chunk = (kbt + k - 1) / k * 64, h = halves(k), wgs = (units + h - 1) / h * k;
+      int64_t ns = (wgs + cus - 1) / cus * chunk * (315 * h * P + 32 * M) / 1000;
+      if (k > 1) ns += M <= kSkinnyFinMaxM && skinny_fin_bits((int)k, chunk) > 0 ? 2000 : 3500 + 8 * M * nbt * 16 * P * k / 1500;
+      if (k == 1 || ns < least) {
+        least = ns;
+        ks = k;
+      }
+    }
+    hpw = halves(ks);
+  }
+  return {(int)hpw, (int)((units + hpw - 1) / hpw), (int)ks};
+}
+
+template <int OP, int NBW, int XB>
+void launch_skinny_blocks(const ScaledSkinnyArgs &a, const ScaledOut &o, dim3 grid, hipStream_t s) {
+  if constexpr (XB > 0) {
+    hipLaunchKernelGGL((scaled_skinny_kernel<OP, NBW, 1, XB>), grid, dim3(512), 0, s, a, o);
+  } else {
+    switch ((o.M + 15) / 16) {
+      case 1: hipLaunchKernelGGL((scaled_skinny_kernel<OP, NBW, 1, 0>), grid, dim3(512), 0, s, a, o); break;
+      case 2: hipLaunchKernelGGL((scaled_skinny_kernel<OP, NBW, 2, 0>), grid, dim3(512), 0, s, a, o); break;
+      case 3: hipLaunchKernelGGL((scaled_skinny_kernel<OP, NBW, 3, 0>), grid, dim3(512), 0, s, a, o); break;
+      default: hipLaunchKernelGGL((scaled_skinny_kernel<OP, NBW, 4, 0>), grid, dim3(512), 0, s, a, o); break;
+    }
+  }
+}
+
+template <int OP, int XB>
+void launch_skinny_rows(const ScaledSkinnyArgs &a, const ScaledOut &o, dim3 grid, hipStream_t s) {
+  const int blocks = (a.hpw + 1) / 2;
+  if constexpr (OP == kGated) {
+    if (blocks == 1) launch_skinny_blocks<OP, 1, XB>(a, o, grid, s);
+    else launch_skinny_blocks<OP, 2, XB>(a, o, grid, s);
+  } else {
+    switch (blocks) {
+      case 1: launch_skinny_blocks<OP, 1, XB>(a, o, grid, s); break;
+      case 2: launch_skinny_blocks<OP, 2, XB>(a, o, grid, s); break;
+      case 3: launch_skinny_blocks<OP, 3, XB>(a, o, grid, s); break;
+      default: launch_skinny_blocks<OP, 4, XB>(a, o, grid, s); break;
+    }
+  }
+}
+
+// Up to 64 rows of a forward call: X of any type (rows already int8 in `rows`
+// when it is null).
+template <int OP>
+int launch_skinny(const void *X, int type, int64_t ldx, int64_t K, const Rows &rows, const int8_t *Bp, ScaledOut o, Scratch &scr) {
+  constexpr int P = OP == kGated ? 2 : 1;
+  hipStream_t s = (hipStream_t)scr.stream;
+  const int64_t Kp = scaled_kp(K), nbt = (o.N + 15) / 16;
+  const ScaledGeom g = skinny_geom<P>(o.M, nbt, Kp, scr.st->num_cus);
+  ScaledSkinnyArgs a = {};
+  a.X = X ? X : rows.q;
+  a.Bp = Bp;
+  a.ldx = X ? ldx : rows.ld;
+  a.x_type = type;
+  a.x_aligned = X && aligned16(X) && ldx * elem_size(type) % 16 == 0;
+  a.K = (int)K; a.Kp = (int)Kp; a.nbt = (int)nbt;
+  a.hpw = g.hpw;
+  a.groups = g.groups;
+  a.kb_per_split = (int)((Kp / 64 + g.ks - 1) / g.ks);
+  a.k_split = (int)((Kp / 64 + a.kb_per_split - 1) / a.kb_per_split);
+  void *w = nullptr;
+  if (a.k_split > 1) {
+    const int bits = o.M <= kSkinnyFinMaxM ? skinny_fin_bits(a.k_split, (int64_t)a.kb_per_split * 64) : 0;
+    if (bits > 0) {
+      const int64_t words = (P == 1 ? (o.M + 1) / 2 : o.M) * nbt * 16;
+      if (int rc = scr.take(kFinWords, (size_t)words * sizeof(uint64_t), &w)) return rc;
+      a.fin = (uint64_t *)w;
+      a.fin_bits = bits;
+    } else {
+      if (int rc = scr.take(kPartials, (size_t)a.k_split * o.M * o.Np * sizeof(int32_t), &w)) return rc;
+      a.ws = (int32_t *)w;
+      if (X) {
+        if (int rc = scr.take(kRows, (size_t)o.M * sizeof(float), &w)) return rc;
+        a.t = (float *)w;
+        o.t = a.t;
+      }
+    }
+  }
+  const dim3 grid((unsigned)(a.groups * a.k_split));
+  if (!X) launch_skinny_rows<OP, 0>(a, o, grid, s);
+  else if (type == VT_TYPE_F32) launch_skinny_rows<OP, 4>(a, o, grid, s);
+  else launch_skinny_rows<OP, 2>(a, o, grid, s);
+  VT_HIP_CHECK(hipGetLastError());
+  if (!a.ws) return VT_OK;
+  if (o.type == VT_TYPE_F32) {
+    ScaledTile<OP, 4> t;
+    (ScaledOut &)t = o;
+    return launch_finish(a.ws, a.k_split, t, s);
+  }
+  ScaledTile<OP, 2> t;
+  (ScaledOut &)t = o;
+  return launch_finish(a.ws, a.k_split, t, s);
 }
 
 template <int OP>
@@ -1248,8 +1658,9 @@ int check_scaled(const ScaledCall &c, bool *empty) {
   *empty = false;
   if (c.M < 0 || c.K < 0 || c.N < 0)
     return fail(VT_EINVAL, "%s: negative size (M=%lld K=%lld N=%lld)", c.who, (long long)c.M, (long long)c.K, (long long)c.N);
-  if (c.M >= kScaledMax || c.K >= kScaledMax || c.N >= kScaledMax / 2)
-    return fail(VT_EINVAL, "%s: size beyond 2^30", c.who);
+  if (c.M >= kScaledMax || c.N >= kScaledMax / 2) return fail(VT_EINVAL, "%s: size beyond 2^30", c.who);
+  if (c.K > kScaledMaxK)
+    return fail(VT_EINVAL, "%s: int32 sums hold K <= %lld (K=%lld)", c.who, (long long)kScaledMaxK, (long long)c.K);
   const bool i8 = c.x_type == VT_TYPE_I8 || c.x_type == VT_TYPE_I8_PADDED;
   if (!float_type(c.x_type) && !i8) return fail(VT_EINVAL, "%s: unknown input type %d", c.who, c.x_type);
   if (!float_type(c.y_type)) return fail(VT_EINVAL, "%s: unknown output type %d", c.who, c.y_type);
@@ -1302,12 +1713,20 @@ int forward(const ScaledCall &c, int act, void *stream) {
   Scratch scr;
   if (int rc = open_scratch(stream, &scr)) return rc;
   const int64_t Kp = scaled_kp(c.K), Np = scaled_np(c.N, c.pair);
-  Rows rows;
-  if (int rc = take_rows(c.X, c.x_type, c.ldx, c.T, c.M, c.K, scr, &rows)) return rc;
   ScaledOut o = {};
-  o.t = rows.t; o.meta = c.meta; o.Y = c.Y; o.ldy = c.ldy;
+  o.meta = c.meta; o.Y = c.Y; o.ldy = c.ldy;
   o.M = (int)c.M; o.N = (int)c.N; o.Np = (int)Np;
   o.act = act; o.type = c.y_type;
+  Rows rows = {};
+  const bool skinny = c.M <= kSkinnyMaxM && Kp > 0;
+  if (skinny && float_type(c.x_type) && c.M <= 16 && c.M * Kp <= kFusedValues)
+    return c.pair ? launch_skinny<kGated>(c.X, c.x_type, c.ldx, c.K, rows, c.Bp, o, scr)
+                  : launch_skinny<kLinear>(c.X, c.x_type, c.ldx, c.K, rows, c.Bp, o, scr);
+  if (int rc = take_rows(c.X, c.x_type, c.ldx, c.T, c.M, c.K, scr, &rows)) return rc;
+  o.t = rows.t;
+  if (skinny)
+    return c.pair ? launch_skinny<kGated>(nullptr, 0, 0, c.K, rows, c.Bp, o, scr)
+                  : launch_skinny<kLinear>(nullptr, 0, 0, c.K, rows, c.Bp, o, scr);
   return c.pair ? launch_scaled<kGated>(rows, c.Bp, Kp, o, scr) : launch_scaled<kLinear>(rows, c.Bp, Kp, o, scr);
 }
 
@@ -1399,8 +1818,9 @@ int vt_quant_rows(const void *X, int32_t x_type, int64_t ldx, int8_t *Q, int64_t
 }
 
 int64_t vt_scaled_size(int64_t K, int64_t N, int32_t pair, int64_t *meta_floats) {
-  if (K < 0 || N < 0 || K >= kScaledMax || N >= kScaledMax / 2)
-    return fail(VT_EINVAL, "vt_scaled_size: needs 0 <= K < 2^30, 0 <= N < 2^29 (K=%lld N=%lld)", (long long)K, (long long)N);
+  if (K < 0 || N < 0 || K > kScaledMaxK || N >= kScaledMax / 2)
+    return fail(VT_EINVAL, "vt_scaled_size: needs 0 <= K <= %lld, 0 <= N < 2^29 (K=%lld N=%lld)", (long long)kScaledMaxK,
+                (long long)K, (long long)N);
   const int64_t Np = scaled_np(N, pair != 0);
   if (meta_floats) *meta_floats = scaled_meta(Np);
   return scaled_kp(K) * Np;
