@@ -542,7 +542,7 @@ struct ScaledTile : ScaledOut {
   }
 
   // The gradient's float32 sums, in tile16's layout, over the row's normaliser
-  // (a power of two: exact).
+  // (a power of two: exact; null for partial sums).
   template <int MI, int NI>
   __device__ __forceinline__ void grad16(const v4f (&acc)[MI][NI], int row0, int col0, int lane,
                                          LDS_AS int8_t *lds) const {
@@ -552,7 +552,7 @@ struct ScaledTile : ScaledOut {
 #pragma unroll
     for (int mi = 0; mi < MI; ++mi)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) un[mi][e] = 1.0f / norm[min(row0 + mi * 16 + 4 * g + e, M - 1)];
+      for (int e = 0; e < 4; ++e) un[mi][e] = norm ? 1.0f / norm[min(row0 + mi * 16 + 4 * g + e, M - 1)] : 1.0f;
     auto swz = [](int row) { return (((row >> 2) & 3) * OE) & (RC - 1); };
 #pragma unroll
     for (int mi = 0; mi < MI; ++mi) {
@@ -979,33 +979,79 @@ struct TermArgs {
   int M, N, Np;
 };
 
+// 16 float16 terms of a row, and what float16 leaves of them.
+__device__ __forceinline__ void put_terms(_Float16 *y, int64_t lo, const float (&v)[16]) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    v8h h, l;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      h[e] = (_Float16)v[8 * i + e];
+      l[e] = (_Float16)(v[8 * i + e] - (float)h[e]);
+    }
+    *(v8h *)(y + 8 * i) = h;
+    if (lo) *(v8h *)(y + lo + 8 * i) = l;
+  }
+}
+
 // One workgroup per row of dy. LINEAR: the row's terms dy s, normalised by
-// their own largest; else only the normaliser of a gated product's terms,
-// from the row's largest |dh|, its scale and the weights' bound: |q| <= 128,
-// |act(g)| <= |g| and |act'| <= 1.13.
-template <int TYPE, bool LINEAR>
+// their own largest; NC pieces of 16 stay in each thread's registers between
+// the maximum and the rounding (0: longer rows, read twice). Else only the
+// normaliser of a gated product's terms, from the row's largest |dh|, its
+// scale and the weights' bound: |q| <= 128, |act(g)| <= |g| and |act'| <= 1.13.
+template <int TYPE, bool ALIGNED, bool LINEAR, int NC>
 __global__ __launch_bounds__(256) void row_terms_kernel(TermArgs p) {
   __shared__ uint32_t red[4];
   typedef typename Elem<TYPE>::T T;
   const int64_t row = blockIdx.x;
   const T *d = (const T *)p.D + row * p.ldd;
+  const int tid = threadIdx.x;
+  float v[NC ? NC : 1][16];
   uint32_t top = 0;
-  for (int j = threadIdx.x; j < p.N; j += 256)
-    top = max(top, magnitude(LINEAR ? (float)d[j] * p.meta[j] : (float)d[j]));
+  auto load = [&](int pos, float (&x)[16]) {
+    load16<TYPE, ALIGNED>(d, pos, p.N, x);
+    if constexpr (LINEAR) {
+      if (pos < p.Np) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const v4f s = *(const v4f *)(p.meta + pos + 4 * i);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[4 * i + e] *= s[e];
+        }
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 16; ++e) top = max(top, magnitude(x[e]));
+  };
+  if constexpr (NC > 0) {
+#pragma unroll
+    for (int i = 0; i < NC; ++i) load((tid + 256 * i) * 16, v[i]);
+  } else {
+    for (int pos = tid * 16; pos < p.N; pos += 4096) load(pos, v[0]);
+  }
   top = block_max<256>(top, red);
   float bound = __uint_as_float(top);
   if (!LINEAR && top < kInfBits) bound *= fabsf(p.t[row]) * p.meta[2 * (int64_t)p.Np] * (128.0f * 1.13f);
   float norm = normaliser(bound);
   // dh times it stays in float32's range, whatever the scales
   if (!LINEAR && top < kInfBits) norm = fminf(norm, normaliser(__uint_as_float(top)) * 0x1p80f);
-  if (threadIdx.x == 0) p.norm[row] = norm;
+  if (tid == 0) p.norm[row] = norm;
   if constexpr (LINEAR) {
     _Float16 *y = p.Y + row * p.Np;
-    for (int j = threadIdx.x; j < p.Np; j += 256) {
-      const float v = j < p.N ? (float)d[j] * p.meta[j] * norm : 0.0f;
-      const _Float16 h = (_Float16)v;
-      y[j] = h;
-      if (p.lo) y[p.lo + j] = (_Float16)(v - (float)h);
+    auto put = [&](int pos, float (&x)[16]) {
+      if (pos >= p.Np) return;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) x[e] *= norm;
+      put_terms(y + pos, p.lo, x);
+    };
+    if constexpr (NC > 0) {
+#pragma unroll
+      for (int i = 0; i < NC; ++i) put((tid + 256 * i) * 16, v[i]);
+    } else {
+      for (int pos = tid * 16; pos < p.Np; pos += 4096) {
+        load(pos, v[0]);
+        put(pos, v[0]);
+      }
     }
   }
 }
@@ -1017,31 +1063,12 @@ __global__ __launch_bounds__(256) void row_terms_kernel(TermArgs p) {
 struct GradArgs {
   const _Float16 *T;     // terms [M][Np]; low halves `lo` elements after them
   const int8_t *Bp;
-  const float *norm;
-  void *X;               // dx [M][ldx]
-  int64_t ldx, lo;
-  int M, K, Kp, Np;
+  int64_t lo;
+  int M, Kp, Np;
   int tiles_m, tiles_n, group_m;
   int planes;            // 2: terms in two halves
+  int splits;            // workgroups along the contraction, each writing its own partial sums
 };
-
-// 8 int8 values as float16, exactly: a byte b = w + 128 below the exponent byte
-// 0x64 is the float16 1024 + b.
-__device__ __forceinline__ v8h bytes_to_half(v2i w) {
-  v8h r;
-  const v2h off = {(_Float16)1152.0f, (_Float16)1152.0f};
-#pragma unroll
-  for (int d = 0; d < 2; ++d) {
-    const uint32_t b = (uint32_t)w[d] ^ 0x80808080u;
-    const v2h lo = __builtin_bit_cast(v2h, __builtin_amdgcn_perm(0x64646464u, b, 0x04010400u)) - off;
-    const v2h hi = __builtin_bit_cast(v2h, __builtin_amdgcn_perm(0x64646464u, b, 0x04030402u)) - off;
-    r[4 * d] = lo[0];
-    r[4 * d + 1] = lo[1];
-    r[4 * d + 2] = hi[0];
-    r[4 * d + 3] = hi[1];
-  }
-  return r;
-}
 
 // v_mfma_f32_16x16x32_f16 accumulating in place in AGPRs (see mfma16_in_place:
 // the same register pressure and the same rules). Its B operand is written by
@@ -1071,7 +1098,8 @@ __device__ __forceinline__ void each(F &&f, std::integer_sequence<int, I...>) {
 //           s + 2. Its MFMAs consume the last fragments of stage s, so after
 //           the barrier at its end stage s may be refilled (by slice s + 3).
 // `planes` 2: the terms' low halves are multiplied by the same weights in a
-// second pass over the slices.
+// second pass over the slices. With `splits`, a workgroup takes its share of the
+// slices and writes float32 partial sums (E = 4).
 template <int E, int BM>
 __global__ __launch_bounds__(256, 1) void grad_dma_kernel(GradArgs p, ScaledTile<kGradOp, E> out) {
   static_assert(BM == 256 || BM == 128, "256x256 or 128x256 tiles");
@@ -1087,8 +1115,9 @@ __global__ __launch_bounds__(256, 1) void grad_dma_kernel(GradArgs p, ScaledTile
   const int total = gridDim.x, w = blockIdx.x;
   const int q = total >> 3, r = total & 7, x = w & 7;
   const int wl = x * q + (x < r ? x : r) + (w >> 3);
-  const int group = p.group_m * p.tiles_n, gid = wl / group, first_m = gid * p.group_m;
-  const int gm = min(p.tiles_m - first_m, p.group_m), within = wl - gid * group;
+  const int tiles = p.tiles_m * p.tiles_n, split = wl / tiles, tile = wl - split * tiles;
+  const int group = p.group_m * p.tiles_n, gid = tile / group, first_m = gid * p.group_m;
+  const int gm = min(p.tiles_m - first_m, p.group_m), within = tile - gid * group;
   const int m0 = (first_m + within % gm) * BM, n0 = (within / gm) * 256;
 
   const int kbt = p.Kp / 64;
@@ -1103,10 +1132,13 @@ __global__ __launch_bounds__(256, 1) void grad_dma_kernel(GradArgs p, ScaledTile
   for (int i = 0; i < DB; ++i)
     b_lane[i] = (uint32_t)((wave * kbt + min(n0 / 64 + i, kbt - 1)) * 1024 + lane * 16);
   const int8_t *const a_tile = (const int8_t *)(p.T + (int64_t)m0 * p.Np);
-  const int8_t *a_next = a_tile, *b_next = p.Bp;
-  const int per_plane = p.Np / 64, slices = per_plane * p.planes;
-  int left = per_plane, d_left = slices;   // slices left of the plane, and to fetch after the next one
+  // This workgroup's slices, of all planes' in turn.
+  const int per_plane = p.Np / 64, all = per_plane * p.planes;
+  const int s_beg = (int)((int64_t)all * split / p.splits), slices = (int)((int64_t)all * (split + 1) / p.splits) - s_beg;
   const int64_t b_step = (int64_t)4 * kbt * 1024;
+  const int plane = s_beg / per_plane, s_in = s_beg - plane * per_plane;
+  const int8_t *a_next = a_tile + (int64_t)s_in * 128 + plane * p.lo * 2, *b_next = p.Bp + s_in * b_step;
+  int left = per_plane - s_in, d_left = slices;   // slices left of the plane, and to fetch after the next one
   // The next slice's bases; past the last one it is fetched again (and not read).
   auto next_slice = [&](const int8_t *&ab, const int8_t *&bb) {
     ab = a_next;
@@ -1150,8 +1182,8 @@ __global__ __launch_bounds__(256, 1) void grad_dma_kernel(GradArgs p, ScaledTile
   auto read_a = [&](int at, int mi) { fa[mi] = ld_lds_b128(smem, at + mi * 2048); };
   auto read_b = [&](int at, int ni) { raw[ni] = ld_lds_tr8(smem, at + (ni >> 2) * 1024 + (ni & 3) * 256); };
   const v2h off = {(_Float16)1152.0f, (_Float16)1152.0f};
-  // Operation o of a half step's 10 NI that turn its raw bytes into float16
-  // (bytes_to_half, one instruction at a time).
+  // Operation o of a half step's 10 NI that turn its raw bytes into float16,
+  // exactly: a byte b = w + 128 below the exponent byte 0x64 is 1024 + b.
   uint32_t biased = 0, pair = 0;
   auto convert = [&](auto op, v4i *gb) __attribute__((always_inline)) {
     constexpr int o = decltype(op)::value, ni = o / 10, d = o / 5 & 1;
@@ -1213,110 +1245,34 @@ __global__ __launch_bounds__(256, 1) void grad_dma_kernel(GradArgs p, ScaledTile
   // results must be there.
   asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier\n\ts_nop 7\n\ts_nop 7" ::: "memory");
   fence_acc();
+  if (p.splits > 1) out.Y = (float *)out.Y + (int64_t)split * p.M * p.Kp;
   out.template grad16<MI, NI>(acc, m0 + wm * 128, n0 + wn * WTN, lane, (LDS_AS int8_t *)smem + wave * 8192);
 }
 
-// 128 x 128 tiles of dx, 4 waves of 64 x 64. The contraction runs over packed
-// columns in steps of 64: the forward pass's packed weights serve as they are,
-// since ds_read_b64_tr_b8 of 8 columns' 16 consecutive k gives a lane 8
-// consecutive columns of one k, the operand of v_mfma_f32_16x16x32_f16.
-template <int TYPE, bool SPLIT>
-__global__ __launch_bounds__(256) void grad_kernel(GradArgs p) {
-  constexpr int BM = 128, BN = 128;
-  constexpr int A_BYTES = BM * 128, B_BYTES = 64 * BN;
-  __shared__ __attribute__((aligned(16))) int8_t smem[2 * A_BYTES * (SPLIT ? 2 : 1) + 2 * B_BYTES];
-  constexpr int A_STAGE = A_BYTES * (SPLIT ? 2 : 1);
-  int8_t *const Bs0 = smem + 2 * A_STAGE;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave >> 1, wn = wave & 1;
-  const int total = gridDim.x, w = blockIdx.x;
-  const int q = total >> 3, r = total & 7, x = w & 7;
-  const int wl = x * q + (x < r ? x : r) + (w >> 3);
-  const int m0 = wl / p.tiles_n * BM, n0 = wl % p.tiles_n * BN;
-  const int kbt = p.Kp / 64;
-  v4i ra[SPLIT ? 8 : 4], rb[2];
-  auto load = [&](int c0) {
+// dx from the partial sums [slices][M][Kp] of a split contraction, over the
+// rows' normalisers: 4 columns of a row per thread.
+struct GradSumArgs {
+  const float *ws;
+  const float *norm;
+  void *X;
+  int64_t ldx;
+  int M, K, Kp, slices, type;
+};
+
+__global__ __launch_bounds__(256) void grad_sum_kernel(GradSumArgs p) {
+  const int64_t row = blockIdx.x;
+  const int col = (blockIdx.y * 256 + threadIdx.x) * 4;
+  if (col >= p.K) return;
+  const float *w = p.ws + row * p.Kp + col;
+  v4f v = *(const v4f *)w;
+  for (int i = 1; i < p.slices; ++i) v += *(const v4f *)(w + (int64_t)i * p.M * p.Kp);
+  v *= 1.0f / p.norm[row];
+  const int64_t at = row * p.ldx + col;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int row = min(m0 + (tid >> 3) + 32 * i, p.M - 1);
-      const _Float16 *src = p.T + (int64_t)row * p.Np + c0 + (tid & 7) * 8;
-      ra[i] = *(const v4i *)src;
-      if constexpr (SPLIT) ra[4 + i] = *(const v4i *)(src + p.lo);
-    }
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int ch = tid + 256 * i, t = ch >> 6;          // tile t: column block t / 2, k block t % 2
-      const int kb = min(n0 / 64 + (t & 1), kbt - 1);
-      rb[i] = *(const v4i *)(p.Bp + ((int64_t)(c0 / 16 + (t >> 1)) * kbt + kb) * 1024 + (ch & 63) * 16);
-    }
-  };
-  auto store = [&](int buf) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int row = (tid >> 3) + 32 * i, off = row * 128 + (((tid & 7) ^ (row & 7)) << 4);
-      st_lds_b128(smem + buf * A_STAGE, off, ra[i]);
-      if constexpr (SPLIT) st_lds_b128(smem + buf * A_STAGE + A_BYTES, off, ra[4 + i]);
-    }
-#pragma unroll
-    for (int i = 0; i < 2; ++i) st_lds_b128(Bs0 + buf * B_BYTES, (tid + 256 * i) * 16, rb[i]);
-  };
-  v4f acc[4][4];
-#pragma unroll
-  for (int mi = 0; mi < 4; ++mi)
-#pragma unroll
-    for (int ni = 0; ni < 4; ++ni) acc[mi][ni] = v4f{0, 0, 0, 0};
-  const int steps = p.Np / 64;
-  if (steps > 0) {
-    load(0);
-    store(0);
-  }
-  __syncthreads();
-  for (int s = 0; s < steps; ++s) {
-    const int buf = s & 1;
-    if (s + 1 < steps) load((s + 1) * 64);
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      v8h fb[4];
-#pragma unroll
-      for (int ni = 0; ni < 4; ++ni) {
-        // lane group g takes columns 8 (g % 2) .. of block 2 h + g / 2; output
-        // block ni of the wave is k block wn, its 16 k's number ni
-        const int g = lane >> 4, j = lane & 15;
-        const int t = (2 * h + (g >> 1)) * 2 + wn;
-        fb[ni] = bytes_to_half(ld_lds_tr8(Bs0 + buf * B_BYTES,
-                                          t * 1024 + (16 * ni + 8 * (g & 1) + (j >> 1)) * 16 + (j & 1) * 8));
-      }
-#pragma unroll
-      for (int mi = 0; mi < 4; ++mi) {
-        const int row = wm * 64 + mi * 16 + (lane & 15);
-        const int off = row * 128 + (((h * 4 + (lane >> 4)) ^ (row & 7)) << 4);
-        const v8h fa = __builtin_bit_cast(v8h, ld_lds_b128(smem + buf * A_STAGE, off));
-#pragma unroll
-        for (int ni = 0; ni < 4; ++ni)
-          acc[mi][ni] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fa, fb[ni], acc[mi][ni], 0, 0, 0);
-        if constexpr (SPLIT) {
-          const v8h fl = __builtin_bit_cast(v8h, ld_lds_b128(smem + buf * A_STAGE + A_BYTES, off));
-#pragma unroll
-          for (int ni = 0; ni < 4; ++ni)
-            acc[mi][ni] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fl, fb[ni], acc[mi][ni], 0, 0, 0);
-        }
-      }
-    }
-    if (s + 1 < steps) store(buf ^ 1);
-    __syncthreads();
-  }
-  typedef typename Elem<TYPE>::T T;
-#pragma unroll
-  for (int mi = 0; mi < 4; ++mi)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int row = m0 + wm * 64 + mi * 16 + 4 * (lane >> 4) + e;
-      if (row >= p.M) continue;
-      const float un = 1.0f / p.norm[row];   // a power of two: exact
-#pragma unroll
-      for (int ni = 0; ni < 4; ++ni) {
-        const int col = n0 + wn * 64 + ni * 16 + (lane & 15);
-        if (col < p.K) ((T *)p.X)[(int64_t)row * p.ldx + col] = (T)(acc[mi][ni][e] * un);
-      }
+  for (int e = 0; e < 4; ++e)
+    if (col + e < p.K) {
+      if (p.type == VT_TYPE_F32) ((float *)p.X)[at + e] = v[e];
+      else ((uint16_t *)p.X)[at + e] = (uint16_t)pack16(v[e], 0.0f, p.type);
     }
 }
 
@@ -1329,6 +1285,8 @@ bool float_type(int type) { return type == VT_TYPE_F32 || type == VT_TYPE_F16 ||
 constexpr int64_t kScaledMax = (int64_t)1 << 30;
 // The longest sums: 131071 products of -128 and -128 stay below 2^31.
 constexpr int64_t kScaledMaxK = 131071;
+// Packed columns: a tile's 256 rows of float16 terms stay within 32-bit offsets.
+constexpr int64_t kScaledMaxN = 65535 * 64;
 // Pitch of int8 rows from which on they are copied before the products.
 constexpr int64_t kFarRows = (int64_t)1 << 23;
 
@@ -1593,46 +1551,102 @@ int launch_scaled(const Rows &rows, const int8_t *Bp, int64_t Kp, const ScaledOu
   return launch_product(rows, Bp, Kp, t, scr);
 }
 
+template <int TYPE, bool ALIGNED, bool LINEAR>
+void launch_row_terms_typed(const TermArgs &a, hipStream_t s) {
+  const dim3 grid((unsigned)a.M);
+  if constexpr (LINEAR) {
+    if (a.Np <= 4096) hipLaunchKernelGGL((row_terms_kernel<TYPE, ALIGNED, true, 1>), grid, dim3(256), 0, s, a);
+    else if (a.Np <= 8192) hipLaunchKernelGGL((row_terms_kernel<TYPE, ALIGNED, true, 2>), grid, dim3(256), 0, s, a);
+    else if (a.Np <= 16384) hipLaunchKernelGGL((row_terms_kernel<TYPE, ALIGNED, true, 4>), grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((row_terms_kernel<TYPE, ALIGNED, true, 0>), grid, dim3(256), 0, s, a);
+  } else {
+    hipLaunchKernelGGL((row_terms_kernel<TYPE, ALIGNED, false, 0>), grid, dim3(256), 0, s, a);
+  }
+}
+
 template <bool LINEAR>
 int launch_row_terms(const TermArgs &a, int type, hipStream_t s) {
-  const dim3 grid((unsigned)a.M);
+  const bool al = aligned16(a.D) && a.ldd * elem_size(type) % 16 == 0;
   switch (type) {
-    case VT_TYPE_F32: hipLaunchKernelGGL((row_terms_kernel<kF32, LINEAR>), grid, dim3(256), 0, s, a); break;
-    case VT_TYPE_F16: hipLaunchKernelGGL((row_terms_kernel<kF16, LINEAR>), grid, dim3(256), 0, s, a); break;
-    default: hipLaunchKernelGGL((row_terms_kernel<kBF16, LINEAR>), grid, dim3(256), 0, s, a); break;
+    case VT_TYPE_F32: al ? launch_row_terms_typed<kF32, true, LINEAR>(a, s) : launch_row_terms_typed<kF32, false, LINEAR>(a, s); break;
+    case VT_TYPE_F16: al ? launch_row_terms_typed<kF16, true, LINEAR>(a, s) : launch_row_terms_typed<kF16, false, LINEAR>(a, s); break;
+    default: al ? launch_row_terms_typed<kBF16, true, LINEAR>(a, s) : launch_row_terms_typed<kBF16, false, LINEAR>(a, s); break;
   }
   VT_HIP_CHECK(hipGetLastError());
   return VT_OK;
 }
 
+// Tiles and splits of a gradient product by the least estimated time: a slice
+// takes a workgroup 0.87 us on 128 x 256 tiles and 1.64 us on 256 x 256 ones
+// (2048 x 4096 x 28672 and 4096^3, one tile per CU), partial sums are written
+// and read at 4 TB/s and take a second launch.
+struct GradGeom {
+  int bm, splits;
+};
+
+GradGeom grad_geom(int64_t M, int64_t Kp, int64_t slices, int cus) {
+  GradGeom best = {128, 1};
+  double least = 0;
+  for (int bm = 256; bm >= 128; bm /= 2)
+    for (int splits = 1; splits <= 32 && splits <= slices; splits *= 2) {
+      const int64_t tiles = (M + bm - 1) / bm * ((Kp + 255) / 256);
+      double ns = (double)((tiles * splits + cus - 1) / cus) * (double)((slices + splits - 1) / splits) * (bm == 256 ? 1640 : 870);
+      if (splits > 1) ns += 3000 + 8.0 * splits * M * Kp / 4000;
+      if (least == 0 || ns < least) {
+        least = ns;
+        best = {bm, splits};
+      }
+    }
+  return best;
+}
+
 template <int E>
-int launch_grad_typed(GradArgs a, const ScaledOut &o, hipStream_t s, int cus) {
+int launch_grad_tiles(const GradArgs &a, int bm, const ScaledOut &o, hipStream_t s) {
   ScaledTile<kGradOp, E> out;
   (ScaledOut &)out = o;
-  const int64_t cols = (a.Kp + 255) / 256;
-  const int64_t t256 = (a.M + 255) / 256 * cols, t128 = (a.M + 127) / 128 * cols;
+  const int64_t wgs = (int64_t)a.tiles_m * a.tiles_n * a.splits;
+  if (wgs > 0x7fffffff) return fail(VT_EUNSUPPORTED, "gradient grid too large");
+  if (bm == 256) hipLaunchKernelGGL((grad_dma_kernel<E, 256>), dim3((unsigned)wgs), dim3(256), 0, s, a, out);
+  else hipLaunchKernelGGL((grad_dma_kernel<E, 128>), dim3((unsigned)wgs), dim3(256), 0, s, a, out);
+  VT_HIP_CHECK(hipGetLastError());
+  return VT_OK;
+}
+
+// An empty contraction: zeros (a kernel, which a captured graph may hold).
+__global__ __launch_bounds__(256) void zero_rows_kernel(ScaledOut o) {
+  const int64_t at = blockIdx.x * o.ldy;
+  for (int j = threadIdx.x; j < o.N; j += 256) {
+    if (o.type == VT_TYPE_F32) ((float *)o.Y)[at + j] = 0.0f;
+    else ((uint16_t *)o.Y)[at + j] = 0;
+  }
+}
+
+int launch_zero(const ScaledOut &o, hipStream_t s) {
+  hipLaunchKernelGGL(zero_rows_kernel, dim3((unsigned)o.M), dim3(256), 0, s, o);
+  VT_HIP_CHECK(hipGetLastError());
+  return VT_OK;
+}
+
+// dx = terms . W^T. o: the gradient, its rows' normalisers and type.
+int launch_grad(GradArgs a, const ScaledOut &o, Scratch &scr) {
+  hipStream_t s = (hipStream_t)scr.stream;
+  const GradGeom g = grad_geom(a.M, a.Kp, (int64_t)a.Np / 64 * a.planes, scr.st->num_cus);
   a.group_m = 4;
-  if (a.Np > 0 && t128 >= 128 && 256ll * a.Np * 2 < (1ll << 31) && 4ll * a.Kp * 16 < (1ll << 31)) {
-    const int64_t r256 = (t256 + cus - 1) / cus * 2, r128 = (t128 + cus - 1) / cus;
-    const bool big = r256 <= r128;
-    a.tiles_m = (a.M + (big ? 255 : 127)) / (big ? 256 : 128);
-    a.tiles_n = (int)cols;
-    if (t128 > 0x7fffffff) return fail(VT_EUNSUPPORTED, "gradient grid too large");
-    if (big) hipLaunchKernelGGL((grad_dma_kernel<E, 256>), dim3((unsigned)t256), dim3(256), 0, s, a, out);
-    else hipLaunchKernelGGL((grad_dma_kernel<E, 128>), dim3((unsigned)t128), dim3(256), 0, s, a, out);
-    VT_HIP_CHECK(hipGetLastError());
-    return VT_OK;
-  }
-  a.tiles_m = (a.M + 127) / 128;
-  a.tiles_n = (a.Kp + 127) / 128;
-  const int64_t tiles = (int64_t)a.tiles_m * a.tiles_n;
-  if (tiles > 0x7fffffff) return fail(VT_EUNSUPPORTED, "gradient grid too large");
-  const dim3 grid((unsigned)tiles);
-  switch (o.type) {
-    case VT_TYPE_F32: hipLaunchKernelGGL((grad_kernel<kF32, true>), grid, dim3(256), 0, s, a); break;
-    case VT_TYPE_F16: hipLaunchKernelGGL((grad_kernel<kF16, false>), grid, dim3(256), 0, s, a); break;
-    default: hipLaunchKernelGGL((grad_kernel<kBF16, false>), grid, dim3(256), 0, s, a); break;
-  }
+  a.tiles_m = (a.M + g.bm - 1) / g.bm;
+  a.tiles_n = (a.Kp + 255) / 256;
+  a.splits = g.splits;
+  if (g.splits == 1)
+    return o.type == VT_TYPE_F32 ? launch_grad_tiles<4>(a, g.bm, o, s) : launch_grad_tiles<2>(a, g.bm, o, s);
+  void *w = nullptr;
+  if (int rc = scr.take(kPartials, (size_t)g.splits * a.M * a.Kp * sizeof(float), &w)) return rc;
+  ScaledOut part = o;
+  part.Y = w;
+  part.ldy = part.N = a.Kp;
+  part.norm = nullptr;
+  part.type = VT_TYPE_F32;
+  if (int rc = launch_grad_tiles<4>(a, g.bm, part, s)) return rc;
+  const GradSumArgs r = {(const float *)w, o.norm, o.Y, o.ldy, a.M, o.N, a.Kp, g.splits, o.type};
+  hipLaunchKernelGGL(grad_sum_kernel, dim3((unsigned)a.M, (unsigned)((o.N + 1023) / 1024)), dim3(256), 0, s, r);
   VT_HIP_CHECK(hipGetLastError());
   return VT_OK;
 }
@@ -1658,7 +1672,9 @@ int check_scaled(const ScaledCall &c, bool *empty) {
   *empty = false;
   if (c.M < 0 || c.K < 0 || c.N < 0)
     return fail(VT_EINVAL, "%s: negative size (M=%lld K=%lld N=%lld)", c.who, (long long)c.M, (long long)c.K, (long long)c.N);
-  if (c.M >= kScaledMax || c.N >= kScaledMax / 2) return fail(VT_EINVAL, "%s: size beyond 2^30", c.who);
+  if (c.M >= kScaledMax) return fail(VT_EINVAL, "%s: size beyond 2^30", c.who);
+  if (c.N > kScaledMaxN / (c.pair ? 2 : 1))
+    return fail(VT_EINVAL, "%s: packed columns beyond %lld (N=%lld)", c.who, (long long)kScaledMaxN, (long long)c.N);
   if (c.K > kScaledMaxK)
     return fail(VT_EINVAL, "%s: int32 sums hold K <= %lld (K=%lld)", c.who, (long long)kScaledMaxK, (long long)c.K);
   const bool i8 = c.x_type == VT_TYPE_I8 || c.x_type == VT_TYPE_I8_PADDED;
@@ -1751,6 +1767,11 @@ int backward(const ScaledCall &c, const int8_t *Q, int q_type, int64_t ldq, cons
   Scratch scr;
   if (int rc = open_scratch(stream, &scr)) return rc;
   hipStream_t s = (hipStream_t)stream;
+  ScaledOut o = {};
+  o.Y = c.Y; o.ldy = c.ldy;
+  o.M = (int)c.M; o.N = (int)c.K;
+  o.type = c.y_type;
+  if (Np == 0) return launch_zero(o, s);
   // Terms in float16, normalised by row; of float32 gradients also what
   // float16 leaves of each (two products).
   const bool split = c.x_type == VT_TYPE_F32;
@@ -1761,25 +1782,22 @@ int backward(const ScaledCall &c, const int8_t *Q, int q_type, int64_t ldq, cons
   _Float16 *terms = (_Float16 *)w;
   float *norm = (float *)((int8_t *)w + t_bytes);
   const TermArgs ta = {c.X, t, c.meta, norm, terms, c.ldx, lo, (int)c.M, (int)c.N, (int)Np};
-  if (!c.pair || c.N == 0) {
+  if (!c.pair) {
     if (int rc = launch_row_terms<true>(ta, c.x_type, s)) return rc;
   } else {
     if (int rc = launch_row_terms<false>(ta, c.x_type, s)) return rc;
     Rows rows;
     if (int rc = take_rows(Q, q_type, ldq, t, c.M, c.K, scr, &rows)) return rc;
-    ScaledOut o = {};
-    o.t = rows.t; o.meta = c.meta; o.D = c.X; o.norm = norm; o.Y = terms;
-    o.ldd = c.ldx; o.lo = lo;
-    o.M = (int)c.M; o.N = (int)c.N; o.Np = (int)Np;
-    o.act = act; o.type = c.x_type;
-    if (int rc = launch_scaled<kTermsOp>(rows, c.Bp, Kp, o, scr)) return rc;
+    ScaledOut f = {};
+    f.t = rows.t; f.meta = c.meta; f.D = c.X; f.norm = norm; f.Y = terms;
+    f.ldd = c.ldx; f.lo = lo;
+    f.M = (int)c.M; f.N = (int)c.N; f.Np = (int)Np;
+    f.act = act; f.type = c.x_type;
+    if (int rc = launch_scaled<kTermsOp>(rows, c.Bp, Kp, f, scr)) return rc;
   }
-  const GradArgs g = {terms, c.Bp, norm, c.Y, c.ldy, lo, (int)c.M, (int)c.K, (int)Kp, (int)Np, 0, 0, 0, split ? 2 : 1};
-  ScaledOut o = {};
-  o.norm = norm; o.Y = c.Y; o.ldy = c.ldy;
-  o.M = (int)c.M; o.N = (int)c.K;
-  o.type = c.y_type;
-  return split ? launch_grad_typed<4>(g, o, s, scr.st->num_cus) : launch_grad_typed<2>(g, o, s, scr.st->num_cus);
+  o.norm = norm;
+  const GradArgs g = {terms, c.Bp, lo, (int)c.M, (int)Kp, (int)Np, 0, 0, 0, split ? 2 : 1, 1};
+  return launch_grad(g, o, scr);
 }
 
 }  // namespace
@@ -1818,9 +1836,9 @@ int vt_quant_rows(const void *X, int32_t x_type, int64_t ldx, int8_t *Q, int64_t
 }
 
 int64_t vt_scaled_size(int64_t K, int64_t N, int32_t pair, int64_t *meta_floats) {
-  if (K < 0 || N < 0 || K > kScaledMaxK || N >= kScaledMax / 2)
-    return fail(VT_EINVAL, "vt_scaled_size: needs 0 <= K <= %lld, 0 <= N < 2^29 (K=%lld N=%lld)", (long long)kScaledMaxK,
-                (long long)K, (long long)N);
+  if (K < 0 || N < 0 || K > kScaledMaxK || N > kScaledMaxN / (pair ? 2 : 1))
+    return fail(VT_EINVAL, "vt_scaled_size: needs 0 <= K <= %lld and 0 <= N <= %lld (K=%lld N=%lld)", (long long)kScaledMaxK,
+                (long long)(kScaledMaxN / (pair ? 2 : 1)), (long long)K, (long long)N);
   const int64_t Np = scaled_np(N, pair != 0);
   if (meta_floats) *meta_floats = scaled_meta(Np);
   return scaled_kp(K) * Np;
@@ -1840,7 +1858,6 @@ int vt_scaled_pack(const int8_t *W0, const int8_t *W1, int64_t ldw0, int64_t ldw
   if (ldw0 > ((int64_t)1 << 40) || ldw1 > ((int64_t)1 << 40)) return fail(VT_EINVAL, "vt_scaled_pack: pitch beyond 2^40");
   if (!aligned16(Bp) || !aligned16(meta)) return fail(VT_EINVAL, "vt_scaled_pack: outputs need 16-byte aligned bases");
   const int64_t Kp = scaled_kp(K), Np = scaled_np(N, pair);
-  if (Np / 64 > 65535) return fail(VT_EUNSUPPORTED, "vt_scaled_pack: N=%lld too large", (long long)N);
   Extent e0, e1, eb;
   if (!operand_extent(W0, 1, 0, K, ldw0, N, 1, &e0) || !operand_extent(Bp, 1, 0, 1, 0, size, 1, &eb) ||
       (pair && !operand_extent(W1, 1, 0, K, ldw1, N, 1, &e1)))
