@@ -23,6 +23,7 @@ typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef __bf16 v4b __attribute__((ext_vector_type(4)));
 typedef __bf16 v8b __attribute__((ext_vector_type(8)));
 typedef float v4f __attribute__((ext_vector_type(4)));
+typedef float v4f_any __attribute__((ext_vector_type(4), aligned(4)));
 
 // K and N of the packed weights. K in whole pairs of 64-deep slices, from 1024
 // on in the 256-deep groups that the persistent kernels take (at most a fifth
@@ -202,10 +203,9 @@ __global__ __launch_bounds__(THREADS) void quant_rows_kernel(QuantArgs p) {
   }
 }
 
-// int8 rows of any pitch and alignment -> rows of Kp bytes, zeros past K.
-__global__ __launch_bounds__(256) void pad_rows_kernel(QuantArgs p) {
-  const int64_t row = blockIdx.y, pos = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 16;
-  if (pos >= p.Kp) return;
+// 16 bytes of an int8 row of any pitch and alignment to a row of Kp bytes,
+// zeros past K.
+__device__ __forceinline__ void pad_piece(const QuantArgs &p, int64_t row, int64_t pos) {
   const int8_t *x = (const int8_t *)p.X + row * p.ldx;
   v4i o = v4i{0, 0, 0, 0};
   if (pos + 16 <= p.K) {
@@ -220,6 +220,11 @@ __global__ __launch_bounds__(256) void pad_rows_kernel(QuantArgs p) {
     }
   }
   *(v4i *)(p.Q + row * p.ldq + pos) = o;
+}
+
+__global__ __launch_bounds__(256) void pad_rows_kernel(QuantArgs p) {
+  const int64_t pos = ((int64_t)blockIdx.y * 256 + threadIdx.x) * 16;
+  if (pos < p.Kp) pad_piece(p, blockIdx.x, pos);
 }
 
 // ---------------------------------------------------------------------------
@@ -340,19 +345,25 @@ __device__ __forceinline__ float normaliser(float bound) {
   return __uint_as_float((uint32_t)(max(-126, min(126, 14 - e)) + 127) << 23);
 }
 
-// What becomes of the int32 sums. OP: the operator; E: bytes of the floating
-// type (2: float16 or bfloat16, by `type`; 4: float32).
-enum ScaledOp { kLinear = 0, kGated = 1, kTermsOp = 2, kGradOp = 3 };
+// f(0), f(1), .. f(N - 1) with compile-time arguments.
+template <class F, int... I>
+__device__ __forceinline__ void each(F &&f, std::integer_sequence<int, I...>) {
+  (f(std::integral_constant<int, I>()), ...);
+}
+
+// What becomes of a product's sums: a linear layer's or gated product's output,
+// the 16-bit gradient terms of a gated product, or the gradient itself.
+enum ScaledOp { kLinear = 0, kGated = 1, kGradTerms = 2, kGrad = 3 };
 
 struct ScaledOut {
   const float *t;      // row scales
   const float *meta;   // channel scales [Np], bias [Np]
-  const void *D;       // kTermsOp: dh [M][ldd]
-  const float *norm;   // kTermsOp, kGradOp: row normalisers
-  void *Y;             // output [M][ldy]; kTermsOp: float16 terms [M][Np]
+  const void *D;       // kGradTerms: dh [M][ldd] of `type`
+  const float *norm;   // kGradTerms, kGrad: row normalisers
+  void *Y;             // output [M][ldy] of `type`; kGradTerms: float16 terms [M][Np]
   int64_t ldy, ldd;
-  int64_t lo;          // kTermsOp: elements from the high to the low halves, 0 for none
-  int M, N, Np;        // N: output columns (dh's for kTermsOp)
+  int64_t lo;          // kGradTerms: elements from the high to the low halves, 0 for none
+  int M, N, Np;        // N: columns of the output (kGradTerms: of dh)
   int act, type;
 };
 
@@ -363,65 +374,257 @@ __device__ __forceinline__ uint32_t pack16(float a, float b, int type) {
   return __builtin_bit_cast(uint32_t, v2h{(_Float16)a, (_Float16)b});
 }
 
-typedef float v4f_any __attribute__((ext_vector_type(4), aligned(4)));
+__device__ __forceinline__ float from16(uint32_t bits, int type) {
+  return type == VT_TYPE_BF16 ? __uint_as_float(bits << 16) : (float)__builtin_bit_cast(_Float16, (uint16_t)bits);
+}
 
-template <int OP, int E>
+// E: bytes of the floating type in tile16 (2 or 4); everything else goes by `type`.
+template <int OP, int E = 2>
 struct ScaledTile : ScaledOut {
   static constexpr bool kScaled = true;
-  // The type that is written: terms are float16 whatever dh's.
-  static constexpr int OE = OP == kTermsOp ? 2 : E;
+  static constexpr int OE = OP == kGradTerms ? 2 : E;   // bytes of what tile16 writes
+  static constexpr int P = OP == kGated || OP == kGradTerms ? 2 : 1;   // projections taken together
 
-  __device__ __forceinline__ float act_value(float g, float &slope) const {
-    return act == VT_ACT_SILU ? act_of<VT_ACT_SILU>(g, slope) : act_of<VT_ACT_GELU>(g, slope);
-  }
-  __device__ __forceinline__ uint32_t pack(float a, float b) const {
-    return pack16(a, b, OP == kTermsOp ? VT_TYPE_F16 : type);
-  }
-  __device__ __forceinline__ void store1(int64_t i, float v) const {
-    if (OE == 4) ((float *)Y)[i] = v;
-    else ((uint16_t *)Y)[i] = (uint16_t)pack(v, 0.0f);
-  }
-  // g and u of a pair of sums -> h, or (kTermsOp) both terms.
-  __device__ __forceinline__ void pair(int32_t ag, int32_t au, float t_row, float sg, float su, float d,
-                                       float &first, float &second) const {
+  // g and u of a pair of sums -> h, or (kGradTerms) the terms of Wg and Wu.
+  __device__ __forceinline__ void pair(int32_t ag, int32_t au, float t_row, float sg, float su, float d, float &first,
+                                       float &second) const {
     const float g = (float)ag * t_row * sg, u = (float)au * t_row * su;
     float slope;
-    const float a = act_value(g, slope);
-    if (OP == kGated) {
+    const float a = act == VT_ACT_SILU ? act_of<VT_ACT_SILU>(g, slope) : act_of<VT_ACT_GELU>(g, slope);
+    if constexpr (OP == kGated) {
       first = a * u;
     } else {
+      // Rounded to 32 bits here: a product fused into the conversion to float16
+      // rounds once, and the low half that is left of it would be another's.
       first = d * u * slope * sg;
       second = d * a * su;
+      asm("" : "+v"(first), "+v"(second));
     }
   }
 
-  // Rows [r0, r0 + ROWS) of `W` output columns from out0 leave the wave's LDS, in
-  // 16-byte pieces of whole rows (vector j of a lane: row (64 j + lane) / RC,
-  // chunk lane % RC). 16-byte chunk k of a row is at k ^ swz(row). Only rows in
-  // [row_min, row_max) and columns in [out_min, the last) are stored.
-  template <int ROWS, int W, class SWZ>
-  __device__ __forceinline__ void store_rows(LDS_AS int8_t *lds, SWZ swz, int r0, int out0, int64_t plane, int lane,
-                                             int row_min, int row_max, int out_min) const {
-    constexpr int PITCH = W * OE, RC = PITCH / 16, PER = 16 / OE;
-    const int out_n = OP == kTermsOp ? Np : N;
-    const int64_t ld = OP == kTermsOp ? Np : ldy;
-#pragma unroll
-    for (int j = 0; j < (ROWS * RC + 63) / 64; ++j) {
-      const int idx = 64 * j + lane, row = idx / RC, k = idx % RC;
-      if (ROWS * RC % 64 && row >= ROWS) break;
-      const v4i w = *(LDS_AS v4i *)(lds + row * PITCH + ((k ^ swz(row)) << 4));
-      const int col = out0 + k * PER;
-      if (r0 + row < row_min || r0 + row >= row_max || col < out_min) continue;
-      int8_t *y = (int8_t *)Y + ((int64_t)(r0 + row) * ld + plane + col) * OE;
-      if (col + PER <= out_n) {
-        __builtin_nontemporal_store(w, (v4i_any *)y);
+  __device__ __forceinline__ int to16() const { return OP == kGradTerms ? VT_TYPE_F16 : type; }
+
+  // `count` (at most 8) elements to y[at ..].
+  __device__ __forceinline__ void store8(int64_t at, const float (&v)[8], int count, int to) const {
+    if (to == VT_TYPE_F32) {
+      float *y = (float *)Y + at;
+      if (count >= 8) {
+        __builtin_nontemporal_store(v4f{v[0], v[1], v[2], v[3]}, (v4f_any *)y);
+        __builtin_nontemporal_store(v4f{v[4], v[5], v[6], v[7]}, (v4f_any *)(y + 4));
       } else {
 #pragma unroll
-        for (int e = 0; e < PER; ++e)
-          if (col + e < out_n) {
-            if constexpr (OE == 4) ((int32_t *)y)[e] = w[e];
-            else ((uint16_t *)y)[e] = (uint16_t)((uint32_t)w[e >> 1] >> (16 * (e & 1)));
+        for (int e = 0; e < 7; ++e)
+          if (e < count) y[e] = v[e];
+      }
+    } else {
+      uint16_t *y = (uint16_t *)Y + at;
+      uint32_t w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = pack16(v[2 * i], v[2 * i + 1], to);
+      if (count >= 8) {
+        __builtin_nontemporal_store(v4i{(int)w[0], (int)w[1], (int)w[2], (int)w[3]}, (v4i_any *)y);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 7; ++e)
+          if (e < count) y[e] = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
+      }
+    }
+  }
+
+  // 8 elements of dh from column j, zero past the last.
+  struct D8 {
+    uint32_t w[8];
+  };
+  __device__ __forceinline__ D8 load_d8(int64_t row, int j) const {
+    D8 d;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) d.w[e] = 0;
+    if (type == VT_TYPE_F32) {
+      const float *x = (const float *)D + row * ldd + j;
+      if (j + 8 <= N) {
+        const v4f a = *(const v4f_any *)x, b = *(const v4f_any *)(x + 4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          d.w[e] = __float_as_uint(a[e]);
+          d.w[4 + e] = __float_as_uint(b[e]);
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 7; ++e)
+          if (j + e < N) d.w[e] = __float_as_uint(x[e]);
+      }
+    } else {
+      const uint16_t *x = (const uint16_t *)D + row * ldd + j;
+      if (j + 8 <= N) {
+        const v4i a = ld_any((const int8_t *)x);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) d.w[e] = (uint32_t)a[e];
+      } else {
+#pragma unroll
+        for (int e = 0; e < 7; ++e)
+          if (j + e < N) d.w[e >> 1] |= (uint32_t)x[e] << (16 * (e & 1));
+      }
+    }
+    return d;
+  }
+  __device__ __forceinline__ float d_value(const D8 &d, int e) const {
+    return type == VT_TYPE_F32 ? __uint_as_float(d.w[e]) : from16(d.w[e >> 1] >> (16 * (e & 1)) & 0xffffu, type);
+  }
+
+  // A wave's sums, MI strips of ROWS rows by WP packed columns from (row0,
+  // col0): write(mi) puts a strip as it lies in the accumulators into the wave's
+  // LDS (rows of 4 WP bytes, 16-byte chunk k of a row at k ^ swz(row)), and the
+  // lanes take it from there row by row, 8 output columns each, so scales, dh
+  // and outputs are whole 16-byte pieces. The strips are a loop (`write` alone
+  // is unrolled): this code runs once per tile, and a short call waits for it
+  // to be fetched (unrolled, the gradient's kernel of 18 KB took 11 us for one
+  // slice). Every strip's dh is loaded one strip ahead, before the stores that
+  // it would otherwise wait for (both count in vmcnt, in order). Rows outside
+  // [row_min, row_max) and packed columns below col_min are not stored.
+  template <int MI, int ROWS, int WP, class WRITE, class SWZ>
+  __device__ __forceinline__ void strips(WRITE write, SWZ swz, int row0, int col0, int row_min, int row_max, int col_min,
+                                         int lane, const LDS_AS int8_t *lds) const {
+    constexpr int LPR = WP / P / 8, RPI = 64 / LPR, IT = ROWS / RPI;   // lanes per row, rows at a time, times
+    static_assert(IT >= 1 && MI * ROWS <= 128, "whole iterations; two registers hold the rows' scales");
+    const int j8 = 8 * (lane % LPR), lr = lane / LPR;
+    const int lp = P == 1 ? j8 : (j8 >> 5) * 64 + (j8 & 31);   // the lane's first packed column, less col0
+    const int pc = col0 + lp, j = (P == 1 ? col0 : col0 / 2) + j8;
+    const int count = OP == kGradTerms ? 8 : N - j;
+    const bool cols = pc >= col_min && pc < Np && count > 0;
+    float s0[8], s1[P == 2 ? 8 : 1], bias[OP == kLinear ? 8 : 1];
+    if constexpr (OP != kGrad) {
+      const float *m = meta + min(pc, Np - 8 - (P == 2 ? 32 : 0));
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        s0[e] = m[e];
+        if constexpr (P == 2) s1[e] = m[32 + e];
+        if constexpr (OP == kLinear) bias[e] = m[Np + e];
+      }
+    }
+    float tr[2], nr[2];
+#pragma unroll
+    for (int h = 0; h < (MI * ROWS > 64 ? 2 : 1); ++h) {
+      const int row = min(row0 + 64 * h + lane, M - 1);
+      if constexpr (OP != kGrad) tr[h] = t[row];
+      if constexpr (OP == kGradTerms) nr[h] = norm[row];
+      if constexpr (OP == kGrad) nr[h] = norm ? 1.0f / norm[row] : 1.0f;
+    }
+    D8 d[OP == kGradTerms ? IT : 1], ahead[OP == kGradTerms ? IT : 1];
+    auto load_d = [&](int mi) {
+      if constexpr (OP == kGradTerms) {
+#pragma unroll
+        for (int it = 0; it < IT; ++it)
+          ahead[it] = load_d8(min(row0 + mi * ROWS + it * RPI + lr, M - 1), min(j, N));
+      }
+    };
+    load_d(0);
+#pragma unroll 1
+    for (int mi = 0; mi < MI; ++mi) {
+      if constexpr (OP == kGradTerms) {
+#pragma unroll
+        for (int it = 0; it < IT; ++it) d[it] = ahead[it];
+        load_d(min(mi + 1, MI - 1));
+      }
+      each([&](auto i) __attribute__((always_inline)) {
+        if (mi == decltype(i)::value) write(i);
+      }, std::make_integer_sequence<int, MI>());
+      const bool second = MI * ROWS > 64 && mi * ROWS >= 64;
+#pragma unroll (IT > 4 ? 2 : IT)
+      for (int it = 0; it < IT; ++it) {
+        const int r = it * RPI + lr, rel = mi * ROWS + r, row = row0 + rel;
+        const LDS_AS int8_t *at = lds + r * (4 * WP);
+        auto chunk = [&](int k) { return *(const LDS_AS v4i *)(at + ((k ^ swz(r)) << 4)); };
+        const v4i a0 = chunk(lp / 4), a1 = chunk(lp / 4 + 1);
+        v4i u0, u1;
+        if constexpr (P == 2) {
+          u0 = chunk(lp / 4 + 8);
+          u1 = chunk(lp / 4 + 9);
+        }
+        float t_row, n_row;
+        if constexpr (OP != kGrad) t_row = __shfl(second ? tr[1] : tr[0], rel & 63);
+        if constexpr (OP == kGradTerms || OP == kGrad) n_row = __shfl(second ? nr[1] : nr[0], rel & 63);
+        float v[8], v2[P == 2 ? 8 : 1];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int a = e < 4 ? a0[e & 3] : a1[e & 3];
+          if constexpr (OP == kLinear) {
+            v[e] = (float)a * t_row * s0[e] + bias[e];
+          } else if constexpr (OP == kGrad) {
+            v[e] = __builtin_bit_cast(float, a) * n_row;
+          } else {
+            const int u = e < 4 ? u0[e & 3] : u1[e & 3];
+            pair(a, u, t_row, s0[e], s1[e], OP == kGradTerms ? d_value(d[it], e) * n_row : 0.0f, v[e], v2[e]);
           }
+        }
+        if (!cols || row < row_min || row >= row_max) continue;
+        if constexpr (OP == kGradTerms) {
+          const int64_t to = (int64_t)row * Np + pc;
+          store8(to, v, 8, VT_TYPE_F16);
+          store8(to + 32, v2, 8, VT_TYPE_F16);
+          if (lo) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              v[e] -= (float)(_Float16)v[e];
+              v2[e] -= (float)(_Float16)v2[e];
+            }
+            store8(to + lo, v, 8, VT_TYPE_F16);
+            store8(to + lo + 32, v2, 8, VT_TYPE_F16);
+          }
+        } else {
+          store8((int64_t)row * ldy + j, v, count, type);
+        }
+      }
+    }
+  }
+
+  // Blocks of 16 x 16 sums (element e of lane l: row 4 (l / 16) + e, column
+  // l % 16) of 16 MI rows and 16 NI packed columns, G block rows to a strip; the
+  // strips' swizzle is store_strip16_lds' (distinct banks for an instruction's
+  // writes).
+  template <int G, int MI, int NI, class ACC>
+  __device__ __forceinline__ void blocks16(const ACC (&acc)[MI][NI], int row0, int col0, int row_min, int col_min, int lane,
+                                           LDS_AS int8_t *lds) const {
+    const int g = lane >> 4, c = lane & 15;
+    strips<MI / G, 16 * G, NI * 16>(
+        [&](auto strip) __attribute__((always_inline)) {
+#pragma unroll
+          for (int i = 0; i < G; ++i)
+#pragma unroll
+            for (int ni = 0; ni < NI; ++ni)
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                *(LDS_AS decltype(acc[0][0][0] + 0) *)(lds + (16 * i + 4 * g + e) * (64 * NI) +
+                                                       ((((ni ^ g) << 2) + (c >> 2)) << 4) + (c & 3) * 4) =
+                    acc[strip * G + i][ni][e];
+        },
+        [](int row) { return ((row >> 2) & 3) << 2; }, row0, col0, row_min, M, col_min, lane, lds);
+  }
+
+  // Rows [r0, r0 + 16) of `W` output columns from out0 leave the wave's LDS, in
+  // 16-byte pieces of whole rows (vector j of a lane: row (64 j + lane) / RC,
+  // chunk lane % RC). 16-byte chunk k of a row is at k ^ swz(row). Rows below
+  // row_min and columns below out_min are the neighbouring tile's.
+  template <int W, class SWZ>
+  __device__ __forceinline__ void store_rows(LDS_AS int8_t *lds, SWZ swz, int r0, int out0, int64_t plane, int lane,
+                                             int row_min, int out_min) const {
+    constexpr int PITCH = W * OE, RC = PITCH / 16, PER = 16 / OE;
+    const int out_n = OP == kGradTerms ? Np : N;
+    const int64_t ld = OP == kGradTerms ? Np : ldy;
+#pragma unroll 4
+    for (int j = 0; j < (16 * RC + 63) / 64; ++j) {
+      const int idx = 64 * j + lane, row = idx / RC, k = idx % RC;
+      LDS_AS int8_t *from = lds + row * PITCH + ((k ^ swz(row)) << 4);
+      const int col = out0 + k * PER;
+      if (r0 + row < row_min || col < out_min) continue;
+      int8_t *y = (int8_t *)Y + ((int64_t)(r0 + row) * ld + plane + col) * OE;
+      if (col + PER <= out_n) {
+        __builtin_nontemporal_store(*(LDS_AS v4i *)from, (v4i_any *)y);
+      } else {
+#pragma unroll 1
+        for (int e = 0; col + e < out_n; ++e) {
+          if constexpr (OE == 4) ((int32_t *)y)[e] = ((LDS_AS int32_t *)from)[e];
+          else ((uint16_t *)y)[e] = ((LDS_AS uint16_t *)from)[e];
+        }
       }
     }
   }
@@ -435,7 +638,7 @@ struct ScaledTile : ScaledOut {
       *(LDS_AS float *)(at + 2 * PITCH) = c;
       *(LDS_AS float *)(at + 3 * PITCH) = d;
     } else {
-      const uint32_t ab = pack(a, b), cd = pack(c, d);
+      const uint32_t ab = pack16(a, b, to16()), cd = pack16(c, d, to16());
       *(LDS_AS uint16_t *)at = (uint16_t)ab;
       *(LDS_AS uint16_t *)(at + PITCH) = (uint16_t)(ab >> 16);
       *(LDS_AS uint16_t *)(at + 2 * PITCH) = (uint16_t)cd;
@@ -449,8 +652,12 @@ struct ScaledTile : ScaledOut {
     else return type == VT_TYPE_BF16 ? __uint_as_float((uint32_t)b << 16) : (float)__builtin_bit_cast(_Float16, b);
   }
 
-  // Blocks of 16 x 16 sums (element e of lane l: row 4 (l / 16) + e, column
-  // l % 16) of 16 MI rows from row0 and 16 NI packed columns from col0. Each
+  // The persistent kernels' tiles, in the same layout but the other order: the
+  // outputs are formed where the sums lie, in registers, and go through the LDS
+  // as they are stored. That is half the LDS traffic for 16-bit outputs, and the
+  // strips, unrolled, overlap: 8192^3 in 403 us against 409 (`strips` unrolled)
+  // and 417 (a loop), gated 2000 x 4096 x 14336 219 against 227 and 232.
+  // Blocks of 16 MI rows from row0 and 16 NI packed columns from col0. Each
   // strip of 16 rows goes through the wave's LDS to whole 16-byte pieces of
   // output rows, chunk k of strip row r at k ^ (OE * ((r / 4) % 4)): the writes
   // of one instruction then fall on distinct banks, as in store_strip16_lds.
@@ -462,24 +669,24 @@ struct ScaledTile : ScaledOut {
   __device__ __forceinline__ void tile16(const v4i (&acc)[MI][NI], int row0, int col0, int row_min, int col_min,
                                          int lane, LDS_AS int8_t *lds) const {
     constexpr int NB = OP == kGated ? NI / 2 : NI;   // blocks of output columns
-    constexpr int ND = OP == kTermsOp ? NI / 2 : 1;  // and of dh's
+    constexpr int ND = OP == kGradTerms ? NI / 2 : 1;  // and of dh's
     constexpr int W = NB * 16, PITCH = W * OE, RC = PITCH / 16;
     const int g = lane >> 4, c = lane & 15;
     float s[NI], bias[OP == kLinear ? NI : 1];
-    v4f tr[OP == kTermsOp ? 2 : MI], nr[2];
-    auto trow = [](int mi) { return OP == kTermsOp ? mi & 1 : mi; };
+    v4f tr[OP == kGradTerms ? 2 : MI], nr[2];
+    auto trow = [](int mi) { return OP == kGradTerms ? mi & 1 : mi; };
 #pragma unroll
     for (int ni = 0; ni < NI; ++ni) {
       s[ni] = meta[col0 + ni * 16 + c];
       if constexpr (OP == kLinear) bias[ni] = meta[Np + col0 + ni * 16 + c];
     }
-    if constexpr (OP != kTermsOp) {
+    if constexpr (OP != kGradTerms) {
 #pragma unroll
       for (int mi = 0; mi < MI; ++mi) tr[mi] = *(const v4f_any *)(t + row0 + mi * 16 + 4 * g);
     }
     DBits d[2][ND][4];
     auto load_strip = [&](int mi) {
-      if constexpr (OP == kTermsOp) {
+      if constexpr (OP == kGradTerms) {
         tr[mi & 1] = *(const v4f_any *)(t + row0 + mi * 16 + 4 * g);
         nr[mi & 1] = *(const v4f_any *)(norm + row0 + mi * 16 + 4 * g);
 #pragma unroll
@@ -499,8 +706,8 @@ struct ScaledTile : ScaledOut {
     auto flush = [&](const float (&v)[NB][4], int mi, int64_t plane) {
 #pragma unroll
       for (int b = 0; b < NB; ++b) put4<PITCH>(lds + wb[b], v[b][0], v[b][1], v[b][2], v[b][3]);
-      store_rows<16, W>(lds, swz, row0 + mi * 16, OP == kGated ? col0 / 2 : col0, plane, lane, EDGE ? row_min : 0, M,
-                        OP == kGated ? col_min / 2 : col_min);
+      store_rows<W>(lds, swz, row0 + mi * 16, OP == kGated ? col0 / 2 : col0, plane, lane, EDGE ? row_min : 0,
+                    OP == kGated ? col_min / 2 : col_min);
     };
 #pragma unroll
     for (int mi = 0; mi < MI; ++mi) {
@@ -516,7 +723,7 @@ struct ScaledTile : ScaledOut {
 #pragma unroll
         for (int b = 0; b < NI / 2; ++b) {
           const int ng = (b >> 1) * 4 + (b & 1);
-          const bool in = OP != kTermsOp || col0 / 2 + b * 16 + c < N;
+          const bool in = OP != kGradTerms || col0 / 2 + b * 16 + c < N;
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             if constexpr (OP == kGated) {
@@ -530,7 +737,7 @@ struct ScaledTile : ScaledOut {
         }
       }
       flush(v, mi, 0);
-      if constexpr (OP == kTermsOp && E == 4) {
+      if constexpr (OP == kGradTerms && E == 4) {
 #pragma unroll
         for (int b = 0; b < NB; ++b)
 #pragma unroll
@@ -541,113 +748,53 @@ struct ScaledTile : ScaledOut {
     }
   }
 
-  // The gradient's float32 sums, in tile16's layout, over the row's normaliser
-  // (a power of two: exact; null for partial sums).
+  // Blocks of 32 x 32 sums (element e of lane l: row 8 (e / 4) + 4 (l / 32) +
+  // e % 4, column l % 32) of 32 MI rows and 64 packed columns; an instruction's
+  // two rows are 4 apart, and chunk k of row r is at k ^ (8 ((r / 4) % 2)).
   template <int MI, int NI>
-  __device__ __forceinline__ void grad16(const v4f (&acc)[MI][NI], int row0, int col0, int lane,
+  __device__ __forceinline__ void tile32(const v16i (&acc)[MI][NI], int row0, int col0, int lane,
                                          LDS_AS int8_t *lds) const {
-    constexpr int W = NI * 16, PITCH = W * OE, RC = PITCH / 16;
-    const int g = lane >> 4, c = lane & 15;
-    float un[MI][4];
+    static_assert(NI == 2, "a gate and an up block");
+    const int g = lane >> 5, c = lane & 31;
+    strips<MI, 32, 64>(
+        [&](auto mi) __attribute__((always_inline)) {
 #pragma unroll
-    for (int mi = 0; mi < MI; ++mi)
+          for (int ni = 0; ni < NI; ++ni)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) un[mi][e] = norm ? 1.0f / norm[min(row0 + mi * 16 + 4 * g + e, M - 1)] : 1.0f;
-    auto swz = [](int row) { return (((row >> 2) & 3) * OE) & (RC - 1); };
-#pragma unroll
-    for (int mi = 0; mi < MI; ++mi) {
-#pragma unroll
-      for (int ni = 0; ni < NI; ++ni)
-        put4<PITCH>(lds + 4 * g * PITCH + (((ni * OE + (c * OE >> 4)) ^ swz(4 * g)) << 4) + (c * OE & 15),
-                    acc[mi][ni][0] * un[mi][0], acc[mi][ni][1] * un[mi][1], acc[mi][ni][2] * un[mi][2],
-                    acc[mi][ni][3] * un[mi][3]);
-      store_rows<16, W>(lds, swz, row0 + mi * 16, col0, 0, lane, 0, M, 0);
-      __builtin_amdgcn_sched_barrier(0);
-    }
+            for (int e = 0; e < 16; ++e)
+              *(LDS_AS int32_t *)(lds + (8 * (e >> 2) + 4 * g + (e & 3)) * 256 + ((((ni ^ g) << 3) + (c >> 2)) << 4) +
+                                  (c & 3) * 4) = acc[mi][ni][e];
+        },
+        [](int row) { return ((row >> 2) & 1) << 3; }, row0, col0, 0, M, 0, lane, lds);
   }
 
   // One element: the sums of packed columns pc (and, of a pair, pc + 32) of a
   // row, to output column j.
   __device__ __forceinline__ void element(int32_t a0, int32_t a1, int row, int pc, int j, float t_row) const {
+    auto put = [&](int64_t at, float v, int to) {
+      if (to == VT_TYPE_F32) ((float *)Y)[at] = v;
+      else ((uint16_t *)Y)[at] = (uint16_t)pack16(v, 0.0f, to);
+    };
     const float s0 = meta[pc];
     if constexpr (OP == kLinear) {
-      if (j < N) store1((int64_t)row * ldy + j, (float)a0 * t_row * s0 + meta[Np + pc]);
+      if (j < N) put((int64_t)row * ldy + j, (float)a0 * t_row * s0 + meta[Np + pc], type);
     } else {
-      float first, second = 0.0f;
-      const float d = OP == kTermsOp && j < N ? d_value(((const DBits *)D)[(int64_t)row * ldd + j]) * norm[row] : 0.0f;
+      float first, second = 0.0f, d = 0.0f;
+      if (OP == kGradTerms && j < N) {
+        const int64_t at = (int64_t)row * ldd + j;
+        d = norm[row] * (type == VT_TYPE_F32 ? ((const float *)D)[at] : from16(((const uint16_t *)D)[at], type));
+      }
       pair(a0, a1, t_row, s0, meta[pc + 32], d, first, second);
       if constexpr (OP == kGated) {
-        if (j < N) store1((int64_t)row * ldy + j, first);
+        if (j < N) put((int64_t)row * ldy + j, first, type);
       } else {
         const int64_t at = (int64_t)row * Np + pc;
-        store1(at, first);
-        store1(at + 32, second);
-        if constexpr (E == 4) {
-          store1(at + lo, first - (float)(_Float16)first);
-          store1(at + lo + 32, second - (float)(_Float16)second);
+        put(at, first, VT_TYPE_F16);
+        put(at + 32, second, VT_TYPE_F16);
+        if (lo) {
+          put(at + lo, first - (float)(_Float16)first, VT_TYPE_F16);
+          put(at + lo + 32, second - (float)(_Float16)second, VT_TYPE_F16);
         }
-      }
-    }
-  }
-
-  // Blocks of 32 x 32 sums (element e of lane l: row 8 (e / 4) + 4 (l / 32) +
-  // e % 4, column l % 32) of 32 MI rows from row0 and 64 packed columns from
-  // col0, one block row at a time through the wave's LDS (whose last reader was
-  // the k loop, before its last barrier): chunk k of row r at k ^ (2 OE * ((r /
-  // 4) % 2)), which puts an instruction's two rows on distinct banks.
-  template <int MI, int NI>
-  __device__ __forceinline__ void tile32(const v16i (&acc)[MI][NI], int row0, int col0, int lane,
-                                         LDS_AS int8_t *lds) const {
-    static_assert(NI == 2, "a gate and an up block");
-    constexpr int W = OP == kGated ? 32 : 64, PITCH = W * OE, RC = PITCH / 16;
-    if (col0 >= Np) return;
-    const int g = lane >> 5, c = lane & 31;
-    const float s0 = meta[col0 + c], s1 = meta[col0 + 32 + c];
-    const float b0 = OP == kLinear ? meta[Np + col0 + c] : 0.0f, b1 = OP == kLinear ? meta[Np + col0 + 32 + c] : 0.0f;
-    const int j = col0 / 2 + c;
-    float tr[MI][16], dr[OP == kTermsOp ? MI : 1][16];
-#pragma unroll
-    for (int mi = 0; mi < MI; ++mi)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int row = min(row0 + mi * 32 + (e >> 2) * 8 + g * 4 + (e & 3), M - 1);
-        tr[mi][e] = t[row];
-        if constexpr (OP == kTermsOp) {
-          const float x = d_value(((const DBits *)D)[(int64_t)row * ldd + min(j, N - 1)]) * norm[row];
-          dr[mi][e] = j < N ? x : 0.0f;
-        }
-      }
-    auto swz = [](int row) { return (((row >> 2) & 1) * 2 * OE) & (RC - 1); };
-    const int w0 = 4 * g * PITCH + (((c * OE >> 4) ^ swz(4 * g)) << 4) + (c * OE & 15);
-    const int w1 = 4 * g * PITCH + (((2 * OE + (c * OE >> 4)) ^ swz(4 * g)) << 4) + (c * OE & 15);
-    auto flush = [&](const float (&a)[16], const float (&b)[16], int mi, int64_t plane) {
-#pragma unroll
-      for (int e = 0; e < 16; e += 4) {
-        put4<PITCH>(lds + w0 + 2 * e * PITCH, a[e], a[e + 1], a[e + 2], a[e + 3]);
-        if constexpr (W == 64) put4<PITCH>(lds + w1 + 2 * e * PITCH, b[e], b[e + 1], b[e + 2], b[e + 3]);
-      }
-      store_rows<32, W>(lds, swz, row0 + mi * 32, OP == kGated ? col0 / 2 : col0, plane, lane, 0, M, 0);
-    };
-#pragma unroll
-    for (int mi = 0; mi < MI; ++mi) {
-      float a[16], b[16];
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        if constexpr (OP == kLinear) {
-          a[e] = (float)acc[mi][0][e] * tr[mi][e] * s0 + b0;
-          b[e] = (float)acc[mi][1][e] * tr[mi][e] * s1 + b1;
-        } else {
-          pair(acc[mi][0][e], acc[mi][1][e], tr[mi][e], s0, s1, OP == kTermsOp ? dr[mi][e] : 0.0f, a[e], b[e]);
-        }
-      }
-      flush(a, b, mi, 0);
-      if constexpr (OP == kTermsOp && E == 4) {
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          a[e] -= (float)(_Float16)a[e];
-          b[e] -= (float)(_Float16)b[e];
-        }
-        flush(a, b, mi, lo);
       }
     }
   }
@@ -659,8 +806,8 @@ __global__ __launch_bounds__(256, 1) void scaled_dma16_kernel(GemmArgs p, Scaled
 }
 
 // The same from int32 sums in memory: `slices` partial sums [M][Np] each.
-template <int OP, int E>
-__global__ __launch_bounds__(256) void finish_kernel(const int32_t *S, int slices, ScaledTile<OP, E> out) {
+template <int OP>
+__global__ __launch_bounds__(256) void finish_kernel(const int32_t *S, int slices, ScaledTile<OP> out) {
   const int row = blockIdx.x, j = blockIdx.y * 256 + threadIdx.x;
   const int pc = OP == kLinear ? j : (int)pair_col(j, 0);
   if (pc >= out.Np) return;
@@ -900,16 +1047,9 @@ __global__ __launch_bounds__(512) void scaled_skinny_kernel(ScaledSkinnyArgs p, 
 
   auto row_t = [&](int row) { return XB ? row_scale(tops[row]).scale : o.t[row]; };
   auto finish = [&](int32_t a0, int32_t a1, int row, int col, float t_row) {
-    const int pc = P == 1 ? col : (int)pair_col(col, 0);
-    if (o.type == VT_TYPE_F32) {
-      ScaledTile<OP, 4> out;
-      (ScaledOut &)out = o;
-      out.element(a0, a1, row, pc, col, t_row);
-    } else {
-      ScaledTile<OP, 2> out;
-      (ScaledOut &)out = o;
-      out.element(a0, a1, row, pc, col, t_row);
-    }
+    ScaledTile<OP> out;
+    (ScaledOut &)out = o;
+    out.element(a0, a1, row, P == 1 ? col : (int)pair_col(col, 0), col, t_row);
   };
   // The sum over the waves of element e of source lane `src` of tile n.
   auto sum = [&](int n, int src, int e) {
@@ -970,6 +1110,7 @@ __global__ __launch_bounds__(512) void scaled_skinny_kernel(ScaledSkinnyArgs p, 
 }
 
 struct TermArgs {
+  QuantArgs pad;       // gated: int8 rows to copy to the pitch of the products (Q null: none)
   const void *D;
   const float *t;      // gated: row scales
   const float *meta;
@@ -1008,6 +1149,10 @@ __global__ __launch_bounds__(256) void row_terms_kernel(TermArgs p) {
   const int tid = threadIdx.x;
   float v[NC ? NC : 1][16];
   uint32_t top = 0;
+  if constexpr (!LINEAR) {
+    if (p.pad.Q)
+      for (int pos = tid * 16; pos < p.pad.Kp; pos += 4096) pad_piece(p.pad, row, pos);
+  }
   auto load = [&](int pos, float (&x)[16]) {
     load16<TYPE, ALIGNED>(d, pos, p.N, x);
     if constexpr (LINEAR) {
@@ -1079,12 +1224,6 @@ __device__ __forceinline__ void mfma16h_in_place(v4f &acc, const v4i &a, const v
   asm volatile("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(acc) : "v"(a), "v"(b));
 }
 
-// f(0), f(1), .. f(N - 1) with compile-time arguments.
-template <class F, int... I>
-__device__ __forceinline__ void each(F &&f, std::integer_sequence<int, I...>) {
-  (f(std::integral_constant<int, I>()), ...);
-}
-
 // BM x 256 tiles of dx (BM 256: waves of 128 x 128; BM 128: of 128 x 64), one
 // tile per workgroup. A slice is 64 packed columns deep: the terms' rows (128
 // bytes, 16-byte chunk c of row r at c ^ (r % 8)) and 4 x 4 whole packed tiles,
@@ -1099,9 +1238,9 @@ __device__ __forceinline__ void each(F &&f, std::integer_sequence<int, I...>) {
 //           the barrier at its end stage s may be refilled (by slice s + 3).
 // `planes` 2: the terms' low halves are multiplied by the same weights in a
 // second pass over the slices. With `splits`, a workgroup takes its share of the
-// slices and writes float32 partial sums (E = 4).
-template <int E, int BM>
-__global__ __launch_bounds__(256, 1) void grad_dma_kernel(GradArgs p, ScaledTile<kGradOp, E> out) {
+// slices and writes float32 partial sums.
+template <int BM>
+__global__ __launch_bounds__(256, 1) void grad_dma_kernel(GradArgs p, ScaledTile<kGrad> out) {
   static_assert(BM == 256 || BM == 128, "256x256 or 128x256 tiles");
   constexpr int WCOLS = BM == 256 ? 2 : 4, WTN = 256 / WCOLS, MI = 8, NI = WTN / 16;
   constexpr int A_BYTES = BM * 128, B_BYTES = 64 * 256, NSTAGE = 3, B_REGION = NSTAGE * A_BYTES;
@@ -1134,7 +1273,7 @@ __global__ __launch_bounds__(256, 1) void grad_dma_kernel(GradArgs p, ScaledTile
   const int8_t *const a_tile = (const int8_t *)(p.T + (int64_t)m0 * p.Np);
   // This workgroup's slices, of all planes' in turn.
   const int per_plane = p.Np / 64, all = per_plane * p.planes;
-  const int s_beg = (int)((int64_t)all * split / p.splits), slices = (int)((int64_t)all * (split + 1) / p.splits) - s_beg;
+  const int s_beg = all * split / p.splits, slices = all * (split + 1) / p.splits - s_beg;   // all * splits < 2^23
   const int64_t b_step = (int64_t)4 * kbt * 1024;
   const int plane = s_beg / per_plane, s_in = s_beg - plane * per_plane;
   const int8_t *a_next = a_tile + (int64_t)s_in * 128 + plane * p.lo * 2, *b_next = p.Bp + s_in * b_step;
@@ -1246,7 +1385,9 @@ __global__ __launch_bounds__(256, 1) void grad_dma_kernel(GradArgs p, ScaledTile
   asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier\n\ts_nop 7\n\ts_nop 7" ::: "memory");
   fence_acc();
   if (p.splits > 1) out.Y = (float *)out.Y + (int64_t)split * p.M * p.Kp;
-  out.template grad16<MI, NI>(acc, m0 + wm * 128, n0 + wn * WTN, lane, (LDS_AS int8_t *)smem + wave * 8192);
+  constexpr int STRIP = 64 * WTN * 4;   // 64 of a wave's rows
+  static_assert(4 * STRIP <= (int)sizeof(smem), "the stages hold every wave's strip");
+  out.blocks16<4>(acc, m0 + wm * 128, n0 + wn * WTN, 0, 0, lane, (LDS_AS int8_t *)smem + wave * STRIP);
 }
 
 // dx from the partial sums [slices][M][Kp] of a split contraction, over the
@@ -1264,8 +1405,16 @@ __global__ __launch_bounds__(256) void grad_sum_kernel(GradSumArgs p) {
   const int col = (blockIdx.y * 256 + threadIdx.x) * 4;
   if (col >= p.K) return;
   const float *w = p.ws + row * p.Kp + col;
-  v4f v = *(const v4f *)w;
-  for (int i = 1; i < p.slices; ++i) v += *(const v4f *)(w + (int64_t)i * p.M * p.Kp);
+  const int64_t step = (int64_t)p.M * p.Kp;
+  v4f v = {0, 0, 0, 0};
+  for (int i = 0; i < p.slices; i += 8) {   // 8 loads in flight; the order of the sums does not depend on them
+    v4f part[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) part[u] = *(const v4f *)(w + min(i + u, p.slices - 1) * step);
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+      if (i + u < p.slices) v += part[u];
+  }
   v *= 1.0f / p.norm[row];
   const int64_t at = row * p.ldx + col;
 #pragma unroll
@@ -1319,12 +1468,19 @@ struct Rows {
   int64_t ld;
 };
 
-// X (any type) -> rows of Kp int8 values: int8 rows that are already so are
-// used where they are (unless they lie too far apart for the tile kernels'
-// 32-bit offsets), others are copied (int8) or rounded to a workspace.
-int take_rows(const void *X, int type, int64_t ldx, const float *T, int64_t M, int64_t K, Scratch &scr, Rows *out) {
+// Whether int8 rows can be read where they are: in whole 16-byte aligned
+// pieces, no further apart than the tile kernels' 32-bit offsets reach.
+bool rows_in_place(const void *X, int type, int64_t ldx, int64_t K) {
+  return ldx <= kFarRows &&
+         (type == VT_TYPE_I8_PADDED || (type == VT_TYPE_I8 && K == scaled_kp(K) && ldx % 16 == 0 && aligned16(X)));
+}
+
+// X (any type) -> rows of Kp int8 values: in place, or copied (int8) or rounded
+// to a workspace. `pad`: a copy is left to the caller, who gets its arguments.
+int take_rows(const void *X, int type, int64_t ldx, const float *T, int64_t M, int64_t K, Scratch &scr, Rows *out,
+              QuantArgs *pad = nullptr) {
   const int64_t Kp = scaled_kp(K);
-  if (ldx <= kFarRows && ((type == VT_TYPE_I8 && K == Kp && ldx % 16 == 0 && aligned16(X)) || type == VT_TYPE_I8_PADDED)) {
+  if (rows_in_place(X, type, ldx, K)) {
     *out = Rows{(const int8_t *)X, T, ldx};
     return VT_OK;
   }
@@ -1333,19 +1489,15 @@ int take_rows(const void *X, int type, int64_t ldx, const float *T, int64_t M, i
   if (int rc = scr.take(kRows, q_bytes + (size_t)M * sizeof(float), &w)) return rc;
   QuantArgs a = {X, (int8_t *)w, (float *)((int8_t *)w + q_bytes), ldx, Kp, K, Kp};
   *out = Rows{a.Q, float_type(type) ? a.T : T, Kp};
-  if (!float_type(type)) {
-    for (int64_t r0 = 0; r0 < M; r0 += 65535) {
-      QuantArgs b = a;
-      b.X = (const int8_t *)X + r0 * ldx;
-      b.Q = a.Q + r0 * Kp;
-      const unsigned rows = (unsigned)std::min<int64_t>(M - r0, 65535);
-      hipLaunchKernelGGL(pad_rows_kernel, dim3((unsigned)((Kp + 4095) / 4096), rows), dim3(256), 0,
-                         (hipStream_t)scr.stream, b);
-    }
-    VT_HIP_CHECK(hipGetLastError());
+  if (float_type(type)) return launch_quant(a, type, M, (hipStream_t)scr.stream);
+  if (pad) {
+    *pad = a;
     return VT_OK;
   }
-  return launch_quant(a, type, M, (hipStream_t)scr.stream);
+  hipLaunchKernelGGL(pad_rows_kernel, dim3((unsigned)M, (unsigned)((Kp + 4095) / 4096)), dim3(256), 0,
+                     (hipStream_t)scr.stream, a);
+  VT_HIP_CHECK(hipGetLastError());
+  return VT_OK;
 }
 
 GemmArgs scaled_args(const Rows &rows, const int8_t *Bp, int64_t M, int64_t Kp, int64_t Np, int bm, int bn) {
@@ -1363,18 +1515,33 @@ GemmArgs scaled_args(const Rows &rows, const int8_t *Bp, int64_t M, int64_t Kp, 
   return a;
 }
 
-template <int OP, int E>
-int launch_finish(const int32_t *sums, int slices, const ScaledTile<OP, E> &out, hipStream_t s) {
+template <int OP>
+int launch_finish(const int32_t *sums, int slices, const ScaledTile<OP> &out, hipStream_t s) {
   const int cols = OP == kLinear ? out.Np : out.Np / 2;
   const dim3 grid((unsigned)out.M, (unsigned)((cols + 255) / 256));
-  hipLaunchKernelGGL((finish_kernel<OP, E>), grid, dim3(256), 0, s, sums, slices, out);
+  hipLaunchKernelGGL((finish_kernel<OP>), grid, dim3(256), 0, s, sums, slices, out);
   VT_HIP_CHECK(hipGetLastError());
   return VT_OK;
 }
 
+template <int OP, int BN>
+void launch_dma16(const GemmArgs &a, const ScaledOut &o, int64_t wgs, hipStream_t s) {
+  if (o.type == VT_TYPE_F32) {
+    ScaledTile<OP, 4> out;
+    (ScaledOut &)out = o;
+    hipLaunchKernelGGL((scaled_dma16_kernel<OP, 4, BN>), dim3((unsigned)wgs), dim3(256), 0, s, a, out);
+  } else {
+    ScaledTile<OP, 2> out;
+    (ScaledOut &)out = o;
+    hipLaunchKernelGGL((scaled_dma16_kernel<OP, 2, BN>), dim3((unsigned)wgs), dim3(256), 0, s, a, out);
+  }
+}
+
 // The int8 product of rows and packed weights, and what follows it, on tiles.
-template <int OP, int E>
-int launch_product(const Rows &rows, const int8_t *Bp, int64_t Kp, const ScaledTile<OP, E> &out, Scratch &scr) {
+template <int OP>
+int launch_scaled(const Rows &rows, const int8_t *Bp, int64_t Kp, const ScaledOut &o, Scratch &scr) {
+  ScaledTile<OP> out;
+  (ScaledOut &)out = o;
   hipStream_t s = (hipStream_t)scr.stream;
   const int cus = scr.st->num_cus;
   const int64_t M = out.M, Np = out.Np;
@@ -1385,10 +1552,10 @@ int launch_product(const Rows &rows, const int8_t *Bp, int64_t Kp, const ScaledT
   const bool persistent = M >= 256 && Np >= 256 && Kp % 256 == 0 && 16 * 1024 * (Kp / 64) < (1ll << 32) - 4096;
   if (persistent && (t256 >= 256 || (Kp >= 2048 && t256 > 128) || (Kp >= 1024 && t256 > 192))) {
     const GemmArgs a = scaled_args(rows, Bp, M, Kp, Np, 256, 256);
-    hipLaunchKernelGGL((scaled_dma16_kernel<OP, E, 256>), dim3((unsigned)std::min<int64_t>(t256, cus)), dim3(256), 0, s, a, out);
+    launch_dma16<OP, 256>(a, o, std::min<int64_t>(t256, cus), s);
   } else if (persistent && Kp >= 1024 && t128 > 128 && t128 <= 256) {
     const GemmArgs a = scaled_args(rows, Bp, M, Kp, Np, 256, 128);
-    hipLaunchKernelGGL((scaled_dma16_kernel<OP, E, 128>), dim3((unsigned)std::min<int64_t>(t128, cus)), dim3(256), 0, s, a, out);
+    launch_dma16<OP, 128>(a, o, std::min<int64_t>(t128, cus), s);
   } else {
     const int ks = mfma_k_split<128, 128>(q);
     if (ks > 1) {
@@ -1410,12 +1577,12 @@ int launch_product(const Rows &rows, const int8_t *Bp, int64_t Kp, const ScaledT
     if (full > 0x7fffffff) return fail(VT_EUNSUPPORTED, "grid of %lld tiles too large", (long long)full);
     if (half <= kHalfTileMaxWgs) {
       const GemmArgs a = scaled_args(rows, Bp, M, Kp, Np, 64, 128);
-      if (short_k) hipLaunchKernelGGL((gemm_mfma_kernel<64, 128, 1, false, true, false, true, ScaledTile<OP, E>>), dim3((unsigned)half), dim3(256), 0, s, a, out);
-      else hipLaunchKernelGGL((gemm_mfma_kernel<64, 128, 1, false, false, false, true, ScaledTile<OP, E>>), dim3((unsigned)half), dim3(256), 0, s, a, out);
+      if (short_k) hipLaunchKernelGGL((gemm_mfma_kernel<64, 128, 1, false, true, false, true, ScaledTile<OP>>), dim3((unsigned)half), dim3(256), 0, s, a, out);
+      else hipLaunchKernelGGL((gemm_mfma_kernel<64, 128, 1, false, false, false, true, ScaledTile<OP>>), dim3((unsigned)half), dim3(256), 0, s, a, out);
     } else {
       const GemmArgs a = scaled_args(rows, Bp, M, Kp, Np, 128, 128);
-      if (short_k) hipLaunchKernelGGL((gemm_mfma_kernel<128, 128, 1, false, true, false, true, ScaledTile<OP, E>>), dim3((unsigned)full), dim3(256), 0, s, a, out);
-      else hipLaunchKernelGGL((gemm_mfma_kernel<128, 128, 1, false, false, false, true, ScaledTile<OP, E>>), dim3((unsigned)full), dim3(256), 0, s, a, out);
+      if (short_k) hipLaunchKernelGGL((gemm_mfma_kernel<128, 128, 1, false, true, false, true, ScaledTile<OP>>), dim3((unsigned)full), dim3(256), 0, s, a, out);
+      else hipLaunchKernelGGL((gemm_mfma_kernel<128, 128, 1, false, false, false, true, ScaledTile<OP>>), dim3((unsigned)full), dim3(256), 0, s, a, out);
     }
   }
   VT_HIP_CHECK(hipGetLastError());
@@ -1529,26 +1696,9 @@ int launch_skinny(const void *X, int type, int64_t ldx, int64_t K, const Rows &r
   else launch_skinny_rows<OP, 2>(a, o, grid, s);
   VT_HIP_CHECK(hipGetLastError());
   if (!a.ws) return VT_OK;
-  if (o.type == VT_TYPE_F32) {
-    ScaledTile<OP, 4> t;
-    (ScaledOut &)t = o;
-    return launch_finish(a.ws, a.k_split, t, s);
-  }
-  ScaledTile<OP, 2> t;
-  (ScaledOut &)t = o;
-  return launch_finish(a.ws, a.k_split, t, s);
-}
-
-template <int OP>
-int launch_scaled(const Rows &rows, const int8_t *Bp, int64_t Kp, const ScaledOut &o, Scratch &scr) {
-  if (o.type == VT_TYPE_F32) {
-    ScaledTile<OP, 4> t;
-    (ScaledOut &)t = o;
-    return launch_product(rows, Bp, Kp, t, scr);
-  }
-  ScaledTile<OP, 2> t;
-  (ScaledOut &)t = o;
-  return launch_product(rows, Bp, Kp, t, scr);
+  ScaledTile<OP> out;
+  (ScaledOut &)out = o;
+  return launch_finish(a.ws, a.k_split, out, s);
 }
 
 template <int TYPE, bool ALIGNED, bool LINEAR>
@@ -1600,14 +1750,13 @@ GradGeom grad_geom(int64_t M, int64_t Kp, int64_t slices, int cus) {
   return best;
 }
 
-template <int E>
 int launch_grad_tiles(const GradArgs &a, int bm, const ScaledOut &o, hipStream_t s) {
-  ScaledTile<kGradOp, E> out;
+  ScaledTile<kGrad> out;
   (ScaledOut &)out = o;
   const int64_t wgs = (int64_t)a.tiles_m * a.tiles_n * a.splits;
   if (wgs > 0x7fffffff) return fail(VT_EUNSUPPORTED, "gradient grid too large");
-  if (bm == 256) hipLaunchKernelGGL((grad_dma_kernel<E, 256>), dim3((unsigned)wgs), dim3(256), 0, s, a, out);
-  else hipLaunchKernelGGL((grad_dma_kernel<E, 128>), dim3((unsigned)wgs), dim3(256), 0, s, a, out);
+  if (bm == 256) hipLaunchKernelGGL(grad_dma_kernel<256>, dim3((unsigned)wgs), dim3(256), 0, s, a, out);
+  else hipLaunchKernelGGL(grad_dma_kernel<128>, dim3((unsigned)wgs), dim3(256), 0, s, a, out);
   VT_HIP_CHECK(hipGetLastError());
   return VT_OK;
 }
@@ -1636,15 +1785,15 @@ int launch_grad(GradArgs a, const ScaledOut &o, Scratch &scr) {
   a.tiles_n = (a.Kp + 255) / 256;
   a.splits = g.splits;
   if (g.splits == 1)
-    return o.type == VT_TYPE_F32 ? launch_grad_tiles<4>(a, g.bm, o, s) : launch_grad_tiles<2>(a, g.bm, o, s);
+    return launch_grad_tiles(a, g.bm, o, s);
   void *w = nullptr;
   if (int rc = scr.take(kPartials, (size_t)g.splits * a.M * a.Kp * sizeof(float), &w)) return rc;
   ScaledOut part = o;
   part.Y = w;
-  part.ldy = part.N = a.Kp;
+  part.ldy = part.N = part.Np = a.Kp;
   part.norm = nullptr;
   part.type = VT_TYPE_F32;
-  if (int rc = launch_grad_tiles<4>(a, g.bm, part, s)) return rc;
+  if (int rc = launch_grad_tiles(a, g.bm, part, s)) return rc;
   const GradSumArgs r = {(const float *)w, o.norm, o.Y, o.ldy, a.M, o.N, a.Kp, g.splits, o.type};
   hipLaunchKernelGGL(grad_sum_kernel, dim3((unsigned)a.M, (unsigned)((o.N + 1023) / 1024)), dim3(256), 0, s, r);
   VT_HIP_CHECK(hipGetLastError());
@@ -1769,7 +1918,7 @@ int backward(const ScaledCall &c, const int8_t *Q, int q_type, int64_t ldq, cons
   hipStream_t s = (hipStream_t)stream;
   ScaledOut o = {};
   o.Y = c.Y; o.ldy = c.ldy;
-  o.M = (int)c.M; o.N = (int)c.K;
+  o.M = (int)c.M; o.N = (int)c.K; o.Np = (int)Kp;
   o.type = c.y_type;
   if (Np == 0) return launch_zero(o, s);
   // Terms in float16, normalised by row; of float32 gradients also what
@@ -1781,19 +1930,19 @@ int backward(const ScaledCall &c, const int8_t *Q, int q_type, int64_t ldq, cons
   if (int rc = scr.take(kTerms, t_bytes + (size_t)c.M * sizeof(float), &w)) return rc;
   _Float16 *terms = (_Float16 *)w;
   float *norm = (float *)((int8_t *)w + t_bytes);
-  const TermArgs ta = {c.X, t, c.meta, norm, terms, c.ldx, lo, (int)c.M, (int)c.N, (int)Np};
+  TermArgs ta = {{}, c.X, t, c.meta, norm, terms, c.ldx, lo, (int)c.M, (int)c.N, (int)Np};
   if (!c.pair) {
     if (int rc = launch_row_terms<true>(ta, c.x_type, s)) return rc;
   } else {
-    if (int rc = launch_row_terms<false>(ta, c.x_type, s)) return rc;
     Rows rows;
-    if (int rc = take_rows(Q, q_type, ldq, t, c.M, c.K, scr, &rows)) return rc;
+    if (int rc = take_rows(Q, q_type, ldq, t, c.M, c.K, scr, &rows, &ta.pad)) return rc;
+    if (int rc = launch_row_terms<false>(ta, c.x_type, s)) return rc;
     ScaledOut f = {};
     f.t = rows.t; f.meta = c.meta; f.D = c.X; f.norm = norm; f.Y = terms;
     f.ldd = c.ldx; f.lo = lo;
     f.M = (int)c.M; f.N = (int)c.N; f.Np = (int)Np;
     f.act = act; f.type = c.x_type;
-    if (int rc = launch_scaled<kTermsOp>(rows, c.Bp, Kp, f, scr)) return rc;
+    if (int rc = launch_scaled<kGradTerms>(rows, c.Bp, Kp, f, scr)) return rc;
   }
   o.norm = norm;
   const GradArgs g = {terms, c.Bp, lo, (int)c.M, (int)Kp, (int)Np, 0, 0, 0, split ? 2 : 1, 1};
