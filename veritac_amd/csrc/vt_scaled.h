@@ -111,14 +111,15 @@ struct Elem<kBF16> {
   typedef __bf16 T;
 };
 
-// 16 elements of a row from `pos`, zero past `len`. ALIGNED: the row starts on
-// 16 bytes, so pieces that lie within the row are read as vectors.
-template <int TYPE, bool ALIGNED>
+// 16 elements of a row from `pos`, zero past `len`. Pieces that lie within the
+// row are read as 16-byte vectors at any alignment (the target's global loads
+// need none; element loads took rows of odd lengths three times as long).
+template <int TYPE>
 __device__ __forceinline__ void load16(const typename Elem<TYPE>::T *row, int64_t pos, int64_t len, float (&v)[16]) {
   typedef typename Elem<TYPE>::T T;
   constexpr int PER = 16 / sizeof(T);
-  if (ALIGNED && pos + 16 <= len) {
-    typedef T VT __attribute__((ext_vector_type(PER)));
+  if (pos + 16 <= len) {
+    typedef T VT __attribute__((ext_vector_type(PER), aligned(sizeof(T))));
 #pragma unroll
     for (int i = 0; i < 16 / PER; ++i) {
       const VT x = *(const VT *)(row + pos + i * PER);
@@ -154,7 +155,7 @@ __device__ __forceinline__ uint32_t block_max(uint32_t m, uint32_t *red) {
 
 // One workgroup per row; a thread holds NC pieces of 16 elements in registers
 // between the maximum and the rounding (NC = 0: longer rows, read twice).
-template <int TYPE, bool ALIGNED, int THREADS, int NC>
+template <int TYPE, int THREADS, int NC>
 __global__ __launch_bounds__(THREADS) void quant_rows_kernel(QuantArgs p) {
   __shared__ uint32_t red[THREADS / 64];
   typedef typename Elem<TYPE>::T T;
@@ -168,13 +169,13 @@ __global__ __launch_bounds__(THREADS) void quant_rows_kernel(QuantArgs p) {
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
       const int64_t pos = (int64_t)(tid + THREADS * i) * 16;
-      load16<TYPE, ALIGNED>(x, pos, p.K, v[i]);
+      load16<TYPE>(x, pos, p.K, v[i]);
 #pragma unroll
       for (int e = 0; e < 16; ++e) top = max(top, magnitude(v[i][e]));
     }
   } else {
     for (int64_t pos = tid * 16; pos < p.K; pos += THREADS * 16) {
-      load16<TYPE, ALIGNED>(x, pos, p.K, v[0]);
+      load16<TYPE>(x, pos, p.K, v[0]);
 #pragma unroll
       for (int e = 0; e < 16; ++e) top = max(top, magnitude(v[0][e]));
     }
@@ -197,7 +198,7 @@ __global__ __launch_bounds__(THREADS) void quant_rows_kernel(QuantArgs p) {
     for (int i = 0; i < NC; ++i) put((int64_t)(tid + THREADS * i) * 16, v[i]);
   } else {
     for (int64_t pos = tid * 16; pos < p.Kp; pos += THREADS * 16) {
-      load16<TYPE, ALIGNED>(x, pos, p.K, v[0]);
+      load16<TYPE>(x, pos, p.K, v[0]);
       put(pos, v[0]);
     }
   }
@@ -832,7 +833,7 @@ struct ScaledSkinnyArgs {
   int32_t *ws;        // [k_split][M][Np] partial sums, or null
   uint64_t *fin;      // finishing words, or null
   int64_t ldx;
-  int x_type, x_aligned;
+  int x_type;
   int K, Kp, nbt;     // nbt: 16-column blocks of a projection
   int hpw, groups, k_split, kb_per_split, fin_bits;
 };
@@ -888,10 +889,10 @@ __global__ __launch_bounds__(512) void scaled_skinny_kernel(ScaledSkinnyArgs p, 
       for (int e = 0; e < XB * 4; ++e) raw[i][e] = 0;
       if (row < M) {
         const int8_t *src = (const int8_t *)p.X + ((int64_t)row * p.ldx + pos) * XB;
-        if (p.x_aligned && pos + 16 <= p.K) {
+        if (pos + 16 <= p.K) {
 #pragma unroll
           for (int v = 0; v < XB; ++v) {
-            const v4i y = *(const v4i *)(src + v * 16);
+            const v4i y = ld_any(src + v * 16);
 #pragma unroll
             for (int e = 0; e < 4; ++e) raw[i][v * 4 + e] = (uint32_t)y[e];
           }
@@ -1140,7 +1141,7 @@ __device__ __forceinline__ void put_terms(_Float16 *y, int64_t lo, const float (
 // the maximum and the rounding (0: longer rows, read twice). Else only the
 // normaliser of a gated product's terms, from the row's largest |dh|, its
 // scale and the weights' bound: |q| <= 128, |act(g)| <= |g| and |act'| <= 1.13.
-template <int TYPE, bool ALIGNED, bool LINEAR, int NC>
+template <int TYPE, bool LINEAR, int NC>
 __global__ __launch_bounds__(256) void row_terms_kernel(TermArgs p) {
   __shared__ uint32_t red[4];
   typedef typename Elem<TYPE>::T T;
@@ -1154,7 +1155,7 @@ __global__ __launch_bounds__(256) void row_terms_kernel(TermArgs p) {
       for (int pos = tid * 16; pos < p.pad.Kp; pos += 4096) pad_piece(p.pad, row, pos);
   }
   auto load = [&](int pos, float (&x)[16]) {
-    load16<TYPE, ALIGNED>(d, pos, p.N, x);
+    load16<TYPE>(d, pos, p.N, x);
     if constexpr (LINEAR) {
       if (pos < p.Np) {
 #pragma unroll
@@ -1439,23 +1440,21 @@ constexpr int64_t kScaledMaxN = 65535 * 64;
 // Pitch of int8 rows from which on they are copied before the products.
 constexpr int64_t kFarRows = (int64_t)1 << 23;
 
-template <int TYPE, bool ALIGNED>
+template <int TYPE>
 void launch_quant_typed(const QuantArgs &a, int64_t M, hipStream_t s) {
   const dim3 grid((unsigned)M);
-  if (a.Kp <= 1024) hipLaunchKernelGGL((quant_rows_kernel<TYPE, ALIGNED, 64, 1>), grid, dim3(64), 0, s, a);
-  else if (a.Kp <= 4096) hipLaunchKernelGGL((quant_rows_kernel<TYPE, ALIGNED, 256, 1>), grid, dim3(256), 0, s, a);
-  else if (a.Kp <= 8192) hipLaunchKernelGGL((quant_rows_kernel<TYPE, ALIGNED, 256, 2>), grid, dim3(256), 0, s, a);
-  else if (a.Kp <= 16384) hipLaunchKernelGGL((quant_rows_kernel<TYPE, ALIGNED, 256, 4>), grid, dim3(256), 0, s, a);
-  else hipLaunchKernelGGL((quant_rows_kernel<TYPE, ALIGNED, 256, 0>), grid, dim3(256), 0, s, a);
+  if (a.Kp <= 1024) hipLaunchKernelGGL((quant_rows_kernel<TYPE, 64, 1>), grid, dim3(64), 0, s, a);
+  else if (a.Kp <= 4096) hipLaunchKernelGGL((quant_rows_kernel<TYPE, 256, 1>), grid, dim3(256), 0, s, a);
+  else if (a.Kp <= 8192) hipLaunchKernelGGL((quant_rows_kernel<TYPE, 256, 2>), grid, dim3(256), 0, s, a);
+  else if (a.Kp <= 16384) hipLaunchKernelGGL((quant_rows_kernel<TYPE, 256, 4>), grid, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((quant_rows_kernel<TYPE, 256, 0>), grid, dim3(256), 0, s, a);
 }
 
 int launch_quant(const QuantArgs &a, int type, int64_t M, hipStream_t s) {
-  const int64_t e = elem_size(type);
-  const bool al = aligned16(a.X) && a.ldx * e % 16 == 0;
   switch (type) {
-    case VT_TYPE_F32: al ? launch_quant_typed<kF32, true>(a, M, s) : launch_quant_typed<kF32, false>(a, M, s); break;
-    case VT_TYPE_F16: al ? launch_quant_typed<kF16, true>(a, M, s) : launch_quant_typed<kF16, false>(a, M, s); break;
-    default: al ? launch_quant_typed<kBF16, true>(a, M, s) : launch_quant_typed<kBF16, false>(a, M, s); break;
+    case VT_TYPE_F32: launch_quant_typed<kF32>(a, M, s); break;
+    case VT_TYPE_F16: launch_quant_typed<kF16>(a, M, s); break;
+    default: launch_quant_typed<kBF16>(a, M, s); break;
   }
   VT_HIP_CHECK(hipGetLastError());
   return VT_OK;
@@ -1666,7 +1665,6 @@ int launch_skinny(const void *X, int type, int64_t ldx, int64_t K, const Rows &r
   a.Bp = Bp;
   a.ldx = X ? ldx : rows.ld;
   a.x_type = type;
-  a.x_aligned = X && aligned16(X) && ldx * elem_size(type) % 16 == 0;
   a.K = (int)K; a.Kp = (int)Kp; a.nbt = (int)nbt;
   a.hpw = g.hpw;
   a.groups = g.groups;
@@ -1701,26 +1699,25 @@ int launch_skinny(const void *X, int type, int64_t ldx, int64_t K, const Rows &r
   return launch_finish(a.ws, a.k_split, out, s);
 }
 
-template <int TYPE, bool ALIGNED, bool LINEAR>
+template <int TYPE, bool LINEAR>
 void launch_row_terms_typed(const TermArgs &a, hipStream_t s) {
   const dim3 grid((unsigned)a.M);
   if constexpr (LINEAR) {
-    if (a.Np <= 4096) hipLaunchKernelGGL((row_terms_kernel<TYPE, ALIGNED, true, 1>), grid, dim3(256), 0, s, a);
-    else if (a.Np <= 8192) hipLaunchKernelGGL((row_terms_kernel<TYPE, ALIGNED, true, 2>), grid, dim3(256), 0, s, a);
-    else if (a.Np <= 16384) hipLaunchKernelGGL((row_terms_kernel<TYPE, ALIGNED, true, 4>), grid, dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((row_terms_kernel<TYPE, ALIGNED, true, 0>), grid, dim3(256), 0, s, a);
+    if (a.Np <= 4096) hipLaunchKernelGGL((row_terms_kernel<TYPE, true, 1>), grid, dim3(256), 0, s, a);
+    else if (a.Np <= 8192) hipLaunchKernelGGL((row_terms_kernel<TYPE, true, 2>), grid, dim3(256), 0, s, a);
+    else if (a.Np <= 16384) hipLaunchKernelGGL((row_terms_kernel<TYPE, true, 4>), grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((row_terms_kernel<TYPE, true, 0>), grid, dim3(256), 0, s, a);
   } else {
-    hipLaunchKernelGGL((row_terms_kernel<TYPE, ALIGNED, false, 0>), grid, dim3(256), 0, s, a);
+    hipLaunchKernelGGL((row_terms_kernel<TYPE, false, 0>), grid, dim3(256), 0, s, a);
   }
 }
 
 template <bool LINEAR>
 int launch_row_terms(const TermArgs &a, int type, hipStream_t s) {
-  const bool al = aligned16(a.D) && a.ldd * elem_size(type) % 16 == 0;
   switch (type) {
-    case VT_TYPE_F32: al ? launch_row_terms_typed<kF32, true, LINEAR>(a, s) : launch_row_terms_typed<kF32, false, LINEAR>(a, s); break;
-    case VT_TYPE_F16: al ? launch_row_terms_typed<kF16, true, LINEAR>(a, s) : launch_row_terms_typed<kF16, false, LINEAR>(a, s); break;
-    default: al ? launch_row_terms_typed<kBF16, true, LINEAR>(a, s) : launch_row_terms_typed<kBF16, false, LINEAR>(a, s); break;
+    case VT_TYPE_F32: launch_row_terms_typed<kF32, LINEAR>(a, s); break;
+    case VT_TYPE_F16: launch_row_terms_typed<kF16, LINEAR>(a, s); break;
+    default: launch_row_terms_typed<kBF16, LINEAR>(a, s); break;
   }
   VT_HIP_CHECK(hipGetLastError());
   return VT_OK;
