@@ -150,7 +150,7 @@ def test_gated(dev, m, k, n, dtype, act):
 
 
 # (m, k, packed columns): enough tiles of 256 x 256 or 256 x 128 for the persistent kernels, ragged ends
-LARGE = [(2100, 200, 8000), (1100, 1024, 3800), (260, 1500, 17000)]
+LARGE = [(4000, 1000, 3904), (2000, 4000, 4032), (260, 1500, 17000), (2100, 200, 8000)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
@@ -158,7 +158,7 @@ LARGE = [(2100, 200, 8000), (1100, 1024, 3800), (260, 1500, 17000)]
 def test_linear_on_whole_chip_tiles(dev, m, k, cols, dtype):
     rng = np.random.default_rng(m + k)
     x, x32 = rows(rng, m, k, dtype)
-    n = cols - 3
+    n = cols - 4
     w, s = weights(rng, k, n)
     bias = rng.normal(0, 0.3, n).astype(np.float32)
     say("linear", m, k, n, dtype)
@@ -372,6 +372,19 @@ def test_gradients_on_whole_chip_tiles(dev, m, k, n, dtype):
     say("gated_grad", m, k, n, dtype)
     dx = scaled.gated_grad(d.to(dev), scaled.quantize_rows(x.to(dev)), packed_pair(dev, w, s, w2, s2))
     ref.check(dx, *ref.gated_grad(d32, q, t, w, s, w2, s2, "silu", dtype != torch.float32), dtype, "gated_grad")
+
+
+@pytest.mark.parametrize("dtype,act", [(torch.float32, "gelu"), (torch.bfloat16, "silu")], ids=["f32-gelu", "bf16-silu"])
+@pytest.mark.parametrize("m,k,n", [(4000, 1000, 1947), (2000, 4000, 2011)])
+def test_gated_grad_terms_on_whole_chip_tiles(dev, m, k, n, dtype, act):
+    rng = np.random.default_rng(m + k + n)
+    d, d32 = gradients(rng, m, n, dtype)
+    (wg, sg), (wu, su) = weights(rng, k, n, -128), weights(rng, k, n)
+    x, x32 = rows(rng, m, k, dtype)
+    q, t = ref.quantize(x32)
+    say("gated_grad", m, k, n, dtype, act)
+    dx = scaled.gated_grad(d.to(dev), scaled.quantize_rows(x.to(dev)), packed_pair(dev, wg, sg, wu, su), act=act)
+    ref.check(dx, *ref.gated_grad(d32, q, t, wg, sg, wu, su, act, dtype != torch.float32), dtype, "gated_grad")
 
 
 @pytest.mark.parametrize("act", ["silu", "gelu"])

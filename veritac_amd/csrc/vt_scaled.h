@@ -1523,6 +1523,65 @@ int launch_finish(const int32_t *sums, int slices, const ScaledTile<OP> &out, hi
   return VT_OK;
 }
 
+// Tiles of the forward products and gradient terms: the kernel with the least
+// estimated time. Fitted to calls over 100 .. 5295 rows, 704 .. 28672 packed
+// columns and K 256 .. 14336 (us, r rounds of tiles over the CUs, s 64-deep
+// slices), each kernel on each of them; the choice is within 5 % of the fastest
+// where that is over 15 us:
+//   persistent 256x256  r (14 + 0.64 s)       whole rounds; 700 x 4096 x 14336
+//                                              52.1 (128x128 tiles 61.5)
+//   persistent 256x128  r (8 + 0.42 s)        5295 x 4864 x 4096 119.5 (256x256
+//                                              127.9, 128x128 135.5)
+//   128x128             5.2 + r (1.6 + 0.287 s), r fractional above 1 (several
+//                                              workgroups share a CU)
+//                                              2566 x 10240 x 1536 56.2 (256x128
+//                                              69.8); 590 x 6912 x 24064 131 (154)
+//   64x128              4.3 + r (0.5 + 0.195 s), r at least 1.2
+//                                              4096 x 256 x 4096 14.5 (128x128
+//                                              16.6, 256x256 18.0)
+//   128x128, K in ks slices: the partial sums' kernel, 3.5 and their traffic
+//                                              1092 x 9728 x 704 22.9 (44.8)
+// Gradient terms take longer after the sums (3 us per round of 128x128 tiles,
+// by the same per element for the others).
+struct TilePlan {
+  int bm, bn, ks;
+  bool persistent;
+  int64_t tiles;
+};
+
+TilePlan tile_plan(bool terms, int64_t M, int64_t Np, int64_t Kp, int cus) {
+  const double slices = Kp / 64.0, more = terms ? 3.0 : 0.0;
+  TilePlan best = {};
+  double least = 0;
+  auto offer = [&](int bm, int bn, int ks, bool persistent) {
+    const int64_t tiles = (M + bm - 1) / bm * ((Np + bn - 1) / bn);
+    const double share = (double)(tiles * ks) / cus;
+    double us;
+    if (persistent) {
+      const double rounds = (double)((tiles + cus - 1) / cus);
+      us = bn == 256 ? rounds * (14 + 0.64 * slices + 3 * more) : rounds * (8 + 0.42 * slices + 1.6 * more);
+    } else if (bm == 64) {
+      us = 4.3 + std::max(share, 1.2) * (0.5 + 0.195 * slices + 0.5 * more);
+    } else {
+      us = 5.2 + std::max(share, 1.0) * (1.6 + 0.287 * slices / ks + (ks > 1 ? 0 : more));
+      if (ks > 1) us += 3.5 + 8.0 * ks * M * Np / 8.0e6;
+    }
+    if (least == 0 || us < least) {
+      least = us;
+      best = {bm, bn, ks, persistent, tiles};
+    }
+  };
+  if (M >= 256 && Np >= 256 && Kp % 256 == 0) {
+    offer(256, 256, 1, true);
+    offer(256, 128, 1, true);
+  }
+  offer(128, 128, 1, false);
+  offer(64, 128, 1, false);
+  for (int ks = 2; ks <= 16; ks *= 2)
+    if (Kp % (128 * ks) == 0 && Kp / ks >= 512) offer(128, 128, ks, false);
+  return best;
+}
+
 template <int OP, int BN>
 void launch_dma16(const GemmArgs &a, const ScaledOut &o, int64_t wgs, hipStream_t s) {
   if (o.type == VT_TYPE_F32) {
@@ -1547,41 +1606,36 @@ int launch_scaled(const Rows &rows, const int8_t *Bp, int64_t Kp, const ScaledOu
   const Problem q = {rows.q, Bp, nullptr, nullptr, M, Np, Kp, rows.ld, Kp / 64, 0, Np, 1, 0, 0, 0, 0};
   void *w = nullptr;
   if (Kp == 0) return launch_finish(nullptr, 0, out, s);
-  const int64_t t256 = (M + 255) / 256 * ((Np + 255) / 256), t128 = (M + 255) / 256 * ((Np + 127) / 128);
-  const bool persistent = M >= 256 && Np >= 256 && Kp % 256 == 0 && 16 * 1024 * (Kp / 64) < (1ll << 32) - 4096;
-  if (persistent && (t256 >= 256 || (Kp >= 2048 && t256 > 128) || (Kp >= 1024 && t256 > 192))) {
-    const GemmArgs a = scaled_args(rows, Bp, M, Kp, Np, 256, 256);
-    launch_dma16<OP, 256>(a, o, std::min<int64_t>(t256, cus), s);
-  } else if (persistent && Kp >= 1024 && t128 > 128 && t128 <= 256) {
-    const GemmArgs a = scaled_args(rows, Bp, M, Kp, Np, 256, 128);
-    launch_dma16<OP, 128>(a, o, std::min<int64_t>(t128, cus), s);
+  const TilePlan plan = tile_plan(OP == kGradTerms, M, Np, Kp, cus);
+  if (plan.tiles > 0x7fffffff) return fail(VT_EUNSUPPORTED, "grid of %lld tiles too large", (long long)plan.tiles);
+  if (plan.ks > 1) {
+    if (int rc = scr.take(kPartials, (size_t)plan.ks * M * Np * sizeof(int32_t), &w)) return rc;
+    const int64_t kc = Kp / plan.ks;
+    Problem sl = q;
+    sl.K = kc;
+    sl.batch = plan.ks;
+    sl.sa = kc;
+    sl.sb = kc / 64 * 1024;
+    sl.C = (int32_t *)w;
+    sl.ldc = Np;
+    sl.sc = M * Np;
+    if (int rc = launch_mfma_tiles<128, 128, true>(sl, s, cus)) return rc;
+    return launch_finish((const int32_t *)w, plan.ks, out, s);
+  }
+  const GemmArgs a = scaled_args(rows, Bp, M, Kp, Np, plan.bm, plan.bn);
+  const bool short_k = Kp <= 128;
+  if (plan.persistent) {
+    const int64_t wgs = std::min<int64_t>(plan.tiles, cus);
+    if (plan.bn == 256) launch_dma16<OP, 256>(a, o, wgs, s);
+    else launch_dma16<OP, 128>(a, o, wgs, s);
   } else {
-    const int ks = mfma_k_split<128, 128>(q);
-    if (ks > 1) {
-      if (int rc = scr.take(kPartials, (size_t)ks * M * Np * sizeof(int32_t), &w)) return rc;
-      const int64_t kc = Kp / ks;
-      Problem sl = q;
-      sl.K = kc;
-      sl.batch = ks;
-      sl.sa = kc;
-      sl.sb = kc / 64 * 1024;
-      sl.C = (int32_t *)w;
-      sl.ldc = Np;
-      sl.sc = M * Np;
-      if (int rc = launch_mfma_tiles<128, 128, true>(sl, s, cus)) return rc;
-      return launch_finish((const int32_t *)w, ks, out, s);
-    }
-    const int64_t half = (M + 63) / 64 * ((Np + 127) / 128), full = (M + 127) / 128 * ((Np + 127) / 128);
-    const bool short_k = Kp <= 128;
-    if (full > 0x7fffffff) return fail(VT_EUNSUPPORTED, "grid of %lld tiles too large", (long long)full);
-    if (half <= kHalfTileMaxWgs) {
-      const GemmArgs a = scaled_args(rows, Bp, M, Kp, Np, 64, 128);
-      if (short_k) hipLaunchKernelGGL((gemm_mfma_kernel<64, 128, 1, false, true, false, true, ScaledTile<OP>>), dim3((unsigned)half), dim3(256), 0, s, a, out);
-      else hipLaunchKernelGGL((gemm_mfma_kernel<64, 128, 1, false, false, false, true, ScaledTile<OP>>), dim3((unsigned)half), dim3(256), 0, s, a, out);
+    const dim3 grid((unsigned)plan.tiles);
+    if (plan.bm == 64) {
+      if (short_k) hipLaunchKernelGGL((gemm_mfma_kernel<64, 128, 1, false, true, false, true, ScaledTile<OP>>), grid, dim3(256), 0, s, a, out);
+      else hipLaunchKernelGGL((gemm_mfma_kernel<64, 128, 1, false, false, false, true, ScaledTile<OP>>), grid, dim3(256), 0, s, a, out);
     } else {
-      const GemmArgs a = scaled_args(rows, Bp, M, Kp, Np, 128, 128);
-      if (short_k) hipLaunchKernelGGL((gemm_mfma_kernel<128, 128, 1, false, true, false, true, ScaledTile<OP>>), dim3((unsigned)full), dim3(256), 0, s, a, out);
-      else hipLaunchKernelGGL((gemm_mfma_kernel<128, 128, 1, false, false, false, true, ScaledTile<OP>>), dim3((unsigned)full), dim3(256), 0, s, a, out);
+      if (short_k) hipLaunchKernelGGL((gemm_mfma_kernel<128, 128, 1, false, true, false, true, ScaledTile<OP>>), grid, dim3(256), 0, s, a, out);
+      else hipLaunchKernelGGL((gemm_mfma_kernel<128, 128, 1, false, false, false, true, ScaledTile<OP>>), grid, dim3(256), 0, s, a, out);
     }
   }
   VT_HIP_CHECK(hipGetLastError());
