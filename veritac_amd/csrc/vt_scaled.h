@@ -371,8 +371,9 @@ struct ScaledOut {
 // Two floats as 16-bit elements, the first in the low half.
 __device__ __forceinline__ uint32_t pack16(float a, float b, int type) {
   typedef __bf16 v2b __attribute__((ext_vector_type(2)));
-  if (type == VT_TYPE_BF16) return __builtin_bit_cast(uint32_t, v2b{(__bf16)a, (__bf16)b});
-  return __builtin_bit_cast(uint32_t, v2h{(_Float16)a, (_Float16)b});
+  const uint32_t bf = __builtin_bit_cast(uint32_t, v2b{(__bf16)a, (__bf16)b});
+  const uint32_t hf = __builtin_bit_cast(uint32_t, v2h{(_Float16)a, (_Float16)b});
+  return type == VT_TYPE_BF16 ? bf : hf;
 }
 
 __device__ __forceinline__ float from16(uint32_t bits, int type) {
@@ -405,31 +406,28 @@ struct ScaledTile : ScaledOut {
 
   __device__ __forceinline__ int to16() const { return OP == kGradTerms ? VT_TYPE_F16 : type; }
 
-  // `count` (at most 8) elements to y[at ..].
-  __device__ __forceinline__ void store8(int64_t at, const float (&v)[8], int count, int to) const {
+  // 8 elements to y[at ..].
+  __device__ __forceinline__ void store8(int64_t at, const float (&v)[8], int to) const {
     if (to == VT_TYPE_F32) {
       float *y = (float *)Y + at;
-      if (count >= 8) {
-        __builtin_nontemporal_store(v4f{v[0], v[1], v[2], v[3]}, (v4f_any *)y);
-        __builtin_nontemporal_store(v4f{v[4], v[5], v[6], v[7]}, (v4f_any *)(y + 4));
-      } else {
-#pragma unroll
-        for (int e = 0; e < 7; ++e)
-          if (e < count) y[e] = v[e];
-      }
+      __builtin_nontemporal_store(v4f{v[0], v[1], v[2], v[3]}, (v4f_any *)y);
+      __builtin_nontemporal_store(v4f{v[4], v[5], v[6], v[7]}, (v4f_any *)(y + 4));
     } else {
-      uint16_t *y = (uint16_t *)Y + at;
-      uint32_t w[4];
+      v4i w;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) w[i] = pack16(v[2 * i], v[2 * i + 1], to);
-      if (count >= 8) {
-        __builtin_nontemporal_store(v4i{(int)w[0], (int)w[1], (int)w[2], (int)w[3]}, (v4i_any *)y);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 7; ++e)
-          if (e < count) y[e] = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
-      }
+      for (int i = 0; i < 4; ++i) w[i] = (int)pack16(v[2 * i], v[2 * i + 1], to);
+      __builtin_nontemporal_store(w, (v4i_any *)((uint16_t *)Y + at));
     }
+  }
+  // `count` (any) of them.
+  __device__ __forceinline__ void store8(int64_t at, const float (&v)[8], int count, int to) const {
+    if (count >= 8) return store8(at, v, to);
+#pragma unroll
+    for (int e = 0; e < 7; ++e)
+      if (e < count) {
+        if (to == VT_TYPE_F32) ((float *)Y)[at + e] = v[e];
+        else ((uint16_t *)Y)[at + e] = (uint16_t)pack16(v[e], 0.0f, to);
+      }
   }
 
   // 8 elements of dh from column j, zero past the last.
@@ -480,18 +478,24 @@ struct ScaledTile : ScaledOut {
   // is unrolled): this code runs once per tile, and a short call waits for it
   // to be fetched (unrolled, the gradient's kernel of 18 KB took 11 us for one
   // slice). Every strip's dh is loaded one strip ahead, before the stores that
-  // it would otherwise wait for (both count in vmcnt, in order). Rows outside
-  // [row_min, row_max) and packed columns below col_min are not stored.
+  // it would otherwise wait for (both count in vmcnt, in order). Rows past
+  // row_max and columns past the last are not stored; a wave that has none of
+  // those runs without their branches (with them an iteration took 550 cycles,
+  // and the epilogue of the gradient's kernel 6.5 us). `early`: the row
+  // normalisers of the wave's first and second 64 rows, when they were loaded
+  // before.
   template <int MI, int ROWS, int WP, class WRITE, class SWZ>
-  __device__ __forceinline__ void strips(WRITE write, SWZ swz, int row0, int col0, int row_min, int row_max, int col_min,
-                                         int lane, const LDS_AS int8_t *lds) const {
+  __device__ __forceinline__ void strips(WRITE write, SWZ swz, int row0, int col0, int row_max, int lane,
+                                         const LDS_AS int8_t *lds, const float *early = nullptr) const {
     constexpr int LPR = WP / P / 8, RPI = 64 / LPR, IT = ROWS / RPI;   // lanes per row, rows at a time, times
     static_assert(IT >= 1 && MI * ROWS <= 128, "whole iterations; two registers hold the rows' scales");
     const int j8 = 8 * (lane % LPR), lr = lane / LPR;
     const int lp = P == 1 ? j8 : (j8 >> 5) * 64 + (j8 & 31);   // the lane's first packed column, less col0
     const int pc = col0 + lp, j = (P == 1 ? col0 : col0 / 2) + j8;
     const int count = OP == kGradTerms ? 8 : N - j;
-    const bool cols = pc >= col_min && pc < Np && count > 0;
+    const bool cols = pc < Np && count > 0;
+    const bool whole = __builtin_amdgcn_readfirstlane(
+        row0 + MI * ROWS <= row_max && (P == 1 ? col0 + WP : col0 / 2 + WP / 2) <= N && col0 + WP <= Np);
     float s0[8], s1[P == 2 ? 8 : 1], bias[OP == kLinear ? 8 : 1];
     if constexpr (OP != kGrad) {
       const float *m = meta + min(pc, Np - 8 - (P == 2 ? 32 : 0));
@@ -508,7 +512,7 @@ struct ScaledTile : ScaledOut {
       const int row = min(row0 + 64 * h + lane, M - 1);
       if constexpr (OP != kGrad) tr[h] = t[row];
       if constexpr (OP == kGradTerms) nr[h] = norm[row];
-      if constexpr (OP == kGrad) nr[h] = norm ? 1.0f / norm[row] : 1.0f;
+      if constexpr (OP == kGrad) nr[h] = early[h];
     }
     D8 d[OP == kGradTerms ? IT : 1], ahead[OP == kGradTerms ? IT : 1];
     auto load_d = [&](int mi) {
@@ -530,7 +534,7 @@ struct ScaledTile : ScaledOut {
         if (mi == decltype(i)::value) write(i);
       }, std::make_integer_sequence<int, MI>());
       const bool second = MI * ROWS > 64 && mi * ROWS >= 64;
-#pragma unroll (IT > 4 ? 2 : IT)
+#pragma unroll (IT > 4 ? 4 : IT)
       for (int it = 0; it < IT; ++it) {
         const int r = it * RPI + lr, rel = mi * ROWS + r, row = row0 + rel;
         const LDS_AS int8_t *at = lds + r * (4 * WP);
@@ -557,21 +561,23 @@ struct ScaledTile : ScaledOut {
             pair(a, u, t_row, s0[e], s1[e], OP == kGradTerms ? d_value(d[it], e) * n_row : 0.0f, v[e], v2[e]);
           }
         }
-        if (!cols || row < row_min || row >= row_max) continue;
         if constexpr (OP == kGradTerms) {
+          if (!whole && (!cols || row >= row_max)) continue;
           const int64_t to = (int64_t)row * Np + pc;
-          store8(to, v, 8, VT_TYPE_F16);
-          store8(to + 32, v2, 8, VT_TYPE_F16);
+          store8(to, v, VT_TYPE_F16);
+          store8(to + 32, v2, VT_TYPE_F16);
           if (lo) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
               v[e] -= (float)(_Float16)v[e];
               v2[e] -= (float)(_Float16)v2[e];
             }
-            store8(to + lo, v, 8, VT_TYPE_F16);
-            store8(to + lo + 32, v2, 8, VT_TYPE_F16);
+            store8(to + lo, v, VT_TYPE_F16);
+            store8(to + lo + 32, v2, VT_TYPE_F16);
           }
-        } else {
+        } else if (whole) {
+          store8((int64_t)row * ldy + j, v, type);
+        } else if (cols && row < row_max) {
           store8((int64_t)row * ldy + j, v, count, type);
         }
       }
@@ -583,8 +589,8 @@ struct ScaledTile : ScaledOut {
   // strips' swizzle is store_strip16_lds' (distinct banks for an instruction's
   // writes).
   template <int G, int MI, int NI, class ACC>
-  __device__ __forceinline__ void blocks16(const ACC (&acc)[MI][NI], int row0, int col0, int row_min, int col_min, int lane,
-                                           LDS_AS int8_t *lds) const {
+  __device__ __forceinline__ void blocks16(const ACC (&acc)[MI][NI], int row0, int col0, int lane, LDS_AS int8_t *lds,
+                                           const float *early) const {
     const int g = lane >> 4, c = lane & 15;
     strips<MI / G, 16 * G, NI * 16>(
         [&](auto strip) __attribute__((always_inline)) {
@@ -598,7 +604,7 @@ struct ScaledTile : ScaledOut {
                                                        ((((ni ^ g) << 2) + (c >> 2)) << 4) + (c & 3) * 4) =
                     acc[strip * G + i][ni][e];
         },
-        [](int row) { return ((row >> 2) & 3) << 2; }, row0, col0, row_min, M, col_min, lane, lds);
+        [](int row) { return ((row >> 2) & 3) << 2; }, row0, col0, M, lane, lds, early);
   }
 
   // Rows [r0, r0 + 16) of `W` output columns from out0 leave the wave's LDS, in
@@ -766,7 +772,7 @@ struct ScaledTile : ScaledOut {
               *(LDS_AS int32_t *)(lds + (8 * (e >> 2) + 4 * g + (e & 3)) * 256 + ((((ni ^ g) << 3) + (c >> 2)) << 4) +
                                   (c & 3) * 4) = acc[mi][ni][e];
         },
-        [](int row) { return ((row >> 2) & 1) << 3; }, row0, col0, 0, M, 0, lane, lds);
+        [](int row) { return ((row >> 2) & 1) << 3; }, row0, col0, M, lane, lds);
   }
 
   // One element: the sums of packed columns pc (and, of a pair, pc + 32) of a
@@ -1141,9 +1147,9 @@ __device__ __forceinline__ void put_terms(_Float16 *y, int64_t lo, const float (
 // the maximum and the rounding (0: longer rows, read twice). Else only the
 // normaliser of a gated product's terms, from the row's largest |dh|, its
 // scale and the weights' bound: |q| <= 128, |act(g)| <= |g| and |act'| <= 1.13.
-template <int TYPE, bool LINEAR, int NC>
-__global__ __launch_bounds__(256) void row_terms_kernel(TermArgs p) {
-  __shared__ uint32_t red[4];
+template <int TYPE, bool LINEAR, int THREADS, int NC>
+__global__ __launch_bounds__(THREADS) void row_terms_kernel(TermArgs p) {
+  __shared__ uint32_t red[THREADS / 64];
   typedef typename Elem<TYPE>::T T;
   const int64_t row = blockIdx.x;
   const T *d = (const T *)p.D + row * p.ldd;
@@ -1152,7 +1158,7 @@ __global__ __launch_bounds__(256) void row_terms_kernel(TermArgs p) {
   uint32_t top = 0;
   if constexpr (!LINEAR) {
     if (p.pad.Q)
-      for (int pos = tid * 16; pos < p.pad.Kp; pos += 4096) pad_piece(p.pad, row, pos);
+      for (int pos = tid * 16; pos < p.pad.Kp; pos += THREADS * 16) pad_piece(p.pad, row, pos);
   }
   auto load = [&](int pos, float (&x)[16]) {
     load16<TYPE>(d, pos, p.N, x);
@@ -1171,11 +1177,11 @@ __global__ __launch_bounds__(256) void row_terms_kernel(TermArgs p) {
   };
   if constexpr (NC > 0) {
 #pragma unroll
-    for (int i = 0; i < NC; ++i) load((tid + 256 * i) * 16, v[i]);
+    for (int i = 0; i < NC; ++i) load((tid + THREADS * i) * 16, v[i]);
   } else {
-    for (int pos = tid * 16; pos < p.N; pos += 4096) load(pos, v[0]);
+    for (int pos = tid * 16; pos < p.N; pos += THREADS * 16) load(pos, v[0]);
   }
-  top = block_max<256>(top, red);
+  top = block_max<THREADS>(top, red);
   float bound = __uint_as_float(top);
   if (!LINEAR && top < kInfBits) bound *= fabsf(p.t[row]) * p.meta[2 * (int64_t)p.Np] * (128.0f * 1.13f);
   float norm = normaliser(bound);
@@ -1192,9 +1198,9 @@ __global__ __launch_bounds__(256) void row_terms_kernel(TermArgs p) {
     };
     if constexpr (NC > 0) {
 #pragma unroll
-      for (int i = 0; i < NC; ++i) put((tid + 256 * i) * 16, v[i]);
+      for (int i = 0; i < NC; ++i) put((tid + THREADS * i) * 16, v[i]);
     } else {
-      for (int pos = tid * 16; pos < p.Np; pos += 4096) {
+      for (int pos = tid * 16; pos < p.Np; pos += THREADS * 16) {
         load(pos, v[0]);
         put(pos, v[0]);
       }
@@ -1260,6 +1266,12 @@ __global__ __launch_bounds__(256, 1) void grad_dma_kernel(GradArgs p, ScaledTile
   const int gm = min(p.tiles_m - first_m, p.group_m), within = tile - gid * group;
   const int m0 = (first_m + within % gm) * BM, n0 = (within / gm) * 256;
 
+  // The normalisers of the wave's rows, loaded ahead of everything.
+  float norms[2] = {1.0f, 1.0f};
+  if (out.norm) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) norms[h] = out.norm[min(m0 + wm * 128 + 64 * h + lane, p.M - 1)];
+  }
   const int kbt = p.Kp / 64;
   const uint32_t lds0 = (uint32_t)(uintptr_t)(LDS_AS int8_t *)smem;
   uint32_t a_lane[DA], b_lane[DB];
@@ -1388,7 +1400,10 @@ __global__ __launch_bounds__(256, 1) void grad_dma_kernel(GradArgs p, ScaledTile
   if (p.splits > 1) out.Y = (float *)out.Y + (int64_t)split * p.M * p.Kp;
   constexpr int STRIP = 64 * WTN * 4;   // 64 of a wave's rows
   static_assert(4 * STRIP <= (int)sizeof(smem), "the stages hold every wave's strip");
-  out.blocks16<4>(acc, m0 + wm * 128, n0 + wn * WTN, 0, 0, lane, (LDS_AS int8_t *)smem + wave * STRIP);
+  float unit[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) unit[h] = out.norm ? 1.0f / norms[h] : 1.0f;
+  out.blocks16<4>(acc, m0 + wm * 128, n0 + wn * WTN, lane, (LDS_AS int8_t *)smem + wave * STRIP, unit);
 }
 
 // dx from the partial sums [slices][M][Kp] of a split contraction, over the
@@ -1757,12 +1772,15 @@ template <int TYPE, bool LINEAR>
 void launch_row_terms_typed(const TermArgs &a, hipStream_t s) {
   const dim3 grid((unsigned)a.M);
   if constexpr (LINEAR) {
-    if (a.Np <= 4096) hipLaunchKernelGGL((row_terms_kernel<TYPE, true, 1>), grid, dim3(256), 0, s, a);
-    else if (a.Np <= 8192) hipLaunchKernelGGL((row_terms_kernel<TYPE, true, 2>), grid, dim3(256), 0, s, a);
-    else if (a.Np <= 16384) hipLaunchKernelGGL((row_terms_kernel<TYPE, true, 4>), grid, dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((row_terms_kernel<TYPE, true, 0>), grid, dim3(256), 0, s, a);
+    if (a.Np <= 1024) hipLaunchKernelGGL((row_terms_kernel<TYPE, true, 64, 1>), grid, dim3(64), 0, s, a);
+    else if (a.Np <= 4096) hipLaunchKernelGGL((row_terms_kernel<TYPE, true, 256, 1>), grid, dim3(256), 0, s, a);
+    else if (a.Np <= 8192) hipLaunchKernelGGL((row_terms_kernel<TYPE, true, 256, 2>), grid, dim3(256), 0, s, a);
+    else if (a.Np <= 16384) hipLaunchKernelGGL((row_terms_kernel<TYPE, true, 256, 4>), grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((row_terms_kernel<TYPE, true, 256, 0>), grid, dim3(256), 0, s, a);
+  } else if (a.N <= 1024) {
+    hipLaunchKernelGGL((row_terms_kernel<TYPE, false, 64, 0>), grid, dim3(64), 0, s, a);
   } else {
-    hipLaunchKernelGGL((row_terms_kernel<TYPE, false, 0>), grid, dim3(256), 0, s, a);
+    hipLaunchKernelGGL((row_terms_kernel<TYPE, false, 256, 0>), grid, dim3(256), 0, s, a);
   }
 }
 
