@@ -552,3 +552,59 @@ def test_offsets_past_32_bits(dev):
     assert torch.equal(z.contiguous(), scaled.linear_grad(dc, W))
     scaled.gated_grad(y, r, G, out=z)
     assert torch.equal(z.contiguous(), scaled.gated_grad(dc, r, G))
+
+
+# --- refusals and the example -----------------------------------------------------
+
+def test_mismatches_are_refused(dev):
+    rng = np.random.default_rng(1)
+    w, s = weights(rng, 96, 40)
+    W, G = packed(dev, w, s), packed_pair(dev, w, s, w, s)
+    x, d = torch.zeros(3, 96, device=dev), torch.zeros(3, 40, device=dev)
+    r = scaled.quantize_rows(x)
+    leaf = torch.zeros(3, 96, device=dev, requires_grad=True)
+    for call, what in ((lambda: scaled.linear(x[:, :95], W), "95 columns"),
+                       (lambda: scaled.linear(x, G), "pack_linear"), (lambda: scaled.gated(x, W), "pack_gated"),
+                       (lambda: scaled.linear(x.cpu(), W), "no CPU path"),
+                       (lambda: scaled.linear(x.double(), W), "float32"),
+                       (lambda: scaled.linear(x, W, out_dtype=torch.int32), "type must be"),
+                       (lambda: scaled.linear(r, W), "need out_dtype"),
+                       (lambda: scaled.linear(x.t().contiguous().t(), W), "unit stride"),
+                       (lambda: scaled.linear(x[:1].expand(3, 96), W), "overlapping rows"),
+                       (lambda: scaled.linear(x, W, out=torch.zeros(3, 41, device=dev)), "out must be"),
+                       (lambda: scaled.linear(x, W, out=torch.zeros(3, 40, device=dev), out_dtype=torch.float16), "out must be"),
+                       (lambda: scaled.linear(x, W, out=torch.zeros(3, 40)), "out must be"),
+                       (lambda: scaled.linear(x, W, out=x.view(-1)[:120].view(3, 40)), "overlaps"),
+                       (lambda: scaled.linear_grad(d[:, :39], W), "39 columns"),
+                       (lambda: scaled.gated_grad(d[:2], r, G), "dh is 2 x 40"),
+                       (lambda: scaled.gated_grad(d, x, G), "QuantRows"),
+                       (lambda: scaled.linear(leaf, W, out=d), "neither out nor stream"),
+                       (lambda: scaled.pack_linear(up(w, dev), up(s, dev)[:39]), "scale of w"),
+                       (lambda: scaled.pack_linear(up(w, dev), up(s, dev), up(s, dev).double()), "bias"),
+                       (lambda: scaled.pack_gated(up(w, dev), up(s, dev), up(w[:95], dev), up(s, dev)), "w_up has shape")):
+        with pytest.raises(Exception, match=what):
+            call()
+    assert torch.equal(scaled.linear(x, W), torch.zeros(3, 40, device=dev))     # and nothing is left broken
+
+
+def test_a_feed_forward_block_in_use(dev):
+    """The example: int8 rounding leaves the block within a few percent of float32 (each of the
+    three roundings of operands to 127 steps of their largest is about 1 % of their size), and an
+    adapter trains through it."""
+    from veritac_amd.specializations.hip_gemm import feed_forward
+    got = feed_forward.main()
+    assert got["prefill"] < 0.06 and got["decode"] < 0.06
+    assert got["loss_last"] < 0.2 * got["loss_first"]
+
+
+def test_captured_blocks_replay_beside_eager_calls(dev):
+    from veritac_amd.specializations.hip_gemm import feed_forward
+    w = [torch.randn(a, b, device=dev) / a**0.5 for a, b in ((512, 1400), (512, 1400), (1400, 512))]
+    block = feed_forward.FeedForward.from_float(*w, act="gelu")
+    step = block.capture(torch.zeros(5, 512, device=dev, dtype=torch.float16))
+    for i in range(4):
+        x = torch.randn(5, 512, device=dev, dtype=torch.float16)
+        want = block(x)
+        step.x.copy_(x)
+        step.replay()
+        assert torch.equal(step.y, want), i

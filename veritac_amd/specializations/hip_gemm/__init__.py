@@ -5,6 +5,7 @@ Import the submodules explicitly (none loads the native library at import):
   runner      benchmark_gemm (the reference runner's benchmark dict)
   inputs      deterministic generators and the benchmark configurations
   scaled      linear layers and gated products on int8 weights and rows with scales
+  feed_forward  a gated feed-forward block of the scaled operators (an example to run)
   replay      Gemmini command streams executed on the GPU
   loopnest    loop-nest JSON emitted as HIP kernels, compiled at run time
   provenance  hardware profile and hash-bound run reports
