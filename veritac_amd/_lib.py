@@ -161,6 +161,8 @@ def _declare(lib):
 def load_library():
     """Load (once) and return the native library; raise HipGemmError if absent."""
     global _lib
+    if _lib is not None:
+        return _lib
     with _lock:
         if _lib is not None:
             return _lib

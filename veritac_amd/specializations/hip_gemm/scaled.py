@@ -193,6 +193,9 @@ def quantize_weight(w, *, stream=None):
 def _rows(name, x):
     """x [..., k] as (a matrix of unit-stride rows, its leading shape)."""
     torch = _torch()
+    # Contiguous matrices on a GPU, the usual call, need no more than this.
+    if type(x) is torch.Tensor and x.is_cuda and x.dtype in _types() and x.dim() == 2 and x.is_contiguous():
+        return x, x.shape[:1]
     if not isinstance(x, torch.Tensor) or x.dtype not in _types():
         raise HipGemmError("%s must be a float32, float16 or bfloat16 torch tensor" % name)
     if x.dim() < 1:
@@ -245,9 +248,13 @@ def _check_weight(W, pair, device, k):
         raise HipGemmError("rows have %d columns, the weights take %d" % (k, W.k))
 
 
-def _output(name, out, m, cols, lead, dtype, device):
-    """(matrix to write, tensor to return, whether it was allocated here)."""
+def _output(name, out, m, cols, lead, dtype, device, like=None):
+    """(matrix to write, tensor to return, whether it was allocated here). `like`:
+    a tensor on the device, whose new_empty takes less time where the type is its."""
     torch = _torch()
+    if out is None and like is not None and like.dtype is dtype:
+        out = like.new_empty((*lead, cols))
+        return out, out, True
     if dtype not in _types():
         raise HipGemmError("%s type must be float32, float16 or bfloat16 (got %s)" % (name, dtype))
     if out is None:
@@ -286,13 +293,14 @@ def _forward(x, W, pair, act, out_dtype, out, stream):
         if out_dtype is None:
             out_dtype = x.dtype if out is None else out.dtype
     m = data.shape[0]
-    o2, ret, allocated = _output("output", out, m, W.n, lead, out_dtype, data.device)
+    device = data.device
+    o2, ret, allocated = _output("output", out, m, W.n, lead, out_dtype, device, data)
     if stream is None:
-        stream = _current_stream(data.device)
+        stream = _current_stream(device)
     elif allocated:
         _keep_for_stream(ret, stream)
     lib = _lib.load_library()
-    ldy = o2.stride(-2) if o2.dim() == 2 and m > 1 and W.n else max(W.n, 1)
+    ldy = max(W.n, 1) if allocated or o2.dim() != 2 or m < 2 or not W.n else o2.stride(-2)
     if pair:
         _lib.check(lib.vt_scaled_gated(data.data_ptr(), kind, _pitch(data), scale, m, k,
                                        W.data.data_ptr(), W.meta.data_ptr(), W.n, act,
@@ -350,7 +358,7 @@ def linear_grad(dy, W, *, out=None, stream=None):
     if d.shape[1] != W.n:
         raise HipGemmError("dy has %d columns, the weights give %d" % (d.shape[1], W.n))
     m = d.shape[0]
-    o2, ret, allocated = _output("gradient", out, m, W.k, lead, dy.dtype, d.device)
+    o2, ret, allocated = _output("gradient", out, m, W.k, lead, dy.dtype, d.device, d)
     if stream is None:
         stream = _current_stream(d.device)
     elif allocated:
@@ -378,7 +386,7 @@ def gated_grad(dh, rows, W, *, act="silu", out=None, stream=None):
     if d.shape[1] != W.n or m != rows.data.shape[0]:
         raise HipGemmError("dh is %d x %d, the rows and weights give %d x %d"
                            % (m, d.shape[1], rows.data.shape[0], W.n))
-    o2, ret, allocated = _output("gradient", out, m, W.k, lead, dh.dtype, d.device)
+    o2, ret, allocated = _output("gradient", out, m, W.k, lead, dh.dtype, d.device, d)
     if stream is None:
         stream = _current_stream(d.device)
     elif allocated:
