@@ -310,28 +310,30 @@ __global__ __launch_bounds__(256) void pack_bound_kernel(ScaledPackArgs p) {
 
 // 2^32 / (1 + exp(-z)): the factor keeps a small value clear of the smallest
 // float32 exponents (which the exponential and the reciprocal drop) until it
-// is multiplied by g. From 2^60 on, exp(z) is all of 1 + exp(z).
+// is multiplied by g. From 2^60 on, exp(z) is all of 1 + exp(z). (fmed3 clamps
+// in one instruction; a NaN reaches the result by its factor g.)
 constexpr float kLogisticUnit = 0x1p-32f;
 __device__ __forceinline__ float logistic32(float z) {
-  const float e = __builtin_amdgcn_exp2f(fminf(z * 1.4426950408889634f, 60.0f) + 32.0f);
-  return e * __builtin_amdgcn_rcpf(1.0f + e * kLogisticUnit);
+  const float e = __builtin_amdgcn_exp2f(__builtin_amdgcn_fmed3f(fmaf(z, 1.4426950408889634f, 32.0f), -200.0f, 92.0f));
+  return e * __builtin_amdgcn_rcpf(fmaf(e, kLogisticUnit, 1.0f));
 }
 
 // act(g), and its slope. gelu is the tanh form: (1 + tanh z) / 2 is
 // 1 / (1 + exp(-2 z)) with z = c (g + a g^3); past |g| = 16 it is 0 or 1, so g
-// is held there inside (its cube would leave float32's range).
-template <int ACT>
+// is held there inside (its cube would leave float32's range). TERMS: for
+// gradient terms, which are rounded to steps of 2^-24 of their row's bound or
+// more, nothing has to be kept of a value below 2^-126.
+template <int ACT, bool TERMS>
 __device__ __forceinline__ float act_of(float g, float &slope) {
-  if (ACT == VT_ACT_SILU) {
-    const float p32 = logistic32(g), p = p32 * kLogisticUnit;
-    slope = p * (1.0f + g * (1.0f - p));
-    return g * p32 * kLogisticUnit;
-  }
   const float c = 0.7978845608028654f, a = 0.044715f;
-  const float h = fminf(fmaxf(g, -16.0f), 16.0f);
-  const float p32 = logistic32(2.0f * c * (h + a * h * h * h)), p = p32 * kLogisticUnit;
-  slope = p + h * 2.0f * p * (1.0f - p) * c * (1.0f + 3.0f * a * h * h);
-  return g * p32 * kLogisticUnit;
+  const float h = ACT == VT_ACT_GELU ? __builtin_amdgcn_fmed3f(g, -16.0f, 16.0f) : g;
+  const float hh = h * h, z = ACT == VT_ACT_GELU ? 2.0f * c * (h * fmaf(a, hh, 1.0f)) : g;
+  const float p32 = TERMS ? 0.0f : logistic32(z);
+  const float p = TERMS ? __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.4426950408889634f))
+                        : p32 * kLogisticUnit;
+  const float dz = ACT == VT_ACT_GELU ? 2.0f * c * fmaf(3.0f * a, hh, 1.0f) : 1.0f;
+  slope = p * fmaf(h * dz, 1.0f - p, 1.0f);
+  return TERMS ? g * p : g * p32 * kLogisticUnit;
 }
 
 // Row normaliser of 16-bit gradient terms: the power of two that takes a bound
@@ -387,12 +389,23 @@ struct ScaledTile : ScaledOut {
   static constexpr int OE = OP == kGradTerms ? 2 : E;   // bytes of what tile16 writes
   static constexpr int P = OP == kGated || OP == kGradTerms ? 2 : 1;   // projections taken together
 
+  // f(the activation, at compile time): one branch around many pairs. A branch
+  // for each kept a wave at one pair's chain of dependent instructions (a tile's
+  // epilogue 10.4 us, with gradient terms 22).
+  template <class F>
+  __device__ __forceinline__ void by_act(F &&f) const {
+    if constexpr (P == 1) f(std::integral_constant<int, VT_ACT_SILU>());
+    else if (act == VT_ACT_SILU) f(std::integral_constant<int, VT_ACT_SILU>());
+    else f(std::integral_constant<int, VT_ACT_GELU>());
+  }
+
   // g and u of a pair of sums -> h, or (kGradTerms) the terms of Wg and Wu.
+  template <int ACT>
   __device__ __forceinline__ void pair(int32_t ag, int32_t au, float t_row, float sg, float su, float d, float &first,
                                        float &second) const {
     const float g = (float)ag * t_row * sg, u = (float)au * t_row * su;
     float slope;
-    const float a = act == VT_ACT_SILU ? act_of<VT_ACT_SILU>(g, slope) : act_of<VT_ACT_GELU>(g, slope);
+    const float a = act_of<ACT, OP == kGradTerms>(g, slope);
     if constexpr (OP == kGated) {
       first = a * u;
     } else {
@@ -549,18 +562,21 @@ struct ScaledTile : ScaledOut {
         if constexpr (OP != kGrad) t_row = __shfl(second ? tr[1] : tr[0], rel & 63);
         if constexpr (OP == kGradTerms || OP == kGrad) n_row = __shfl(second ? nr[1] : nr[0], rel & 63);
         float v[8], v2[P == 2 ? 8 : 1];
+        by_act([&](auto kind) __attribute__((always_inline)) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int a = e < 4 ? a0[e & 3] : a1[e & 3];
-          if constexpr (OP == kLinear) {
-            v[e] = (float)a * t_row * s0[e] + bias[e];
-          } else if constexpr (OP == kGrad) {
-            v[e] = __builtin_bit_cast(float, a) * n_row;
-          } else {
-            const int u = e < 4 ? u0[e & 3] : u1[e & 3];
-            pair(a, u, t_row, s0[e], s1[e], OP == kGradTerms ? d_value(d[it], e) * n_row : 0.0f, v[e], v2[e]);
+          for (int e = 0; e < 8; ++e) {
+            const int a = e < 4 ? a0[e & 3] : a1[e & 3];
+            if constexpr (OP == kLinear) {
+              v[e] = (float)a * t_row * s0[e] + bias[e];
+            } else if constexpr (OP == kGrad) {
+              v[e] = __builtin_bit_cast(float, a) * n_row;
+            } else {
+              const int u = e < 4 ? u0[e & 3] : u1[e & 3];
+              pair<decltype(kind)::value>(a, u, t_row, s0[e], s1[e], OP == kGradTerms ? d_value(d[it], e) * n_row : 0.0f,
+                                          v[e], v2[e]);
+            }
           }
-        }
+        });
         if constexpr (OP == kGradTerms) {
           if (!whole && (!cols || row >= row_max)) continue;
           const int64_t to = (int64_t)row * Np + pc;
@@ -680,8 +696,8 @@ struct ScaledTile : ScaledOut {
     constexpr int W = NB * 16, PITCH = W * OE, RC = PITCH / 16;
     const int g = lane >> 4, c = lane & 15;
     float s[NI], bias[OP == kLinear ? NI : 1];
-    v4f tr[OP == kGradTerms ? 2 : MI], nr[2];
-    auto trow = [](int mi) { return OP == kGradTerms ? mi & 1 : mi; };
+    v4f tr[OP == kGradTerms ? 1 : MI], nr;
+    auto trow = [](int mi) { return OP == kGradTerms ? 0 : mi; };
 #pragma unroll
     for (int ni = 0; ni < NI; ++ni) {
       s[ni] = meta[col0 + ni * 16 + c];
@@ -691,21 +707,23 @@ struct ScaledTile : ScaledOut {
 #pragma unroll
       for (int mi = 0; mi < MI; ++mi) tr[mi] = *(const v4f_any *)(t + row0 + mi * 16 + 4 * g);
     }
-    DBits d[2][ND][4];
-    auto load_strip = [&](int mi) {
+    DBits d[ND][4];
+    auto load_scales = [&](int mi) {
       if constexpr (OP == kGradTerms) {
-        tr[mi & 1] = *(const v4f_any *)(t + row0 + mi * 16 + 4 * g);
-        nr[mi & 1] = *(const v4f_any *)(norm + row0 + mi * 16 + 4 * g);
-#pragma unroll
-        for (int b = 0; b < ND; ++b) {
-          const int j = min(col0 / 2 + b * 16 + c, N - 1);
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            d[mi & 1][b][e] = ((const DBits *)D)[(int64_t)(row0 + mi * 16 + 4 * g + e) * ldd + j];
-        }
+        tr[0] = *(const v4f_any *)(t + row0 + mi * 16 + 4 * g);
+        nr = *(const v4f_any *)(norm + row0 + mi * 16 + 4 * g);
       }
     };
-    load_strip(0);
+    auto load_block = [&](int mi, int b) {
+      const int j = min(col0 / 2 + b * 16 + c, N - 1);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) d[b][e] = ((const DBits *)D)[(int64_t)(row0 + mi * 16 + 4 * g + e) * ldd + j];
+    };
+    if constexpr (OP == kGradTerms) {
+      load_scales(0);
+#pragma unroll
+      for (int b = 0; b < ND; ++b) load_block(0, b);
+    }
     auto swz = [](int row) { return (((row >> 2) & 3) * OE) & (RC - 1); };
     int wb[NB];
 #pragma unroll
@@ -716,10 +734,9 @@ struct ScaledTile : ScaledOut {
       store_rows<W>(lds, swz, row0 + mi * 16, OP == kGated ? col0 / 2 : col0, plane, lane, EDGE ? row_min : 0,
                     OP == kGated ? col_min / 2 : col_min);
     };
-#pragma unroll
-    for (int mi = 0; mi < MI; ++mi) {
+    each([&](auto strip) __attribute__((always_inline)) {
+      constexpr int mi = decltype(strip)::value;
       float v[NB][4];
-      if (mi + 1 < MI) load_strip(mi + 1);
       __builtin_amdgcn_sched_barrier(0);
       if constexpr (OP == kLinear) {
 #pragma unroll
@@ -727,21 +744,33 @@ struct ScaledTile : ScaledOut {
 #pragma unroll
           for (int e = 0; e < 4; ++e) v[ni][e] = (float)acc[mi][ni][e] * tr[trow(mi)][e] * s[ni] + bias[ni];
       } else {
+        by_act([&](auto kind) __attribute__((always_inline)) {
 #pragma unroll
-        for (int b = 0; b < NI / 2; ++b) {
-          const int ng = (b >> 1) * 4 + (b & 1);
-          const bool in = OP != kGradTerms || col0 / 2 + b * 16 + c < N;
+          for (int b = 0; b < NI / 2; ++b) {
+            const int ng = (b >> 1) * 4 + (b & 1);
+            const bool in = OP != kGradTerms || col0 / 2 + b * 16 + c < N;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            if constexpr (OP == kGated) {
-              float none;
-              pair(acc[mi][ng][e], acc[mi][ng + 2][e], tr[trow(mi)][e], s[ng], s[ng + 2], 0.0f, v[b][e], none);
-            } else {
-              const float de = in ? d_value(d[mi & 1][b][e]) * nr[mi & 1][e] : 0.0f;
-              pair(acc[mi][ng][e], acc[mi][ng + 2][e], tr[trow(mi)][e], s[ng], s[ng + 2], de, v[ng][e], v[ng + 2][e]);
+            for (int e = 0; e < 4; ++e) {
+              const int32_t ag = acc[mi][ng][e], au = acc[mi][ng + 2][e];
+              if constexpr (OP == kGated) {
+                float none;
+                pair<decltype(kind)::value>(ag, au, tr[trow(mi)][e], s[ng], s[ng + 2], 0.0f, v[b][e], none);
+              } else {
+                const float de = in ? d_value(d[b][e]) * nr[e] : 0.0f;
+                pair<decltype(kind)::value>(ag, au, tr[trow(mi)][e], s[ng], s[ng + 2], de, v[ng][e], v[ng + 2][e]);
+              }
+            }
+            // A block's dh of the next strip takes the registers of this one's, and
+            // four pairs' chains run at a time: more spilled registers.
+            if constexpr (OP == kGradTerms) {
+              __builtin_amdgcn_sched_barrier(0);
+              if constexpr (mi + 1 < MI) {
+                load_block(mi + 1, b);
+                if (b == NI / 2 - 1) load_scales(mi + 1);
+              }
             }
           }
-        }
+        });
       }
       flush(v, mi, 0);
       if constexpr (OP == kGradTerms && E == 4) {
@@ -752,7 +781,7 @@ struct ScaledTile : ScaledOut {
         flush(v, mi, lo);
       }
       __builtin_amdgcn_sched_barrier(0);
-    }
+    }, std::make_integer_sequence<int, MI>());
   }
 
   // Blocks of 32 x 32 sums (element e of lane l: row 8 (e / 4) + 4 (l / 32) +
@@ -791,7 +820,9 @@ struct ScaledTile : ScaledOut {
         const int64_t at = (int64_t)row * ldd + j;
         d = norm[row] * (type == VT_TYPE_F32 ? ((const float *)D)[at] : from16(((const uint16_t *)D)[at], type));
       }
-      pair(a0, a1, t_row, s0, meta[pc + 32], d, first, second);
+      by_act([&](auto kind) __attribute__((always_inline)) {
+        pair<decltype(kind)::value>(a0, a1, t_row, s0, meta[pc + 32], d, first, second);
+      });
       if constexpr (OP == kGated) {
         if (j < N) put((int64_t)row * ldy + j, first, type);
       } else {
