@@ -481,7 +481,8 @@ int vt_gemm_i8_packed(const int8_t *A, const int8_t *Bp, const int32_t *D, int32
  * a 16-byte aligned base and zeros in columns K .. vt_quant_pitch(K) - 1, as
  * vt_quant_rows writes them (then they are used in place). Outputs have any
  * pitch and their elements' alignment; an output may not share memory with an
- * input. M = 0 and empty outputs are no-ops, K = 0 sums are zero.
+ * input. M = 0 and empty outputs are no-ops, K = 0 sums are zero. Sizes: K up
+ * to 131071 (sums of int32), M up to 2^24 - 1.
  *
  * Intermediate rows, sums and terms live in per-stream workspaces, as
  * vt_gemm_i8's do (a call made once on a stream may be captured there).

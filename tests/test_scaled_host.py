@@ -69,6 +69,18 @@ def test_native_refusals(lib, kw):
     assert "vt_scaled_linear" in _lib.last_error()
 
 
+FAR = 1 << 44      # addresses this far apart
+
+
+def many_rows(lib, m):
+    return [linear(lib, M=m, X=FAR, Y=2 * FAR), lib.vt_quant_rows(FAR, F32, 64, 2 * FAR, 128, 3 * FAR, m, 64, None)]
+
+
+def test_more_rows_than_a_launch_takes(lib):
+    # a workgroup per row of up to 256 threads: 2^24 rows would be 2^32 threads
+    assert many_rows(lib, 1 << 24) == [_lib.VT_EINVAL] * 2
+
+
 def test_empty_calls_need_no_device(lib):
     assert linear(lib, M=0, X=None, Y=None) == _lib.VT_OK
     assert linear(lib, N=0, Y=None, B=None) == _lib.VT_OK
@@ -80,6 +92,7 @@ def test_valid_calls_end_without_a_device(lib):
     for kw in ({}, dict(xt=BF16, yt=F16), dict(xt=I8, T=BASE * 5), dict(xt=I8P, ldx=128, T=BASE * 5), dict(K=0, X=None, B=None),
                dict(X=BASE + 4), dict(Y=BASE * 4 + 4, ldy=33)):
         assert linear(lib, **kw) == _lib.VT_ENODEV, kw
+    assert many_rows(lib, (1 << 24) - 1) == [_lib.VT_ENODEV] * 2
 
 
 def test_other_entries_refuse(lib):
