@@ -374,6 +374,21 @@ def test_gradients_on_whole_chip_tiles(dev, m, k, n, dtype):
     ref.check(dx, *ref.gated_grad(d32, q, t, w, s, w2, s2, "silu", dtype != torch.float32), dtype, "gated_grad")
 
 
+# contractions split over workgroups on those tiles, in parts of unequal length
+@pytest.mark.parametrize("m,k,n,dtype", [(2050, 1000, 3000, torch.float32), (2050, 500, 4000, torch.float32),
+                                         (2050, 2000, 4000, torch.float32), (1100, 1025, 8000, torch.bfloat16),
+                                         (2050, 2000, 8000, torch.float16)])
+def test_split_contractions_on_large_tiles(dev, m, k, n, dtype):
+    rng = np.random.default_rng(m + k + n)
+    d, d32 = gradients(rng, m, n, dtype)
+    w, s = weights(rng, k, n, -128)
+    say("linear_grad", m, k, n, dtype)
+    W = packed(dev, w, s)
+    dx = scaled.linear_grad(d.to(dev), W)
+    ref.check(dx, *ref.linear_grad(d32, w, s, dtype != torch.float32), dtype, "linear_grad")
+    assert torch.equal(dx, scaled.linear_grad(d.to(dev), W))      # the sums' order is fixed
+
+
 @pytest.mark.parametrize("dtype,act", [(torch.float32, "gelu"), (torch.bfloat16, "silu")], ids=["f32-gelu", "bf16-silu"])
 @pytest.mark.parametrize("m,k,n", [(4000, 1000, 1947), (2000, 4000, 2011)])
 def test_gated_grad_terms_on_whole_chip_tiles(dev, m, k, n, dtype, act):

@@ -39,10 +39,10 @@ def operands(text):
 
 
 def test_grad_kernels_are_all_there(asm):
-    assert len(names(asm, "grad_dma_kernel")) == 2 and len(names(asm, "scaled_dma16_kernel")) == 12
+    assert len(names(asm, "grad_dma_kernel")) == 3 and len(names(asm, "scaled_dma16_kernel")) == 12
 
 
-@pytest.mark.parametrize("which", range(2))
+@pytest.mark.parametrize("which", range(3))
 def test_mfma_operands_are_two_instructions_old(asm, which):
     code = instructions(asm, names(asm, "grad_dma_kernel")[which])
     mfmas = 0
@@ -65,7 +65,7 @@ def test_mfma_operands_are_two_instructions_old(asm, which):
     assert mfmas == rows // 2      # one slice's two halves, in the loop
 
 
-@pytest.mark.parametrize("which", range(2))
+@pytest.mark.parametrize("which", range(3))
 def test_nothing_else_in_the_loop_waits_for_vector_memory(asm, which):
     code = instructions(asm, names(asm, "grad_dma_kernel")[which])
     at = [i for i, t in enumerate(code) if t.startswith("v_mfma_f32_16x16x32_f16")]
@@ -94,7 +94,7 @@ def test_the_int8_k_loop_is_undisturbed(asm, which):
     m0_belongs_to_dmas(code)
 
 
-@pytest.mark.parametrize("which", range(2))
+@pytest.mark.parametrize("which", range(3))
 def test_accumulators_stay_in_place(asm, which):
     """Between the first and the last MFMA no accumulator is copied or read."""
     code = instructions(asm, names(asm, "grad_dma_kernel")[which])

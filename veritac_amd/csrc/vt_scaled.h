@@ -1275,8 +1275,8 @@ __device__ __forceinline__ void mfma16h_in_place(v4f &acc, const v4i &a, const v
   asm volatile("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(acc) : "v"(a), "v"(b));
 }
 
-// BM x 256 tiles of dx (BM 256: waves of 128 x 128; BM 128: of 128 x 64), one
-// tile per workgroup. A slice is 64 packed columns deep: the terms' rows (128
+// BM x 256 tiles of dx (BM 256: waves of 128 x 128; 128: of 128 x 64; 64: of
+// 64 x 64, two workgroups to a CU), one tile per workgroup. A slice is 64 packed columns deep: the terms' rows (128
 // bytes, 16-byte chunk c of row r at c ^ (r % 8)) and 4 x 4 whole packed tiles,
 // both by DMA into three LDS stages, two slices ahead. A slice is multiplied in
 // two halves of 32; half (s, h) multiplies fragments read in the half before,
@@ -1296,11 +1296,12 @@ __device__ __forceinline__ void mfma16h_in_place(v4f &acc, const v4i &a, const v
 // on 128 x 256 tiles in 381 - 417 (1150 - 1260). The conversions, 10 vector
 // operations per B operand of 32 x 16 weights, issue between the MFMAs: 1.35
 // vector instructions to one. A call of few slices is bound by what surrounds
-// them: 10 us for 100 x 333 over 2432 packed columns.
+// them, which 64-row tiles halve: 100 x 333 over 2432 packed columns in 13.4 us
+// with its terms and sums, on 128-row tiles 16.5.
 template <int BM>
 __global__ __launch_bounds__(256, 1) void grad_dma_kernel(GradArgs p, ScaledTile<kGrad> out) {
-  static_assert(BM == 256 || BM == 128, "256x256 or 128x256 tiles");
-  constexpr int WCOLS = BM == 256 ? 2 : 4, WTN = 256 / WCOLS, MI = 8, NI = WTN / 16;
+  static_assert(BM == 256 || BM == 128 || BM == 64, "256x256, 128x256 or 64x256 tiles");
+  constexpr int WCOLS = BM == 256 ? 2 : 4, WTN = 256 / WCOLS, MI = BM == 64 ? 4 : 8, NI = WTN / 16;
   constexpr int A_BYTES = BM * 128, B_BYTES = 64 * 256, NSTAGE = 3, B_REGION = NSTAGE * A_BYTES;
   constexpr int DA = A_BYTES / 4096, DB = 4, DMAS = DA + DB, FIRST = DMAS / 2;
   __shared__ __attribute__((aligned(1024))) int8_t smem[NSTAGE * (A_BYTES + B_BYTES)];
@@ -1396,7 +1397,8 @@ __global__ __launch_bounds__(256, 1) void grad_dma_kernel(GradArgs p, ScaledTile
     else gb[ni][2 * d + (o % 5 == 4)] = __builtin_bit_cast(int, __builtin_bit_cast(v2h, pair) - off);
   };
   constexpr int SLOTS = MI * NI, CONV0 = SLOTS / 4, DSTEP = SLOTS / (DMAS / 2 + 1);
-  static_assert(CONV0 + 5 * NI <= SLOTS - 2, "conversions end two slots before the half step does");
+  constexpr int OPS = BM == 64 ? 4 : 2, CONV1 = CONV0 + 10 * NI / OPS;   // conversions' operations in a slot
+  static_assert(CONV1 <= SLOTS - 2, "conversions end two slots before the half step does");
   // One half step: MFMAs from fa and fb (odd rows right to left, so a row's
   // first reuses the last B operand); the next half's fragments from at_a and
   // at_b, B's converted into gb; DMAs d0 .. d1 - 1 of a slice into `stage`.
@@ -1408,10 +1410,10 @@ __global__ __launch_bounds__(256, 1) void grad_dma_kernel(GradArgs p, ScaledTile
       mfma16h_in_place(acc[mi][ni], fa[mi], fb[ni]);
       if constexpr (slot < NI) read_b(at_b, slot);
       if constexpr (pos == NI - 1) read_a(at_a, mi);
-      if constexpr (slot >= CONV0 && slot < CONV0 + 5 * NI) {
-        convert(std::integral_constant<int, 2 * (slot - CONV0)>(), gb);
-        convert(std::integral_constant<int, 2 * (slot - CONV0) + 1>(), gb);
-      }
+      if constexpr (slot >= CONV0 && slot < CONV1)
+        each([&](auto o) __attribute__((always_inline)) {
+          convert(std::integral_constant<int, OPS * (slot - CONV0) + decltype(o)::value>(), gb);
+        }, std::make_integer_sequence<int, OPS>());
       if constexpr (slot % DSTEP == 2 && d0 + slot / DSTEP < d1) dma(d0 + slot / DSTEP, stage, ab, bb);
       __builtin_amdgcn_sched_barrier(0);
     }, std::make_integer_sequence<int, SLOTS>());
@@ -1854,25 +1856,35 @@ int launch_row_terms(const TermArgs &a, int type, hipStream_t s) {
   return VT_OK;
 }
 
-// Tiles and splits of a gradient product by the least estimated time: a slice
-// takes a workgroup 0.87 us on 128 x 256 tiles and 1.64 us on 256 x 256 ones
-// (2048 x 4096 x 28672 and 4096^3, one tile per CU), partial sums are written
-// and read at 4 TB/s and take a second launch.
+// Tiles and splits of a gradient product by the least estimated time (us). A
+// slice takes a workgroup, on an idle card and on a busy one (the clock falls),
+//   64 x 256     0.48 .. 0.53, as if two workgroups on a CU ran one behind the
+//                other; 3.7 around the slices, half of it under the other workgroup
+//   128 x 256    0.66 .. 0.87; 6.3
+//   256 x 256    1.17 .. 1.55; 10
+// and partial sums are written and read at 4 TB/s and take a second launch. On 37
+// shapes, every tile timed at 1, 2, 4, .. 32 splits, the choice among those is
+// within 5 % of the fastest: 100 x 333 over 2432 columns 13.4 on 64-row tiles (128: 16.5), 1024 x 4096 over
+// 4096 45.8 (53.5; 256: 66.8), 1088 rows of that 56.2 on 128-row tiles (64: 63.2),
+// 4096^3 124 on 256-row tiles (128: 137, 64: 151).
 struct GradGeom {
   int bm, splits;
 };
 
 GradGeom grad_geom(int64_t M, int64_t Kp, int64_t slices, int cus) {
+  static const struct { int bm; double idle, busy, around, next; } kTiles[] = {
+      {256, 1.17, 1.55, 10.0, 10.0}, {128, 0.66, 0.87, 6.3, 6.3}, {64, 0.48, 0.53, 3.7, 1.85}};
   GradGeom best = {128, 1};
   double least = 0;
-  for (int bm = 256; bm >= 128; bm /= 2)
-    for (int splits = 1; splits <= 32 && splits <= slices; splits *= 2) {
-      const int64_t tiles = (M + bm - 1) / bm * ((Kp + 255) / 256);
-      double ns = (double)((tiles * splits + cus - 1) / cus) * (double)((slices + splits - 1) / splits) * (bm == 256 ? 1640 : 870);
-      if (splits > 1) ns += 3000 + 8.0 * splits * M * Kp / 4000;
-      if (least == 0 || ns < least) {
-        least = ns;
-        best = {bm, splits};
+  for (const auto &t : kTiles)
+    for (int splits = 1; splits <= 32 && splits <= slices; splits += splits < 8 ? 1 : splits / 4) {
+      const int64_t wgs = (M + t.bm - 1) / t.bm * ((Kp + 255) / 256) * splits, rounds = (wgs + cus - 1) / cus;
+      const double slice = t.idle + (t.busy - t.idle) * std::min(1.0, (double)wgs / cus);
+      double us = (double)rounds * (double)((slices + splits - 1) / splits) * slice + t.around + (double)(rounds - 1) * t.next;
+      if (splits > 1) us += 2.5 + 8.0 * splits * M * Kp / 4e6;
+      if (least == 0 || us < least) {
+        least = us;
+        best = {t.bm, splits};
       }
     }
   return best;
@@ -1884,7 +1896,8 @@ int launch_grad_tiles(const GradArgs &a, int bm, const ScaledOut &o, hipStream_t
   const int64_t wgs = (int64_t)a.tiles_m * a.tiles_n * a.splits;
   if (wgs > 0x7fffffff) return fail(VT_EUNSUPPORTED, "gradient grid too large");
   if (bm == 256) hipLaunchKernelGGL(grad_dma_kernel<256>, dim3((unsigned)wgs), dim3(256), 0, s, a, out);
-  else hipLaunchKernelGGL(grad_dma_kernel<128>, dim3((unsigned)wgs), dim3(256), 0, s, a, out);
+  else if (bm == 128) hipLaunchKernelGGL(grad_dma_kernel<128>, dim3((unsigned)wgs), dim3(256), 0, s, a, out);
+  else hipLaunchKernelGGL(grad_dma_kernel<64>, dim3((unsigned)wgs), dim3(256), 0, s, a, out);
   VT_HIP_CHECK(hipGetLastError());
   return VT_OK;
 }
