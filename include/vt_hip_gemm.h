@@ -474,7 +474,8 @@ int vt_gemm_i8_packed(const int8_t *A, const int8_t *Bp, const int32_t *D, int32
  * gradients are those in x^ = q t (straight through the rounding); weights,
  * scales and bias are constants. Gradient terms (dy s, or the factors of Wg and
  * Wu above) are float16 with one power of two per row, in two halves (22 bits)
- * when the gradients are float32; their products are summed in float32.
+ * unless the gradients are bfloat16 (one, 11 bits); their products are summed in
+ * float32.
  *
  * Rows: X [M][ldx] of x_type; VT_TYPE_I8 rows come with their scales T [M].
  * VT_TYPE_I8_PADDED rows also have ldx >= vt_quant_pitch(K), a multiple of 16,

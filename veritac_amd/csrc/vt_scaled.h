@@ -390,8 +390,9 @@ __device__ __forceinline__ float from16(uint32_t bits, int type) {
   return type == VT_TYPE_BF16 ? __uint_as_float(bits << 16) : (float)__builtin_bit_cast(_Float16, (uint16_t)bits);
 }
 
-// E: bytes of the floating type in tile16 (2 or 4); everything else goes by `type`.
-template <int OP, int E = 2>
+// E: bytes of the floating type in tile16 (2 or 4), and LOW whether it writes
+// the low halves of gradient terms; everything else goes by `type` and `lo`.
+template <int OP, int E = 2, bool LOW = E == 4>
 struct ScaledTile : ScaledOut {
   static constexpr bool kScaled = true;
   static constexpr int OE = OP == kGradTerms ? 2 : E;   // bytes of what tile16 writes
@@ -781,7 +782,7 @@ struct ScaledTile : ScaledOut {
         });
       }
       flush(v, mi, 0);
-      if constexpr (OP == kGradTerms && E == 4) {
+      if constexpr (OP == kGradTerms && LOW) {
 #pragma unroll
         for (int b = 0; b < NB; ++b)
 #pragma unroll
@@ -848,6 +849,13 @@ struct ScaledTile : ScaledOut {
 
 template <int OP, int E, int BN>
 __global__ __launch_bounds__(256, 1) void scaled_dma16_kernel(GemmArgs p, ScaledTile<OP, E> out) {
+  dma16_tiles<false, true, true, BN, false>(p, out);
+}
+
+// Terms of float16 gradients: 16-bit dh, and low halves. (A branch on `lo` in the
+// kernel for both 16-bit types cost the bfloat16 one registers and 1.5 - 3 %.)
+template <int BN>
+__global__ __launch_bounds__(256, 1) void terms_low_dma16_kernel(GemmArgs p, ScaledTile<kGradTerms, 2, true> out) {
   dma16_tiles<false, true, true, BN, false>(p, out);
 }
 
@@ -1664,6 +1672,10 @@ void launch_dma16(const GemmArgs &a, const ScaledOut &o, int64_t wgs, hipStream_
     ScaledTile<OP, 4> out;
     (ScaledOut &)out = o;
     hipLaunchKernelGGL((scaled_dma16_kernel<OP, 4, BN>), dim3((unsigned)wgs), dim3(256), 0, s, a, out);
+  } else if (OP == kGradTerms && o.lo) {
+    ScaledTile<kGradTerms, 2, true> out;
+    (ScaledOut &)out = o;
+    hipLaunchKernelGGL((terms_low_dma16_kernel<BN>), dim3((unsigned)wgs), dim3(256), 0, s, a, out);
   } else {
     ScaledTile<OP, 2> out;
     (ScaledOut &)out = o;
@@ -2062,9 +2074,13 @@ int backward(const ScaledCall &c, const int8_t *Q, int q_type, int64_t ldq, cons
   o.M = (int)c.M; o.N = (int)c.K; o.Np = (int)Kp;
   o.type = c.y_type;
   if (Np == 0) return launch_zero(o, s);
-  // Terms in float16, normalised by row; of float32 gradients also what
-  // float16 leaves of each (two products).
-  const bool split = c.x_type == VT_TYPE_F32;
+  // Terms in float16, normalised by row, and in a second half what float16
+  // leaves of each: two products, 22 bits. Only bfloat16 gradients do without:
+  // their own rounding to 8 bits is 8 times that of an 11-bit term, so the error
+  // grows by 1 / 128 (1.7e-3 of the result's norm either way, 4096^3), and the
+  // second product would double the largest part of the call. Float16 gradients
+  // have as many bits as such a term: one half alone gave 1.4 times their error.
+  const bool split = c.x_type != VT_TYPE_BF16;
   const int64_t lo = split ? c.M * Np : 0;
   void *w = nullptr;
   const size_t t_bytes = ((size_t)c.M * Np * 2 * (split ? 2 : 1) + 255) / 256 * 256;
