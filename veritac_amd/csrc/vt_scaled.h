@@ -316,14 +316,15 @@ __global__ __launch_bounds__(256) void pack_bound_kernel(ScaledPackArgs p) {
 // What follows the int32 sums
 // ---------------------------------------------------------------------------
 
-// 2^32 / (1 + exp(-z)): the factor keeps a small value clear of the smallest
-// float32 exponents (which the exponential and the reciprocal drop) until it
-// is multiplied by g. From 2^60 on, exp(z) is all of 1 + exp(z). (fmed3 clamps
-// in one instruction; a NaN reaches the result by its factor g.)
-constexpr float kLogisticUnit = 0x1p-32f;
-__device__ __forceinline__ float logistic32(float z) {
-  const float e = __builtin_amdgcn_exp2f(__builtin_amdgcn_fmed3f(fmaf(z, 1.4426950408889634f, 32.0f), -200.0f, 92.0f));
-  return e * __builtin_amdgcn_rcpf(fmaf(e, kLogisticUnit, 1.0f));
+// g / (1 + exp(-z)) as (g y) (y / (1 + y^2)) with y = exp(z / 2) = 2^x: a small value
+// stays clear of the smallest float32 exponents (which the exponential and the
+// reciprocal drop) until it is multiplied by g, and z keeps all of its bits. (32
+// added to the exponent instead took those near z = 0: 4.5 roundings of the
+// product instead of 1.5.) From y = 2^13 on, y^2 is all of 1 + y^2 in 24 bits. (fmed3
+// clamps in one instruction; a NaN reaches the result by its factor g.)
+__device__ __forceinline__ float logistic_of(float g, float x) {
+  const float y = __builtin_amdgcn_exp2f(__builtin_amdgcn_fmed3f(x, -200.0f, 13.0f));
+  return (g * y) * (y * __builtin_amdgcn_rcpf(fmaf(y, y, 1.0f)));
 }
 
 // act(g), and its slope. gelu is the tanh form: (1 + tanh z) / 2 is
@@ -335,13 +336,13 @@ template <int ACT, bool TERMS>
 __device__ __forceinline__ float act_of(float g, float &slope) {
   const float c = 0.7978845608028654f, a = 0.044715f;
   const float h = ACT == VT_ACT_GELU ? __builtin_amdgcn_fmed3f(g, -16.0f, 16.0f) : g;
-  const float hh = h * h, z = ACT == VT_ACT_GELU ? 2.0f * c * (h * fmaf(a, hh, 1.0f)) : g;
-  const float p32 = TERMS ? 0.0f : logistic32(z);
-  const float p = TERMS ? __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.4426950408889634f))
-                        : p32 * kLogisticUnit;
+  const float hh = h * h, z = ACT == VT_ACT_GELU ? h * fmaf(a, hh, 1.0f) : g;   // gelu: over 2 c
+  const float log2e = (ACT == VT_ACT_GELU ? 2.0f * c : 1.0f) * 1.4426950408889634f;
+  if constexpr (!TERMS) return logistic_of(g, z * (0.5f * log2e));
+  const float p = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -log2e));
   const float dz = ACT == VT_ACT_GELU ? 2.0f * c * fmaf(3.0f * a, hh, 1.0f) : 1.0f;
   slope = p * fmaf(h * dz, 1.0f - p, 1.0f);
-  return TERMS ? g * p : g * p32 * kLogisticUnit;
+  return g * p;
 }
 
 // Row normaliser of 16-bit gradient terms: the power of two that takes a bound
