@@ -1,0 +1,44 @@
+"""Scaled calls with stream=: what a call copies and fills on its way is in order with its kernels, also
+while torch's current stream has work of its own queued up."""
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from test_gpu_scaled import dev, say, up, weights  # noqa: F401
+from veritac_amd.specializations.hip_gemm import scaled
+
+pytestmark = pytest.mark.gpu
+
+
+class Busy:
+    """Some 30 ms of work on torch's current stream, and a stream beside it that starts where that one
+    stands now."""
+
+    def __init__(self, dev):
+        self.a = torch.randn(4096, 4096, device=dev)
+        self.b = torch.empty_like(self.a)
+        self.side = torch.cuda.Stream(dev)
+
+    def __enter__(self):
+        torch.cuda.synchronize()
+        for _ in range(20):
+            torch.mm(self.a, self.a, out=self.b)
+        return self.side.cuda_stream
+
+    def __exit__(self, *exc):
+        torch.cuda.synchronize()
+
+
+def test_packing_beside_a_busy_stream(dev):
+    rng = np.random.default_rng(1)
+    (w, s), (w2, s2) = weights(rng, 300, 200), weights(rng, 300, 200)
+    w, s, w2, s2, bias = (up(v, dev) for v in (w, s, w2, s2, rng.normal(0, 1, 200).astype(np.float32)))
+    want = [scaled.pack_linear(w, s, bias), scaled.pack_gated(w, s, w2, s2)]
+    busy = Busy(dev)
+    for _ in range(3):
+        say("pack on a side stream")
+        with busy as side:
+            got = [scaled.pack_linear(w, s, bias, stream=side), scaled.pack_gated(w, s, w2, s2, stream=side)]
+        for a, b in zip(got, want):
+            assert torch.equal(a.data, b.data) and torch.equal(a.meta, b.meta)

@@ -21,9 +21,10 @@ gradients by themselves.
 Same conventions as backend.run: device tensors only, every mismatch raises
 HipGemmError before anything is launched, work is enqueued on torch's current
 stream or on `stream` (a raw hipStream_t handle, whose order against the
-operands' producers is the caller's), and a call made once on a stream can be
-captured into a HIP graph there. Rows may have any pitch and alignment; their
-last dimension has unit stride.
+operands' producers is the caller's; what a call allocates and copies itself is
+on that stream too), and a call made once on a stream can be captured into a
+HIP graph there. Rows may have any pitch and alignment; their last dimension
+has unit stride.
 """
 from __future__ import annotations
 
@@ -103,6 +104,36 @@ class ScaledWeight:
             self.k, self.n, "gated" if self.pair else "linear", self.device)
 
 
+def _enqueued(on, stream, call, record=True):
+    """call(), with the raw handle `stream` as torch's current stream of the device
+    of `on`: the copies and memory that the call makes on its way are then in
+    order with its kernels. Its results (unless the caller holds them already)
+    are recorded as used on the stream that was current, where the caller goes
+    on with them."""
+    device = getattr(on, "device", None)
+    if stream is None or getattr(device, "type", None) != "cuda":
+        return call()
+    torch = _torch()
+    with torch.cuda.device(device):
+        before = torch.cuda.current_stream(device)
+        if stream == before.cuda_stream:
+            return call()
+        with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=device)):
+            result = call()
+        if record:
+            for t in _tensors(result):
+                t.record_stream(before)
+        return result
+
+
+def _tensors(result):
+    if isinstance(result, QuantRows):
+        return result.data, result.scale
+    if isinstance(result, ScaledWeight):
+        return result.data, result.meta
+    return result if isinstance(result, tuple) else (result,)
+
+
 def _gpu(name, t):
     if t.device.type != "cuda":
         raise HipGemmError("%s must be on a gfx950 GPU (got %s); hip_gemm has no CPU path"
@@ -142,23 +173,18 @@ def _pitch(t):
     return t.stride(0) if t.shape[0] > 1 and t.shape[1] else max(t.shape[1], 1)
 
 
-def _pack(w0, s0, w1, s1, bias, stream):
+def _pack(w0, s0, w1, s1, bias):
     torch = _torch()
     k, n = w0.shape
     size, floats = _lib.scaled_size(k, n, w1 is not None)
     data = torch.empty(size, dtype=torch.int8, device=w0.device)
-    meta = torch.zeros(floats, dtype=torch.float32, device=w0.device)
-    if stream is None:
-        stream = _current_stream(w0.device)
-    else:
-        _keep_for_stream(data, stream)
-        _keep_for_stream(meta, stream)
+    meta = torch.empty(floats, dtype=torch.float32, device=w0.device)   # written whole (and not read if n = 0)
     lib = _lib.load_library()
     _lib.check(lib.vt_scaled_pack(
         w0.data_ptr(), None if w1 is None else w1.data_ptr(), _pitch(w0),
         0 if w1 is None else _pitch(w1), s0.data_ptr(), None if s1 is None else s1.data_ptr(),
-        None if bias is None else bias.data_ptr(), k, n, data.data_ptr(), meta.data_ptr(), stream),
-        "vt_scaled_pack")
+        None if bias is None else bias.data_ptr(), k, n, data.data_ptr(), meta.data_ptr(),
+        _current_stream(w0.device)), "vt_scaled_pack")
     return ScaledWeight(data, meta, k, n, w1 is not None)
 
 
@@ -168,7 +194,7 @@ def pack_linear(w, scale, bias=None, *, stream=None):
     _weight("w", w, scale)
     if bias is not None:
         _channels("bias", bias, w.shape[1], w.device)
-    return _pack(w, scale, None, None, bias, stream)
+    return _enqueued(w, stream, lambda: _pack(w, scale, None, None, bias))
 
 
 def pack_gated(w_gate, s_gate, w_up, s_up, *, stream=None):
@@ -177,7 +203,7 @@ def pack_gated(w_gate, s_gate, w_up, s_up, *, stream=None):
     `gated_grad`."""
     _weight("w_gate", w_gate, s_gate)
     _weight("w_up", w_up, s_up, w_gate.shape, w_gate.device)
-    return _pack(w_gate, s_gate, w_up, s_up, None, stream)
+    return _enqueued(w_gate, stream, lambda: _pack(w_gate, s_gate, w_up, s_up, None))
 
 
 def quantize_weight(w, *, stream=None):
