@@ -42,3 +42,14 @@ def test_packing_beside_a_busy_stream(dev):
             got = [scaled.pack_linear(w, s, bias, stream=side), scaled.pack_gated(w, s, w2, s2, stream=side)]
         for a, b in zip(got, want):
             assert torch.equal(a.data, b.data) and torch.equal(a.meta, b.meta)
+
+
+def test_quantising_weights_beside_a_busy_stream(dev):
+    w = torch.randn(700, 300, device=dev)
+    want = scaled.quantize_weight(w)
+    busy = Busy(dev)
+    for _ in range(3):
+        say("quantize_weight on a side stream")
+        with busy as side:
+            got = scaled.quantize_weight(w, stream=side)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])

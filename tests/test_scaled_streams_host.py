@@ -97,6 +97,8 @@ CALLS = {
     "pack_linear": lambda w, s, L, G, r, x, d, **kw: scaled.pack_linear(w, s, **kw),
     "pack_linear bias": lambda w, s, L, G, r, x, d, **kw: scaled.pack_linear(w, s, s, **kw),
     "pack_gated": lambda w, s, L, G, r, x, d, **kw: scaled.pack_gated(w, s, w, s, **kw),
+    "quantize_weight": lambda w, s, L, G, r, x, d, **kw: scaled.quantize_weight(torch.ones(K, N), **kw),
+    "quantize_rows": lambda w, s, L, G, r, x, d, **kw: scaled.quantize_rows(x, **kw),
 }
 
 

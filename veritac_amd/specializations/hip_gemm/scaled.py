@@ -212,8 +212,11 @@ def quantize_weight(w, *, stream=None):
     torch = _torch()
     if not isinstance(w, torch.Tensor) or w.dim() != 2:
         raise HipGemmError("w must be a floating torch tensor [k, n]")
-    r = quantize_rows(w.detach().t().contiguous(), stream=stream)
-    return r.data[:, :r.k].t().contiguous(), r.scale
+
+    def both():
+        r = _quantize(w.detach().t().contiguous())
+        return r.data[:, :r.k].t().contiguous(), r.scale
+    return _enqueued(w, stream, both)
 
 
 def _rows(name, x):
@@ -246,20 +249,19 @@ def _rows(name, x):
 def quantize_rows(x, *, stream=None):
     """Floating rows x [..., k] -> QuantRows: each row by its largest magnitude,
     rounded to the nearest, ties to even."""
+    return _enqueued(x, stream, lambda: _quantize(x))
+
+
+def _quantize(x):
     torch = _torch()
     x2, lead = _rows("x", x)
     m, k = x2.shape
     pitch = _lib.quant_pitch(k)
     data = torch.empty((m, pitch), dtype=torch.int8, device=x.device)
     scale = torch.empty(m, dtype=torch.float32, device=x.device)
-    if stream is None:
-        stream = _current_stream(x.device)
-    else:
-        _keep_for_stream(data, stream)
-        _keep_for_stream(scale, stream)
     lib = _lib.load_library()
     _lib.check(lib.vt_quant_rows(x2.data_ptr(), _types()[x.dtype], _pitch(x2), data.data_ptr(), pitch,
-                                 scale.data_ptr(), m, k, stream), "vt_quant_rows")
+                                 scale.data_ptr(), m, k, _current_stream(x.device)), "vt_quant_rows")
     return QuantRows(data, scale, k=k, padded=True, shape=tuple(lead) + (k,))
 
 
