@@ -53,3 +53,29 @@ def test_quantising_weights_beside_a_busy_stream(dev):
         with busy as side:
             got = scaled.quantize_weight(w, stream=side)
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_rows_that_are_copied_beside_a_busy_stream(dev):
+    """Rows of three dimensions whose leading two do not flatten."""
+    rng = np.random.default_rng(2)
+    w, s = weights(rng, 256, 192)
+    L = scaled.pack_linear(up(w, dev), up(s, dev))
+    G = scaled.pack_gated(up(w, dev), up(s, dev), up(w, dev), up(s, dev))
+    x = torch.randn(40, 30, 256, device=dev).transpose(0, 1)
+    d = torch.randn(40, 30, 192, device=dev).transpose(0, 1)
+    r = scaled.quantize_rows(x)
+    calls = [lambda **kw: scaled.quantize_rows(x, **kw).data, lambda **kw: scaled.linear(x, L, **kw),
+             lambda **kw: scaled.gated(x, G, **kw), lambda **kw: scaled.linear_grad(d, L, **kw),
+             lambda **kw: scaled.gated_grad(d, r, G, **kw)]
+    want = [f() for f in calls]
+    busy = Busy(dev)
+    say("copied rows on a side stream")
+    for _ in range(2):
+        with busy as side:
+            got = [f(stream=side) for f in calls]
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    # and their memory is not handed out while the side stream may still read it
+    with busy as side:
+        got = [f(stream=side) for f in calls for _ in range(3)]
+        spoil = [torch.full((40 * 30 * 256,), float("nan"), device=dev) for _ in range(8)]
+    assert all(torch.equal(a, b) for a, b in zip(got, [v for v in want for _ in range(3)])) and len(spoil) == 8

@@ -99,6 +99,11 @@ CALLS = {
     "pack_gated": lambda w, s, L, G, r, x, d, **kw: scaled.pack_gated(w, s, w, s, **kw),
     "quantize_weight": lambda w, s, L, G, r, x, d, **kw: scaled.quantize_weight(torch.ones(K, N), **kw),
     "quantize_rows": lambda w, s, L, G, r, x, d, **kw: scaled.quantize_rows(x, **kw),
+    "linear": lambda w, s, L, G, r, x, d, **kw: scaled.linear(x, L, **kw),
+    "linear of int8 rows": lambda w, s, L, G, r, x, d, **kw: scaled.linear(r, L, out_dtype=torch.float32, **kw),
+    "gated": lambda w, s, L, G, r, x, d, **kw: scaled.gated(x, G, **kw),
+    "linear_grad": lambda w, s, L, G, r, x, d, **kw: scaled.linear_grad(d, L, **kw),
+    "gated_grad": lambda w, s, L, G, r, x, d, **kw: scaled.gated_grad(d, r, G, **kw),
 }
 
 
@@ -122,3 +127,10 @@ def test_all_work_of_a_call_is_on_its_stream(log, name):
         # memory of the side stream's, used on the caller's from here on
         assert {p for p, s in log.recorded if s == MAIN} == (pointers(result) if want == SIDE else set())
 
+
+def test_a_given_output_is_the_caller_s(log):
+    w, s, L, G, r, x, d = operands()
+    out = torch.empty(3, 2, N)
+    del log.work[:]
+    assert scaled.linear(x, L, out=out, stream=SIDE) is out and not log.recorded
+    assert {w[1] for w in log.work} == {SIDE}

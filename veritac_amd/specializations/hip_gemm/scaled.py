@@ -30,7 +30,7 @@ from __future__ import annotations
 
 from ... import _lib
 from ..._lib import HipGemmError
-from .backend import _current_stream, _keep_for_stream, _torch
+from .backend import _current_stream, _torch
 
 ACTIVATIONS = tuple(_lib.ACT_IDS)
 
@@ -302,7 +302,7 @@ def _output(name, out, m, cols, lead, dtype, device, like=None):
     return o2, out, False
 
 
-def _forward(x, W, pair, act, out_dtype, out, stream):
+def _forward(x, W, pair, act, out_dtype, out):
     if isinstance(x, QuantRows):
         data, k = x.data, x.k
         _gpu("x", data)
@@ -323,10 +323,7 @@ def _forward(x, W, pair, act, out_dtype, out, stream):
     m = data.shape[0]
     device = data.device
     o2, ret, allocated = _output("output", out, m, W.n, lead, out_dtype, device, data)
-    if stream is None:
-        stream = _current_stream(device)
-    elif allocated:
-        _keep_for_stream(ret, stream)
+    stream = _current_stream(device)
     lib = _lib.load_library()
     ldy = max(W.n, 1) if allocated or o2.dim() != 2 or m < 2 or not W.n else o2.stride(-2)
     if pair:
@@ -363,7 +360,9 @@ def linear(x, W, *, out_dtype=None, out=None, stream=None):
         if out is not None or stream is not None:
             raise HipGemmError("a differentiable call takes neither out nor stream")
         return _functions()[0].apply(x, W, out_dtype)
-    return _forward(x, W, False, 0, out_dtype, out, stream)
+    if stream is not None:
+        return _enqueued(x, stream, lambda: _forward(x, W, False, 0, out_dtype, out), out is None)
+    return _forward(x, W, False, 0, out_dtype, out)
 
 
 def gated(x, W, *, act="silu", out_dtype=None, out=None, stream=None):
@@ -375,27 +374,29 @@ def gated(x, W, *, act="silu", out_dtype=None, out=None, stream=None):
         if out is not None or stream is not None:
             raise HipGemmError("a differentiable call takes neither out nor stream")
         return _functions()[1].apply(x, W, act, out_dtype)
-    return _forward(x, W, True, a, out_dtype, out, stream)
+    if stream is not None:
+        return _enqueued(x, stream, lambda: _forward(x, W, True, a, out_dtype, out), out is None)
+    return _forward(x, W, True, a, out_dtype, out)
 
 
 def linear_grad(dy, W, *, out=None, stream=None):
     """dx = (dy * scale) . w^T, the gradient of `linear` in its rounded rows, for
     dy [..., n] of any floating type; dx [..., k] has the same."""
+    return _enqueued(dy, stream, lambda: _linear_grad(dy, W, out), out is None)
+
+
+def _linear_grad(dy, W, out):
     d, lead = _rows("dy", dy)
     _check_weight(W, False, d.device, None)
     if d.shape[1] != W.n:
         raise HipGemmError("dy has %d columns, the weights give %d" % (d.shape[1], W.n))
     m = d.shape[0]
-    o2, ret, allocated = _output("gradient", out, m, W.k, lead, dy.dtype, d.device, d)
-    if stream is None:
-        stream = _current_stream(d.device)
-    elif allocated:
-        _keep_for_stream(ret, stream)
+    o2, ret, _ = _output("gradient", out, m, W.k, lead, dy.dtype, d.device, d)
     ldx = o2.stride(-2) if o2.dim() == 2 and m > 1 and W.k else max(W.k, 1)
     lib = _lib.load_library()
     _lib.check(lib.vt_scaled_linear_grad(d.data_ptr(), _types()[dy.dtype], _pitch(d), m, W.k,
                                          W.data.data_ptr(), W.meta.data_ptr(), W.n, o2.data_ptr(),
-                                         ldx, stream), "vt_scaled_linear_grad")
+                                         ldx, _current_stream(d.device)), "vt_scaled_linear_grad")
     return ret
 
 
@@ -404,6 +405,10 @@ def gated_grad(dh, rows, W, *, act="silu", out=None, stream=None):
     QuantRows of the forward pass (quantize_rows of its x). dx [..., k] has dh's
     type."""
     a = _act_id(act)
+    return _enqueued(dh, stream, lambda: _gated_grad(dh, rows, W, a, out), out is None)
+
+
+def _gated_grad(dh, rows, W, a, out):
     d, lead = _rows("dh", dh)
     if not isinstance(rows, QuantRows):
         raise HipGemmError("rows must be the QuantRows of the forward pass")
@@ -414,18 +419,14 @@ def gated_grad(dh, rows, W, *, act="silu", out=None, stream=None):
     if d.shape[1] != W.n or m != rows.data.shape[0]:
         raise HipGemmError("dh is %d x %d, the rows and weights give %d x %d"
                            % (m, d.shape[1], rows.data.shape[0], W.n))
-    o2, ret, allocated = _output("gradient", out, m, W.k, lead, dh.dtype, d.device, d)
-    if stream is None:
-        stream = _current_stream(d.device)
-    elif allocated:
-        _keep_for_stream(ret, stream)
+    o2, ret, _ = _output("gradient", out, m, W.k, lead, dh.dtype, d.device, d)
     ldx = o2.stride(-2) if o2.dim() == 2 and m > 1 and W.k else max(W.k, 1)
     lib = _lib.load_library()
     _lib.check(lib.vt_scaled_gated_grad(
         d.data_ptr(), _types()[dh.dtype], _pitch(d), rows.data.data_ptr(),
         _lib.TYPE_I8_PADDED if rows.padded else _lib.TYPE_I8, _pitch(rows.data),
         rows.scale.data_ptr(), m, W.k, W.data.data_ptr(), W.meta.data_ptr(), W.n, a, o2.data_ptr(),
-        ldx, stream), "vt_scaled_gated_grad")
+        ldx, _current_stream(d.device)), "vt_scaled_gated_grad")
     return ret
 
 
@@ -443,7 +444,7 @@ def _functions():
             @staticmethod
             def forward(ctx, x, W, out_dtype):
                 ctx.W, ctx.dtype = W, x.dtype
-                return _forward(x, W, False, 0, out_dtype, None, None)
+                return _forward(x, W, False, 0, out_dtype, None)
 
             @staticmethod
             @torch.autograd.function.once_differentiable
@@ -457,7 +458,7 @@ def _functions():
                 rows = quantize_rows(x)
                 ctx.W, ctx.act, ctx.dtype, ctx.shape = W, act, x.dtype, rows.shape
                 ctx.save_for_backward(rows.data, rows.scale)
-                return _forward(rows, W, True, _act_id(act), out_dtype or x.dtype, None, None)
+                return _forward(rows, W, True, _act_id(act), out_dtype or x.dtype, None)
 
             @staticmethod
             @torch.autograd.function.once_differentiable
