@@ -28,9 +28,11 @@ has unit stride.
 """
 from __future__ import annotations
 
+import math
+
 from ... import _lib
 from ..._lib import HipGemmError
-from .backend import _current_stream, _torch
+from .backend import _current_stream, _is_int, _torch
 
 ACTIVATIONS = tuple(_lib.ACT_IDS)
 
@@ -51,6 +53,7 @@ class QuantRows:
     `data` is int8 [m, >= k] and `scale` float32 [m], both on one GPU. Rows
     made by quantize_rows are padded with zeros to the pitch that the products
     read in place (`padded`); others are copied so by the calls that need it.
+    `shape`: what the rows were flattened from, [..., k] of m rows in all.
     """
 
     __slots__ = ("data", "scale", "k", "padded", "shape")
@@ -66,10 +69,19 @@ class QuantRows:
             raise HipGemmError("scale is on %s, data on %s" % (scale.device, data.device))
         if not _unit_rows(data):
             raise HipGemmError("data must have unit stride in its last dimension")
-        self.data, self.scale = data, scale
-        self.k = data.shape[1] if k is None else k
-        self.padded = padded
-        self.shape = (data.shape[0], self.k) if shape is None else shape
+        m, width = data.shape
+        if k is None:
+            k = width
+        elif not _is_int(k) or not 0 <= k <= width:
+            raise HipGemmError("k must be 0 .. %d, the width of data (got %r)" % (width, k))
+        if padded and width < _lib.quant_pitch(k):
+            raise HipGemmError("padded rows of k = %d are at least %d wide (got %d)"
+                               % (k, _lib.quant_pitch(k), width))
+        shape = (m, k) if shape is None else tuple(shape)
+        if not shape or not all(_is_int(d) and d >= 0 for d in shape) or shape[-1] != k \
+                or math.prod(shape[:-1]) != m:
+            raise HipGemmError("shape must be [..., %d] of %d rows (got %s)" % (k, m, shape))
+        self.data, self.scale, self.k, self.padded, self.shape = data, scale, k, padded, shape
 
     @property
     def device(self):
