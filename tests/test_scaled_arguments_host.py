@@ -1,4 +1,4 @@
-"""QuantRows hold what the kernels may read and write: sizes that the tensors do not
+"""QuantRows and ScaledWeight hold what the kernels may read and write: sizes that the tensors do not
 have are refused where the object is made, without a GPU."""
 import pytest
 
@@ -44,3 +44,24 @@ def test_rows_of_any_leading_shape():
     assert rows(3, 0).shape == (3, 0)
     assert rows(3, 0, padded=True).k == 0
 
+
+def weight(k=100, n=60, pair=False, data=None, meta=None):
+    size, floats = _lib.scaled_size(100, 60, pair)
+    return scaled.ScaledWeight(torch.zeros(size, dtype=torch.int8) if data is None else data,
+                               torch.zeros(floats) if meta is None else meta, k, n, pair)
+
+
+def test_packed_weights_have_their_size():
+    size, floats = _lib.scaled_size(100, 60, False)
+    assert weight().n == 60 and weight(pair=True).pair
+    for call, what in ((lambda: weight(k=200), "data"), (lambda: weight(n=65), "data"),
+                       (lambda: weight(data=torch.zeros(size - 1, dtype=torch.int8)), "data"),
+                       (lambda: weight(data=torch.zeros(size)), "data"),
+                       (lambda: weight(data=torch.zeros(2 * size, dtype=torch.int8)[::2]), "data"),
+                       (lambda: weight(data=[0] * size), "data"),
+                       (lambda: weight(meta=torch.zeros(floats - 1)), "meta"),
+                       (lambda: weight(meta=torch.zeros(floats, dtype=torch.float64)), "meta"),
+                       (lambda: weight(meta=torch.zeros(2 * floats)[::2]), "meta"),
+                       (lambda: weight(k=-1), "K")):
+        with pytest.raises(HipGemmError, match=what):
+            call()

@@ -105,6 +105,14 @@ class ScaledWeight:
     __slots__ = ("data", "meta", "k", "n", "pair")
 
     def __init__(self, data, meta, k, n, pair):
+        torch = _torch()
+        size, floats = _lib.scaled_size(k, n, pair)
+        if not isinstance(data, torch.Tensor) or data.dtype != torch.int8 or data.shape != (size,) \
+                or not data.is_contiguous():
+            raise HipGemmError("data must be a contiguous int8 tensor of %d bytes" % size)
+        if not isinstance(meta, torch.Tensor) or meta.dtype != torch.float32 or meta.shape != (floats,) \
+                or not meta.is_contiguous() or meta.device != data.device:
+            raise HipGemmError("meta must be a contiguous float32 tensor [%d] on %s" % (floats, data.device))
         self.data, self.meta, self.k, self.n, self.pair = data, meta, k, n, pair
 
     @property
