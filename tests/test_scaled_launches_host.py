@@ -1,0 +1,41 @@
+"""What the scaled operators launch, on the CPU: their host code runs against a HIP runtime that only logs
+(fake_hip.cpp). Operand addresses are made up and never read."""
+import pytest
+
+from test_workspaces_host import run  # noqa: F401
+
+CALLS = """
+lib = _lib.load_library()
+F32, F16, BF16, I8, I8P = 1, 2, 3, 4, 5
+BASE = [(1 + i) << 43 for i in range(6)]
+
+def ok(rc):
+    assert rc == 0, (rc, _lib.last_error())
+
+def linear(m, k, n, x=BF16, y=BF16, ldx=None, stream=STREAM):
+    ok(lib.vt_scaled_linear(BASE[0], x, k if ldx is None else ldx, BASE[1], m, k, BASE[2], BASE[3], n, BASE[4], y, n, stream))
+
+def gated(m, k, n, x=BF16, y=BF16, ldx=None, act=0, stream=STREAM):
+    ok(lib.vt_scaled_gated(BASE[0], x, k if ldx is None else ldx, BASE[1], m, k, BASE[2], BASE[3], n, act, BASE[4], y, n, stream))
+
+def linear_grad(m, k, n, t=BF16, stream=STREAM):
+    ok(lib.vt_scaled_linear_grad(BASE[0], t, n, m, k, BASE[2], BASE[3], n, BASE[4], k, stream))
+
+def gated_grad(m, k, n, t=BF16, x=I8, ldx=None, stream=STREAM):
+    ok(lib.vt_scaled_gated_grad(BASE[0], t, n, BASE[5], x, k if ldx is None else ldx, BASE[1], m, k, BASE[2], BASE[3], n, 0,
+                                BASE[4], k, stream))
+"""
+
+
+@pytest.mark.parametrize("op", ["linear", "gated"])
+@pytest.mark.parametrize("kind,ldx", [("I8", 0), ("I8", 1), ("I8", 16), ("I8P", 0), ("I8P", 1), ("I8P", 16), ("F32", 0),
+                                      ("BF16", 5)])
+def test_empty_sums_need_no_rows(run, op, kind, ldx):
+    """K = 0: the bias or zeros, whatever the rows; no launch of an empty grid."""
+    seen = run(CALLS + """
+import json
+%s(5, 0, 40, x=%s, ldx=%d)
+print(json.dumps([e[3] for e in launches()]))
+""" % (op, kind, ldx))
+    assert "finish_kernel" in seen[-1] and len(seen) == (1 if kind.startswith("I8") else 2)
+    assert all(int(e.split(" ")[0]) > 0 for e in seen)

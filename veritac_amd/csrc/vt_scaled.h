@@ -1564,7 +1564,7 @@ bool rows_in_place(const void *X, int type, int64_t ldx, int64_t K) {
 int take_rows(const void *X, int type, int64_t ldx, const float *T, int64_t M, int64_t K, Scratch &scr, Rows *out,
               QuantArgs *pad = nullptr) {
   const int64_t Kp = scaled_kp(K);
-  if (rows_in_place(X, type, ldx, K)) {
+  if (rows_in_place(X, type, ldx, K) || (Kp == 0 && !float_type(type))) {   // no values: nothing to copy
     *out = Rows{(const int8_t *)X, T, ldx};
     return VT_OK;
   }
@@ -1996,7 +1996,7 @@ int check_scaled(const ScaledCall &c, bool *empty) {
   if (c.ldx < need) return fail(VT_EINVAL, "%s: input pitch %lld < %lld", c.who, (long long)c.ldx, (long long)need);
   if (c.ldy < c.yc) return fail(VT_EINVAL, "%s: output pitch %lld < %lld", c.who, (long long)c.ldy, (long long)c.yc);
   if (c.ldx > ((int64_t)1 << 40) || c.ldy > ((int64_t)1 << 40)) return fail(VT_EINVAL, "%s: pitch beyond 2^40", c.who);
-  if (c.x_type == VT_TYPE_I8_PADDED && (c.ldx % 16 || !aligned16(c.X)))
+  if (c.x_type == VT_TYPE_I8_PADDED && Kp > 0 && (c.ldx % 16 || !aligned16(c.X)))
     return fail(VT_EINVAL, "%s: padded int8 rows need a pitch of whole 16 bytes and a 16-byte aligned base", c.who);
   if ((uintptr_t)c.X % elem_size(c.x_type) || (uintptr_t)c.Y % elem_size(c.y_type) || !aligned16(c.Bp) || !aligned16(c.meta))
     return fail(VT_EINVAL, "%s: operands are not aligned to their elements, or packed weights not to 16 bytes", c.who);
