@@ -279,6 +279,13 @@ const char *vt_last_error(void);
 /* hipStreamSynchronize(stream), reporting asynchronous kernel errors. */
 int vt_sync(void *stream);
 
+/* A new non-blocking stream of default priority on the current device, which
+ * stays until the process ends. Workspaces belong to a stream's handle, so a
+ * graph captured on a stream that nothing else uses shares them with no other
+ * call, wherever it is replayed (handles from a framework's pool come round
+ * again). Without a counterpart in the reference. */
+int vt_stream_create(void **stream);
+
 /* Number of usable gfx950 devices (0 if none); no error on a GPU-less host. */
 int vt_device_count(void);
 

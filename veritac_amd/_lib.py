@@ -38,7 +38,7 @@ VARIANTS = tuple(VARIANT_IDS)
 
 # Every function include/vt_hip_gemm.h declares.
 EXPORTS = ("vt_gemm_i8", "vt_gemm_i8_noalloc", "vt_gemm_check", "vt_gemm_route", "vt_gemm_select", "vt_variant_info", "vt_variant_name",
-           "vt_last_error", "vt_sync", "vt_device_count", "vt_abi_version", "vt_replay_i8",
+           "vt_last_error", "vt_sync", "vt_stream_create", "vt_device_count", "vt_abi_version", "vt_replay_i8",
            "vt_device_query", "vt_packed_b_size", "vt_pack_b_i8", "vt_gemm_i8_packed",
            "vt_rtc_compile", "vt_rtc_code_size", "vt_rtc_launch", "vt_rtc_release",
            "vt_quant_pitch", "vt_quant_rows", "vt_scaled_size", "vt_scaled_pack", "vt_scaled_linear",
@@ -113,6 +113,8 @@ def _declare(lib):
     lib.vt_variant_name.restype = ctypes.c_char_p
     lib.vt_last_error.argtypes = []
     lib.vt_last_error.restype = ctypes.c_char_p
+    lib.vt_stream_create.argtypes = [ctypes.POINTER(p)]
+    lib.vt_stream_create.restype = ctypes.c_int
     lib.vt_sync.argtypes = [p]
     lib.vt_sync.restype = ctypes.c_int
     lib.vt_device_count.argtypes = []
@@ -291,6 +293,13 @@ def gemm_noalloc_raw(A_ptr, B_ptr, D_ptr, C_ptr, M, N, K, lda, ldb, ldd, ldc, ba
 
 def sync(stream=None):
     return check(load_library().vt_sync(stream), "vt_sync")
+
+
+def stream_create():
+    """Raw handle of a new stream on the current device, nobody else's (vt_stream_create)."""
+    out = ctypes.c_void_p()
+    check(load_library().vt_stream_create(ctypes.byref(out)), "vt_stream_create")
+    return out.value
 
 
 def replay_raw(prog_ptr, n_ops, A_ptr, B_ptr, C_ptr, m, n, k, scratchpad_rows,

@@ -4331,6 +4331,18 @@ int vt_device_query(int32_t device, vt_device_info *info, int64_t info_size) {
   return VT_OK;
 }
 
+int vt_stream_create(void **stream) {
+  g_err.clear();
+  if (!stream) return fail(VT_EINVAL, "vt_stream_create: stream is null");
+  int dev = 0;
+  DeviceState *st = nullptr;
+  if (int rc = current_device(&dev, &st)) return rc;
+  hipStream_t s = nullptr;
+  VT_HIP_CHECK(hipStreamCreateWithFlags(&s, hipStreamNonBlocking));
+  *stream = (void *)s;
+  return VT_OK;
+}
+
 int vt_sync(void *stream) {
   int count = 0;
   if (hipGetDeviceCount(&count) != hipSuccess || count <= 0)

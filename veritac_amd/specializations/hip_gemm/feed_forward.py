@@ -15,6 +15,9 @@ far they are from the same block in float32.
 """
 from __future__ import annotations
 
+import weakref
+
+from ... import _lib
 from ..._lib import HipGemmError
 from . import scaled
 from .backend import _torch
@@ -45,8 +48,29 @@ class FeedForward:
 
     def capture(self, x):
         """The block on rows like x as a HIP graph: an object with static `x` and
-        `y` and replay(). Its stream's workspaces are made here."""
+        `y` and replay(), with workspaces of its own, which are made here."""
         return _CapturedBlock(self, x)
+
+
+# Streams that no captured block uses any more, by device index. The library
+# keeps workspaces by stream handle: a block's stream is neither torch's (whose
+# pool hands out each of 32 handles again and again) nor another block's, so
+# replays and eager calls may run beside each other on any streams.
+_free_streams = {}
+
+
+def _own_stream(device, owner):
+    """A stream for `owner` alone, back among the free ones when it is gone."""
+    torch = _torch()
+    free = _free_streams.setdefault(device.index, [])
+    with torch.cuda.device(device):
+        try:
+            handle = free.pop()
+            torch.cuda.synchronize(device)      # what its last owner enqueued
+        except IndexError:
+            handle = _lib.stream_create()
+    weakref.finalize(owner, free.append, handle)
+    return torch.cuda.ExternalStream(handle, device=device)
 
 
 class _CapturedBlock:
@@ -55,8 +79,8 @@ class _CapturedBlock:
         self.x = x.detach().clone()
         self.h = torch.empty((*x.shape[:-1], block.gate_up.n), dtype=x.dtype, device=x.device)
         self.y = torch.empty((*x.shape[:-1], block.down.n), dtype=x.dtype, device=x.device)
-        self.stream = torch.cuda.Stream(x.device)
         self.graph = torch.cuda.CUDAGraph()
+        self.stream = _own_stream(x.device, self.graph)
 
         def step():
             scaled.gated(self.x, block.gate_up, act=block.act, out=self.h)
@@ -73,7 +97,7 @@ class _CapturedBlock:
 
     def replay(self):
         """Enqueues the step on torch's current stream; y is ready in its order.
-        Graphs captured on one stream share its workspaces: replay them in order."""
+        Replays of one block share its x, y and workspaces: order them."""
         self.graph.replay()
         return self.y
 
