@@ -16,7 +16,10 @@ x may require gradients: linear and gated are then differentiable in it, with
 the rounding to int8 passed straight through (the gradient is the one in the
 rounded rows) and weights, scales and bias held constant. gated keeps its int8
 rows for that, not the two products. linear_grad and gated_grad are those
-gradients by themselves.
+gradients by themselves. Nothing else is differentiable: quantize_rows (so
+training goes through floating rows, which each product rounds for itself),
+the two gradients and forward mode raise HipGemmError rather than leave a
+gradient out.
 
 Same conventions as backend.run: device tensors only, every mismatch raises
 HipGemmError before anything is launched, work is enqueued on torch's current
@@ -268,7 +271,9 @@ def _rows(name, x):
 
 def quantize_rows(x, *, stream=None):
     """Floating rows x [..., k] -> QuantRows: each row by its largest magnitude,
-    rounded to the nearest, ties to even."""
+    rounded to the nearest, ties to even. Not differentiable: train through
+    floating rows, which linear and gated take as they are."""
+    _constant("quantize_rows", x, "give linear and gated the floating rows")
     return _enqueued(x, stream, lambda: _quantize(x))
 
 
@@ -359,9 +364,26 @@ def _forward(x, W, pair, act, out_dtype, out):
     return ret
 
 
+_forward_ad = None      # torch.autograd.forward_ad, from the first call on
+
+
 def _wants_grad(x):
-    torch = _torch()
-    return isinstance(x, torch.Tensor) and x.requires_grad and torch.is_grad_enabled()
+    global _forward_ad
+    requires = getattr(x, "requires_grad", None)
+    if requires is None:        # not a tensor
+        return False
+    if _forward_ad is None:
+        _forward_ad = _torch().autograd.forward_ad
+    # outside of its levels nothing has a tangent (asking for one takes 0.3 us)
+    if getattr(_forward_ad, "_current_level", 0) >= 0 and _forward_ad.unpack_dual(x).tangent is not None:
+        raise HipGemmError("the scaled operators have no forward-mode derivative")
+    return requires and _torch().is_grad_enabled()
+
+
+def _constant(name, x, instead):
+    """Refuses an input whose gradient would be left out silently."""
+    if _wants_grad(x):
+        raise HipGemmError("%s passes no gradient on to its input: %s, or detach it" % (name, instead))
 
 
 def _act_id(act):
@@ -402,6 +424,7 @@ def gated(x, W, *, act="silu", out_dtype=None, out=None, stream=None):
 def linear_grad(dy, W, *, out=None, stream=None):
     """dx = (dy * scale) . w^T, the gradient of `linear` in its rounded rows, for
     dy [..., n] of any floating type; dx [..., k] has the same."""
+    _constant("linear_grad", dy, "there is no second derivative")
     return _enqueued(dy, stream, lambda: _linear_grad(dy, W, out), out is None)
 
 
@@ -425,6 +448,7 @@ def gated_grad(dh, rows, W, *, act="silu", out=None, stream=None):
     QuantRows of the forward pass (quantize_rows of its x). dx [..., k] has dh's
     type."""
     a = _act_id(act)
+    _constant("gated_grad", dh, "there is no second derivative")
     return _enqueued(dh, stream, lambda: _gated_grad(dh, rows, W, a, out), out is None)
 
 
@@ -475,7 +499,7 @@ def _functions():
         class Gated(torch.autograd.Function):
             @staticmethod
             def forward(ctx, x, W, act, out_dtype):
-                rows = quantize_rows(x)
+                rows = _quantize(x)
                 ctx.W, ctx.act, ctx.dtype, ctx.shape = W, act, x.dtype, rows.shape
                 ctx.save_for_backward(rows.data, rows.scale)
                 return _forward(rows, W, True, _act_id(act), out_dtype or x.dtype, None)
