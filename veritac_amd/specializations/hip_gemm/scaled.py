@@ -493,7 +493,7 @@ def _functions():
             @staticmethod
             @torch.autograd.function.once_differentiable
             def backward(ctx, dy):
-                dx = linear_grad(_unit_stride(dy), ctx.W)
+                dx = linear_grad(_incoming(dy, ctx.dtype), ctx.W)
                 return dx.to(ctx.dtype), None, None
 
         class Gated(torch.autograd.Function):
@@ -509,16 +509,20 @@ def _functions():
             def backward(ctx, dh):
                 data, scale = ctx.saved_tensors
                 rows = QuantRows(data, scale, k=ctx.W.k, padded=True, shape=ctx.shape)
-                dx = gated_grad(_unit_stride(dh), rows, ctx.W, act=ctx.act)
+                dx = gated_grad(_incoming(dh, ctx.dtype), rows, ctx.W, act=ctx.act)
                 return dx.to(ctx.dtype), None, None, None
 
         _function_classes = Linear, Gated
     return _function_classes
 
 
-def _unit_stride(d):
-    """An incoming gradient as rows: autograd may hand a broadcast or transposed
-    one."""
+def _incoming(d, dtype):
+    """An incoming gradient as rows (autograd may hand a broadcast or transposed
+    one), of a type that holds both its values and the gradient of `dtype` that
+    is made of them: an output of fewer bits or less range than x takes neither
+    from x's gradient."""
+    if d.dtype != dtype:
+        d = d.to(_torch().promote_types(d.dtype, dtype))
     if d.dim() and (d.stride(-1) != 1 or not d.is_contiguous()):
         return d.contiguous()
     return d
