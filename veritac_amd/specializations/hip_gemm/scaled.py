@@ -328,6 +328,8 @@ def _output(name, out, m, cols, lead, dtype, device, like=None):
 
 
 def _forward(x, W, pair, act, out_dtype, out):
+    if out is not None and not isinstance(out, _torch().Tensor):
+        raise HipGemmError("out must be a torch tensor (got %s)" % type(out).__name__)
     if isinstance(x, QuantRows):
         data, k = x.data, x.k
         _gpu("x", data)
@@ -387,7 +389,7 @@ def _constant(name, x, instead):
 
 
 def _act_id(act):
-    if act not in _lib.ACT_IDS:
+    if not isinstance(act, str) or act not in _lib.ACT_IDS:
         raise HipGemmError("act must be one of %s (got %r)" % (list(ACTIVATIONS), act))
     return _lib.ACT_IDS[act]
 
