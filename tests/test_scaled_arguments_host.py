@@ -65,3 +65,30 @@ def test_packed_weights_have_their_size():
                        (lambda: weight(k=-1), "K")):
         with pytest.raises(HipGemmError, match=what):
             call()
+
+
+def test_packing_needs_operands_apart_and_aligned():
+    lib, p = _lib.load_library(), 1 << 20
+    K, N = 64, 32
+    ok = dict(W0=p, W1=None, ld0=N, ld1=0, s0=2 * p, s1=None, bias=3 * p, Bp=4 * p, meta=5 * p)
+    pair = dict(ok, W1=6 * p, ld1=N, s1=7 * p, bias=None)
+    at = {"W0": K * N - 4, "W1": K * N - 4, "s0": 4 * N - 4, "s1": 4 * N - 4, "bias": 4 * N - 4}      # last elements
+
+    def call(a):
+        return lib.vt_scaled_pack(a["W0"], a["W1"], a["ld0"], a["ld1"], a["s0"], a["s1"], a["bias"], K, N, a["Bp"], a["meta"],
+                                  None)
+    for base, names in ((ok, ("W0", "s0", "bias", "Bp")), (pair, ("W0", "W1", "s0", "s1", "Bp"))):
+        for name in names:
+            assert call(dict(base, **{name: base["meta"] - (at.get(name, 128 * 64 - 16) // 16 * 16)})) == _lib.VT_EINVAL, name
+            if name[0] in "sb":
+                assert call(dict(base, **{name: base[name] + 2})) == _lib.VT_EINVAL, name
+                assert call(dict(base, **{name: base["Bp"]})) == _lib.VT_EINVAL, name
+    assert lib.vt_scaled_linear(p, _lib.TYPE_I8, 64, 2 * p + 1, 4, 64, 3 * p, 4 * p, 32, 5 * p, _lib.TYPE_F32, 32,
+                                None) == _lib.VT_EINVAL
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="no call here reaches a device")
+def test_packing_takes_operands_side_by_side():
+    lib, p = _lib.load_library(), 1 << 20
+    assert lib.vt_scaled_pack(p, None, 32, 0, p + 64 * 32, None, p + 64 * 32 + 128, 64, 32, 2 * p, 2 * p + 128 * 64,
+                              None) == _lib.VT_ENODEV

@@ -2009,6 +2009,7 @@ int check_scaled(const ScaledCall &c, bool *empty) {
   if ((c.X && overlaps(ey, ex)) || (c.Bp && overlaps(ey, eb)) || overlaps(ey, em))
     return fail(VT_EINVAL, "%s: the output overlaps an input in memory", c.who);
   if (c.T) {
+    if ((uintptr_t)c.T % 4) return fail(VT_EINVAL, "%s: scales are not aligned to their elements", c.who);
     if (!operand_extent(c.T, 1, 0, 1, 0, c.M, 4, &et)) return fail(VT_EINVAL, "%s: extent beyond 2^56 bytes", c.who);
     if (overlaps(ey, et)) return fail(VT_EINVAL, "%s: the output overlaps an input in memory", c.who);
   }
@@ -2170,8 +2171,16 @@ int vt_scaled_pack(const int8_t *W0, const int8_t *W1, int64_t ldw0, int64_t ldw
   if (!operand_extent(W0, 1, 0, K, ldw0, N, 1, &e0) || !operand_extent(Bp, 1, 0, 1, 0, size, 1, &eb) ||
       (pair && !operand_extent(W1, 1, 0, K, ldw1, N, 1, &e1)))
     return fail(VT_EINVAL, "vt_scaled_pack: extent beyond 2^56 bytes");
+  if ((uintptr_t)s0 % 4 || (uintptr_t)s1 % 4 || (uintptr_t)bias % 4)
+    return fail(VT_EINVAL, "vt_scaled_pack: scales and bias need their elements' alignment");
   if (K > 0 && (overlaps(e0, eb) || (pair && overlaps(e1, eb))))
     return fail(VT_EINVAL, "vt_scaled_pack: Bp overlaps the weights in memory");
+  Extent em, ev;
+  bool shared = !operand_extent(meta, 1, 0, 1, 0, scaled_meta(Np), 4, &em) ||
+                (K > 0 && (overlaps(em, eb) || overlaps(em, e0) || (pair && overlaps(em, e1))));
+  for (const float *v : {s0, s1, bias})
+    if (v) shared |= !operand_extent(v, 1, 0, 1, 0, N, 4, &ev) || overlaps(ev, em) || (K > 0 && overlaps(ev, eb));
+  if (shared) return fail(VT_EINVAL, "vt_scaled_pack: meta shares memory with another operand, or scales with Bp");
   Scratch scr;
   if (int rc = open_scratch(stream, &scr)) return rc;
   const ScaledPackArgs a = {W0, W1, s0, s1, bias, Bp, meta, ldw0, ldw1, (int)K, (int)N, (int)Kp, (int)Np};
