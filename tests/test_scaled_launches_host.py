@@ -1,7 +1,12 @@
 """What the scaled operators launch, on the CPU: their host code runs against a HIP runtime that only logs
 (fake_hip.cpp). Operand addresses are made up and never read."""
+import re
+import subprocess
+
 import pytest
 
+from scaled_cases import CASES
+from veritac_amd import _lib
 from test_workspaces_host import run  # noqa: F401
 
 CALLS = """
@@ -39,3 +44,40 @@ print(json.dumps([e[3] for e in launches()]))
 """ % (op, kind, ldx))
     assert "finish_kernel" in seen[-1] and len(seen) == (1 if kind.startswith("I8") else 2)
     assert all(int(e.split(" ")[0]) > 0 for e in seen)
+
+
+def compiled():
+    """The operators' kernels in the built library, by the stubs that launch them (packing aside)."""
+    text = subprocess.run(["nm", _lib.load_library()._name], check=True, capture_output=True, text=True).stdout
+    found = set()
+    for stub in re.findall(r"\S*__device_stub__\S+", text):
+        if re.search("scaled_skinny|dma16_kernel.*ScaledTile|mfma_kernel.*ScaledTile|grad_dma|grad_sum|quant_rows|pad_rows|"
+                     "row_terms|finish_kernel|zero_rows", stub):
+            found.add(re.sub(r"(\d+)__device_stub__", lambda m: str(int(m.group(1)) - 15), stub))
+    return found
+
+
+# sizes that need none of the products
+SIMPLE = """
+linear(300, 100, 70, x=I8)
+linear_grad(3, 64, 0)
+"""
+
+
+def test_every_kernel_has_a_case(run):
+    """The cases that the GPU tests check reach every kernel that is built, so none stays that no call reaches
+    and a change of the rules that choose them cannot leave one untested."""
+    seen = run(CALLS + SIMPLE + """
+kinds = {"f32": F32, "f16": F16, "bf16": BF16}
+for op, m, k, n, t, rows in %r:
+    x = I8 if rows == "i8" else kinds[t]
+    if op == "linear": linear(m, k, n, x=x, y=kinds[t])
+    elif op == "gated": gated(m, k, n, x=x, y=kinds[t])
+    elif op == "linear_grad": linear_grad(m, k, n, kinds[t])
+    else: gated_grad(m, k, n, kinds[t])
+import json
+print(json.dumps(sorted({e[3].split(" ")[1] for e in launches()})))
+""" % (CASES,))
+    names = compiled()
+    assert len(names) > 90
+    assert not names - set(seen), sorted(names - set(seen))

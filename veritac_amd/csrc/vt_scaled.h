@@ -1660,7 +1660,7 @@ TilePlan tile_plan(bool terms, int64_t M, int64_t Np, int64_t Kp, int cus) {
     offer(256, 256, 1, true);
     offer(256, 128, 1, true);
   }
-  offer(128, 128, 1, false);
+  if (Kp > 128) offer(128, 128, 1, false);   // their kernel is built for more than one pair of slices
   offer(64, 128, 1, false);
   for (int ks = 2; ks <= 16; ++ks)
     if (Kp % (128 * ks) == 0 && Kp / ks >= 512) offer(128, 128, ks, false);
@@ -1712,7 +1712,6 @@ int launch_scaled(const Rows &rows, const int8_t *Bp, int64_t Kp, const ScaledOu
     return launch_finish((const int32_t *)w, plan.ks, out, s);
   }
   const GemmArgs a = scaled_args(rows, Bp, M, Kp, Np, plan.bm, plan.bn);
-  const bool short_k = Kp <= 128;
   if (plan.persistent) {
     const int64_t wgs = std::min<int64_t>(plan.tiles, cus);
     if (plan.bn == 256) launch_dma16<OP, 256>(a, o, wgs, s);
@@ -1720,11 +1719,10 @@ int launch_scaled(const Rows &rows, const int8_t *Bp, int64_t Kp, const ScaledOu
   } else {
     const dim3 grid((unsigned)plan.tiles);
     if (plan.bm == 64) {
-      if (short_k) hipLaunchKernelGGL((gemm_mfma_kernel<64, 128, 1, false, true, false, true, ScaledTile<OP>>), grid, dim3(256), 0, s, a, out);
+      if (Kp <= 128) hipLaunchKernelGGL((gemm_mfma_kernel<64, 128, 1, false, true, false, true, ScaledTile<OP>>), grid, dim3(256), 0, s, a, out);
       else hipLaunchKernelGGL((gemm_mfma_kernel<64, 128, 1, false, false, false, true, ScaledTile<OP>>), grid, dim3(256), 0, s, a, out);
     } else {
-      if (short_k) hipLaunchKernelGGL((gemm_mfma_kernel<128, 128, 1, false, true, false, true, ScaledTile<OP>>), grid, dim3(256), 0, s, a, out);
-      else hipLaunchKernelGGL((gemm_mfma_kernel<128, 128, 1, false, false, false, true, ScaledTile<OP>>), grid, dim3(256), 0, s, a, out);
+      hipLaunchKernelGGL((gemm_mfma_kernel<128, 128, 1, false, false, false, true, ScaledTile<OP>>), grid, dim3(256), 0, s, a, out);
     }
   }
   VT_HIP_CHECK(hipGetLastError());
