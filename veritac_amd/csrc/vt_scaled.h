@@ -1518,6 +1518,11 @@ constexpr int64_t kScaledMaxK = 131071;
 constexpr int64_t kScaledMaxM = ((int64_t)1 << 24) - 1;
 // Packed columns: a tile's 256 rows of float16 terms stay within 32-bit offsets.
 constexpr int64_t kScaledMaxN = 65535 * 64;
+// Bytes of int8 rows, of gradient terms or of partial sums that a call keeps at
+// once: calls of more take their rows in parts, and split contractions less. (A
+// part is 1 ms of work and more: 8192 x 4096 over 2 x 14336 float32 gradients in
+// two parts of 470 MB.)
+constexpr int64_t kScaledBytes = (int64_t)512 << 20;
 // Pitch of int8 rows from which on they are copied before the products.
 constexpr int64_t kFarRows = (int64_t)1 << 23;
 
@@ -1889,6 +1894,7 @@ GradGeom grad_geom(int64_t M, int64_t Kp, int64_t slices, int cus) {
   double least = 0;
   for (const auto &t : kTiles)
     for (int splits = 1; splits <= 32 && splits <= slices; splits += splits < 8 ? 1 : splits / 4) {
+      if (splits > 1 && splits * M * Kp * 4 > kScaledBytes) break;
       const int64_t wgs = (M + t.bm - 1) / t.bm * ((Kp + 255) / 256) * splits, rounds = (wgs + cus - 1) / cus;
       const double slice = t.idle + (t.busy - t.idle) * std::min(1.0, (double)wgs / cus);
       double us = (double)rounds * (double)((slices + splits - 1) / splits) * slice + t.around + (double)(rounds - 1) * t.next;
@@ -2023,11 +2029,26 @@ int open_scratch(void *stream, Scratch *scr) {
   return VT_OK;
 }
 
-int forward(const ScaledCall &c, int act, void *stream) {
-  bool empty = false;
-  if (int rc = check_scaled(c, &empty)) return rc;
-  if (act != VT_ACT_SILU && act != VT_ACT_GELU) return fail(VT_EINVAL, "%s: unknown activation %d", c.who, act);
-  if (empty) return VT_OK;
+// Rows that a call of M takes at a time, whose workspaces hold row_bytes each:
+// parts of equal numbers of whole tiles, 64 rows at least.
+int64_t rows_at_once(int64_t M, int64_t row_bytes) {
+  const int64_t tile = 256 * row_bytes <= kScaledBytes ? 256 : 64;
+  const int64_t most = std::max(kScaledBytes / row_bytes / tile * tile, tile);
+  if (M <= most) return M;
+  const int64_t parts = (M + most - 1) / most;
+  return ((M + parts - 1) / parts + tile - 1) / tile * tile;
+}
+
+// Rows [r, r + rows) of a call.
+ScaledCall part_of(ScaledCall c, int64_t r, int64_t rows) {
+  if (c.X) c.X = (const int8_t *)c.X + r * c.ldx * elem_size(c.x_type);
+  if (c.T) c.T += r;
+  c.Y = (int8_t *)c.Y + r * c.ldy * elem_size(c.y_type);
+  c.M = rows;
+  return c;
+}
+
+int forward_rows(const ScaledCall &c, int act, void *stream) {
   Scratch scr;
   if (int rc = open_scratch(stream, &scr)) return rc;
   const int64_t Kp = scaled_kp(c.K), Np = scaled_np(c.N, c.pair);
@@ -2048,39 +2069,37 @@ int forward(const ScaledCall &c, int act, void *stream) {
   return c.pair ? launch_scaled<kGated>(rows, c.Bp, Kp, o, scr) : launch_scaled<kLinear>(rows, c.Bp, Kp, o, scr);
 }
 
-// The gradient in x^: D [M][ldd] of N columns, X the output [M][ldx] of K.
-int backward(const ScaledCall &c, const int8_t *Q, int q_type, int64_t ldq, const float *t, int act, void *stream) {
+int forward(const ScaledCall &c, int act, void *stream) {
   bool empty = false;
   if (int rc = check_scaled(c, &empty)) return rc;
   if (act != VT_ACT_SILU && act != VT_ACT_GELU) return fail(VT_EINVAL, "%s: unknown activation %d", c.who, act);
-  if (!float_type(c.x_type) || c.x_type != c.y_type)
-    return fail(VT_EINVAL, "%s: the gradients have one floating type", c.who);
-  const int64_t Kp = scaled_kp(c.K), Np = scaled_np(c.N, c.pair);
-  if (c.pair) {
-    if (q_type != VT_TYPE_I8 && q_type != VT_TYPE_I8_PADDED)
-      return fail(VT_EINVAL, "%s: the rows are int8 with scales", c.who);
-    if (!empty) {
-      ScaledCall r = c;   // the same checks of the int8 rows against the output
-      r.X = Q; r.x_type = q_type; r.ldx = ldq; r.xc = c.K; r.T = t;
-      if (int rc = check_scaled(r, &empty)) return rc;
-    }
-  }
   if (empty) return VT_OK;
+  const bool copied = !rows_in_place(c.X, c.x_type, c.ldx, c.K);
+  const int64_t step = copied ? rows_at_once(c.M, scaled_kp(c.K) + 4) : c.M;
+  for (int64_t r = 0; r < c.M; r += step)
+    if (int rc = forward_rows(part_of(c, r, std::min(step, c.M - r)), act, stream)) return rc;
+  return VT_OK;
+}
+
+// Terms in float16, normalised by row, and in a second half what float16
+// leaves of each: two products, 22 bits. Only bfloat16 gradients do without:
+// their own rounding to 8 bits is 8 times that of an 11-bit term, so the error
+// grows by 1 / 128 (1.7e-3 of the result's norm either way, 4096^3), and the
+// second product would double the largest part of the call. Float16 gradients
+// have as many bits as such a term: one half alone gave 1.4 times their error.
+bool two_halves(int type) { return type != VT_TYPE_BF16; }
+
+int backward_rows(const ScaledCall &c, const int8_t *Q, int q_type, int64_t ldq, const float *t, int act, void *stream) {
   Scratch scr;
   if (int rc = open_scratch(stream, &scr)) return rc;
   hipStream_t s = (hipStream_t)stream;
+  const int64_t Kp = scaled_kp(c.K), Np = scaled_np(c.N, c.pair);
   ScaledOut o = {};
   o.Y = c.Y; o.ldy = c.ldy;
   o.M = (int)c.M; o.N = (int)c.K; o.Np = (int)Kp;
   o.type = c.y_type;
   if (Np == 0) return launch_zero(o, s);
-  // Terms in float16, normalised by row, and in a second half what float16
-  // leaves of each: two products, 22 bits. Only bfloat16 gradients do without:
-  // their own rounding to 8 bits is 8 times that of an 11-bit term, so the error
-  // grows by 1 / 128 (1.7e-3 of the result's norm either way, 4096^3), and the
-  // second product would double the largest part of the call. Float16 gradients
-  // have as many bits as such a term: one half alone gave 1.4 times their error.
-  const bool split = c.x_type != VT_TYPE_BF16;
+  const bool split = two_halves(c.x_type);
   const int64_t lo = split ? c.M * Np : 0;
   void *w = nullptr;
   const size_t t_bytes = ((size_t)c.M * Np * 2 * (split ? 2 : 1) + 255) / 256 * 256;
@@ -2104,6 +2123,33 @@ int backward(const ScaledCall &c, const int8_t *Q, int q_type, int64_t ldq, cons
   o.norm = norm;
   const GradArgs g = {terms, c.Bp, lo, (int)c.M, (int)Kp, (int)Np, 0, 0, 0, split ? 2 : 1, 1};
   return launch_grad(g, o, scr);
+}
+
+// The gradient in x^: D [M][ldd] of N columns, X the output [M][ldx] of K.
+int backward(const ScaledCall &c, const int8_t *Q, int q_type, int64_t ldq, const float *t, int act, void *stream) {
+  bool empty = false;
+  if (int rc = check_scaled(c, &empty)) return rc;
+  if (act != VT_ACT_SILU && act != VT_ACT_GELU) return fail(VT_EINVAL, "%s: unknown activation %d", c.who, act);
+  if (!float_type(c.x_type) || c.x_type != c.y_type)
+    return fail(VT_EINVAL, "%s: the gradients have one floating type", c.who);
+  if (c.pair) {
+    if (q_type != VT_TYPE_I8 && q_type != VT_TYPE_I8_PADDED)
+      return fail(VT_EINVAL, "%s: the rows are int8 with scales", c.who);
+    if (!empty) {
+      ScaledCall r = c;   // the same checks of the int8 rows against the output
+      r.X = Q; r.x_type = q_type; r.ldx = ldq; r.xc = c.K; r.T = t;
+      if (int rc = check_scaled(r, &empty)) return rc;
+    }
+  }
+  if (empty) return VT_OK;
+  int64_t row_bytes = scaled_np(c.N, c.pair) * (two_halves(c.x_type) ? 4 : 2) + 4;
+  if (c.pair && !rows_in_place(Q, q_type, ldq, c.K)) row_bytes = std::max(row_bytes, scaled_kp(c.K) + 4);
+  const int64_t step = rows_at_once(c.M, row_bytes);
+  for (int64_t r = 0; r < c.M; r += step)
+    if (int rc = backward_rows(part_of(c, r, std::min(step, c.M - r)), c.pair ? Q + r * ldq : nullptr, q_type, ldq,
+                               c.pair ? t + r : nullptr, act, stream))
+      return rc;
+  return VT_OK;
 }
 
 }  // namespace
