@@ -493,7 +493,8 @@ int vt_gemm_i8_packed(const int8_t *A, const int8_t *Bp, const int32_t *D, int32
  * to 131071 (sums of int32), M up to 2^24 - 1.
  *
  * Intermediate rows, sums and terms live in per-stream workspaces, as
- * vt_gemm_i8's do (a call made once on a stream may be captured there).
+ * vt_gemm_i8's do (a call made once on a stream may be captured there), at most
+ * 512 MiB of each for a call: one of more rows takes them in parts.
  */
 #define VT_TYPE_F32 1
 #define VT_TYPE_F16 2
