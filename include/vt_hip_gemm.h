@@ -547,6 +547,43 @@ int vt_scaled_gated_grad(const void *dH, int32_t type, int64_t ldd, const int8_t
                          int64_t ldx, void *stream);
 
 /*
+ * Norms in front of the scaled operators.
+ *
+ *   h_ij = x_ij + r_ij, rounded to the type (x without R)
+ *   y_ij = h_ij gain_j / sqrt(mean_j h_ij^2 + eps)
+ *
+ * vt_norm: X [M][ldx], the residual R [M][ldr] (null: none; H is null then
+ * too) -> H [M][ldh] and Y [M][ldy] of the same floating type, or (T given) Y
+ * as the int8 rows that vt_quant_rows would make of y, with their scales T [M]:
+ * Y [M][ldy] of vt_quant_pitch(K) bytes, 16-byte aligned. gain [K] is float32 or
+ * of the type. eps >= 0. Squares are summed in float32; a row whose squares leave
+ * its range is scaled by a power of two first. A row that holds NaN or an
+ * infinity gives NaN where 32-bit arithmetic does, and int8 rows of scale NaN.
+ *
+ * vt_norm_grad: dY and H as above, and (or null) the gradient dH of h from
+ * elsewhere -> dX, the gradient of x and of r, and (or null) dgain [K] of the
+ * gain's type:
+ *   dx_ij = (z_ij - n_ij mean_j(z_ij n_ij)) / sqrt(..) + dh_ij
+ *   dgain_j = sum_i dy_ij n_ij,  z = dy gain, n = h / sqrt(..)
+ * Partial sums of dgain live in a per-stream workspace and are added in one
+ * order: results repeat bit for bit. M = 0 gives dgain = 0.
+ *
+ * vt_dequant_rows: Y [M][ldy] = Q [M][ldq] of K columns times T [M], rounded to
+ * y_type. No output may share memory with another operand, but for H, which
+ * may be R itself (same base and pitch).
+ */
+int vt_norm(const void *X, int64_t ldx, const void *R, int64_t ldr, int32_t type, const void *gain,
+            int32_t gain_type, float eps, void *H, int64_t ldh, void *Y, int64_t ldy, float *T,
+            int64_t M, int64_t K, void *stream);
+
+int vt_norm_grad(const void *dY, int64_t ldd, const void *H, int64_t ldh, const void *dH,
+                 int64_t lde, int32_t type, const void *gain, int32_t gain_type, float eps,
+                 void *dX, int64_t ldx, void *dgain, int64_t M, int64_t K, void *stream);
+
+int vt_dequant_rows(const int8_t *Q, int64_t ldq, const float *T, void *Y, int32_t y_type,
+                    int64_t ldy, int64_t M, int64_t K, void *stream);
+
+/*
  * Run-time compiled loop-nest kernels.
  *
  * The reference turns a loop nest (its `Stmt` JSON, README.md:456-503) into

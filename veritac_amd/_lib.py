@@ -42,7 +42,8 @@ EXPORTS = ("vt_gemm_i8", "vt_gemm_i8_noalloc", "vt_gemm_check", "vt_gemm_route",
            "vt_device_query", "vt_packed_b_size", "vt_pack_b_i8", "vt_gemm_i8_packed",
            "vt_rtc_compile", "vt_rtc_code_size", "vt_rtc_launch", "vt_rtc_release",
            "vt_quant_pitch", "vt_quant_rows", "vt_scaled_size", "vt_scaled_pack", "vt_scaled_linear",
-           "vt_scaled_gated", "vt_scaled_linear_grad", "vt_scaled_gated_grad")
+           "vt_scaled_gated", "vt_scaled_linear_grad", "vt_scaled_gated_grad",
+           "vt_norm", "vt_norm_grad", "vt_dequant_rows")
 
 # Replay operation codes and status codes (VT_REPLAY_* in include/vt_hip_gemm.h).
 REPLAY_MVIN, REPLAY_LATCH_B, REPLAY_COMPUTE, REPLAY_MVOUT = 1, 2, 3, 4
@@ -153,6 +154,13 @@ def _declare(lib):
     lib.vt_scaled_gated_grad.argtypes = [p, i32, i64, p, i32, i64, p, i64, i64, p, p, i64, i32, p,
                                          i64, p]
     lib.vt_scaled_gated_grad.restype = ctypes.c_int
+    f32 = ctypes.c_float
+    lib.vt_norm.argtypes = [p, i64, p, i64, i32, p, i32, f32, p, i64, p, i64, p, i64, i64, p]
+    lib.vt_norm.restype = ctypes.c_int
+    lib.vt_norm_grad.argtypes = [p, i64, p, i64, p, i64, i32, p, i32, f32, p, i64, p, i64, i64, p]
+    lib.vt_norm_grad.restype = ctypes.c_int
+    lib.vt_dequant_rows.argtypes = [p, i64, p, p, i32, i64, i64, i64, p]
+    lib.vt_dequant_rows.restype = ctypes.c_int
     u32 = ctypes.c_uint32
     lib.vt_rtc_launch.argtypes = [p, u32, u32, u32, u32, u32, u32, ctypes.POINTER(p), p]
     lib.vt_rtc_launch.restype = ctypes.c_int

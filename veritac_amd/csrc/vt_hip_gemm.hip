@@ -4715,3 +4715,4 @@ void vt_rtc_release(vt_rtc_program *p) {
 }  // extern "C"
 
 #include "vt_scaled.h"
+#include "vt_norm.h"

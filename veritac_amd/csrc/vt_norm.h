@@ -1,0 +1,594 @@
+// vt_norm.h -- root-mean-square norm of rows, with the residual's addition in
+// front and int8 rows with scales, or rows of x's type, behind, and its
+// gradients. Part of vt_hip_gemm.hip's translation unit, after vt_scaled.h.
+//
+//   h_ij = x_ij + r_ij, rounded to x's type (x itself without r)
+//   y_ij = h_ij g_j / sqrt(mean_j h_ij^2 + eps)
+//   rows: z = h g, top_i = max_j |z_ij|, q = round(z (127 / top)), t = top / 127 / sqrt(..)
+//   dx_ij = (z_ij - n_ij mean_j(z_ij n_ij)) / sqrt(..) + dh_ij, z = dy g, n = h / sqrt(..)
+//   dg_j = sum_i dy_ij n_ij
+//
+// A row's int8 values do not depend on its norm, which is a factor of its scale
+// only, so one reduction (of the squares' sum and the largest |z|) serves both.
+// Everything is float32 between the loads and the one rounding at the store.
+
+namespace {
+
+// 8 elements of a row from `pos`, zero past `len`, as 16-byte vectors at any
+// alignment where all 8 are there.
+template <int TYPE>
+__device__ __forceinline__ void load8(const typename Elem<TYPE>::T *row, int64_t pos, int64_t len, float (&v)[8]) {
+  typedef typename Elem<TYPE>::T T;
+  constexpr int PER = 16 / sizeof(T);
+  if (pos + 8 <= len) {
+    typedef T VT __attribute__((ext_vector_type(PER), aligned(sizeof(T))));
+#pragma unroll
+    for (int i = 0; i < 8 / PER; ++i) {
+      const VT x = *(const VT *)(row + pos + i * PER);
+#pragma unroll
+      for (int e = 0; e < PER; ++e) v[i * PER + e] = (float)x[e];
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = pos + e < len ? (float)row[pos + e] : 0.0f;
+  }
+}
+
+template <int TYPE>
+__device__ __forceinline__ void store8(typename Elem<TYPE>::T *row, int64_t pos, int64_t len, const float (&v)[8]) {
+  typedef typename Elem<TYPE>::T T;
+  constexpr int PER = 16 / sizeof(T);
+  if (pos + 8 <= len) {
+    typedef T VT __attribute__((ext_vector_type(PER), aligned(sizeof(T))));
+#pragma unroll
+    for (int i = 0; i < 8 / PER; ++i) {
+      VT x;
+#pragma unroll
+      for (int e = 0; e < PER; ++e) x[e] = (T)v[i * PER + e];
+      *(VT *)(row + pos + i * PER) = x;
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (pos + e < len) row[pos + e] = (T)v[e];
+  }
+}
+
+// The norm's weights, float32 or of the rows' type.
+template <int TYPE>
+__device__ __forceinline__ void load_gain(const void *g, bool wide, int64_t pos, int64_t len, float (&v)[8]) {
+  if (wide || TYPE == kF32) load8<kF32>((const float *)g, pos, len, v);
+  else load8<TYPE>((const typename Elem<TYPE>::T *)g, pos, len, v);
+}
+
+// Sum and maximum over a workgroup, of two values at once.
+template <int THREADS, class A, class B, class FA, class FB>
+__device__ __forceinline__ void block_two(A &a, B &b, FA fa, FB fb, uint64_t *red) {
+#pragma unroll
+  for (int o = 32; o; o >>= 1) {
+    a = fa(a, __builtin_bit_cast(A, __shfl_xor(__builtin_bit_cast(int, a), o)));
+    b = fb(b, __builtin_bit_cast(B, __shfl_xor(__builtin_bit_cast(int, b), o)));
+  }
+  if constexpr (THREADS > 64) {
+    if ((threadIdx.x & 63) == 0)
+      red[threadIdx.x >> 6] = (uint64_t)__builtin_bit_cast(uint32_t, a) << 32 | __builtin_bit_cast(uint32_t, b);
+    __syncthreads();
+    uint64_t w = red[0];
+    a = __builtin_bit_cast(A, (uint32_t)(w >> 32));
+    b = __builtin_bit_cast(B, (uint32_t)w);
+#pragma unroll
+    for (int i = 1; i < THREADS / 64; ++i) {
+      w = red[i];
+      a = fa(a, __builtin_bit_cast(A, (uint32_t)(w >> 32)));
+      b = fb(b, __builtin_bit_cast(B, (uint32_t)w));
+    }
+    __syncthreads();   // red is the next row's after this
+  }
+}
+
+__device__ __forceinline__ float add_f(float a, float b) { return a + b; }
+__device__ __forceinline__ uint32_t max_u(uint32_t a, uint32_t b) { return max(a, b); }
+
+// The power of two that a row is scaled by: 1, unless the squares' sum has left
+// float32's range at the top, or is so small beside an eps of next to nothing
+// that squares were lost at the bottom.
+__device__ __forceinline__ float row_factor(float squares, float eps) {
+  if (magnitude(squares) >= kInfBits) return 0x1p-80f;
+  return squares < 0x1p-80f && eps < 0x1p-60f ? 0x1p80f : 1.0f;
+}
+
+// 1 / sqrt(mean + eps) of a row scaled by f, over f: n = (h f) * this.
+__device__ __forceinline__ float inverse_rms(float squares, float f, float k, float eps) {
+  return 1.0f / sqrtf(squares / k + eps * f * f);
+}
+
+struct NormArgs {
+  const void *X, *R, *G;   // R null: no residual
+  void *H, *Y;             // H: h, null without a residual; Y: [M][ldy] of the type, or int8 rows
+  float *T;                // scales of int8 rows, null: Y is floating
+  int64_t ldx, ldr, ldh, ldy, M, K, Kp;
+  float eps;
+  int gain32;
+};
+
+// A workgroup takes rows w, w + grid, ..; a thread holds NC pieces of 8 elements
+// of the row and of the gain in registers (NC = 0: longer rows, read again after
+// the reduction, and the gain with them). Bound by one read of x and r and one
+// write of h and y.
+template <int TYPE, int THREADS, int NC, bool ROWS>
+__global__ __launch_bounds__(THREADS) void norm_kernel(NormArgs p) {
+  __shared__ uint64_t red[THREADS / 64];
+  typedef typename Elem<TYPE>::T T;
+  constexpr int N = NC ? NC : 1;
+  const int tid = threadIdx.x;
+  float g[N][8];
+  auto pos_of = [&](int i) { return (int64_t)(tid + THREADS * i) * 8; };
+  if constexpr (NC > 0) {
+#pragma unroll
+    for (int i = 0; i < NC; ++i) load_gain<TYPE>(p.G, p.gain32, pos_of(i), p.K, g[i]);
+  }
+  for (int64_t row = blockIdx.x; row < p.M; row += gridDim.x) {
+    const T *x = (const T *)p.X + row * p.ldx, *r = (const T *)p.R + row * p.ldr;
+    // h of a piece, in x's precision; again: as the thread has stored it (over r, maybe)
+    auto load_h = [&](int64_t pos, float (&v)[8], bool again) {
+      if (again && p.H) {
+        load8<TYPE>((const T *)p.H + row * p.ldh, pos, p.K, v);
+        return;
+      }
+      load8<TYPE>(x, pos, p.K, v);
+      if (p.R) {
+        float w[8];
+        load8<TYPE>(r, pos, p.K, w);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = (float)(T)(v[e] + w[e]);
+      }
+    };
+    float v[N][8];
+    float squares = 0.0f;
+    uint32_t top = 0;
+    auto gather = [&](const float (&h)[8], const float (&w)[8], float f) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float a = h[e] * f;
+        squares = fmaf(a, a, squares);
+        if constexpr (ROWS) top = max(top, magnitude(a * w[e]));
+      }
+    };
+    auto all = [&](float f, bool first) {
+      squares = 0.0f;
+      top = 0;
+      if constexpr (NC > 0) {
+#pragma unroll
+        for (int i = 0; i < NC; ++i) gather(v[i], g[i], f);
+      } else {
+        for (int64_t pos = tid * 8; pos < p.K; pos += THREADS * 8) {
+          load_h(pos, v[0], !first);
+          if (first && p.H) store8<TYPE>((T *)p.H + row * p.ldh, pos, p.K, v[0]);
+          load_gain<TYPE>(p.G, p.gain32, pos, p.K, g[0]);
+          gather(v[0], g[0], f);
+        }
+      }
+      block_two<THREADS>(squares, top, add_f, max_u, red);
+    };
+    if constexpr (NC > 0) {
+#pragma unroll
+      for (int i = 0; i < NC; ++i) load_h(pos_of(i), v[i], false);
+      if (p.H) {
+#pragma unroll
+        for (int i = 0; i < NC; ++i) store8<TYPE>((T *)p.H + row * p.ldh, pos_of(i), p.K, v[i]);
+      }
+    }
+    all(1.0f, true);
+    const float f = row_factor(squares, p.eps);
+    if (f != 1.0f) all(f, false);
+    const float inv = inverse_rms(squares, f, (float)p.K, p.eps);
+    const RowScale s = row_scale(top);
+    if (ROWS && tid == 0) p.T[row] = p.K ? s.scale * inv : 0.0f;
+    auto put = [&](int64_t pos, const float (&h)[8], const float (&w)[8]) {
+      if constexpr (ROWS) {
+        if (pos >= p.Kp) return;
+        uint32_t b[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) b[e] = round_byte(h[e] * f * w[e], s.inv);
+        v2i o = {pack_bytes(b[0], b[1], b[2], b[3]), pack_bytes(b[4], b[5], b[6], b[7])};
+        if (s.inv == 0.0f) o = v2i{0, 0};
+        *(v2i *)((int8_t *)p.Y + row * p.ldy + pos) = o;
+      } else {
+        float y[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] = h[e] * f * w[e] * inv;
+        store8<TYPE>((T *)p.Y + row * p.ldy, pos, p.K, y);
+      }
+    };
+    if constexpr (NC > 0) {
+#pragma unroll
+      for (int i = 0; i < NC; ++i) put(pos_of(i), v[i], g[i]);
+    } else {
+      for (int64_t pos = tid * 8; pos < (ROWS ? p.Kp : p.K); pos += THREADS * 8) {
+        load_h(pos, v[0], true);
+        load_gain<TYPE>(p.G, p.gain32, pos, p.K, g[0]);
+        put(pos, v[0], g[0]);
+      }
+    }
+  }
+}
+
+struct NormGradArgs {
+  const void *D, *H, *G, *E;   // dy, h, the gain and the residual's own gradient (or null)
+  void *X;                     // dx
+  float *part;                 // [groups][K] partial sums of the gain's gradient, null: not wanted
+  float *stats;                // NC = 0: two floats a row
+  int64_t ldd, ldh, lde, ldx, M, K;
+  float eps;
+  int gain32;
+};
+
+// What dx needs of a row scaled by f: dx = inv f (z - h f c) + dh, n = h f inv.
+struct RowStats {
+  float f, inv, c;
+};
+
+// A workgroup takes rows w, w + grid, .. whole, and keeps its part of the gain's
+// gradient in registers over them.
+template <int TYPE, int THREADS, int NC>
+__global__ __launch_bounds__(THREADS) void norm_grad_kernel(NormGradArgs p) {
+  __shared__ uint64_t red[THREADS / 64];
+  typedef typename Elem<TYPE>::T T;
+  const int tid = threadIdx.x;
+  float g[NC][8], sum[NC][8];
+  auto pos_of = [&](int i) { return (int64_t)(tid + THREADS * i) * 8; };
+#pragma unroll
+  for (int i = 0; i < NC; ++i) {
+    load_gain<TYPE>(p.G, p.gain32, pos_of(i), p.K, g[i]);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum[i][e] = 0.0f;
+  }
+  for (int64_t row = blockIdx.x; row < p.M; row += gridDim.x) {
+    float d[NC][8], h[NC][8], x[NC][8];
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      load8<TYPE>((const T *)p.D + row * p.ldd, pos_of(i), p.K, d[i]);
+      load8<TYPE>((const T *)p.H + row * p.ldh, pos_of(i), p.K, h[i]);
+      if (p.E) load8<TYPE>((const T *)p.E + row * p.lde, pos_of(i), p.K, x[i]);
+    }
+    float squares, dot;
+    auto all = [&](float f) {
+      squares = dot = 0.0f;
+#pragma unroll
+      for (int i = 0; i < NC; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float a = h[i][e] * f;
+          squares = fmaf(a, a, squares);
+          dot = fmaf(d[i][e] * g[i][e], a, dot);
+        }
+      block_two<THREADS>(squares, dot, add_f, add_f, red);
+    };
+    all(1.0f);
+    const float f = row_factor(squares, p.eps);
+    if (f != 1.0f) all(f);
+    const float inv = inverse_rms(squares, f, (float)p.K, p.eps), c = dot / (float)p.K * inv * inv;
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float a = h[i][e] * f;
+        sum[i][e] = fmaf(d[i][e], a * inv, sum[i][e]);
+        const float y = (d[i][e] * g[i][e] - a * c) * (inv * f);
+        x[i][e] = p.E ? x[i][e] + y : y;
+      }
+      store8<TYPE>((T *)p.X + row * p.ldx, pos_of(i), p.K, x[i]);
+    }
+  }
+  if (p.part) {
+#pragma unroll
+    for (int i = 0; i < NC; ++i) store8<kF32>(p.part + blockIdx.x * p.K, pos_of(i), p.K, sum[i]);
+  }
+}
+
+// Rows too long for a workgroup's registers: first what dx needs of each row,
+template <int TYPE>
+__global__ __launch_bounds__(1024) void norm_stats_kernel(NormGradArgs p) {
+  __shared__ uint64_t red[16];
+  typedef typename Elem<TYPE>::T T;
+  const int64_t row = blockIdx.x;
+  float squares, dot;
+  auto all = [&](float f) {
+    squares = dot = 0.0f;
+    for (int64_t pos = threadIdx.x * 8; pos < p.K; pos += 8192) {
+      float d[8], h[8], g[8];
+      load8<TYPE>((const T *)p.D + row * p.ldd, pos, p.K, d);
+      load8<TYPE>((const T *)p.H + row * p.ldh, pos, p.K, h);
+      load_gain<TYPE>(p.G, p.gain32, pos, p.K, g);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float a = h[e] * f;
+        squares = fmaf(a, a, squares);
+        dot = fmaf(d[e] * g[e], a, dot);
+      }
+    }
+    block_two<1024>(squares, dot, add_f, add_f, red);
+  };
+  all(1.0f);
+  const float f = row_factor(squares, p.eps);
+  if (f != 1.0f) all(f);
+  if (threadIdx.x == 0) {
+    const float inv = inverse_rms(squares, f, (float)p.K, p.eps);
+    float *s = p.stats + row * 3;
+    s[0] = f;
+    s[1] = inv;
+    s[2] = dot / (float)p.K * inv * inv;
+  }
+}
+
+// then dx and the gain's gradient, 2048 columns of rows w, w + gridDim.x, .. each.
+template <int TYPE>
+__global__ __launch_bounds__(256) void norm_apply_kernel(NormGradArgs p) {
+  typedef typename Elem<TYPE>::T T;
+  const int64_t pos = ((int64_t)blockIdx.y * 256 + threadIdx.x) * 8;
+  float g[8], sum[8];
+  load_gain<TYPE>(p.G, p.gain32, pos, p.K, g);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) sum[e] = 0.0f;
+  for (int64_t row = blockIdx.x; row < p.M; row += gridDim.x) {
+    const float *s = p.stats + row * 3;
+    const float f = s[0], inv = s[1], c = s[2];
+    float d[8], h[8], x[8];
+    load8<TYPE>((const T *)p.D + row * p.ldd, pos, p.K, d);
+    load8<TYPE>((const T *)p.H + row * p.ldh, pos, p.K, h);
+    if (p.E) load8<TYPE>((const T *)p.E + row * p.lde, pos, p.K, x);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float a = h[e] * f;
+      sum[e] = fmaf(d[e], a * inv, sum[e]);
+      const float y = (d[e] * g[e] - a * c) * (inv * f);
+      x[e] = p.E ? x[e] + y : y;
+    }
+    store8<TYPE>((T *)p.X + row * p.ldx, pos, p.K, x);
+  }
+  if (p.part) store8<kF32>(p.part + blockIdx.x * p.K, pos, p.K, sum);
+}
+
+// The sums of `groups` rows of K partial sums, in one order: 64 columns a
+// workgroup, its four waves every fourth row, 8 loads in flight.
+struct GainSumArgs {
+  const float *part;
+  void *out;
+  int64_t K;
+  int groups, type;
+};
+
+__global__ __launch_bounds__(256) void gain_sum_kernel(GainSumArgs p) {
+  __shared__ float red[4][64];
+  const int c = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t col = (int64_t)blockIdx.x * 64 + c;
+  float s = 0.0f;
+  if (col < p.K) {
+    for (int i = wave; i < p.groups; i += 32) {
+      float v[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) v[u] = i + 4 * u < p.groups ? p.part[(int64_t)(i + 4 * u) * p.K + col] : 0.0f;
+#pragma unroll
+      for (int u = 0; u < 8; ++u) s += v[u];
+    }
+  }
+  red[wave][c] = s;
+  __syncthreads();
+  if (wave || col >= p.K) return;
+  s = (red[0][c] + red[1][c]) + (red[2][c] + red[3][c]);
+  if (p.type == VT_TYPE_F32) ((float *)p.out)[col] = s;
+  else ((uint16_t *)p.out)[col] = (uint16_t)pack16(s, 0.0f, p.type);
+}
+
+// int8 rows as the values they stand for.
+struct DequantArgs {
+  const int8_t *Q;
+  const float *T;
+  void *Y;
+  int64_t ldq, ldy, M, K;
+};
+
+template <int TYPE>
+__global__ __launch_bounds__(256) void dequant_kernel(DequantArgs p) {
+  typedef typename Elem<TYPE>::T T;
+  const int64_t pieces = (p.K + 7) / 8;
+  for (int64_t row = blockIdx.x; row < p.M; row += gridDim.x) {
+    const float t = p.T[row];
+    const int8_t *q = p.Q + row * p.ldq;
+    for (int64_t i = threadIdx.x; i < pieces; i += 256) {
+      const int64_t pos = i * 8;
+      typedef int8_t V8 __attribute__((ext_vector_type(8), aligned(1)));
+      float v[8];
+      if (pos + 8 <= p.K) {
+        const V8 b = *(const V8 *)(q + pos);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = (float)b[e] * t;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = pos + e < p.K ? (float)q[pos + e] * t : 0.0f;
+      }
+      store8<TYPE>((T *)p.Y + row * p.ldy, pos, p.K, v);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------
+
+// Workgroups for rows of `threads` threads each: as many as are resident at once.
+int64_t resident(int64_t rows, int threads, int cus) { return std::min<int64_t>(rows, (int64_t)cus * (2048 / threads)); }
+
+template <int TYPE, bool ROWS>
+void launch_norm_typed(const NormArgs &a, int cus, hipStream_t s) {
+  const int64_t k = ROWS ? a.Kp : a.K;
+  auto grid = [&](int threads) { return dim3((unsigned)resident(a.M, threads, cus)); };
+  if (k <= 512) hipLaunchKernelGGL((norm_kernel<TYPE, 64, 1, ROWS>), grid(64), dim3(64), 0, s, a);
+  else if (k <= 2048) hipLaunchKernelGGL((norm_kernel<TYPE, 256, 1, ROWS>), grid(256), dim3(256), 0, s, a);
+  else if (k <= 4096) hipLaunchKernelGGL((norm_kernel<TYPE, 512, 1, ROWS>), grid(512), dim3(512), 0, s, a);
+  else if (k <= 8192) hipLaunchKernelGGL((norm_kernel<TYPE, 1024, 1, ROWS>), grid(1024), dim3(1024), 0, s, a);
+  else if (k <= 16384) hipLaunchKernelGGL((norm_kernel<TYPE, 1024, 2, ROWS>), grid(1024), dim3(1024), 0, s, a);
+  else hipLaunchKernelGGL((norm_kernel<TYPE, 1024, 0, ROWS>), grid(1024), dim3(1024), 0, s, a);
+}
+
+template <int TYPE>
+int launch_norm(const NormArgs &a, int cus, hipStream_t s) {
+  if (a.T) launch_norm_typed<TYPE, true>(a, cus, s);
+  else launch_norm_typed<TYPE, false>(a, cus, s);
+  VT_HIP_CHECK(hipGetLastError());
+  return VT_OK;
+}
+
+// Longest rows whose gradients a workgroup holds in registers.
+constexpr int64_t kNormGradRow = 8192;
+
+template <int TYPE>
+int launch_norm_grad(NormGradArgs a, void *dgain, int gain_type, Scratch &scr) {
+  hipStream_t s = (hipStream_t)scr.stream;
+  const int cus = scr.st->num_cus;
+  const int threads = a.K <= 512 ? 64 : a.K <= 2048 ? 256 : a.K <= 4096 ? 512 : a.K <= kNormGradRow ? 1024 : 256;
+  // One workgroup more of a row's size costs the gain's sums a row more to read.
+  const int64_t groups = a.K <= kNormGradRow ? std::min<int64_t>(a.M, (int64_t)cus * (1024 / threads))
+                                             : std::min<int64_t>(a.M, std::max<int64_t>(1, cus * 8 / ((a.K + 2047) / 2048)));
+  void *w = nullptr;
+  if (dgain || a.K > kNormGradRow) {
+    const size_t part = dgain ? ((size_t)groups * a.K * sizeof(float) + 255) / 256 * 256 : 0;
+    const size_t stats = a.K > kNormGradRow ? (size_t)a.M * 3 * sizeof(float) : 0;
+    if (int rc = scr.take(kPartials, part + stats, &w)) return rc;
+    a.part = dgain ? (float *)w : nullptr;
+    a.stats = (float *)((int8_t *)w + part);
+  }
+  const dim3 grid((unsigned)groups);
+  if (a.M == 0) ;   // dgain = 0
+  else if (threads == 64) hipLaunchKernelGGL((norm_grad_kernel<TYPE, 64, 1>), grid, dim3(64), 0, s, a);
+  else if (a.K <= 2048) hipLaunchKernelGGL((norm_grad_kernel<TYPE, 256, 1>), grid, dim3(256), 0, s, a);
+  else if (threads == 512) hipLaunchKernelGGL((norm_grad_kernel<TYPE, 512, 1>), grid, dim3(512), 0, s, a);
+  else if (threads == 1024) hipLaunchKernelGGL((norm_grad_kernel<TYPE, 1024, 1>), grid, dim3(1024), 0, s, a);
+  else {
+    hipLaunchKernelGGL((norm_stats_kernel<TYPE>), dim3((unsigned)a.M), dim3(1024), 0, s, a);
+    VT_HIP_CHECK(hipGetLastError());
+    hipLaunchKernelGGL((norm_apply_kernel<TYPE>), dim3((unsigned)groups, (unsigned)((a.K + 2047) / 2048)), dim3(256), 0, s, a);
+  }
+  VT_HIP_CHECK(hipGetLastError());
+  if (!dgain) return VT_OK;
+  const GainSumArgs g = {a.part, dgain, a.K, (int)groups, gain_type};
+  hipLaunchKernelGGL(gain_sum_kernel, dim3((unsigned)((a.K + 63) / 64)), dim3(256), 0, s, g);
+  VT_HIP_CHECK(hipGetLastError());
+  return VT_OK;
+}
+
+// An operand of a call: [rows][ld] of `cols` elements of `elem` bytes, from a
+// base and rows aligned to `align` of them. Null and empty ones are left out.
+struct Operand {
+  const char *name;
+  const void *p;
+  int64_t rows, ld, cols, elem;
+  bool out;
+  int64_t align = 1;
+};
+
+// Pitches, alignment and extents of up to 16 operands, and that no output
+// shares memory with another operand.
+int check_operands(const char *who, const Operand *o, int count) {
+  Extent e[16];
+  for (int i = 0; i < count; ++i) {
+    if (!o[i].p || o[i].rows == 0 || o[i].cols == 0) continue;
+    if (o[i].rows > 1 && (o[i].ld < o[i].cols || o[i].ld > ((int64_t)1 << 40)))
+      return fail(VT_EINVAL, "%s: pitch of %s (%lld) must be %lld .. 2^40", who, o[i].name, (long long)o[i].ld, (long long)o[i].cols);
+    if ((uintptr_t)o[i].p % (o[i].elem * o[i].align) || (o[i].rows > 1 && o[i].ld % o[i].align))
+      return fail(VT_EINVAL, "%s: %s is not aligned to %lld bytes", who, o[i].name, (long long)(o[i].elem * o[i].align));
+    if (!operand_extent(o[i].p, 1, 0, o[i].rows, o[i].ld, o[i].cols, o[i].elem, &e[i]))
+      return fail(VT_EINVAL, "%s: extent of %s beyond 2^56 bytes", who, o[i].name);
+    for (int j = 0; j < i; ++j)
+      if (o[j].p && o[j].rows && o[j].cols && (o[i].out || o[j].out) && overlaps(e[i], e[j]))
+        return fail(VT_EINVAL, "%s: %s and %s share memory", who, o[j].name, o[i].name);
+  }
+  return VT_OK;
+}
+
+int check_norm_sizes(const char *who, int64_t M, int64_t K, int32_t type, int32_t gain_type, float eps) {
+  if (M < 0 || K < 0 || M > kScaledMaxM || K >= kScaledMax)
+    return fail(VT_EINVAL, "%s: needs 0 <= M <= %lld, 0 <= K < 2^30 (M=%lld K=%lld)", who, (long long)kScaledMaxM, (long long)M,
+                (long long)K);
+  if (!float_type(type)) return fail(VT_EINVAL, "%s: unknown type %d", who, (int)type);
+  if (gain_type != VT_TYPE_F32 && gain_type != type)
+    return fail(VT_EINVAL, "%s: the gain is float32 or of the rows' type (got %d)", who, (int)gain_type);
+  if (!(eps >= 0.0f) || eps > 3.0e38f) return fail(VT_EINVAL, "%s: eps must be a number of at least 0", who);
+  return VT_OK;
+}
+
+// f(the element type, at compile time).
+template <class F>
+int by_type(int type, F &&f) {
+  switch (type) {
+    case VT_TYPE_F32: return f(std::integral_constant<int, kF32>());
+    case VT_TYPE_F16: return f(std::integral_constant<int, kF16>());
+    default: return f(std::integral_constant<int, kBF16>());
+  }
+}
+
+}  // namespace
+
+extern "C" {
+
+int vt_norm(const void *X, int64_t ldx, const void *R, int64_t ldr, int32_t type, const void *gain, int32_t gain_type,
+            float eps, void *H, int64_t ldh, void *Y, int64_t ldy, float *T, int64_t M, int64_t K, void *stream) {
+  g_err.clear();
+  const char *who = "vt_norm";
+  if (int rc = check_norm_sizes(who, M, K, type, gain_type, eps)) return rc;
+  if (M == 0 || (K == 0 && !T)) return VT_OK;
+  if (K > 0 && (!X || !gain || !Y || !R != !H)) return fail(VT_EINVAL, "%s: an operand is null, or only one of R and H given", who);
+  const int64_t e = elem_size(type), Kp = scaled_kp(K);
+  const bool in_place = H == R && ldh == ldr;
+  const Operand o[] = {{"X", X, M, ldx, K, e, false}, {"R", in_place ? nullptr : R, M, ldr, K, e, false},
+                       {"gain", gain, 1, K, K, elem_size(gain_type), false}, {"H", H, M, ldh, K, e, true},
+                       {"Y", Y, M, ldy, T ? Kp : K, T ? 1 : e, true, T ? 16 : 1}, {"T", T, 1, M, M, 4, true}};
+  if (int rc = check_operands(who, o, 6)) return rc;
+  Scratch scr;
+  if (int rc = open_scratch(stream, &scr)) return rc;
+  const NormArgs a = {X, R, gain, H, Y, T, ldx, ldr, ldh, ldy, M, K, Kp, eps, gain_type == VT_TYPE_F32};
+  return by_type(type, [&](auto t) { return launch_norm<decltype(t)::value>(a, scr.st->num_cus, (hipStream_t)stream); });
+}
+
+int vt_norm_grad(const void *dY, int64_t ldd, const void *H, int64_t ldh, const void *dH, int64_t lde, int32_t type,
+                 const void *gain, int32_t gain_type, float eps, void *dX, int64_t ldx, void *dgain, int64_t M, int64_t K,
+                 void *stream) {
+  g_err.clear();
+  const char *who = "vt_norm_grad";
+  if (int rc = check_norm_sizes(who, M, K, type, gain_type, eps)) return rc;
+  if (K == 0 || (M == 0 && !dgain)) return VT_OK;
+  if (!gain || (M > 0 && (!dY || !H || !dX))) return fail(VT_EINVAL, "%s: an operand is null", who);
+  const int64_t e = elem_size(type), ge = elem_size(gain_type);
+  const Operand o[] = {{"dY", dY, M, ldd, K, e, false}, {"H", H, M, ldh, K, e, false}, {"dH", dH, M, lde, K, e, false},
+                       {"gain", gain, 1, K, K, ge, false}, {"dX", dX, M, ldx, K, e, true}, {"dgain", dgain, 1, K, K, ge, true}};
+  if (int rc = check_operands(who, o, 6)) return rc;
+  Scratch scr;
+  if (int rc = open_scratch(stream, &scr)) return rc;
+  const NormGradArgs a = {dY, H, gain, dH, dX, nullptr, nullptr, ldd, ldh, lde, ldx, M, K, eps, gain_type == VT_TYPE_F32};
+  return by_type(type, [&](auto t) { return launch_norm_grad<decltype(t)::value>(a, dgain, gain_type, scr); });
+}
+
+int vt_dequant_rows(const int8_t *Q, int64_t ldq, const float *T, void *Y, int32_t y_type, int64_t ldy, int64_t M, int64_t K,
+                    void *stream) {
+  g_err.clear();
+  const char *who = "vt_dequant_rows";
+  if (M < 0 || K < 0 || M > kScaledMaxM || K >= kScaledMax)
+    return fail(VT_EINVAL, "%s: needs 0 <= M <= %lld, 0 <= K < 2^30 (M=%lld K=%lld)", who, (long long)kScaledMaxM, (long long)M,
+                (long long)K);
+  if (!float_type(y_type)) return fail(VT_EINVAL, "%s: unknown output type %d", who, (int)y_type);
+  if (M == 0 || K == 0) return VT_OK;
+  if (!Q || !T || !Y) return fail(VT_EINVAL, "%s: an operand is null", who);
+  const Operand o[] = {{"Q", Q, M, ldq, K, 1, false}, {"T", T, 1, M, M, 4, false}, {"Y", Y, M, ldy, K, elem_size(y_type), true}};
+  if (int rc = check_operands(who, o, 3)) return rc;
+  Scratch scr;
+  if (int rc = open_scratch(stream, &scr)) return rc;
+  const DequantArgs a = {Q, T, Y, ldq, ldy, M, K};
+  const dim3 grid((unsigned)resident(M, 256, scr.st->num_cus));
+  return by_type(y_type, [&](auto t) {
+    hipLaunchKernelGGL((dequant_kernel<decltype(t)::value>), grid, dim3(256), 0, (hipStream_t)stream, a);
+    VT_HIP_CHECK(hipGetLastError());
+    return VT_OK;
+  });
+}
+
+}  // extern "C"

@@ -31,6 +31,7 @@ has unit stride.
 """
 from __future__ import annotations
 
+import contextlib
 import math
 
 from ... import _lib
@@ -90,9 +91,20 @@ class QuantRows:
     def device(self):
         return self.data.device
 
-    def dequantize(self):
-        """The rows as float32 [..., k]."""
-        return (self.data[:, :self.k].float() * self.scale[:, None]).reshape(self.shape)
+    def dequantize(self, dtype=None):
+        """The rows as float32 [..., k], or rounded to float16 or bfloat16."""
+        torch = _torch()
+        dtype = torch.float32 if dtype is None else dtype
+        if dtype not in _types():
+            raise HipGemmError("dtype must be float32, float16 or bfloat16 (got %s)" % (dtype,))
+        if self.data.device.type != "cuda":
+            return (self.data[:, :self.k].float() * self.scale[:, None]).reshape(self.shape).to(dtype)
+        y = torch.empty(self.shape, dtype=dtype, device=self.device)
+        with _on(self.device):
+            _lib.check(_lib.load_library().vt_dequant_rows(
+                self.data.data_ptr(), _pitch(self.data), self.scale.data_ptr(), y.data_ptr(), _types()[dtype],
+                max(self.k, 1), self.data.shape[0], self.k, _current_stream(self.device)), "vt_dequant_rows")
+        return y
 
     def __repr__(self):
         return "QuantRows(m=%d, k=%d, device=%s)" % (self.data.shape[0], self.k, self.device)
@@ -127,12 +139,12 @@ class ScaledWeight:
             self.k, self.n, "gated" if self.pair else "linear", self.device)
 
 
-def _enqueued(on, stream, call, record=True):
+def _enqueued(on, stream, call, record=True, held=()):
     """call(), with the raw handle `stream` as torch's current stream of the device
     of `on`: the copies and memory that the call makes on its way are then in
-    order with its kernels. Its results (unless the caller holds them already)
-    are recorded as used on the stream that was current, where the caller goes
-    on with them."""
+    order with its kernels. Its results (unless the caller holds them already:
+    all of them, or those in `held`) are recorded as used on the stream that was
+    current, where the caller goes on with them."""
     device = getattr(on, "device", None)
     if stream is None or getattr(device, "type", None) != "cuda":
         return call()
@@ -145,8 +157,20 @@ def _enqueued(on, stream, call, record=True):
             result = call()
         if record:
             for t in _tensors(result):
-                t.record_stream(before)
+                if not any(t is h for h in held):
+                    t.record_stream(before)
         return result
+
+
+def _on(device):
+    """A context with `device` current: the library launches on the device that is."""
+    torch = _torch()
+    if device.index is None or torch._C._cuda_getDevice() == device.index:
+        return _HERE
+    return torch.cuda.device(device)
+
+
+_HERE = contextlib.nullcontext()
 
 
 def _tensors(result):
@@ -154,7 +178,9 @@ def _tensors(result):
         return result.data, result.scale
     if isinstance(result, ScaledWeight):
         return result.data, result.meta
-    return result if isinstance(result, tuple) else (result,)
+    if not isinstance(result, tuple):
+        return (result,)
+    return tuple(t for r in result if r is not None for t in _tensors(r))
 
 
 def _gpu(name, t):
