@@ -584,6 +584,45 @@ int vt_dequant_rows(const int8_t *Q, int64_t ldq, const float *T, void *Y, int32
                     int64_t ldy, int64_t M, int64_t K, void *stream);
 
 /*
+ * Softmax cross entropy over an int8 linear layer's outputs, l = vt_scaled_linear
+ * of X, and its gradient in the layer's int8 rows (straight through the rounding;
+ * weights, scales and bias constant). The logits are not kept, forward or
+ * backward, but for up to 64 rows, in a workspace.
+ *
+ *   loss_i = log(sum_j exp(l_ij)) - l_i,target_i
+ *   dx_ik = g_i sum_j (exp(l_ij) / sum_j exp(l_ij) - [j = target_i]) s_j W_kj
+ *
+ * target [M] is int32 or int64. A row whose target is `ignored` has loss 0 and no
+ * gradient; any other target outside 0 .. N - 1, and a row whose logits hold NaN
+ * or +infinity, gives NaN in its own row's loss and gradient. A bias of -infinity
+ * takes a class out. loss [M] float32; state [4 M] float32, 16-byte aligned, is
+ * what the gradient needs of the rows. reduction: VT_REDUCE_MEAN over the rows
+ * that have a target (NaN if none has), or VT_REDUCE_SUM, writes *reduced, and
+ * *count = how many rows have a target.
+ *
+ * vt_cross_entropy_grad: Q, T the int8 rows of the forward pass, state its
+ * output; g_i = dloss[i * dloss_step] (dloss_step 0 or 1), over *count if count
+ * is given. Gradient terms are 16-bit as vt_scaled_linear_grad's, by dX's type.
+ * Calls of many rows take them in parts, so that a workspace of at most 512 MiB
+ * holds a part's terms.
+ */
+#define VT_TARGET_I32 1
+#define VT_TARGET_I64 2
+#define VT_REDUCE_NONE 0
+#define VT_REDUCE_MEAN 1
+#define VT_REDUCE_SUM 2
+
+int vt_cross_entropy(const void *X, int32_t x_type, int64_t ldx, const float *T, int64_t M,
+                     int64_t K, const int8_t *Bp, const float *meta, int64_t N, const void *target,
+                     int32_t target_type, int64_t ignored, float *loss, float *state,
+                     int32_t reduction, float *reduced, float *count, void *stream);
+
+int vt_cross_entropy_grad(const int8_t *Q, int32_t q_type, int64_t ldq, const float *T, int64_t M,
+                          int64_t K, const int8_t *Bp, const float *meta, int64_t N,
+                          const float *state, const float *dloss, int64_t dloss_step,
+                          const float *count, void *dX, int32_t type, int64_t ldx, void *stream);
+
+/*
  * Run-time compiled loop-nest kernels.
  *
  * The reference turns a loop nest (its `Stmt` JSON, README.md:456-503) into

@@ -43,7 +43,7 @@ EXPORTS = ("vt_gemm_i8", "vt_gemm_i8_noalloc", "vt_gemm_check", "vt_gemm_route",
            "vt_rtc_compile", "vt_rtc_code_size", "vt_rtc_launch", "vt_rtc_release",
            "vt_quant_pitch", "vt_quant_rows", "vt_scaled_size", "vt_scaled_pack", "vt_scaled_linear",
            "vt_scaled_gated", "vt_scaled_linear_grad", "vt_scaled_gated_grad",
-           "vt_norm", "vt_norm_grad", "vt_dequant_rows")
+           "vt_norm", "vt_norm_grad", "vt_dequant_rows", "vt_cross_entropy", "vt_cross_entropy_grad")
 
 # Replay operation codes and status codes (VT_REPLAY_* in include/vt_hip_gemm.h).
 REPLAY_MVIN, REPLAY_LATCH_B, REPLAY_COMPUTE, REPLAY_MVOUT = 1, 2, 3, 4
@@ -161,6 +161,10 @@ def _declare(lib):
     lib.vt_norm_grad.restype = ctypes.c_int
     lib.vt_dequant_rows.argtypes = [p, i64, p, p, i32, i64, i64, i64, p]
     lib.vt_dequant_rows.restype = ctypes.c_int
+    lib.vt_cross_entropy.argtypes = [p, i32, i64, p, i64, i64, p, p, i64, p, i32, i64, p, p, i32, p, p, p]
+    lib.vt_cross_entropy.restype = ctypes.c_int
+    lib.vt_cross_entropy_grad.argtypes = [p, i32, i64, p, i64, i64, p, p, i64, p, p, i64, p, p, i32, i64, p]
+    lib.vt_cross_entropy_grad.restype = ctypes.c_int
     u32 = ctypes.c_uint32
     lib.vt_rtc_launch.argtypes = [p, u32, u32, u32, u32, u32, u32, ctypes.POINTER(p), p]
     lib.vt_rtc_launch.restype = ctypes.c_int
@@ -363,6 +367,9 @@ def gemm_packed_raw(A_ptr, Bp_ptr, D_ptr, C_ptr, M, N, K, lda, ldd, ldc, batch=1
 # VT_TYPE_* and VT_ACT_* of the scaled operators
 TYPE_F32, TYPE_F16, TYPE_BF16, TYPE_I8, TYPE_I8_PADDED = 1, 2, 3, 4, 5
 ACT_IDS = {"silu": 0, "gelu": 1}
+# VT_TARGET_* and VT_REDUCE_* of the loss
+TARGET_I32, TARGET_I64 = 1, 2
+REDUCE_IDS = {"none": 0, "mean": 1, "sum": 2}
 
 
 def quant_pitch(k):

@@ -42,8 +42,8 @@ __host__ __device__ constexpr int64_t pair_col(int64_t j, int which) {
   return (j >> 5) * 64 + which * 32 + (j & 31);
 }
 
-// Float side of packed weights: np scales, np bias terms, and the bound of a
-// gated product's gradient terms (pack_bound_kernel).
+// Float side of packed weights: np scales, np bias terms, and the bound of
+// gradient terms (pack_bound_kernel, pack_top_kernel).
 constexpr int64_t scaled_meta(int64_t np) { return 2 * np + 16; }
 
 enum ElemType { kF32 = VT_TYPE_F32, kF16 = VT_TYPE_F16, kBF16 = VT_TYPE_BF16 };
@@ -310,6 +310,15 @@ __global__ __launch_bounds__(256) void pack_bound_kernel(ScaledPackArgs p) {
 #pragma unroll
   for (int o = 32; o; o >>= 1) bits = max(bits, (uint32_t)__shfl_xor((int)bits, o));
   if (c == 0) atomicMax((uint32_t *)(p.meta + 2 * (int64_t)p.Np), bits);
+}
+
+// A linear layer's: max over j of |s_j|, which bounds a loss' gradient terms.
+__global__ __launch_bounds__(1024) void pack_top_kernel(ScaledPackArgs p) {
+  __shared__ uint32_t red[16];
+  uint32_t bits = 0;
+  for (int j = threadIdx.x; j < p.N; j += 1024) bits = max(bits, magnitude(p.s0[j]));
+  bits = block_max<1024>(bits, red);
+  if (threadIdx.x == 0) p.meta[2 * (int64_t)p.Np] = __uint_as_float(bits);
 }
 
 // ---------------------------------------------------------------------------
@@ -1639,7 +1648,8 @@ struct TilePlan {
   int64_t tiles;
 };
 
-TilePlan tile_plan(bool terms, int64_t M, int64_t Np, int64_t Kp, int cus) {
+// `slice`: whether K may be split.
+TilePlan tile_plan(bool terms, int64_t M, int64_t Np, int64_t Kp, int cus, bool slice = true) {
   const double slices = Kp / 64.0, more = terms ? 3.0 : 0.0;
   TilePlan best = {};
   double least = 0;
@@ -1667,7 +1677,7 @@ TilePlan tile_plan(bool terms, int64_t M, int64_t Np, int64_t Kp, int cus) {
   }
   if (Kp > 128) offer(128, 128, 1, false);   // their kernel is built for more than one pair of slices
   offer(64, 128, 1, false);
-  for (int ks = 2; ks <= 16; ++ks)
+  for (int ks = 2; slice && ks <= 16; ++ks)
     if (Kp % (128 * ks) == 0 && Kp / ks >= 512) offer(128, 128, ks, false);
   return best;
 }
@@ -2048,9 +2058,7 @@ ScaledCall part_of(ScaledCall c, int64_t r, int64_t rows) {
   return c;
 }
 
-int forward_rows(const ScaledCall &c, int act, void *stream) {
-  Scratch scr;
-  if (int rc = open_scratch(stream, &scr)) return rc;
+int forward_rows(const ScaledCall &c, int act, Scratch &scr) {
   const int64_t Kp = scaled_kp(c.K), Np = scaled_np(c.N, c.pair);
   ScaledOut o = {};
   o.meta = c.meta; o.Y = c.Y; o.ldy = c.ldy;
@@ -2076,8 +2084,11 @@ int forward(const ScaledCall &c, int act, void *stream) {
   if (empty) return VT_OK;
   const bool copied = !rows_in_place(c.X, c.x_type, c.ldx, c.K);
   const int64_t step = copied ? rows_at_once(c.M, scaled_kp(c.K) + 4) : c.M;
-  for (int64_t r = 0; r < c.M; r += step)
-    if (int rc = forward_rows(part_of(c, r, std::min(step, c.M - r)), act, stream)) return rc;
+  for (int64_t r = 0; r < c.M; r += step) {
+    Scratch scr;
+    if (int rc = open_scratch(stream, &scr)) return rc;
+    if (int rc = forward_rows(part_of(c, r, std::min(step, c.M - r)), act, scr)) return rc;
+  }
   return VT_OK;
 }
 
@@ -2233,8 +2244,10 @@ int vt_scaled_pack(const int8_t *W0, const int8_t *W1, int64_t ldw0, int64_t ldw
   VT_HIP_CHECK(hipGetLastError());
   if (pair) {
     hipLaunchKernelGGL(pack_bound_kernel, dim3((unsigned)((N + 63) / 64)), dim3(256), 0, (hipStream_t)stream, a);
-    VT_HIP_CHECK(hipGetLastError());
+  } else {
+    hipLaunchKernelGGL(pack_top_kernel, dim3(1), dim3(1024), 0, (hipStream_t)stream, a);
   }
+  VT_HIP_CHECK(hipGetLastError());
   return VT_OK;
 }
 
