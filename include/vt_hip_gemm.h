@@ -623,6 +623,48 @@ int vt_cross_entropy_grad(const int8_t *Q, int32_t q_type, int64_t ldq, const fl
                           const float *count, void *dX, int32_t type, int64_t ldx, void *stream);
 
 /*
+ * Low-rank adapters of many requests beside an int8 linear layer, and their
+ * gradients. Row i has adapter a = which[i] (which null: 0); a negative one is
+ * none, and one of L or more gives the row NaN.
+ *
+ *   u_ir = scale sum_k x_ik down[a][r][k]
+ *   y_ij = vt_scaled_linear's y_ij + sum_r u_ir up[a][j][r]
+ *   h_ir = scale sum_j dy_ij up[a][j][r]
+ *   dx_ik = vt_scaled_linear_grad's dx_ik + sum_r h_ir down[a][r][k]
+ *   ddown[a][r][k] = sum_i h_ir x_ik, dup[a][j][r] = sum_i dy_ij u_ir, over a's rows
+ *
+ * One floating type for the adapters, the outputs, dY and all gradients; X has it
+ * too, or is int8 rows with scales (forward only), which x then stands for. Sums
+ * are float32; u and h enter the second product in two 16-bit halves (16 bits in
+ * bfloat16, 22 in float16) or as they are; y and dx are rounded once. The
+ * gradients of down and up are summed in one order: results repeat bit for bit.
+ *
+ * vt_adapter_size: bytes of the layouts that one direction reads of L adapters of
+ * rank R (1 .. 128); negative: VT_E*. vt_adapter_pack: down [L][R][K] and up
+ * [L][N][R] -> P, 16-byte aligned: back 0 for vt_adapted_linear, 1 for
+ * vt_adapted_grad.
+ *
+ * vt_adapted_linear: U [M][R rounded up to 16] float32, 16-byte aligned, is
+ * written; vt_adapted_grad's dUp needs it again. vt_adapted_grad: H like U is
+ * written; dX, dDown, dUp may be null where they are not wanted (then X without
+ * dDown and U without dUp too). Otherwise as vt_scaled_linear and its gradient.
+ */
+int64_t vt_adapter_size(int64_t K, int64_t N, int64_t R, int64_t L, int32_t type);
+
+int vt_adapter_pack(const void *down, const void *up, int32_t type, int64_t K, int64_t N, int64_t R,
+                    int64_t L, int32_t back, void *P, void *stream);
+
+int vt_adapted_linear(const void *X, int32_t x_type, int64_t ldx, const float *T, int64_t M,
+                      int64_t K, const int8_t *Bp, const float *meta, int64_t N, const void *P,
+                      int64_t R, int64_t L, float scale, const int32_t *which, float *U, void *Y,
+                      int32_t type, int64_t ldy, void *stream);
+
+int vt_adapted_grad(const void *dY, int32_t type, int64_t ldd, const void *X, int64_t ldx, int64_t M,
+                    int64_t K, const int8_t *Bp, const float *meta, int64_t N, const void *P,
+                    int64_t R, int64_t L, float scale, const int32_t *which, const float *U,
+                    float *H, void *dX, int64_t lddx, void *dDown, void *dUp, void *stream);
+
+/*
  * Run-time compiled loop-nest kernels.
  *
  * The reference turns a loop nest (its `Stmt` JSON, README.md:456-503) into

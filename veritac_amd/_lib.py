@@ -43,7 +43,8 @@ EXPORTS = ("vt_gemm_i8", "vt_gemm_i8_noalloc", "vt_gemm_check", "vt_gemm_route",
            "vt_rtc_compile", "vt_rtc_code_size", "vt_rtc_launch", "vt_rtc_release",
            "vt_quant_pitch", "vt_quant_rows", "vt_scaled_size", "vt_scaled_pack", "vt_scaled_linear",
            "vt_scaled_gated", "vt_scaled_linear_grad", "vt_scaled_gated_grad",
-           "vt_norm", "vt_norm_grad", "vt_dequant_rows", "vt_cross_entropy", "vt_cross_entropy_grad")
+           "vt_norm", "vt_norm_grad", "vt_dequant_rows", "vt_cross_entropy", "vt_cross_entropy_grad",
+           "vt_adapter_size", "vt_adapter_pack", "vt_adapted_linear", "vt_adapted_grad")
 
 # Replay operation codes and status codes (VT_REPLAY_* in include/vt_hip_gemm.h).
 REPLAY_MVIN, REPLAY_LATCH_B, REPLAY_COMPUTE, REPLAY_MVOUT = 1, 2, 3, 4
@@ -165,6 +166,14 @@ def _declare(lib):
     lib.vt_cross_entropy.restype = ctypes.c_int
     lib.vt_cross_entropy_grad.argtypes = [p, i32, i64, p, i64, i64, p, p, i64, p, p, i64, p, p, i32, i64, p]
     lib.vt_cross_entropy_grad.restype = ctypes.c_int
+    lib.vt_adapter_size.argtypes = [i64, i64, i64, i64, i32]
+    lib.vt_adapter_size.restype = ctypes.c_int64
+    lib.vt_adapter_pack.argtypes = [p, p, i32, i64, i64, i64, i64, i32, p, p]
+    lib.vt_adapter_pack.restype = ctypes.c_int
+    lib.vt_adapted_linear.argtypes = [p, i32, i64, p, i64, i64, p, p, i64, p, i64, i64, f32, p, p, p, i32, i64, p]
+    lib.vt_adapted_linear.restype = ctypes.c_int
+    lib.vt_adapted_grad.argtypes = [p, i32, i64, p, i64, i64, i64, p, p, i64, p, i64, i64, f32, p, p, p, p, i64, p, p, p]
+    lib.vt_adapted_grad.restype = ctypes.c_int
     u32 = ctypes.c_uint32
     lib.vt_rtc_launch.argtypes = [p, u32, u32, u32, u32, u32, u32, ctypes.POINTER(p), p]
     lib.vt_rtc_launch.restype = ctypes.c_int
@@ -387,6 +396,14 @@ def scaled_size(k, n, pair):
     if size < 0:
         check(int(size), "vt_scaled_size")
     return size, meta.value
+
+
+def adapter_size(k, n, rank, count, type_id):
+    """Bytes of one direction's layouts of adapters, vt_adapter_size."""
+    size = load_library().vt_adapter_size(k, n, rank, count, type_id)
+    if size < 0:
+        check(int(size), "vt_adapter_size")
+    return size
 
 
 class RtcProgram:

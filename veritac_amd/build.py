@@ -16,7 +16,7 @@ PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG_DIR)
 SOURCES = [os.path.join(PKG_DIR, "csrc", "vt_hip_gemm.hip")]
 # device and host code that SOURCES include
-PARTS = [os.path.join(PKG_DIR, "csrc", name) for name in ("vt_scaled.h", "vt_norm.h", "vt_loss.h")]
+PARTS = [os.path.join(PKG_DIR, "csrc", name) for name in ("vt_scaled.h", "vt_norm.h", "vt_loss.h", "vt_adapter.h")]
 INCLUDE = os.path.join(ROOT, "include")
 LIB_PATH = os.path.join(PKG_DIR, "libvt_hip_gemm.so")
 ARCH = "gfx950"

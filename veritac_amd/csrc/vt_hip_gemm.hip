@@ -4717,3 +4717,4 @@ void vt_rtc_release(vt_rtc_program *p) {
 #include "vt_scaled.h"
 #include "vt_norm.h"
 #include "vt_loss.h"
+#include "vt_adapter.h"

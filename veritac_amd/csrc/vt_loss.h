@@ -346,11 +346,6 @@ struct LossTermsTile : ScaledTile<kGradTerms, 2, LOW> {
   }
 };
 
-template <class OUT, int BN>
-__global__ __launch_bounds__(256, 1) void loss_dma16_kernel(GemmArgs p, OUT out) {
-  dma16_tiles<false, true, true, BN, false>(p, out);
-}
-
 // Logits of a few rows (float32 [M][N] of a workspace) -> their parts: one
 // workgroup for 4096 columns of a row.
 constexpr int kLogitChunk = 4096;
@@ -491,28 +486,6 @@ __global__ __launch_bounds__(256) void loss_scale_kernel(LossScaleArgs p) {
 // Host side
 // ---------------------------------------------------------------------------
 
-// The product of rows and packed weights on tiles, whose sums OUT takes (a plan
-// without K slices).
-template <class OUT>
-int launch_loss(const TilePlan &plan, const Rows &rows, const int8_t *Bp, int64_t Kp, const OUT &out, Scratch &scr) {
-  hipStream_t s = (hipStream_t)scr.stream;
-  if (plan.tiles > 0x7fffffff) return fail(VT_EUNSUPPORTED, "grid of %lld tiles too large", (long long)plan.tiles);
-  const GemmArgs a = scaled_args(rows, Bp, out.M, Kp, out.Np, plan.bm, plan.bn);
-  const dim3 grid((unsigned)plan.tiles);
-  if (plan.persistent) {
-    const dim3 wgs((unsigned)std::min<int64_t>(plan.tiles, scr.st->num_cus));
-    if (plan.bn == 256) hipLaunchKernelGGL((loss_dma16_kernel<OUT, 256>), wgs, dim3(256), 0, s, a, out);
-    else hipLaunchKernelGGL((loss_dma16_kernel<OUT, 128>), wgs, dim3(256), 0, s, a, out);
-  } else if (plan.bm == 64) {
-    if (Kp <= 128) hipLaunchKernelGGL((gemm_mfma_kernel<64, 128, 1, false, true, false, true, OUT>), grid, dim3(256), 0, s, a, out);
-    else hipLaunchKernelGGL((gemm_mfma_kernel<64, 128, 1, false, false, false, true, OUT>), grid, dim3(256), 0, s, a, out);
-  } else {
-    hipLaunchKernelGGL((gemm_mfma_kernel<128, 128, 1, false, false, false, true, OUT>), grid, dim3(256), 0, s, a, out);
-  }
-  VT_HIP_CHECK(hipGetLastError());
-  return VT_OK;
-}
-
 struct LossCall {
   ScaledCall c;
   Targets targets;
@@ -562,7 +535,7 @@ int loss_rows(const LossCall &l, bool logits, void *stream) {
     out.part = (v2f *)r.part;
     out.mine = (float *)r.mine;
     out.targets = l.targets;
-    if (int rc = launch_loss(plan, rows, c.Bp, Kp, out, scr)) return rc;
+    if (int rc = launch_tiles(plan, rows, c.Bp, Kp, out, scr)) return rc;
   }
   if (M >= 512) hipLaunchKernelGGL(loss_rows_kernel<16>, dim3((unsigned)((M + 15) / 16)), dim3(1024), 0, s, r);
   else hipLaunchKernelGGL(loss_rows_kernel<1>, dim3((unsigned)M), dim3(1024), 0, s, r);
@@ -594,10 +567,10 @@ int loss_grad_rows(const ScaledCall &c, const RowState *state, const float *dlos
   auto terms = [&](auto out) {
     (ScaledOut &)out = f;
     out.state = state;
-    return launch_loss(plan, rows, c.Bp, Kp, out, scr);
+    return launch_tiles(plan, rows, c.Bp, Kp, out, scr);
   };
   if (int rc = split ? terms(LossTermsTile<true>()) : terms(LossTermsTile<false>())) return rc;
-  ScaledOut o = {};
+  ScaledTile<kGrad> o = {};
   o.Y = c.Y; o.ldy = c.ldy;
   o.M = (int)c.M; o.N = (int)c.K; o.Np = (int)Kp;
   o.type = c.y_type; o.norm = norm;

@@ -869,9 +869,15 @@ __global__ __launch_bounds__(256, 1) void terms_low_dma16_kernel(GemmArgs p, Sca
   dma16_tiles<false, true, true, BN, false>(p, out);
 }
 
+// The product on the persistent kernels with any other output.
+template <class OUT, int BN>
+__global__ __launch_bounds__(256, 1) void out_dma16_kernel(GemmArgs p, OUT out) {
+  dma16_tiles<false, true, true, BN, false>(p, out);
+}
+
 // The same from int32 sums in memory: `slices` partial sums [M][Np] each.
-template <int OP>
-__global__ __launch_bounds__(256) void finish_kernel(const int32_t *S, int slices, ScaledTile<OP> out) {
+template <int OP, class OUT>
+__device__ __forceinline__ void finish_rows(const int32_t *S, int slices, const OUT &out) {
   const int row = blockIdx.x, j = blockIdx.y * 256 + threadIdx.x;
   const int pc = OP == kLinear ? j : (int)pair_col(j, 0);
   if (pc >= out.Np) return;
@@ -884,6 +890,11 @@ __global__ __launch_bounds__(256) void finish_kernel(const int32_t *S, int slice
     s += (int64_t)out.M * out.Np;
   }
   out.element(a0, a1, row, pc, j, out.t[row]);
+}
+
+template <int OP>
+__global__ __launch_bounds__(256) void finish_kernel(const int32_t *S, int slices, ScaledTile<OP> out) {
+  finish_rows<OP>(S, slices, out);
 }
 
 // ---------------------------------------------------------------------------
@@ -920,9 +931,9 @@ constexpr int kFusedValues = 16384;
 //
 // K slices finish through 64-bit words as in packed_skinny_kernel: the words'
 // two sums are two rows of a column (P = 1) or the two projections of one
-// element (P = 2).
-template <int OP, int NBW, int MB, int XB>
-__global__ __launch_bounds__(512) void scaled_skinny_kernel(ScaledSkinnyArgs p, ScaledOut o) {
+// element (P = 2). O: ScaledOut, or an output with an element() of its own.
+template <int OP, int NBW, int MB, int XB, class O>
+__device__ __forceinline__ void skinny_rows(const ScaledSkinnyArgs &p, const O &o) {
   constexpr int P = OP == kGated ? 2 : 1, NT = NBW * P, WAVES = 8, S = packed_stages(NT);
   static_assert(XB == 0 || MB == 1, "rows are rounded here for M <= 16");
   __shared__ v4i red[WAVES * NT * 64];
@@ -1114,9 +1125,13 @@ __global__ __launch_bounds__(512) void scaled_skinny_kernel(ScaledSkinnyArgs p, 
 
   auto row_t = [&](int row) { return XB ? row_scale(tops[row]).scale : o.t[row]; };
   auto finish = [&](int32_t a0, int32_t a1, int row, int col, float t_row) {
-    ScaledTile<OP> out;
-    (ScaledOut &)out = o;
-    out.element(a0, a1, row, P == 1 ? col : (int)pair_col(col, 0), col, t_row);
+    if constexpr (std::is_same<O, ScaledOut>::value) {
+      ScaledTile<OP> out;
+      (ScaledOut &)out = o;
+      out.element(a0, a1, row, P == 1 ? col : (int)pair_col(col, 0), col, t_row);
+    } else {
+      o.element(a0, a1, row, P == 1 ? col : (int)pair_col(col, 0), col, t_row);
+    }
   };
   // The sum over the waves of element e of source lane `src` of tile n.
   auto sum = [&](int n, int src, int e) {
@@ -1174,6 +1189,11 @@ __global__ __launch_bounds__(512) void scaled_skinny_kernel(ScaledSkinnyArgs p, 
       }
     }
   }
+}
+
+template <int OP, int NBW, int MB, int XB>
+__global__ __launch_bounds__(512) void scaled_skinny_kernel(ScaledSkinnyArgs p, ScaledOut o) {
+  skinny_rows<OP, NBW, MB, XB>(p, o);
 }
 
 struct TermArgs {
@@ -1316,8 +1336,8 @@ __device__ __forceinline__ void mfma16h_in_place(v4f &acc, const v4i &a, const v
 // vector instructions to one. A call of few slices is bound by what surrounds
 // them, which 64-row tiles halve: 100 x 333 over 2432 packed columns in 13.4 us
 // with its terms and sums, on 128-row tiles 16.5.
-template <int BM>
-__global__ __launch_bounds__(256, 1) void grad_dma_kernel(GradArgs p, ScaledTile<kGrad> out) {
+template <int BM, class OUT>
+__device__ __forceinline__ void grad_tiles(const GradArgs &p, OUT &out) {
   static_assert(BM == 256 || BM == 128 || BM == 64, "256x256, 128x256 or 64x256 tiles");
   constexpr int WCOLS = BM == 256 ? 2 : 4, WTN = 256 / WCOLS, MI = BM == 64 ? 4 : 8, NI = WTN / 16;
   constexpr int A_BYTES = BM * 128, B_BYTES = 64 * 256, NSTAGE = 3, B_REGION = NSTAGE * A_BYTES;
@@ -1474,7 +1494,12 @@ __global__ __launch_bounds__(256, 1) void grad_dma_kernel(GradArgs p, ScaledTile
   float unit[2];
 #pragma unroll
   for (int h = 0; h < 2; ++h) unit[h] = out.norm ? 1.0f / norms[h] : 1.0f;
-  out.blocks16<4>(acc, m0 + wm * 128, n0 + wn * WTN, lane, (LDS_AS int8_t *)smem + wave * STRIP, unit);
+  out.template blocks16<4>(acc, m0 + wm * 128, n0 + wn * WTN, lane, (LDS_AS int8_t *)smem + wave * STRIP, unit);
+}
+
+template <int BM>
+__global__ __launch_bounds__(256, 1) void grad_dma_kernel(GradArgs p, ScaledTile<kGrad> out) {
+  grad_tiles<BM>(p, out);
 }
 
 // dx from the partial sums [slices][M][Kp] of a split contraction, over the
@@ -1489,7 +1514,9 @@ struct GradSumArgs {
   int M, K, Kp, slices, type;
 };
 
-__global__ __launch_bounds__(256) void grad_sum_kernel(GradSumArgs p) {
+// `more`: what else an element (row, column) holds.
+template <class MORE>
+__device__ __forceinline__ void sum_grad_slices(const GradSumArgs &p, MORE &&more) {
   const int64_t row = blockIdx.x;
   const int col = (blockIdx.y * 256 + threadIdx.x) * 4;
   if (col >= p.K) return;
@@ -1509,9 +1536,14 @@ __global__ __launch_bounds__(256) void grad_sum_kernel(GradSumArgs p) {
 #pragma unroll
   for (int e = 0; e < 4; ++e)
     if (col + e < p.K) {
-      if (p.type == VT_TYPE_F32) ((float *)p.X)[at + e] = v[e];
-      else ((uint16_t *)p.X)[at + e] = (uint16_t)pack16(v[e], 0.0f, p.type);
+      const float x = v[e] + more((int)row, col + e);
+      if (p.type == VT_TYPE_F32) ((float *)p.X)[at + e] = x;
+      else ((uint16_t *)p.X)[at + e] = (uint16_t)pack16(x, 0.0f, p.type);
     }
+}
+
+__global__ __launch_bounds__(256) void grad_sum_kernel(GradSumArgs p) {
+  sum_grad_slices(p, [](int, int) { return 0.0f; });
 }
 
 // ---------------------------------------------------------------------------
@@ -1699,6 +1731,40 @@ void launch_dma16(const GemmArgs &a, const ScaledOut &o, int64_t wgs, hipStream_
   }
 }
 
+// The int8 product of rows and packed weights on a plan's K slices: *out int32
+// sums [ks][M][Np].
+int sliced_sums(const TilePlan &plan, const Rows &rows, const int8_t *Bp, int64_t M, int64_t Np, int64_t Kp, Scratch &scr,
+                const int32_t **out) {
+  void *w = nullptr;
+  if (int rc = scr.take(kPartials, (size_t)plan.ks * M * Np * sizeof(int32_t), &w)) return rc;
+  const int64_t kc = Kp / plan.ks;
+  const Problem sl = {rows.q, Bp, nullptr, (int32_t *)w, M, Np, kc, rows.ld, Kp / 64, 0, Np, plan.ks, kc, kc / 64 * 1024, 0, M * Np};
+  *out = (const int32_t *)w;
+  return launch_mfma_tiles<128, 128, true>(sl, (hipStream_t)scr.stream, scr.st->num_cus);
+}
+
+// The product on a plan without K slices, whose sums OUT takes on kernels of its
+// own type.
+template <class OUT>
+int launch_tiles(const TilePlan &plan, const Rows &rows, const int8_t *Bp, int64_t Kp, const OUT &out, Scratch &scr) {
+  hipStream_t s = (hipStream_t)scr.stream;
+  if (plan.tiles > 0x7fffffff) return fail(VT_EUNSUPPORTED, "grid of %lld tiles too large", (long long)plan.tiles);
+  const GemmArgs a = scaled_args(rows, Bp, out.M, Kp, out.Np, plan.bm, plan.bn);
+  const dim3 grid((unsigned)plan.tiles);
+  if (plan.persistent) {
+    const dim3 wgs((unsigned)std::min<int64_t>(plan.tiles, scr.st->num_cus));
+    if (plan.bn == 256) hipLaunchKernelGGL((out_dma16_kernel<OUT, 256>), wgs, dim3(256), 0, s, a, out);
+    else hipLaunchKernelGGL((out_dma16_kernel<OUT, 128>), wgs, dim3(256), 0, s, a, out);
+  } else if (plan.bm == 64) {
+    if (Kp <= 128) hipLaunchKernelGGL((gemm_mfma_kernel<64, 128, 1, false, true, false, true, OUT>), grid, dim3(256), 0, s, a, out);
+    else hipLaunchKernelGGL((gemm_mfma_kernel<64, 128, 1, false, false, false, true, OUT>), grid, dim3(256), 0, s, a, out);
+  } else {
+    hipLaunchKernelGGL((gemm_mfma_kernel<128, 128, 1, false, false, false, true, OUT>), grid, dim3(256), 0, s, a, out);
+  }
+  VT_HIP_CHECK(hipGetLastError());
+  return VT_OK;
+}
+
 // The int8 product of rows and packed weights, and what follows it, on tiles.
 template <int OP>
 int launch_scaled(const Rows &rows, const int8_t *Bp, int64_t Kp, const ScaledOut &o, Scratch &scr) {
@@ -1707,24 +1773,13 @@ int launch_scaled(const Rows &rows, const int8_t *Bp, int64_t Kp, const ScaledOu
   hipStream_t s = (hipStream_t)scr.stream;
   const int cus = scr.st->num_cus;
   const int64_t M = out.M, Np = out.Np;
-  const Problem q = {rows.q, Bp, nullptr, nullptr, M, Np, Kp, rows.ld, Kp / 64, 0, Np, 1, 0, 0, 0, 0};
-  void *w = nullptr;
   if (Kp == 0) return launch_finish(nullptr, 0, out, s);
   const TilePlan plan = tile_plan(OP == kGradTerms, M, Np, Kp, cus);
   if (plan.tiles > 0x7fffffff) return fail(VT_EUNSUPPORTED, "grid of %lld tiles too large", (long long)plan.tiles);
   if (plan.ks > 1) {
-    if (int rc = scr.take(kPartials, (size_t)plan.ks * M * Np * sizeof(int32_t), &w)) return rc;
-    const int64_t kc = Kp / plan.ks;
-    Problem sl = q;
-    sl.K = kc;
-    sl.batch = plan.ks;
-    sl.sa = kc;
-    sl.sb = kc / 64 * 1024;
-    sl.C = (int32_t *)w;
-    sl.ldc = Np;
-    sl.sc = M * Np;
-    if (int rc = launch_mfma_tiles<128, 128, true>(sl, s, cus)) return rc;
-    return launch_finish((const int32_t *)w, plan.ks, out, s);
+    const int32_t *sums = nullptr;
+    if (int rc = sliced_sums(plan, rows, Bp, M, Np, Kp, scr, &sums)) return rc;
+    return launch_finish(sums, plan.ks, out, s);
   }
   const GemmArgs a = scaled_args(rows, Bp, M, Kp, Np, plan.bm, plan.bn);
   if (plan.persistent) {
@@ -1778,22 +1833,30 @@ ScaledGeom skinny_geom(int64_t M, int64_t nbt, int64_t Kp, int cus) {
   return {(int)hpw, (int)((units + hpw - 1) / hpw), (int)ks};
 }
 
-template <int OP, int NBW, int XB>
-void launch_skinny_blocks(const ScaledSkinnyArgs &a, const ScaledOut &o, dim3 grid, hipStream_t s) {
+// O: ScaledOut, or an output that launches its own kernels.
+template <int OP, int NBW, int MB, int XB, class O>
+void launch_skinny_one(const ScaledSkinnyArgs &a, const O &o, dim3 grid, hipStream_t s) {
+  if constexpr (std::is_same<O, ScaledOut>::value)
+    hipLaunchKernelGGL((scaled_skinny_kernel<OP, NBW, MB, XB>), grid, dim3(512), 0, s, a, o);
+  else O::template skinny<NBW, MB, XB>(a, o, grid, s);
+}
+
+template <int OP, int NBW, int XB, class O>
+void launch_skinny_blocks(const ScaledSkinnyArgs &a, const O &o, dim3 grid, hipStream_t s) {
   if constexpr (XB > 0) {
-    hipLaunchKernelGGL((scaled_skinny_kernel<OP, NBW, 1, XB>), grid, dim3(512), 0, s, a, o);
+    launch_skinny_one<OP, NBW, 1, XB>(a, o, grid, s);
   } else {
     switch ((o.M + 15) / 16) {
-      case 1: hipLaunchKernelGGL((scaled_skinny_kernel<OP, NBW, 1, 0>), grid, dim3(512), 0, s, a, o); break;
-      case 2: hipLaunchKernelGGL((scaled_skinny_kernel<OP, NBW, 2, 0>), grid, dim3(512), 0, s, a, o); break;
-      case 3: hipLaunchKernelGGL((scaled_skinny_kernel<OP, NBW, 3, 0>), grid, dim3(512), 0, s, a, o); break;
-      default: hipLaunchKernelGGL((scaled_skinny_kernel<OP, NBW, 4, 0>), grid, dim3(512), 0, s, a, o); break;
+      case 1: launch_skinny_one<OP, NBW, 1, 0>(a, o, grid, s); break;
+      case 2: launch_skinny_one<OP, NBW, 2, 0>(a, o, grid, s); break;
+      case 3: launch_skinny_one<OP, NBW, 3, 0>(a, o, grid, s); break;
+      default: launch_skinny_one<OP, NBW, 4, 0>(a, o, grid, s); break;
     }
   }
 }
 
-template <int OP, int XB>
-void launch_skinny_rows(const ScaledSkinnyArgs &a, const ScaledOut &o, dim3 grid, hipStream_t s) {
+template <int OP, int XB, class O>
+void launch_skinny_rows(const ScaledSkinnyArgs &a, const O &o, dim3 grid, hipStream_t s) {
   const int blocks = (a.hpw + 1) / 2;
   if constexpr (OP == kGated) {
     if (blocks == 1) launch_skinny_blocks<OP, 1, XB>(a, o, grid, s);
@@ -1810,8 +1873,8 @@ void launch_skinny_rows(const ScaledSkinnyArgs &a, const ScaledOut &o, dim3 grid
 
 // Up to 64 rows of a forward call: X of any type (rows already int8 in `rows`
 // when it is null).
-template <int OP>
-int launch_skinny(const void *X, int type, int64_t ldx, int64_t K, const Rows &rows, const int8_t *Bp, ScaledOut o, Scratch &scr) {
+template <int OP, class O>
+int launch_skinny(const void *X, int type, int64_t ldx, int64_t K, const Rows &rows, const int8_t *Bp, O o, Scratch &scr) {
   constexpr int P = OP == kGated ? 2 : 1;
   hipStream_t s = (hipStream_t)scr.stream;
   const int64_t Kp = scaled_kp(K), nbt = (o.N + 15) / 16;
@@ -1850,9 +1913,13 @@ int launch_skinny(const void *X, int type, int64_t ldx, int64_t K, const Rows &r
   else launch_skinny_rows<OP, 2>(a, o, grid, s);
   VT_HIP_CHECK(hipGetLastError());
   if (!a.ws) return VT_OK;
-  ScaledTile<OP> out;
-  (ScaledOut &)out = o;
-  return launch_finish(a.ws, a.k_split, out, s);
+  if constexpr (std::is_same<O, ScaledOut>::value) {
+    ScaledTile<OP> out;
+    (ScaledOut &)out = o;
+    return launch_finish(a.ws, a.k_split, out, s);
+  } else {
+    return O::finish(a.ws, a.k_split, o, s);
+  }
 }
 
 template <int TYPE, bool LINEAR>
@@ -1917,12 +1984,13 @@ GradGeom grad_geom(int64_t M, int64_t Kp, int64_t slices, int cus) {
   return best;
 }
 
-int launch_grad_tiles(const GradArgs &a, int bm, const ScaledOut &o, hipStream_t s) {
-  ScaledTile<kGrad> out;
-  (ScaledOut &)out = o;
+// OUT: ScaledTile<kGrad>, or an output that launches its own kernels.
+template <class OUT>
+int launch_grad_tiles(const GradArgs &a, int bm, const OUT &out, hipStream_t s) {
   const int64_t wgs = (int64_t)a.tiles_m * a.tiles_n * a.splits;
   if (wgs > 0x7fffffff) return fail(VT_EUNSUPPORTED, "gradient grid too large");
-  if (bm == 256) hipLaunchKernelGGL(grad_dma_kernel<256>, dim3((unsigned)wgs), dim3(256), 0, s, a, out);
+  if constexpr (!std::is_same<OUT, ScaledTile<kGrad>>::value) OUT::tiles(a, bm, out, dim3((unsigned)wgs), s);
+  else if (bm == 256) hipLaunchKernelGGL(grad_dma_kernel<256>, dim3((unsigned)wgs), dim3(256), 0, s, a, out);
   else if (bm == 128) hipLaunchKernelGGL(grad_dma_kernel<128>, dim3((unsigned)wgs), dim3(256), 0, s, a, out);
   else hipLaunchKernelGGL(grad_dma_kernel<64>, dim3((unsigned)wgs), dim3(256), 0, s, a, out);
   VT_HIP_CHECK(hipGetLastError());
@@ -1945,7 +2013,8 @@ int launch_zero(const ScaledOut &o, hipStream_t s) {
 }
 
 // dx = terms . W^T. o: the gradient, its rows' normalisers and type.
-int launch_grad(GradArgs a, const ScaledOut &o, Scratch &scr) {
+template <class OUT = ScaledTile<kGrad>>
+int launch_grad(GradArgs a, const OUT &o, Scratch &scr) {
   hipStream_t s = (hipStream_t)scr.stream;
   const GradGeom g = grad_geom(a.M, a.Kp, (int64_t)a.Np / 64 * a.planes, scr.st->num_cus);
   a.group_m = 4;
@@ -1956,14 +2025,17 @@ int launch_grad(GradArgs a, const ScaledOut &o, Scratch &scr) {
     return launch_grad_tiles(a, g.bm, o, s);
   void *w = nullptr;
   if (int rc = scr.take(kPartials, (size_t)g.splits * a.M * a.Kp * sizeof(float), &w)) return rc;
-  ScaledOut part = o;
+  ScaledTile<kGrad> part;
+  (ScaledOut &)part = o;
   part.Y = w;
   part.ldy = part.N = part.Np = a.Kp;
   part.norm = nullptr;
   part.type = VT_TYPE_F32;
   if (int rc = launch_grad_tiles(a, g.bm, part, s)) return rc;
   const GradSumArgs r = {(const float *)w, o.norm, o.Y, o.ldy, a.M, o.N, a.Kp, g.splits, o.type};
-  hipLaunchKernelGGL(grad_sum_kernel, dim3((unsigned)a.M, (unsigned)((o.N + 1023) / 1024)), dim3(256), 0, s, r);
+  const dim3 grid((unsigned)a.M, (unsigned)((o.N + 1023) / 1024));
+  if constexpr (!std::is_same<OUT, ScaledTile<kGrad>>::value) OUT::sums(r, o, grid, s);
+  else hipLaunchKernelGGL(grad_sum_kernel, grid, dim3(256), 0, s, r);
   VT_HIP_CHECK(hipGetLastError());
   return VT_OK;
 }
@@ -2131,9 +2203,11 @@ int backward_rows(const ScaledCall &c, const int8_t *Q, int q_type, int64_t ldq,
     f.act = act; f.type = c.x_type;
     if (int rc = launch_scaled<kGradTerms>(rows, c.Bp, Kp, f, scr)) return rc;
   }
-  o.norm = norm;
+  ScaledTile<kGrad> dx;
+  (ScaledOut &)dx = o;
+  dx.norm = norm;
   const GradArgs g = {terms, c.Bp, lo, (int)c.M, (int)Kp, (int)Np, 0, 0, 0, split ? 2 : 1, 1};
-  return launch_grad(g, o, scr);
+  return launch_grad(g, dx, scr);
 }
 
 // The gradient in x^: D [M][ldd] of N columns, X the output [M][ldx] of K.
