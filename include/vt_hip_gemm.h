@@ -641,18 +641,19 @@ int vt_cross_entropy_grad(const int8_t *Q, int32_t q_type, int64_t ldq, const fl
  *
  * vt_adapter_size: bytes of the layouts that one direction reads of L adapters of
  * rank R (1 .. 128); negative: VT_E*. vt_adapter_pack: down [L][R][K] and up
- * [L][N][R] -> P, 16-byte aligned: back 0 for vt_adapted_linear, 1 for
- * vt_adapted_grad.
+ * [L][N][R] -> P, what vt_adapted_linear reads, and back, what vt_adapted_grad
+ * does, both 16-byte aligned (null: not wanted).
  *
  * vt_adapted_linear: U [M][R rounded up to 16] float32, 16-byte aligned, is
- * written; vt_adapted_grad's dUp needs it again. vt_adapted_grad: H like U is
- * written; dX, dDown, dUp may be null where they are not wanted (then X without
- * dDown and U without dUp too). Otherwise as vt_scaled_linear and its gradient.
+ * written (Y null: U alone). vt_adapted_grad: H like U is written; dX, dDown and
+ * dUp may be null where they are not wanted, and X and U without dDown and dUp.
+ * U is the forward pass' (P null), or made again from X and P. Otherwise as
+ * vt_scaled_linear and its gradient.
  */
 int64_t vt_adapter_size(int64_t K, int64_t N, int64_t R, int64_t L, int32_t type);
 
 int vt_adapter_pack(const void *down, const void *up, int32_t type, int64_t K, int64_t N, int64_t R,
-                    int64_t L, int32_t back, void *P, void *stream);
+                    int64_t L, void *P, void *back, void *stream);
 
 int vt_adapted_linear(const void *X, int32_t x_type, int64_t ldx, const float *T, int64_t M,
                       int64_t K, const int8_t *Bp, const float *meta, int64_t N, const void *P,
@@ -661,8 +662,9 @@ int vt_adapted_linear(const void *X, int32_t x_type, int64_t ldx, const float *T
 
 int vt_adapted_grad(const void *dY, int32_t type, int64_t ldd, const void *X, int64_t ldx, int64_t M,
                     int64_t K, const int8_t *Bp, const float *meta, int64_t N, const void *P,
-                    int64_t R, int64_t L, float scale, const int32_t *which, const float *U,
-                    float *H, void *dX, int64_t lddx, void *dDown, void *dUp, void *stream);
+                    const void *back, int64_t R, int64_t L, float scale, const int32_t *which,
+                    float *U, float *H, void *dX, int64_t lddx, void *dDown, void *dUp,
+                    void *stream);
 
 /*
  * Run-time compiled loop-nest kernels.

@@ -168,11 +168,11 @@ def _declare(lib):
     lib.vt_cross_entropy_grad.restype = ctypes.c_int
     lib.vt_adapter_size.argtypes = [i64, i64, i64, i64, i32]
     lib.vt_adapter_size.restype = ctypes.c_int64
-    lib.vt_adapter_pack.argtypes = [p, p, i32, i64, i64, i64, i64, i32, p, p]
+    lib.vt_adapter_pack.argtypes = [p, p, i32, i64, i64, i64, i64, p, p, p]
     lib.vt_adapter_pack.restype = ctypes.c_int
     lib.vt_adapted_linear.argtypes = [p, i32, i64, p, i64, i64, p, p, i64, p, i64, i64, f32, p, p, p, i32, i64, p]
     lib.vt_adapted_linear.restype = ctypes.c_int
-    lib.vt_adapted_grad.argtypes = [p, i32, i64, p, i64, i64, i64, p, p, i64, p, i64, i64, f32, p, p, p, p, i64, p, p, p]
+    lib.vt_adapted_grad.argtypes = [p, i32, i64, p, i64, i64, i64, p, p, i64, p, p, i64, i64, f32, p, p, p, p, i64, p, p, p]
     lib.vt_adapted_grad.restype = ctypes.c_int
     u32 = ctypes.c_uint32
     lib.vt_rtc_launch.argtypes = [p, u32, u32, u32, u32, u32, u32, ctypes.POINTER(p), p]

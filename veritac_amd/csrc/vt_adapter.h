@@ -35,10 +35,9 @@ AdapterLayout adapter_layout(int64_t K, int64_t N, int64_t R, int64_t L) {
 }
 
 struct AdapterPackArgs {
-  const uint8_t *A, *B;   // down [L][R][K], up [L][N][R]
-  uint8_t *first, *second;
+  const uint8_t *A, *B;       // down [L][R][K], up [L][N][R]
+  uint8_t *first[2], *second[2];   // forward and backward, null: not wanted
   int K, N, R, Kp, Np, Rp;
-  int back, elem;
 };
 
 // A workgroup lays out 64 of an adapter's long side by all of its rank, through
@@ -59,12 +58,17 @@ __global__ __launch_bounds__(256) void adapter_pack_kernel(AdapterPackArgs p) {
     tile[j][r] = v;
   }
   __syncthreads();
-  // forward, down keeps its order and up too; backward both turn
-  const bool rank_inner = up != (p.back != 0);
-  T *dst = (T *)(up != (p.back != 0) ? p.second : p.first) + (int64_t)a * p.Rp * lenp;
-  for (int i = threadIdx.x; i < 64 * p.Rp; i += 256) {
-    if (rank_inner) dst[(int64_t)(j0 + i / p.Rp) * p.Rp + i % p.Rp] = tile[i / p.Rp][i % p.Rp];
-    else dst[(int64_t)(i >> 6) * lenp + j0 + (i & 63)] = tile[i & 63][i >> 6];
+#pragma unroll
+  for (int back = 0; back < 2; ++back) {
+    // forward, down keeps its order and up too; backward both turn
+    const bool rank_inner = up != (back != 0);
+    uint8_t *to = rank_inner ? p.second[back] : p.first[back];
+    if (!to) continue;
+    T *dst = (T *)to + (int64_t)a * p.Rp * lenp;
+    for (int i = threadIdx.x; i < 64 * p.Rp; i += 256) {
+      if (rank_inner) dst[(int64_t)(j0 + i / p.Rp) * p.Rp + i % p.Rp] = tile[i / p.Rp][i % p.Rp];
+      else dst[(int64_t)(i >> 6) * lenp + j0 + (i & 63)] = tile[i & 63][i >> 6];
+    }
   }
 }
 
@@ -81,6 +85,13 @@ struct ShrinkArgs {
   int64_t ldx;
   float scale;
   int M, len, lenp, L, Rp;
+  int8_t *Q;            // few rows: also rounds floating rows to int8 rows of lenp (null: not)
+  float *T;             // and their scales
+};
+
+// One or two of them over the same rows, by blockIdx.z.
+struct ShrinkPair {
+  ShrinkArgs of[2];
 };
 
 // 8 elements of a row from `pos` as floats, zero past `len`; int8 rows too.
@@ -110,18 +121,22 @@ __device__ __forceinline__ float shrink_factor(const ShrinkArgs &p, int row, int
 }
 
 // Up to 64 rows, each with an adapter of its own maybe: 16 ranks of a row to a
-// workgroup, a wave for each, 8 columns a lane. Bound by the latency of its few
-// loads and, with many adapters, by reading them.
+// workgroup, a wave for each, 8 columns a lane. The first of a row's workgroups
+// rounds it too, where the int8 product needs that done: the row is in its cache,
+// and a launch less. Bound by the latency of its few loads and, with many
+// adapters, by reading them.
 template <int TYPE, bool I8>
-__global__ __launch_bounds__(1024) void shrink_rows_kernel(ShrinkArgs p) {
+__global__ __launch_bounds__(1024) void shrink_rows_kernel(ShrinkPair pair) {
+  __shared__ uint32_t red[16];
+  const ShrinkArgs &p = pair.of[blockIdx.z];
   typedef typename Elem<TYPE>::T T;
   const int row = blockIdx.x, rank = blockIdx.y * 16 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int a = p.which ? p.which[row] : 0;
+  const void *x = I8 ? (const void *)((const int8_t *)p.X + row * p.ldx) : (const void *)((const T *)p.X + row * p.ldx);
   float s = 0.0f;
   if (a >= 0 && a < p.L) {
-    const void *x = I8 ? (const void *)((const int8_t *)p.X + row * p.ldx) : (const void *)((const T *)p.X + row * p.ldx);
     const T *w = (const T *)p.P + ((int64_t)a * p.Rp + rank) * p.lenp;
-#pragma unroll 4
+#pragma unroll 8
     for (int pos = lane * 8; pos < p.lenp; pos += 512) {
       float v[8], b[8];
       load_row8<TYPE, I8>(x, pos, p.len, v);
@@ -133,6 +148,29 @@ __global__ __launch_bounds__(1024) void shrink_rows_kernel(ShrinkArgs p) {
     for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o);
   }
   if (lane == 0) p.U[(int64_t)row * p.Rp + rank] = a < 0 ? 0.0f : s * shrink_factor<I8>(p, row, a);
+  if constexpr (!I8) {
+    if (!p.Q || blockIdx.y) return;
+    uint32_t top = 0;
+    for (int pos = threadIdx.x * 8; pos < p.len; pos += 8192) {
+      float v[8];
+      load8<TYPE>((const T *)x, pos, p.len, v);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) top = max(top, magnitude(v[e]));
+    }
+    top = block_max<1024>(top, red);
+    const RowScale r = row_scale(top);
+    if (threadIdx.x == 0) p.T[row] = r.scale;
+    for (int pos = threadIdx.x * 8; pos < p.lenp; pos += 8192) {
+      float v[8];
+      uint32_t b[8];
+      load8<TYPE>((const T *)x, pos, p.len, v);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) b[e] = round_byte(v[e], r.inv);
+      v2i o = {pack_bytes(b[0], b[1], b[2], b[3]), pack_bytes(b[4], b[5], b[6], b[7])};
+      if (r.inv == 0.0f) o = v2i{0, 0};
+      *(v2i *)(p.Q + (int64_t)row * p.lenp + pos) = o;
+    }
+  }
 }
 
 // A 16 x 32 by 32 x 16 product (16 x 16 x 16 steps of 4 in float32) of fragments
@@ -200,54 +238,66 @@ __device__ __forceinline__ void each_adapter(int a, F &&f) {
   }
 }
 
-// More rows: 16 rows by 16 ranks to a workgroup, whose 8 waves take 32-deep
-// slices in turn (4 of them in flight) and join through LDS.
-template <int TYPE, bool I8>
-__global__ __launch_bounds__(512) void shrink_tiles_kernel(ShrinkArgs p) {
+// More rows: 16 rows by 16 NR ranks to a workgroup, whose 16 waves take
+// neighbouring runs of U 32-deep slices (whole lines of the rows) and join through
+// LDS. Bound by what it reads of the rows (once for every 16 NR ranks) and of
+// their adapters (once for every 16 rows, from L2).
+template <int TYPE, bool I8, int NR>
+__global__ __launch_bounds__(1024) void shrink_tiles_kernel(ShrinkPair pair) {
   typedef typename Elem<TYPE>::T T;
-  constexpr int WAVES = 8, U = 4;
-  __shared__ float red[WAVES][16][17];
+  constexpr int WAVES = 16, U = TYPE == kF32 ? 2 : 4;
+  __shared__ float red[WAVES][16][16 * NR + 1];
+  const ShrinkArgs &p = pair.of[blockIdx.z];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, c = lane & 15;
-  const int row0 = blockIdx.x * 16, rank0 = blockIdx.y * 16;
+  const int row0 = blockIdx.x * 16, rank0 = blockIdx.y * 16 * NR;
   const int row = min(row0 + c, p.M - 1);
   int a = p.which ? p.which[row] : 0;
   if (a >= p.L) a = -1;
   const void *x = I8 ? (const void *)((const int8_t *)p.X + row * p.ldx) : (const void *)((const T *)p.X + row * p.ldx);
   const T *w = (const T *)p.P + (int64_t)(rank0 + c) * p.lenp + 8 * g;
   const int64_t step = (int64_t)p.Rp * p.lenp;
-  v4f acc = {0, 0, 0, 0};
-  for (int k0 = wave * 32; k0 < p.lenp; k0 += WAVES * U * 32) {
+  v4f acc[NR];
+#pragma unroll
+  for (int n = 0; n < NR; ++n) acc[n] = v4f{0, 0, 0, 0};
+  for (int k0 = wave * U * 32; k0 < p.lenp; k0 += WAVES * U * 32) {
     Frag<TYPE> xa[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       float v[8];
-      load_row8<TYPE, I8>(x, k0 + u * WAVES * 32 + 8 * g, p.len, v);
+      load_row8<TYPE, I8>(x, k0 + u * 32 + 8 * g, p.len, v);
       xa[u] = to_frag<TYPE>(v);
     }
     each_adapter(a, [&](int cur, uint32_t rows) {
-      Frag<TYPE> b[U];
-      v4f part = {0, 0, 0, 0};
+      Frag<TYPE> b[NR][U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) b[u] = load_frag<TYPE>(w + cur * step + min(k0 + u * WAVES * 32, p.lenp - 32));
+      for (int n = 0; n < NR; ++n)
 #pragma unroll
-      for (int u = 0; u < U; ++u) part = mfma16<TYPE>(xa[u], b[u], part);
+        for (int u = 0; u < U; ++u)
+          b[n][u] = load_frag<TYPE>(w + cur * step + (int64_t)n * 16 * p.lenp + min(k0 + u * 32, p.lenp - 32));
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (rows >> (4 * g + e) & 1) acc[e] += part[e];
+      for (int n = 0; n < NR; ++n) {
+        v4f part = {0, 0, 0, 0};
+#pragma unroll
+        for (int u = 0; u < U; ++u) part = mfma16<TYPE>(xa[u], b[n][u], part);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (rows >> (4 * g + e) & 1) acc[n][e] += part[e];
+      }
     });
   }
 #pragma unroll
-  for (int e = 0; e < 4; ++e) red[wave][4 * g + e][c] = acc[e];
-  __syncthreads();
-  if (threadIdx.x < 256) {
-    const int r = threadIdx.x >> 4, rank = threadIdx.x & 15, i = row0 + r;
-    if (i < p.M) {
-      float s = 0.0f;
+  for (int n = 0; n < NR; ++n)
 #pragma unroll
-      for (int v = 0; v < WAVES; ++v) s += red[v][r][rank];
-      const int ad = p.which ? p.which[i] : 0;
-      p.U[(int64_t)i * p.Rp + rank0 + rank] = ad < 0 ? 0.0f : s * shrink_factor<I8>(p, i, ad);
-    }
+    for (int e = 0; e < 4; ++e) red[wave][4 * g + e][16 * n + c] = acc[n][e];
+  __syncthreads();
+  for (int t = threadIdx.x; t < 256 * NR; t += 1024) {
+    const int r = t / (16 * NR), rank = t % (16 * NR), i = row0 + r;
+    if (i >= p.M) continue;
+    float s = 0.0f;
+#pragma unroll
+    for (int v = 0; v < WAVES; ++v) s += red[v][r][rank];
+    const int ad = p.which ? p.which[i] : 0;
+    p.U[(int64_t)i * p.Rp + rank0 + rank] = ad < 0 ? 0.0f : s * shrink_factor<I8>(p, i, ad);
   }
 }
 
@@ -289,81 +339,139 @@ __device__ __forceinline__ float low_rank_element(const LowRank &l, int row, int
   return s;
 }
 
+// E elements of it at once, so that their loads are under way together; those with
+// a row below 0 are left out.
+template <int TYPE, int E>
+__device__ __forceinline__ void low_rank_elements(const LowRank &l, const int (&row)[E], const int (&col)[E], float (&s)[E]) {
+  const float *u[E];
+  const typename Elem<TYPE>::T *v[E];
+  bool in[E];
+#pragma unroll
+  for (int i = 0; i < E; ++i) {
+    const int a = row[i] < 0 ? -1 : adapter_of(l, row[i]);
+    in[i] = a >= 0;
+    u[i] = l.U + (int64_t)max(row[i], 0) * l.Rp;
+    v[i] = (const typename Elem<TYPE>::T *)l.V + (max(a, 0) * l.colsp + (row[i] < 0 ? 0 : col[i])) * l.Rp;
+    s[i] = 0.0f;
+  }
+  for (int r = 0; r < l.Rp; r += 8) {
+    Frag<TYPE> b[E];
+    v4f x[E], y[E];
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      b[i] = load_frag<TYPE>(v[i] + r);
+      x[i] = *(const v4f *)(u[i] + r);
+      y[i] = *(const v4f *)(u[i] + r + 4);
+    }
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[i] = fmaf(x[i][e], (float)b[i].v[e], s[i]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[i] = fmaf(y[i][e], (float)b[i].v[4 + e], s[i]);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < E; ++i) s[i] = in[i] ? s[i] : 0.0f;
+}
+
 __device__ __forceinline__ float low_rank_element(const LowRank &l, int type, int row, int64_t col) {
   if (type == VT_TYPE_F32) return low_rank_element<kF32>(l, row, col);
   return type == VT_TYPE_F16 ? low_rank_element<kF16>(l, row, col) : low_rank_element<kBF16>(l, row, col);
 }
 
 // Blocks of 16 x 16 in the accumulators' layout: d[ni] element e is row row0 +
-// 4 (lane / 16) + e, column col0 + 16 ni + lane % 16. Columns below colsp, any rows.
+// 4 (lane / 16) + e, column col0 + 16 ni + lane % 16. Columns below colsp, any rows;
+// a: adapter_of row row0 + lane % 16.
 // 16-bit adapters: 16 ranks are one 32-deep product, of u in two halves (16 bits
 // of it in bfloat16, 22 in float16; u is then as exact as the 16-bit y that it is
 // added to needs, 2^-8 of a step) against the same 16 values. float16 halves are of
 // u times a power of two for each row, so that none overflows or is lost.
+// All loads of 16 S ranks are under way together: there is one wave to a SIMD
+// here, and nothing else hides them.
 template <int TYPE, int NI>
-__device__ __forceinline__ void low_rank16(const LowRank &l, int row0, int col0, int lane, v4f (&d)[NI]) {
+__device__ __forceinline__ void low_rank16(const LowRank &l, int a, int row0, int col0, int lane, v4f (&d)[NI]) {
   typedef typename Elem<TYPE>::T T;
+  constexpr int S = NI <= 4 && TYPE != kF32 ? 4 : 2;
   const int g = lane >> 4, c = lane & 15, row = min(row0 + c, l.rows - 1);
-  const float *u = l.U + (int64_t)row * l.Rp;
+  const float *u = l.U + (int64_t)row * l.Rp + (TYPE == kF32 ? 4 * g : 8 * (g & 1));
 #pragma unroll
   for (int ni = 0; ni < NI; ++ni) d[ni] = v4f{0, 0, 0, 0};
-  each_adapter(adapter_of(l, row), [&](int cur, uint32_t rows) {
-    const T *v = (const T *)l.V + (cur * l.colsp + col0 + c) * l.Rp;
+  each_adapter(a, [&](int cur, uint32_t rows) {
+    const T *v = (const T *)l.V + (cur * l.colsp + col0 + c) * l.Rp + (TYPE == kF32 ? 4 * g : 8 * (g & 1));
     v4f t[NI];
 #pragma unroll
     for (int ni = 0; ni < NI; ++ni) t[ni] = v4f{0, 0, 0, 0};
-    if constexpr (TYPE == kF32) {
-      for (int r = 0; r < l.Rp; r += 16) {
-        const v4f a = *(const v4f *)(u + r + 4 * g);
+    auto ranks = [&](auto count, int r) __attribute__((always_inline)) {
+      constexpr int N = decltype(count)::value;
+      if constexpr (TYPE == kF32) {
+        v4f x[N], b[N][NI];
 #pragma unroll
-        for (int ni = 0; ni < NI; ++ni) {
-          const v4f b = *(const v4f *)(v + (int64_t)ni * 16 * l.Rp + r + 4 * g);
+        for (int s = 0; s < N; ++s) {
+          x[s] = *(const v4f *)(u + r + 16 * s);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) t[ni] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], b[e], t[ni], 0, 0, 0);
-        }
-      }
-    } else {
-      for (int r = 0; r < l.Rp; r += 16) {
-        const int at = r + 8 * (g & 1);
-        const v4f a0 = *(const v4f *)(u + at), a1 = *(const v4f *)(u + at + 4);
-        float f[8];
-        uint32_t top = 0;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          f[e] = e < 4 ? a0[e & 3] : a1[e & 3];
-          top = max(top, magnitude(f[e]));
-        }
-        float back = 1.0f;
-        if constexpr (TYPE == kF16) {
-          top = max(top, (uint32_t)__shfl_xor((int)top, 16));
-          const float norm = normaliser(__uint_as_float(top));
-          back = 1.0f / norm;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) f[e] *= norm;
+          for (int ni = 0; ni < NI; ++ni) b[s][ni] = *(const v4f *)(v + (int64_t)ni * 16 * l.Rp + r + 16 * s);
         }
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float hi = (float)(T)f[e];
-          // (inf - inf of an infinite u would make a NaN of its low half)
-          f[e] = g < 2 ? hi : magnitude(hi) < kInfBits ? f[e] - hi : 0.0f;
+        for (int s = 0; s < N; ++s)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int ni = 0; ni < NI; ++ni) t[ni] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[s][e], b[s][ni][e], t[ni], 0, 0, 0);
+      } else {
+        v4f x[N][2];
+        Frag<TYPE> b[N][NI];
+#pragma unroll
+        for (int s = 0; s < N; ++s) {
+          x[s][0] = *(const v4f *)(u + r + 16 * s);
+          x[s][1] = *(const v4f *)(u + r + 16 * s + 4);
+#pragma unroll
+          for (int ni = 0; ni < NI; ++ni) b[s][ni] = load_frag<TYPE>(v + (int64_t)ni * 16 * l.Rp + r + 16 * s);
         }
-        const Frag<TYPE> a = to_frag<TYPE>(f);
-        if constexpr (TYPE == kF16) {
-          v4f un;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) un[e] = __shfl(back, 4 * g + e);
+        for (int s = 0; s < N; ++s) {
+          float f[8];
+          uint32_t top = 0;
 #pragma unroll
-          for (int ni = 0; ni < NI; ++ni) {
-            const v4f p = mfma16<TYPE>(a, load_frag<TYPE>(v + (int64_t)ni * 16 * l.Rp + at), v4f{0, 0, 0, 0});
-#pragma unroll
-            for (int e = 0; e < 4; ++e) t[ni][e] = fmaf(p[e], un[e], t[ni][e]);
+          for (int e = 0; e < 8; ++e) {
+            f[e] = x[s][e >> 2][e & 3];
+            top = max(top, magnitude(f[e]));
           }
-        } else {
+          float back = 1.0f;
+          if constexpr (TYPE == kF16) {
+            top = max(top, (uint32_t)__shfl_xor((int)top, 16));
+            const float norm = normaliser(__uint_as_float(top));
+            back = 1.0f / norm;
 #pragma unroll
-          for (int ni = 0; ni < NI; ++ni) t[ni] = mfma16<TYPE>(a, load_frag<TYPE>(v + (int64_t)ni * 16 * l.Rp + at), t[ni]);
+            for (int e = 0; e < 8; ++e) f[e] *= norm;
+          }
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float hi = (float)(T)f[e];
+            // (inf - inf of an infinite u would make a NaN of its low half)
+            f[e] = g < 2 ? hi : magnitude(hi) < kInfBits ? f[e] - hi : 0.0f;
+          }
+          const Frag<TYPE> h = to_frag<TYPE>(f);
+          if constexpr (TYPE == kF16) {
+            v4f un;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) un[e] = __shfl(back, 4 * g + e);
+#pragma unroll
+            for (int ni = 0; ni < NI; ++ni) {
+              const v4f p = mfma16<TYPE>(h, b[s][ni], v4f{0, 0, 0, 0});
+#pragma unroll
+              for (int e = 0; e < 4; ++e) t[ni][e] = fmaf(p[e], un[e], t[ni][e]);
+            }
+          } else {
+#pragma unroll
+            for (int ni = 0; ni < NI; ++ni) t[ni] = mfma16<TYPE>(h, b[s][ni], t[ni]);
+          }
         }
       }
-    }
+    };
+    int r = 0;
+    for (; r + 16 * S <= l.Rp; r += 16 * S) ranks(std::integral_constant<int, S>(), r);
+    for (; r < l.Rp; r += 16) ranks(std::integral_constant<int, 1>(), r);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const bool mine = rows >> (4 * g + e) & 1;
@@ -373,43 +481,70 @@ __device__ __forceinline__ void low_rank16(const LowRank &l, int row0, int col0,
   });
 }
 
+// The adapters of a wave's 128 rows from row0: lane l holds rows l and 64 + l.
+struct RowAdapters {
+  int a[2];
+};
+__device__ __forceinline__ RowAdapters row_adapters(const LowRank &l, int row0, int lane) {
+  RowAdapters r;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) r.a[h] = adapter_of(l, min(row0 + 64 * h + lane, l.rows - 1));
+  return r;
+}
+// That of row rel + lane % 16 (rel a multiple of 16).
+__device__ __forceinline__ int adapter_at(const RowAdapters &r, int rel, int lane) {
+  return __shfl(rel >= 64 ? r.a[1] : r.a[0], (rel & 63) + (lane & 15));
+}
+
 // A linear layer's outputs with adapters. TYPE: of adapters and outputs.
 template <int TYPE>
 struct AdaptedTile : ScaledTile<kLinear, TYPE == kF32 ? 4 : 2> {
   LowRank low;
   static constexpr int OE = TYPE == kF32 ? 4 : 2;
 
+  // A strip of 16 rows at a time in a loop, of which only the reading of the sums
+  // is unrolled: as straight code the low-rank products (3 times, for ranks in
+  // fours, ones and several adapters) leave the instruction cache with every strip.
+  // Rows and columns that a moved-back tile shares with its neighbour come out the
+  // same in both.
   template <int MI, int NI, bool EDGE>
-  __device__ __forceinline__ void tile16(const v4i (&acc)[MI][NI], int row0, int col0, int row_min, int col_min, int lane,
-                                         LDS_AS int8_t *lds) const {
-    constexpr int W = NI * 16, PITCH = W * OE, RC = PITCH / 16;
-    const int g = lane >> 4, c = lane & 15;
+  __device__ __forceinline__ void tile16(const v4i (&acc)[MI][NI], int row0, int col0, int, int, int lane, LDS_AS int8_t *lds) const {
+    constexpr int W = NI * 16, LPR = W / 8, RPI = 64 / LPR, IT = 16 / RPI;
+    const int g = lane >> 4, c = lane & 15, j8 = 8 * (lane % LPR), lr = lane / LPR;
     float s[NI], b[NI];
 #pragma unroll
     for (int ni = 0; ni < NI; ++ni) {
       s[ni] = this->meta[col0 + ni * 16 + c];
       b[ni] = this->meta[this->Np + col0 + ni * 16 + c];
     }
-    auto swz = [](int row) { return (((row >> 2) & 3) * OE) & (RC - 1); };
-    int wb[NI];
-#pragma unroll
-    for (int ni = 0; ni < NI; ++ni) wb[ni] = 4 * g * PITCH + (((ni * OE + (c * OE >> 4)) ^ swz(4 * g)) << 4) + (c * OE & 15);
-    each([&](auto strip) __attribute__((always_inline)) {
-      constexpr int mi = decltype(strip)::value;
+    const RowAdapters ra = row_adapters(low, row0, lane);
+#pragma unroll 1
+    for (int mi = 0; mi < MI; ++mi) {
       const v4f tr = *(const v4f_any *)(this->t + row0 + mi * 16 + 4 * g);
       v4f d[NI];
-      low_rank16<TYPE, NI>(low, row0 + mi * 16, col0, lane, d);
-      __builtin_amdgcn_sched_barrier(0);
+      low_rank16<TYPE, NI>(low, adapter_at(ra, mi * 16, lane), row0 + mi * 16, col0, lane, d);
+      // chunk k of strip row r at k ^ (4 (r / 4 % 4)): an instruction's writes fall on distinct banks
+      each([&](auto strip) __attribute__((always_inline)) {
+        constexpr int i = decltype(strip)::value;
+        if (mi != i) return;
 #pragma unroll
-      for (int ni = 0; ni < NI; ++ni) {
-        float v[4];
+        for (int ni = 0; ni < NI; ++ni)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = ((float)acc[mi][ni][e] * tr[e] * s[ni] + b[ni]) + d[ni][e];
-        this->template put4<PITCH>(lds + wb[ni], v[0], v[1], v[2], v[3]);
+          for (int e = 0; e < 4; ++e)
+            *(LDS_AS float *)(lds + (4 * g + e) * (W * 4) + ((((ni ^ g) << 2) + (c >> 2)) << 4) + (c & 3) * 4) =
+                ((float)acc[i][ni][e] * tr[e] * s[ni] + b[ni]) + d[ni][e];
+      }, std::make_integer_sequence<int, MI>());
+#pragma unroll
+      for (int it = 0; it < IT; ++it) {
+        const int r = it * RPI + lr;
+        const LDS_AS int8_t *at = lds + r * (W * 4);
+        const int swz = ((r >> 2) & 3) << 2;
+        const v4f x = *(const LDS_AS v4f *)(at + (((j8 >> 2) ^ swz) << 4)), y = *(const LDS_AS v4f *)(at + ((((j8 >> 2) + 1) ^ swz) << 4));
+        const float v[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+        if (col0 + j8 < this->N)
+          this->store8((int64_t)(row0 + mi * 16 + r) * this->ldy + col0 + j8, v, this->N - (col0 + j8), this->type);
       }
-      this->template store_rows<W>(lds, swz, row0 + mi * 16, col0, 0, lane, EDGE ? row_min : 0, col_min);
-      __builtin_amdgcn_sched_barrier(0);
-    }, std::make_integer_sequence<int, MI>());
+    }
   }
 
   // 32 x 32 blocks (element e of lane l: row 8 (e / 4) + 4 (l / 32) + e % 4, column
@@ -422,6 +557,7 @@ struct AdaptedTile : ScaledTile<kLinear, TYPE == kF32 ? 4 : 2> {
     if (col0 >= this->Np) return;   // the same for the whole wave, behind the last barrier
     const int g = lane >> 5, c = lane & 31;
     LDS_AS float *f = (LDS_AS float *)lds;   // [32][64]
+    const RowAdapters ra = row_adapters(low, row0, lane);
     each([&](auto strip) __attribute__((always_inline)) {
       constexpr int mi = decltype(strip)::value;
       const int first = row0 + mi * 32;
@@ -429,7 +565,7 @@ struct AdaptedTile : ScaledTile<kLinear, TYPE == kF32 ? 4 : 2> {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         v4f d[4];
-        low_rank16<TYPE, 4>(low, first + 16 * h, col0, lane, d);
+        low_rank16<TYPE, 4>(low, adapter_at(ra, mi * 32 + 16 * h, lane), first + 16 * h, col0, lane, d);
 #pragma unroll
         for (int ni = 0; ni < 4; ++ni)
 #pragma unroll
@@ -459,9 +595,19 @@ struct AdaptedTile : ScaledTile<kLinear, TYPE == kF32 ? 4 : 2> {
     }, std::make_integer_sequence<int, MI>());
   }
 
+  // The adapters' part of E elements, before the sums are there.
+  template <int E>
+  __device__ __forceinline__ void ahead(const int (&row)[E], const int (&col)[E], float (&d)[E]) const {
+    if (this->type == VT_TYPE_F32) low_rank_elements<kF32>(low, row, col, d);
+    else if (this->type == VT_TYPE_F16) low_rank_elements<kF16>(low, row, col, d);
+    else low_rank_elements<kBF16>(low, row, col, d);
+  }
   __device__ __forceinline__ void element(int32_t a0, int32_t, int row, int pc, int j, float t_row) const {
+    if (j < this->N) element_with(a0, row, pc, j, t_row, low_rank_element(low, this->type, row, j));
+  }
+  __device__ __forceinline__ void element_with(int32_t a0, int row, int pc, int j, float t_row, float d) const {
     if (j >= this->N) return;
-    const float v = ((float)a0 * t_row * this->meta[pc] + this->meta[this->Np + pc]) + low_rank_element(low, this->type, row, j);
+    const float v = ((float)a0 * t_row * this->meta[pc] + this->meta[this->Np + pc]) + d;
     const int64_t at = (int64_t)row * this->ldy + j;
     if (this->type == VT_TYPE_F32) ((float *)this->Y)[at] = v;
     else ((uint16_t *)this->Y)[at] = (uint16_t)pack16(v, 0.0f, this->type);
@@ -478,6 +624,7 @@ struct AdaptedGrad : ScaledTile<kGrad> {
                                            const float *early) const {
     const int g = lane >> 4, c = lane & 15;
     const float one[2] = {1.0f, 1.0f};
+    const RowAdapters ra = row_adapters(low, row0, lane);
     this->template strips<MI / G, 16 * G, NI * 16>(
         [&](auto strip) __attribute__((always_inline)) {
 #pragma unroll
@@ -486,7 +633,7 @@ struct AdaptedGrad : ScaledTile<kGrad> {
             const int rel = (first + i) * 16;
             v4f d[NI];
             // columns past the last are not stored, and read from before it
-            low_rank16<TYPE, NI>(low, row0 + rel, min(col0, (int)low.colsp - NI * 16), lane, d);
+            low_rank16<TYPE, NI>(low, adapter_at(ra, rel, lane), row0 + rel, min(col0, (int)low.colsp - NI * 16), lane, d);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const float unit = __shfl(rel >= 64 ? early[1] : early[0], (rel + 4 * g + e) & 63);
@@ -535,21 +682,29 @@ struct OuterArgs {
   int M, cols, colsp, L, R, Rp, splits, turned;
 };
 
+// One or two of them over the same rows: the first `x0` of blockIdx.x are the first's.
+struct OuterPair {
+  OuterArgs of[2];
+  int x0;
+};
+
 // 16 ranks by 128 columns of one adapter over one range of rows to a workgroup.
 // Its waves take 4 rows at a time in turn, as 4-deep float32 products (nothing is
 // rounded on the way, whatever the type): lane l holds 8 columns of row l / 16,
 // and product j takes column j of every lane's. The rows of other adapters are
 // left out by a list of this one's rows, made in order 1024 rows at a time.
 template <int TYPE>
-__global__ __launch_bounds__(256) void outer_kernel(OuterArgs p) {
+__global__ __launch_bounds__(256) void outer_kernel(OuterPair pair) {
   typedef typename Elem<TYPE>::T T;
   constexpr int ROWS = 1024;
+  const int which_of = (int)blockIdx.x >= pair.x0, block = blockIdx.x - (which_of ? pair.x0 : 0);
+  const OuterArgs &p = pair.of[which_of];
   __shared__ int list[ROWS];
   __shared__ int counts[4][4];
   __shared__ float red[4][16][132];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, c = lane & 15;
   const int ranks = p.Rp / 16, tiles = (p.cols + 127) / 128;
-  const int tile = blockIdx.x % tiles, rank0 = blockIdx.x / tiles % ranks * 16;
+  const int tile = block % tiles, rank0 = block / tiles % ranks * 16;
   const int a = blockIdx.y, split = blockIdx.z;
   const int col = tile * 128 + 8 * c;
   const int beg = (int)((int64_t)p.M * split / p.splits), end = (int)((int64_t)p.M * (split + 1) / p.splits);
@@ -582,7 +737,7 @@ __global__ __launch_bounds__(256) void outer_kernel(OuterArgs p) {
       n = total;
       __syncthreads();
     }
-    constexpr int U = 4;
+    constexpr int U = TYPE == kF32 ? 4 : 8;
     for (int i0 = wave * 4 * U; i0 < n; i0 += 16 * U) {
       float h[U], z[U][8];
 #pragma unroll
@@ -626,9 +781,11 @@ __global__ __launch_bounds__(256) void outer_kernel(OuterArgs p) {
 
 // The splits' sums, in one order.
 template <int TYPE>
-__global__ __launch_bounds__(256) void outer_sum_kernel(OuterArgs p) {
+__global__ __launch_bounds__(256) void outer_sum_kernel(OuterPair pair) {
   typedef typename Elem<TYPE>::T T;
-  const int64_t count = (int64_t)p.R * p.cols, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int which_of = (int)blockIdx.x >= pair.x0;
+  const OuterArgs &p = pair.of[which_of];
+  const int64_t count = (int64_t)p.R * p.cols, i = (int64_t)(blockIdx.x - (which_of ? pair.x0 : 0)) * 256 + threadIdx.x;
   if (i >= count) return;
   const int a = blockIdx.y;
   const int r = (int)(p.turned ? i % p.R : i / p.cols), k = (int)(p.turned ? i / p.R : i % p.cols);
@@ -649,44 +806,69 @@ __global__ __launch_bounds__(256) void outer_sum_kernel(OuterArgs p) {
 // Host side
 // ---------------------------------------------------------------------------
 
+// `count` (1 or 2) of them over the same rows.
 template <int TYPE, bool I8>
-int launch_shrink(const ShrinkArgs &a, hipStream_t s) {
-  if (a.M <= kSkinnyMaxM)
-    hipLaunchKernelGGL((shrink_rows_kernel<TYPE, I8>), dim3((unsigned)a.M, (unsigned)(a.Rp / 16)), dim3(1024), 0, s, a);
-  else
-    hipLaunchKernelGGL((shrink_tiles_kernel<TYPE, I8>), dim3((unsigned)((a.M + 15) / 16), (unsigned)(a.Rp / 16)), dim3(512), 0, s, a);
+int launch_shrink(const ShrinkPair &a, int count, int cus, hipStream_t s) {
+  const int64_t M = a.of[0].M, blocks = (M + 15) / 16, ranks = a.of[0].Rp / 16;
+  if (M <= kSkinnyMaxM) {
+    hipLaunchKernelGGL((shrink_rows_kernel<TYPE, I8>), dim3((unsigned)M, (unsigned)ranks, (unsigned)count), dim3(1024), 0, s, a);
+  } else {
+    // as many ranks to a workgroup as leave most CUs one
+    const bool two = ranks % 2 == 0 && blocks * (ranks / 2) * count >= cus * 3 / 4;
+    if (two && TYPE != kF32 && ranks % 4 == 0 && blocks * (ranks / 4) * count >= cus * 3 / 4)
+      hipLaunchKernelGGL((shrink_tiles_kernel<TYPE, I8, TYPE == kF32 ? 2 : 4>), dim3((unsigned)blocks, (unsigned)(ranks / 4), (unsigned)count), dim3(1024), 0, s, a);
+    else if (two)
+      hipLaunchKernelGGL((shrink_tiles_kernel<TYPE, I8, 2>), dim3((unsigned)blocks, (unsigned)(ranks / 2), (unsigned)count), dim3(1024), 0, s, a);
+    else
+      hipLaunchKernelGGL((shrink_tiles_kernel<TYPE, I8, 1>), dim3((unsigned)blocks, (unsigned)ranks, (unsigned)count), dim3(1024), 0, s, a);
+  }
   VT_HIP_CHECK(hipGetLastError());
   return VT_OK;
 }
 
-int shrink(const ShrinkArgs &a, int type, bool i8, hipStream_t s) {
+int shrink(const ShrinkPair &a, int count, int type, bool i8, const Scratch &scr) {
   return by_type(type, [&](auto t) {
     constexpr int TYPE = decltype(t)::value;
-    return i8 ? launch_shrink<TYPE, true>(a, s) : launch_shrink<TYPE, false>(a, s);
+    hipStream_t s = (hipStream_t)scr.stream;
+    return i8 ? launch_shrink<TYPE, true>(a, count, scr.st->num_cus, s) : launch_shrink<TYPE, false>(a, count, scr.st->num_cus, s);
   });
 }
 
+// `count` (1 or 2) of them over the same rows and adapters.
 template <int TYPE>
-int launch_outer(OuterArgs a, Scratch &scr) {
+int launch_outer(OuterPair a, int count, Scratch &scr) {
   hipStream_t s = (hipStream_t)scr.stream;
-  const int64_t per = (int64_t)((a.cols + 127) / 128) * (a.Rp / 16), wgs = per * a.L;
-  // Rows are split until there are two workgroups for each CU, of 64 rows at
+  const OuterArgs &f = a.of[0];
+  int64_t wgs = 0, bytes[2] = {0, 0}, blocks[2] = {0, 0}, sums = 0;
+  for (int i = 0; i < count; ++i) {
+    const OuterArgs &o = a.of[i];
+    blocks[i] = (int64_t)((o.cols + 127) / 128) * (o.Rp / 16);
+    bytes[i] = (int64_t)o.L * o.Rp * o.colsp * sizeof(float);
+    wgs += blocks[i];
+  }
+  // Rows are split until there are four workgroups for each CU, of 64 rows at
   // least, as far as the partial sums stay within their bound.
-  const int64_t bytes = (int64_t)a.L * a.Rp * a.colsp * sizeof(float);
-  int64_t splits = std::max<int64_t>(1, std::min<int64_t>({(2 * scr.st->num_cus + wgs - 1) / wgs, (a.M + 63) / 64, kScaledBytes / bytes}));
-  a.splits = (int)splits;
-  if (splits > 1) {
-    void *w = nullptr;
-    if (int rc = scr.take(kPartials, (size_t)(splits * bytes), &w)) return rc;
-    a.part = (float *)w;
+  const int64_t all = wgs * f.L, cus = scr.st->num_cus;
+  const int64_t splits = std::max<int64_t>(1, std::min<int64_t>({(4 * cus + all - 1) / all, (f.M + 63) / 64, kScaledBytes / (bytes[0] + bytes[1])}));
+  if (wgs > 0x7fffffff) return fail(VT_EUNSUPPORTED, "gradient grid too large");
+  void *w = nullptr;
+  if (splits > 1)
+    if (int rc = scr.take(kPartials, (size_t)(splits * (bytes[0] + bytes[1])), &w)) return rc;
+  for (int i = 0; i < count; ++i) {
+    a.of[i].splits = (int)splits;
+    if (splits > 1) a.of[i].part = (float *)((int8_t *)w + (i ? splits * bytes[0] : 0));
   }
-  if (per > 0x7fffffff) return fail(VT_EUNSUPPORTED, "gradient grid too large");
-  hipLaunchKernelGGL((outer_kernel<TYPE>), dim3((unsigned)per, (unsigned)a.L, (unsigned)splits), dim3(256), 0, s, a);
+  a.x0 = (int)blocks[0];
+  hipLaunchKernelGGL((outer_kernel<TYPE>), dim3((unsigned)wgs, (unsigned)f.L, (unsigned)splits), dim3(256), 0, s, a);
   VT_HIP_CHECK(hipGetLastError());
-  if (splits > 1) {
-    hipLaunchKernelGGL((outer_sum_kernel<TYPE>), dim3((unsigned)(((int64_t)a.R * a.cols + 255) / 256), (unsigned)a.L), dim3(256), 0, s, a);
-    VT_HIP_CHECK(hipGetLastError());
+  if (splits == 1) return VT_OK;
+  for (int i = 0; i < count; ++i) {
+    blocks[i] = ((int64_t)a.of[i].R * a.of[i].cols + 255) / 256;
+    sums += blocks[i];
   }
+  a.x0 = (int)blocks[0];
+  hipLaunchKernelGGL((outer_sum_kernel<TYPE>), dim3((unsigned)sums, (unsigned)f.L), dim3(256), 0, s, a);
+  VT_HIP_CHECK(hipGetLastError());
   return VT_OK;
 }
 
@@ -717,8 +899,15 @@ struct AdaptedDx : AdaptedGrad<TYPE> {
   }
 };
 
-// Rows of a forward call, whose u is there.
-int adapted_rows(const ScaledCall &c, const LowRank &low, Scratch &scr) {
+// Whether u's kernel rounds a call's rows too: those that the weights' stream does
+// not round itself.
+bool shrink_rounds(const ScaledCall &c) {
+  const int64_t Kp = scaled_kp(c.K);
+  return float_type(c.x_type) && c.M <= kSkinnyMaxM && Kp > 0 && !(c.M <= 16 && c.M * Kp <= kFusedValues);
+}
+
+// Rows of a forward call, whose u is there (and `ready`: the rows rounded).
+int adapted_rows(const ScaledCall &c, const LowRank &low, const Rows *ready, Scratch &scr) {
   const int64_t Kp = scaled_kp(c.K), Np = scaled_np(c.N, false);
   AdaptedSkinny o = {};
   o.meta = c.meta; o.Y = c.Y; o.ldy = c.ldy;
@@ -729,7 +918,8 @@ int adapted_rows(const ScaledCall &c, const LowRank &low, Scratch &scr) {
   const bool skinny = c.M <= kSkinnyMaxM && Kp > 0;
   if (skinny && float_type(c.x_type) && c.M <= 16 && c.M * Kp <= kFusedValues)
     return launch_skinny<kLinear>(c.X, c.x_type, c.ldx, c.K, rows, c.Bp, o, scr);
-  if (int rc = take_rows(c.X, c.x_type, c.ldx, c.T, c.M, c.K, scr, &rows)) return rc;
+  if (ready) rows = *ready;
+  else if (int rc = take_rows(c.X, c.x_type, c.ldx, c.T, c.M, c.K, scr, &rows)) return rc;
   o.t = rows.t;
   if (skinny) return launch_skinny<kLinear>(nullptr, 0, 0, c.K, rows, c.Bp, o, scr);
   hipStream_t s = (hipStream_t)scr.stream;
@@ -783,12 +973,7 @@ LowRank low_at(LowRank l, int64_t r, int64_t rows) {
 struct AdapterCall {
   const char *who;
   int type;
-  const void *P;
-  int64_t L, R, K, N, M;
-  bool back;
-  float scale;
-  const int32_t *which;
-  float *U;
+  int64_t L, R, K, N;
 };
 
 int check_adapters(const AdapterCall &c) {
@@ -806,29 +991,31 @@ int check_adapters(const AdapterCall &c) {
 extern "C" {
 
 int64_t vt_adapter_size(int64_t K, int64_t N, int64_t R, int64_t L, int32_t type) {
-  const AdapterCall c = {"vt_adapter_size", type, nullptr, L, R, K, N, 0, false, 0.0f, nullptr, nullptr};
+  const AdapterCall c = {"vt_adapter_size", type, L, R, K, N};
   if (int rc = check_adapters(c)) return rc;
   const AdapterLayout l = adapter_layout(K, N, R, L);
   return (l.first(false) + l.second(false)) * elem_size(type);
 }
 
-int vt_adapter_pack(const void *down, const void *up, int32_t type, int64_t K, int64_t N, int64_t R, int64_t L, int32_t back,
-                    void *P, void *stream) {
+int vt_adapter_pack(const void *down, const void *up, int32_t type, int64_t K, int64_t N, int64_t R, int64_t L, void *P,
+                    void *back, void *stream) {
   g_err.clear();
   const char *who = "vt_adapter_pack";
-  const AdapterCall c = {who, type, P, L, R, K, N, 0, back != 0, 0.0f, nullptr, nullptr};
+  const AdapterCall c = {who, type, L, R, K, N};
   if (int rc = check_adapters(c)) return rc;
   const AdapterLayout l = adapter_layout(K, N, R, L);
   const int64_t e = elem_size(type), size = l.first(false) + l.second(false);
-  if (size == 0) return VT_OK;
-  if (!P || (K > 0 && !down) || (N > 0 && !up)) return fail(VT_EINVAL, "%s: an operand is null", who);
+  if (size == 0 || (!P && !back)) return VT_OK;
+  if ((K > 0 && !down) || (N > 0 && !up)) return fail(VT_EINVAL, "%s: an operand is null", who);
   const Operand o[] = {{"down", down, 1, L * R * K, L * R * K, e, false}, {"up", up, 1, L * R * N, L * R * N, e, false},
-                       {"P", P, 1, size, size, e, true, 16 / e}};
-  if (int rc = check_operands(who, o, 3)) return rc;
+                       {"P", P, 1, size, size, e, true, 16 / e}, {"back", back, 1, size, size, e, true, 16 / e}};
+  if (int rc = check_operands(who, o, 4)) return rc;
   Scratch scr;
   if (int rc = open_scratch(stream, &scr)) return rc;
-  const AdapterPackArgs a = {(const uint8_t *)down, (const uint8_t *)up, (uint8_t *)P, (uint8_t *)P + l.first(back != 0) * e,
-                             (int)K, (int)N, (int)R, (int)l.Kp, (int)l.Np, (int)l.Rp, back != 0, (int)e};
+  AdapterPackArgs a = {(const uint8_t *)down, (const uint8_t *)up, {(uint8_t *)P, (uint8_t *)back}, {nullptr, nullptr},
+                       (int)K, (int)N, (int)R, (int)l.Kp, (int)l.Np, (int)l.Rp};
+  for (int i = 0; i < 2; ++i)
+    if (a.first[i]) a.second[i] = a.first[i] + l.first(i != 0) * e;
   const dim3 grid((unsigned)(std::max(l.Kp, l.Np) / 64), (unsigned)L, 2);
   if (e == 4) hipLaunchKernelGGL(adapter_pack_kernel<uint32_t>, grid, dim3(256), 0, (hipStream_t)stream, a);
   else hipLaunchKernelGGL(adapter_pack_kernel<uint16_t>, grid, dim3(256), 0, (hipStream_t)stream, a);
@@ -842,7 +1029,7 @@ int vt_adapted_linear(const void *X, int32_t x_type, int64_t ldx, const float *T
   g_err.clear();
   const char *who = "vt_adapted_linear";
   const ScaledCall c = {who, X, x_type, ldx, K, T, Bp, meta, Y, type, ldy, N, M, K, N, false};
-  const AdapterCall ad = {who, type, P, L, R, K, N, M, false, scale, which, U};
+  const AdapterCall ad = {who, type, L, R, K, N};
   if (int rc = check_adapters(ad)) return rc;
   const int64_t Rp = rank_pad(R);
   ScaledCall checked = c;
@@ -864,54 +1051,66 @@ int vt_adapted_linear(const void *X, int32_t x_type, int64_t ldx, const float *T
                        {"scales", meta, 1, 0, scaled_meta(l.Np), 4, false}, {"adapters", P, 1, size, size, e, false, 16 / e},
                        {"which", which, 1, M, M, 4, false}, {"U", U, 1, M * Rp, M * Rp, 4, true, 4}, {"Y", Y, M, ldy, N, e, true}};
   if (int rc = check_operands(who, o, 8)) return rc;
-  const bool copied = !rows_in_place(X, x_type, ldx, K);
-  const int64_t step = copied ? rows_at_once(M, l.Kp + 4) : M;
   const LowRank low = {U, (const int8_t *)P + l.first(false) * e, which, l.Np, (int)L, (int)Rp, (int)M};
-  {
+  ShrinkPair pair = {};
+  pair.of[0] = ShrinkArgs{X, T, P, which, U, ldx, scale, (int)M, (int)K, (int)l.Kp, (int)L, (int)Rp, nullptr, nullptr};
+  const bool out = Y && !empty;
+  // few rows are one part
+  const int64_t step = rows_in_place(X, x_type, ldx, K) ? M : rows_at_once(M, l.Kp + 4);
+  for (int64_t r = 0; r < M && (out || r == 0); r += step) {
     Scratch scr;
     if (int rc = open_scratch(stream, &scr)) return rc;
-    const ShrinkArgs a = {X, T, P, which, U, ldx, scale, (int)M, (int)K, (int)l.Kp, (int)L, (int)Rp};
-    if (int rc = shrink(a, type, i8, (hipStream_t)stream)) return rc;
-  }
-  if (empty || !Y) return VT_OK;
-  for (int64_t r = 0; r < M; r += step) {
-    Scratch scr;
-    if (int rc = open_scratch(stream, &scr)) return rc;
-    const int64_t rows = std::min(step, M - r);
-    if (int rc = adapted_rows(part_of(c, r, rows), low_at(low, r, rows), scr)) return rc;
+    Rows rows = {};
+    const bool rounds = out && shrink_rounds(c);
+    if (rounds) {
+      void *w = nullptr;
+      if (int rc = scr.take(kRows, (size_t)M * (l.Kp + sizeof(float)), &w)) return rc;
+      pair.of[0].Q = (int8_t *)w;
+      pair.of[0].T = (float *)((int8_t *)w + M * l.Kp);
+      rows = Rows{pair.of[0].Q, pair.of[0].T, l.Kp};
+    }
+    if (r == 0)
+      if (int rc = shrink(pair, 1, type, i8, scr)) return rc;
+    if (!out) break;
+    const int64_t count = std::min(step, M - r);
+    if (int rc = adapted_rows(part_of(c, r, count), low_at(low, r, count), rounds ? &rows : nullptr, scr)) return rc;
   }
   return VT_OK;
 }
 
 int vt_adapted_grad(const void *dY, int32_t type, int64_t ldd, const void *X, int64_t ldx, int64_t M, int64_t K, const int8_t *Bp,
-                    const float *meta, int64_t N, const void *P, int64_t R, int64_t L, float scale, const int32_t *which,
-                    const float *U, float *H, void *dX, int64_t lddx, void *dDown, void *dUp, void *stream) {
+                    const float *meta, int64_t N, const void *P, const void *back, int64_t R, int64_t L, float scale,
+                    const int32_t *which, float *U, float *H, void *dX, int64_t lddx, void *dDown, void *dUp, void *stream) {
   g_err.clear();
   const char *who = "vt_adapted_grad";
   const int64_t Rp = rank_pad(R);
   const ScaledCall c = {who, dY, type, ldd, N, nullptr, Bp, meta, dX ? dX : H, dX ? type : VT_TYPE_F32, dX ? lddx : Rp, dX ? K : Rp, M, K, N, false};
-  const AdapterCall ad = {who, type, P, L, R, K, N, M, true, scale, which, H};
+  const AdapterCall ad = {who, type, L, R, K, N};
   if (int rc = check_adapters(ad)) return rc;
   bool empty = false;
   if (int rc = check_scaled(c, &empty)) return rc;
   const AdapterLayout l = adapter_layout(K, N, R, L);
   const int64_t e = elem_size(type), size = l.first(true) + l.second(true);
-  if (M > 0 && (!H || (size > 0 && !P) || (dUp && !U) || (dDown && K > 0 && !X)))
+  const bool again = P && dUp;   // u has to be made again
+  if (M > 0 && (!H || (size > 0 && !back) || (dUp && !U) || ((dDown || again) && K > 0 && !X)))
     return fail(VT_EINVAL, "%s: adapters, X, U or H are null", who);
   const Operand o[] = {{"dY", dY, M, ldd, N, e, false}, {"X", X, M, ldx, K, e, false}, {"weights", Bp, 1, 0, l.Kp * l.Np, 1, false},
                        {"scales", meta, 1, 0, scaled_meta(l.Np), 4, false}, {"adapters", P, 1, size, size, e, false, 16 / e},
-                       {"which", which, 1, M, M, 4, false}, {"U", U, 1, M * Rp, M * Rp, 4, false, 4},
+                       {"adapters", back, 1, size, size, e, false, 16 / e}, {"which", which, 1, M, M, 4, false},
+                       {"U", dUp ? U : nullptr, 1, M * Rp, M * Rp, 4, again, 4},
                        {"H", H, 1, M * Rp, M * Rp, 4, true, 4}, {"dX", dX, M, lddx, K, e, true},
                        {"dDown", dDown, 1, L * R * K, L * R * K, e, true}, {"dUp", dUp, 1, L * R * N, L * R * N, e, true}};
-  if (int rc = check_operands(who, o, 11)) return rc;
+  if (int rc = check_operands(who, o, 12)) return rc;
   if (M > 0) {
     Scratch scr;
     if (int rc = open_scratch(stream, &scr)) return rc;
-    const ShrinkArgs a = {dY, nullptr, P, which, H, ldd, scale, (int)M, (int)N, (int)l.Np, (int)L, (int)Rp};
-    if (int rc = shrink(a, type, false, (hipStream_t)stream)) return rc;
+    ShrinkPair a = {};
+    a.of[0] = ShrinkArgs{dY, nullptr, back, which, H, ldd, scale, (int)M, (int)N, (int)l.Np, (int)L, (int)Rp, nullptr, nullptr};
+    a.of[1] = ShrinkArgs{X, nullptr, P, which, U, ldx, scale, (int)M, (int)K, (int)l.Kp, (int)L, (int)Rp, nullptr, nullptr};
+    if (int rc = shrink(a, again ? 2 : 1, type, false, scr)) return rc;
   }
   if (dX && M > 0 && K > 0) {
-    const LowRank low = {H, (const int8_t *)P + l.first(true) * e, which, l.Kp, (int)L, (int)Rp, (int)M};
+    const LowRank low = {H, (const int8_t *)back + l.first(true) * e, which, l.Kp, (int)L, (int)Rp, (int)M};
     const int64_t step = rows_at_once(M, l.Np * (two_halves(type) ? 4 : 2) + 4);
     for (int64_t r = 0; r < M; r += step) {
       const int64_t rows = std::min(step, M - r);
@@ -927,13 +1126,14 @@ int vt_adapted_grad(const void *dY, int32_t type, int64_t ldd, const void *X, in
   }
   Scratch scr;
   if (int rc = open_scratch(stream, &scr)) return rc;
-  auto outer = [&](const float *h, const void *z, int64_t ldz, int64_t cols, int64_t colsp, void *out, bool turned) {
-    if (!out || cols == 0) return (int)VT_OK;
-    const OuterArgs a = {h, z, which, nullptr, out, ldz, (int)M, (int)cols, (int)colsp, (int)L, (int)R, (int)Rp, 1, turned};
-    return by_type(type, [&](auto t) { return launch_outer<decltype(t)::value>(a, scr); });
-  };
-  if (int rc = outer(H, X, ldx, K, l.Kp, dDown, false)) return rc;
-  return outer(U, dY, ldd, N, l.Np, dUp, true);
+  OuterPair a = {};
+  int count = 0;
+  if (dDown && K > 0)
+    a.of[count++] = OuterArgs{H, X, which, nullptr, dDown, ldx, (int)M, (int)K, (int)l.Kp, (int)L, (int)R, (int)Rp, 1, 0};
+  if (dUp && N > 0)
+    a.of[count++] = OuterArgs{U, dY, which, nullptr, dUp, ldd, (int)M, (int)N, (int)l.Np, (int)L, (int)R, (int)Rp, 1, 1};
+  if (count == 0) return VT_OK;
+  return by_type(type, [&](auto t) { return launch_outer<decltype(t)::value>(a, count, scr); });
 }
 
 }  // extern "C"

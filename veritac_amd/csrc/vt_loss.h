@@ -196,6 +196,9 @@ struct LseTile : ScaledOut {
 template <bool LOW>
 struct LossTermsTile : ScaledTile<kGradTerms, 2, LOW> {
   const RowState *state;
+  const float *dloss, *count;   // count null: not a mean
+  float *norm_out;
+  int64_t step;                 // of dloss: 1 for one a row, 0 for one in all
 
   struct Row {
     float t, top, log_sum, norm;
@@ -224,64 +227,88 @@ struct LossTermsTile : ScaledTile<kGradTerms, 2, LOW> {
     return v;
   }
 
+  // What the gradient product divides a row by: its normaliser over the gradient
+  // that reaches its loss.
+  __device__ __forceinline__ void put_norm(int row, const Row &r) const {
+    float g = dloss[row * step];
+    if (count) g /= *count;
+    norm_out[row] = r.target == kIgnored ? __builtin_inff() : r.norm / g;
+  }
+
+  // A strip of 16 rows at a time in a loop: its sums go through the wave's LDS to 8
+  // columns of a row a lane, which then needs one row's state, and the code stays
+  // in the instruction cache (unrolled, and a branch for the target in each of its
+  // parts, the kernel took 606 us at 2048 x 4096 x 65536).
   template <int MI, int NI, bool EDGE>
   __device__ __forceinline__ void tile16(const v4i (&acc)[MI][NI], int row0, int col0, int row_min, int col_min, int lane,
                                          LDS_AS int8_t *lds) const {
-    constexpr int OE = 2, W = NI * 16, PITCH = W * OE, RC = PITCH / 16;
-    const int g = lane >> 4, c = lane & 15;
-    float s[NI], b[NI];
+    constexpr int W = NI * 16, LPR = W / 8, RPI = 64 / LPR, IT = 16 / RPI;
+    const int g = lane >> 4, c = lane & 15, j8 = 8 * (lane % LPR), lr = lane / LPR, col = col0 + j8;
+    float s[8], b[8];
 #pragma unroll
-    for (int ni = 0; ni < NI; ++ni) {
-      const int j = col0 + ni * 16 + c;
-      s[ni] = this->meta[j];
-      b[ni] = j < this->N ? this->meta[this->Np + j] : -__builtin_inff();   // no class: p = 0
+    for (int e = 0; e < 8; ++e) {
+      s[e] = this->meta[col + e];
+      b[e] = col + e < this->N ? this->meta[this->Np + col + e] : -__builtin_inff();   // no class: p = 0
     }
-    auto swz = [](int row) { return (((row >> 2) & 3) * OE) & (RC - 1); };
-    int wb[NI];
+    Row next[IT];
 #pragma unroll
-    for (int ni = 0; ni < NI; ++ni) wb[ni] = 4 * g * PITCH + (((ni * OE + (c * OE >> 4)) ^ swz(4 * g)) << 4) + (c * OE & 15);
-    Row next[4];
+    for (int it = 0; it < IT; ++it) next[it] = row_at(row0 + it * RPI + lr);
+#pragma unroll 1
+    for (int mi = 0; mi < MI; ++mi) {
+      Row now[IT];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) next[e] = row_at(row0 + 4 * g + e);
-    each([&](auto strip) __attribute__((always_inline)) {
-      constexpr int mi = decltype(strip)::value;
-      Row r[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        r[e] = next[e];
-        if constexpr (mi + 1 < MI) next[e] = row_at(row0 + (mi + 1) * 16 + 4 * g + e);
+      for (int it = 0; it < IT; ++it) {
+        now[it] = next[it];
+        next[it] = row_at(row0 + min(mi + 1, MI - 1) * 16 + it * RPI + lr);
       }
-      float v[NI][4];
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int ni = 0; ni < NI; ++ni)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[ni][e] = term(acc[mi][ni][e], r[e], s[ni], b[ni]);
-      bool some = false;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) some |= (unsigned)(r[e].target - col0) < (unsigned)W;
-      if (__ballot(some)) {
+      // chunk k of strip row r at k ^ (4 (r / 4 % 4)): an instruction's writes fall on distinct banks
+      each([&](auto strip) __attribute__((always_inline)) {
+        constexpr int i = decltype(strip)::value;
+        if (mi != i) return;
 #pragma unroll
         for (int ni = 0; ni < NI; ++ni)
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            if (r[e].target == col0 + ni * 16 + c) v[ni][e] = target_term(acc[mi][ni][e], r[e], s[ni], b[ni]);
+            *(LDS_AS int32_t *)(lds + (4 * g + e) * (W * 4) + ((((ni ^ g) << 2) + (c >> 2)) << 4) + (c & 3) * 4) = acc[i][ni][e];
+      }, std::make_integer_sequence<int, MI>());
+#pragma unroll
+      for (int it = 0; it < IT; ++it) {
+        const int r = it * RPI + lr, row = row0 + mi * 16 + r, swz = ((r >> 2) & 3) << 2;
+        const LDS_AS int8_t *at = lds + r * (W * 4);
+        const v4i x = *(const LDS_AS v4i *)(at + (((j8 >> 2) ^ swz) << 4)), y = *(const LDS_AS v4i *)(at + ((((j8 >> 2) + 1) ^ swz) << 4));
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = term(e < 4 ? x[e & 3] : y[e & 3], now[it], s[e], b[e]);
+        const int rel = now[it].target - col;
+        if (__ballot((unsigned)rel < 8u)) {
+#pragma unroll 1
+          for (int e = 0; e < 8; ++e) {
+            int32_t sum = 0;
+            float se = 0.0f, be = 0.0f;
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+              if (k == e) {
+                sum = k < 4 ? x[k & 3] : y[k & 3];
+                se = s[k];
+                be = b[k];
+              }
+            const float w = target_term(sum, now[it], se, be);
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+              if (k == e && rel == e) v[k] = w;
+          }
+        }
+        if (EDGE && (row < row_min || col < col_min)) continue;
+        const int64_t to = (int64_t)row * this->Np + col;
+        this->store8(to, v, VT_TYPE_F16);
+        if constexpr (LOW) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] -= (float)(_Float16)v[e];
+          this->store8(to + this->lo, v, VT_TYPE_F16);
+        }
+        if (col == 0) put_norm(row, now[it]);
       }
-      auto flush = [&](int64_t plane) {
-#pragma unroll
-        for (int ni = 0; ni < NI; ++ni) this->template put4<PITCH>(lds + wb[ni], v[ni][0], v[ni][1], v[ni][2], v[ni][3]);
-        this->template store_rows<W>(lds, swz, row0 + mi * 16, col0, plane, lane, EDGE ? row_min : 0, col_min);
-      };
-      flush(0);
-      if constexpr (LOW) {
-#pragma unroll
-        for (int ni = 0; ni < NI; ++ni)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) v[ni][e] -= (float)(_Float16)v[ni][e];
-        flush(this->lo);
-      }
-      __builtin_amdgcn_sched_barrier(0);
-    }, std::make_integer_sequence<int, MI>());
+    }
   }
 
   template <int MI, int NI>
@@ -309,6 +336,7 @@ struct LossTermsTile : ScaledTile<kGradTerms, 2, LOW> {
         for (int ni = 0; ni < NI; ++ni) v[ni][e] = term(acc[mi][ni][e], r, s[ni], b[ni]);
         some |= (unsigned)(r.target - col0) < 64u;
       }
+      if (col0 == 0 && lane < 32 && first + lane < M) put_norm(first + lane, row_at(first + lane));
       if (__ballot(some)) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
@@ -463,25 +491,6 @@ __global__ __launch_bounds__(1024) void loss_sum_kernel(LossSumArgs p) {
   *p.count = (float)n;
 }
 
-// The rows' normalisers over the gradient that reaches their losses: what the
-// gradient product divides by.
-struct LossScaleArgs {
-  const RowState *state;
-  const float *dloss, *count;   // count null: not a mean
-  float *norm;
-  int64_t step;                 // of dloss: 1 for one a row, 0 for one in all
-  int M;
-};
-
-__global__ __launch_bounds__(256) void loss_scale_kernel(LossScaleArgs p) {
-  const int row = blockIdx.x * 256 + threadIdx.x;
-  if (row >= p.M) return;
-  const RowState s = p.state[row];
-  float g = p.dloss[row * p.step];
-  if (p.count) g /= *p.count;
-  p.norm[row] = s.target == kIgnored ? __builtin_inff() : s.norm / g;
-}
-
 // ---------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------
@@ -546,7 +555,6 @@ int loss_rows(const LossCall &l, bool logits, void *stream) {
 int loss_grad_rows(const ScaledCall &c, const RowState *state, const float *dloss, int64_t step, const float *count, void *stream) {
   Scratch scr;
   if (int rc = open_scratch(stream, &scr)) return rc;
-  hipStream_t s = (hipStream_t)stream;
   const int64_t Kp = scaled_kp(c.K), Np = scaled_np(c.N, false);
   const bool split = two_halves(c.y_type);
   const int64_t lo = split ? c.M * Np : 0;
@@ -556,9 +564,6 @@ int loss_grad_rows(const ScaledCall &c, const RowState *state, const float *dlos
   float *norm = (float *)((int8_t *)w + t_bytes);
   Rows rows;
   if (int rc = take_rows(c.X, c.x_type, c.ldx, c.T, c.M, c.K, scr, &rows)) return rc;
-  const LossScaleArgs a = {state, dloss, count, norm, step, (int)c.M};
-  hipLaunchKernelGGL(loss_scale_kernel, dim3((unsigned)((c.M + 255) / 256)), dim3(256), 0, s, a);
-  VT_HIP_CHECK(hipGetLastError());
   ScaledOut f = {};
   f.t = rows.t; f.meta = c.meta; f.Y = w;
   f.lo = lo;
@@ -567,6 +572,10 @@ int loss_grad_rows(const ScaledCall &c, const RowState *state, const float *dlos
   auto terms = [&](auto out) {
     (ScaledOut &)out = f;
     out.state = state;
+    out.dloss = dloss;
+    out.count = count;
+    out.step = step;
+    out.norm_out = norm;
     return launch_tiles(plan, rows, c.Bp, Kp, out, scr);
   };
   if (int rc = split ? terms(LossTermsTile<true>()) : terms(LossTermsTile<false>())) return rc;

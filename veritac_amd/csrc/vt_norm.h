@@ -350,7 +350,7 @@ __global__ __launch_bounds__(256) void norm_apply_kernel(NormGradArgs p) {
 }
 
 // The sums of `groups` rows of K partial sums, in one order: 64 columns a
-// workgroup, its four waves every fourth row, 8 loads in flight.
+// workgroup, its 16 waves every 16th row, 8 loads in flight.
 struct GainSumArgs {
   const float *part;
   void *out;
@@ -358,16 +358,16 @@ struct GainSumArgs {
   int groups, type;
 };
 
-__global__ __launch_bounds__(256) void gain_sum_kernel(GainSumArgs p) {
-  __shared__ float red[4][64];
+__global__ __launch_bounds__(1024) void gain_sum_kernel(GainSumArgs p) {
+  __shared__ float red[16][64];
   const int c = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t col = (int64_t)blockIdx.x * 64 + c;
   float s = 0.0f;
   if (col < p.K) {
-    for (int i = wave; i < p.groups; i += 32) {
+    for (int i = wave; i < p.groups; i += 128) {
       float v[8];
 #pragma unroll
-      for (int u = 0; u < 8; ++u) v[u] = i + 4 * u < p.groups ? p.part[(int64_t)(i + 4 * u) * p.K + col] : 0.0f;
+      for (int u = 0; u < 8; ++u) v[u] = i + 16 * u < p.groups ? p.part[(int64_t)(i + 16 * u) * p.K + col] : 0.0f;
 #pragma unroll
       for (int u = 0; u < 8; ++u) s += v[u];
     }
@@ -375,7 +375,8 @@ __global__ __launch_bounds__(256) void gain_sum_kernel(GainSumArgs p) {
   red[wave][c] = s;
   __syncthreads();
   if (wave || col >= p.K) return;
-  s = (red[0][c] + red[1][c]) + (red[2][c] + red[3][c]);
+#pragma unroll
+  for (int i = 1; i < 16; ++i) s += red[i][c];
   if (p.type == VT_TYPE_F32) ((float *)p.out)[col] = s;
   else ((uint16_t *)p.out)[col] = (uint16_t)pack16(s, 0.0f, p.type);
 }
@@ -472,7 +473,7 @@ int launch_norm_grad(NormGradArgs a, void *dgain, int gain_type, Scratch &scr) {
   VT_HIP_CHECK(hipGetLastError());
   if (!dgain) return VT_OK;
   const GainSumArgs g = {a.part, dgain, a.K, (int)groups, gain_type};
-  hipLaunchKernelGGL(gain_sum_kernel, dim3((unsigned)((a.K + 63) / 64)), dim3(256), 0, s, g);
+  hipLaunchKernelGGL(gain_sum_kernel, dim3((unsigned)((a.K + 63) / 64)), dim3(1024), 0, s, g);
   VT_HIP_CHECK(hipGetLastError());
   return VT_OK;
 }

@@ -1085,10 +1085,35 @@ __device__ __forceinline__ void skinny_rows(const ScaledSkinnyArgs &p, const O &
       if (p.ws && wl == 0 && tid < M) p.t[tid] = row_scale(tops[tid]).scale;
     }
   };
+  // What an output of its own adds to this thread's elements, its loads behind the
+  // first weights'.
+  constexpr bool AHEAD = !std::is_same<O, ScaledOut>::value;
+  constexpr int EPT = (NBW * 256 + 511) / 512;   // elements of a row block
+  float more[MB][EPT];
+  auto look_ahead = [&]() {
+    if constexpr (AHEAD) {
+      if ((MB == 1 && p.fin) || p.ws) return;
+      __builtin_amdgcn_sched_barrier(0);
+      int row[MB * EPT], col[MB * EPT];
+      float d[MB * EPT];
+#pragma unroll
+      for (int i = 0; i < MB * EPT; ++i) {
+        const int t = tid + 512 * (i % EPT), n = t >> 8, c = t & 15;
+        row[i] = (i / EPT) * 16 + ((t >> 4) & 15);
+        col[i] = (nb0 + n) * 16 + c;
+        if (t >= NBW * 256 || row[i] >= M || col[i] >= o.N || c < col_lo(n) || c >= col_hi(n)) row[i] = -1;
+      }
+      o.ahead(row, col, d);
+#pragma unroll
+      for (int i = 0; i < MB * EPT; ++i) more[i / EPT][i % EPT] = d[i];
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
   if (steps >= S) {
 #pragma unroll
     for (int s = 0; s < S; ++s) load_b(s, b[s]);
     if constexpr (XB > 0) __builtin_amdgcn_sched_barrier(0);
+    look_ahead();
     round_rows();
 #pragma unroll
     for (int s = 0; s < S; ++s) load_a(s, a[s]);
@@ -1113,6 +1138,7 @@ __device__ __forceinline__ void skinny_rows(const ScaledSkinnyArgs &p, const O &
     for (int s = 0; s < S; ++s)
       if (s < steps) load_b(s, b[s]);
     if constexpr (XB > 0) __builtin_amdgcn_sched_barrier(0);
+    look_ahead();
     round_rows();
 #pragma unroll
     for (int s = 0; s < S; ++s)
@@ -1174,14 +1200,18 @@ __device__ __forceinline__ void skinny_rows(const ScaledSkinnyArgs &p, const O &
 #pragma unroll
     for (int n = 0; n < NT; ++n) red[(wave * NT + n) * 64 + lane] = acc[mb][n];
     __syncthreads();
-    for (int t = tid; t < NBW * 256; t += 512) {
+#pragma unroll
+    for (int i = 0; i < EPT; ++i) {
+      const int t = tid + 512 * i;
+      if (t >= NBW * 256) break;
       const int n = t >> 8, r16 = (t >> 4) & 15, c = t & 15;
       const int src = (r16 >> 2) * 16 + c, e = r16 & 3, row = mb * 16 + r16;
       if (row >= M || c < col_lo(n) || c >= col_hi(n)) continue;
       const int32_t s0 = sum(n, src, e), s1 = P == 1 ? 0 : sum(n + NBW, src, e);
       const int col = (nb0 + n) * 16 + c;
       if (!p.ws) {
-        finish(s0, s1, row, col, row_t(row));
+        if constexpr (AHEAD) o.element_with(s0, row, col, col, row_t(row), more[mb][i]);
+        else finish(s0, s1, row, col, row_t(row));
       } else {
         int32_t *ws = p.ws + ((int64_t)split * M + row) * o.Np;
         ws[P == 1 ? col : pair_col(col, 0)] = s0;

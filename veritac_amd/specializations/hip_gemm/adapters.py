@@ -82,23 +82,28 @@ def _pair(down, up):
     return down, up
 
 
-def _layout(down, up, back):
-    """One direction's layouts of checked adapters."""
+def _layout(down, up, forward, back):
+    """The layouts of checked adapters that each direction reads, or None."""
     torch = _torch()
     (count, rank, k), n = down.shape, up.shape[1]
     kind = _types()[down.dtype]
     down, up = down.contiguous(), up.contiguous()
-    data = torch.empty(_lib.adapter_size(k, n, rank, count, kind), dtype=torch.uint8, device=down.device)
+    size = _lib.adapter_size(k, n, rank, count, kind)
+    f, b = (torch.empty(size, dtype=torch.uint8, device=down.device) if w else None for w in (forward, back))
     with _on(down.device):
         _lib.check(_lib.load_library().vt_adapter_pack(
-            down.data_ptr(), up.data_ptr(), kind, k, n, rank, count, int(back), data.data_ptr(),
-            _current_stream(down.device)), "vt_adapter_pack")
-    return data
+            down.data_ptr(), up.data_ptr(), kind, k, n, rank, count, _ptr(f), _ptr(b), _current_stream(down.device)),
+            "vt_adapter_pack")
+    return f, b
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
 
 
 def _pack(down, up, scaling):
     down, up = _pair(down.detach(), up.detach())
-    return Adapters(_layout(down, up, False), down.dtype, down.shape[0], down.shape[1], down.shape[2], up.shape[1], scaling)
+    return Adapters(_layout(down, up, True, False)[0], down.dtype, down.shape[0], down.shape[1], down.shape[2], up.shape[1], scaling)
 
 
 def pack_adapters(down, up, *, scaling=1.0, stream=None):
@@ -216,26 +221,18 @@ def _adapted_grad(dy, x, W, down, up, scaling, which, u, wanted):
         raise HipGemmError("dy has %d columns, the adapters give %d and the weights %d" % (d.shape[1], n, W.n))
     w = _which(which, lead, device)
     kind = _types()[dy.dtype]
-    lib = _lib.load_library()
     with _on(device):
-        if wanted[2] and u is None:
-            # u as the forward pass makes it, and no output
-            u = _u(m, rank, device)
-            A = _layout(down, up, False)
-            _lib.check(lib.vt_adapted_linear(
-                x2.data_ptr(), kind, _pitch(x2), None, m, k, W.data.data_ptr(), W.meta.data_ptr(), n, A.data_ptr(),
-                rank, count, scaling, None if w is None else w.data_ptr(), u.data_ptr(), None, kind, max(n, 1),
-                _current_stream(device)), "vt_adapted_linear")
-        A = _layout(down, up, True)
+        again = wanted[2] and u is None     # u as the forward pass makes it
+        forward, back = _layout(down, up, again, True)
+        u = _u(m, rank, device) if again else u
         h = _u(m, rank, device)
         dx = torch.empty((*lead, k), dtype=dy.dtype, device=device) if wanted[0] else None
         dd = torch.empty(shapes[0], dtype=dy.dtype, device=device) if wanted[1] else None
         du = torch.empty(shapes[1], dtype=dy.dtype, device=device) if wanted[2] else None
-        ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
-        _lib.check(lib.vt_adapted_grad(
-            d.data_ptr(), kind, _pitch(d), ptr(x2), 0 if x2 is None else _pitch(x2), m, k, W.data.data_ptr(),
-            W.meta.data_ptr(), n, A.data_ptr(), rank, count, scaling, ptr(w), ptr(u), h.data_ptr(), ptr(dx), max(k, 1),
-            ptr(dd), ptr(du), _current_stream(device)), "vt_adapted_grad")
+        _lib.check(_lib.load_library().vt_adapted_grad(
+            d.data_ptr(), kind, _pitch(d), _ptr(x2), 0 if x2 is None else _pitch(x2), m, k, W.data.data_ptr(),
+            W.meta.data_ptr(), n, _ptr(forward), back.data_ptr(), rank, count, scaling, _ptr(w), _ptr(u), h.data_ptr(),
+            _ptr(dx), max(k, 1), _ptr(dd), _ptr(du), _current_stream(device)), "vt_adapted_grad")
     return dx, dd, du
 
 

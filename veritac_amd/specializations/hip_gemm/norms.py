@@ -47,6 +47,9 @@ def _like(name, t, x, lead):
 
 def _matrix(name, given, like, lead, k):
     """(matrix to write, tensor to return) of an output of the rows' type."""
+    if given is None and len(lead) == 1:
+        o2 = like.new_empty((like.shape[0], k))
+        return o2, o2
     o2, ret, _ = scaled._output(name, given, like.shape[0], k, lead, like.dtype, like.device, like)
     return (o2 if o2.dim() == 2 else o2.reshape(like.shape[0], k)), ret
 
@@ -65,9 +68,9 @@ def _forward(x, gain, residual, eps, rows, out, h_out):
         h2, h = _matrix("h", h_out, x2, lead, k)
     if rows:
         pitch = _lib.quant_pitch(k)
-        y2 = torch.empty((m, pitch), dtype=torch.int8, device=x2.device)
-        scale = torch.empty(m, dtype=torch.float32, device=x2.device)
-        y = scaled.QuantRows(y2, scale, k=k, padded=True, shape=tuple(lead) + (k,))
+        y2 = x2.new_empty((m, pitch), dtype=torch.int8)
+        scale = x2.new_empty(m, dtype=torch.float32)
+        y = scaled.QuantRows._made(y2, scale, k, (*lead, k))
     else:
         scale = None
         y2, y = _matrix("output", out, x2, lead, k)
@@ -92,6 +95,8 @@ def norm(x, gain, *, residual=None, eps=1e-6, out=None, h_out=None, stream=None)
             raise HipGemmError("a differentiable call takes neither out, h_out nor stream")
         y, h = _function().apply(x, gain, residual, eps)
         return y if residual is None else (y, h)
+    if stream is None:
+        return _forward(x, gain, residual, eps, False, out, h_out)
     given = (() if out is None else (out,)) + (() if h_out is None else (h_out,))
     return scaled._enqueued(x, stream, lambda: _forward(x, gain, residual, eps, False, out, h_out), held=given)
 
@@ -101,6 +106,8 @@ def norm_rows(x, gain, *, residual=None, eps=1e-6, h_out=None, stream=None):
     (rows, h). Not differentiable: train through norm."""
     for t in (x, gain, residual):
         scaled._constant("norm_rows", t, "train through norm, whose rows linear and gated round for themselves")
+    if stream is None:
+        return _forward(x, gain, residual, eps, True, None, h_out)
     given = () if h_out is None else (h_out,)
     return scaled._enqueued(x, stream, lambda: _forward(x, gain, residual, eps, True, None, h_out), held=given)
 

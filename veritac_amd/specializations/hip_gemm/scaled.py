@@ -87,6 +87,13 @@ class QuantRows:
             raise HipGemmError("shape must be [..., %d] of %d rows (got %s)" % (k, m, shape))
         self.data, self.scale, self.k, self.padded, self.shape = data, scale, k, padded, shape
 
+    @classmethod
+    def _made(cls, data, scale, k, shape):
+        """Padded rows that the library has just written, without the checks."""
+        rows = object.__new__(cls)
+        rows.data, rows.scale, rows.k, rows.padded, rows.shape = data, scale, k, True, shape
+        return rows
+
     @property
     def device(self):
         return self.data.device
@@ -97,13 +104,15 @@ class QuantRows:
         dtype = torch.float32 if dtype is None else dtype
         if dtype not in _types():
             raise HipGemmError("dtype must be float32, float16 or bfloat16 (got %s)" % (dtype,))
-        if self.data.device.type != "cuda":
-            return (self.data[:, :self.k].float() * self.scale[:, None]).reshape(self.shape).to(dtype)
-        y = torch.empty(self.shape, dtype=dtype, device=self.device)
-        with _on(self.device):
+        data, k = self.data, self.k
+        device = data.device
+        if device.type != "cuda":
+            return (data[:, :k].float() * self.scale[:, None]).reshape(self.shape).to(dtype)
+        y = data.new_empty(self.shape, dtype=dtype)
+        with _on(device):
             _lib.check(_lib.load_library().vt_dequant_rows(
-                self.data.data_ptr(), _pitch(self.data), self.scale.data_ptr(), y.data_ptr(), _types()[dtype],
-                max(self.k, 1), self.data.shape[0], self.k, _current_stream(self.device)), "vt_dequant_rows")
+                data.data_ptr(), _pitch(data), self.scale.data_ptr(), y.data_ptr(), _types()[dtype], max(k, 1),
+                data.shape[0], k, _current_stream(device)), "vt_dequant_rows")
         return y
 
     def __repr__(self):
@@ -313,7 +322,7 @@ def _quantize(x):
     lib = _lib.load_library()
     _lib.check(lib.vt_quant_rows(x2.data_ptr(), _types()[x.dtype], _pitch(x2), data.data_ptr(), pitch,
                                  scale.data_ptr(), m, k, _current_stream(x.device)), "vt_quant_rows")
-    return QuantRows(data, scale, k=k, padded=True, shape=tuple(lead) + (k,))
+    return QuantRows._made(data, scale, k, tuple(lead) + (k,))
 
 
 def _check_weight(W, pair, device, k):
