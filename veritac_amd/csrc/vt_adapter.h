@@ -11,19 +11,26 @@
 // u and h are float32 [M][Rp] and come from a kernel of their own; the second
 // product is added where the int8 product's (or the gradient's) sums lie in
 // registers, so y and dx are rounded and written once. Adapters are laid out
-// with the rank padded to Rp (whole 16s) and the long side to that of the packed
-// weights, zeros in between, once with the contraction's index innermost for each
-// product that reads them.
+// with the rank padded to Rp and the long side to that of the packed weights, zeros
+// in between, once for each product that reads them, as that product's fragments:
+// a wave's load of one is contiguous.
 
 namespace {
 
 typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 
 constexpr int kMaxRank = 128, kMaxAdapters = 65535;   // adapters: a side of a grid
-constexpr int64_t rank_pad(int64_t R) { return (R + 15) / 16 * 16; }
+// 16 ranks, or whole 32s: the depth of a 16-bit matrix instruction, half of it for
+// the second half of u where the rank is small.
+constexpr int64_t rank_pad(int64_t R) { return R <= 16 ? 16 : (R + 31) / 32 * 32; }
 
-// One pair of an adapter's layouts: [L][Rp][Kp] for x . A^T and [L][Np][Rp] for
-// u . B^T forward, [L][Rp][Np] for dy . B and [L][Kp][Rp] for h . A backward.
+// One pair of an adapter's layouts, for x . A^T and u . B^T forward, dy . B and h . A
+// backward.
+//   first   [L][Rp / 16][len / 32] fragments of 16 ranks by 32 columns: 8 columns of
+//           rank r % 16 at ((column / 8 % 4) * 16 + r % 16) * 8
+//   second  [L][columns / 16][Rp / G] fragments of 16 columns by G ranks (G = 32, or 16
+//           where Rp is, or in float32): E ranks (8, in float32 4) of column c % 16 at
+//           ((rank / E % (G / E)) * 16 + c % 16) * E
 struct AdapterLayout {
   int64_t Kp, Np, Rp, L;
   int64_t first(bool back) const { return L * Rp * (back ? Np : Kp); }
@@ -58,16 +65,27 @@ __global__ __launch_bounds__(256) void adapter_pack_kernel(AdapterPackArgs p) {
     tile[j][r] = v;
   }
   __syncthreads();
+  constexpr int E = sizeof(T) == 4 ? 4 : 8;
+  const int G = sizeof(T) == 4 || p.Rp == 16 ? 16 : 32;
 #pragma unroll
   for (int back = 0; back < 2; ++back) {
-    // forward, down keeps its order and up too; backward both turn
-    const bool rank_inner = up != (back != 0);
-    uint8_t *to = rank_inner ? p.second[back] : p.first[back];
+    // forward, down is first and up second; backward the other way
+    const bool second = up != (back != 0);
+    uint8_t *to = second ? p.second[back] : p.first[back];
     if (!to) continue;
     T *dst = (T *)to + (int64_t)a * p.Rp * lenp;
     for (int i = threadIdx.x; i < 64 * p.Rp; i += 256) {
-      if (rank_inner) dst[(int64_t)(j0 + i / p.Rp) * p.Rp + i % p.Rp] = tile[i / p.Rp][i % p.Rp];
-      else dst[(int64_t)(i >> 6) * lenp + j0 + (i & 63)] = tile[i & 63][i >> 6];
+      if (second) {
+        // 4 blocks of 16 columns, contiguous
+        const int nb = i / (16 * p.Rp), w = i % (16 * p.Rp), f = w % (16 * G);
+        const int r = w / (16 * G) * G + f / (16 * E) * E + f % E, c = f / E % 16;
+        dst[(int64_t)j0 * p.Rp + i] = tile[nb * 16 + c][r];
+      } else {
+        // 2 fragments of 32 columns for each 16 ranks
+        const int rb = i / 1024, w = i % 1024, f = w % 512;
+        const int r = rb * 16 + f / 8 % 16, j = w / 512 * 32 + f / 128 * 8 + f % 8;
+        dst[((int64_t)rb * (lenp / 32) + j0 / 32) * 512 + w] = tile[j][r];
+      }
     }
   }
 }
@@ -94,88 +112,8 @@ struct ShrinkPair {
   ShrinkArgs of[2];
 };
 
-// 8 elements of a row from `pos` as floats, zero past `len`; int8 rows too.
-template <int TYPE, bool I8>
-__device__ __forceinline__ void load_row8(const void *row, int pos, int len, float (&v)[8]) {
-  if constexpr (I8) {
-    const int8_t *q = (const int8_t *)row;
-    typedef int8_t V8 __attribute__((ext_vector_type(8), aligned(1)));
-    if (pos + 8 <= len) {
-      const V8 b = *(const V8 *)(q + pos);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = (float)b[e];
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = pos + e < len ? (float)q[pos + e] : 0.0f;
-    }
-  } else {
-    load8<TYPE>((const typename Elem<TYPE>::T *)row, pos, len, v);
-  }
-}
-
-// What a row's sums are multiplied by: a NaN for an adapter that is not there.
-template <bool I8>
-__device__ __forceinline__ float shrink_factor(const ShrinkArgs &p, int row, int a) {
-  if (a >= p.L) return __uint_as_float(0x7fc00000u);
-  return I8 ? p.scale * p.t[row] : p.scale;
-}
-
-// Up to 64 rows, each with an adapter of its own maybe: 16 ranks of a row to a
-// workgroup, a wave for each, 8 columns a lane. The first of a row's workgroups
-// rounds it too, where the int8 product needs that done: the row is in its cache,
-// and a launch less. Bound by the latency of its few loads and, with many
-// adapters, by reading them.
-template <int TYPE, bool I8>
-__global__ __launch_bounds__(1024) void shrink_rows_kernel(ShrinkPair pair) {
-  __shared__ uint32_t red[16];
-  const ShrinkArgs &p = pair.of[blockIdx.z];
-  typedef typename Elem<TYPE>::T T;
-  const int row = blockIdx.x, rank = blockIdx.y * 16 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-  const int a = p.which ? p.which[row] : 0;
-  const void *x = I8 ? (const void *)((const int8_t *)p.X + row * p.ldx) : (const void *)((const T *)p.X + row * p.ldx);
-  float s = 0.0f;
-  if (a >= 0 && a < p.L) {
-    const T *w = (const T *)p.P + ((int64_t)a * p.Rp + rank) * p.lenp;
-#pragma unroll 8
-    for (int pos = lane * 8; pos < p.lenp; pos += 512) {
-      float v[8], b[8];
-      load_row8<TYPE, I8>(x, pos, p.len, v);
-      load8<TYPE>(w, pos, p.lenp, b);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) s = fmaf(v[e], b[e], s);
-    }
-#pragma unroll
-    for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o);
-  }
-  if (lane == 0) p.U[(int64_t)row * p.Rp + rank] = a < 0 ? 0.0f : s * shrink_factor<I8>(p, row, a);
-  if constexpr (!I8) {
-    if (!p.Q || blockIdx.y) return;
-    uint32_t top = 0;
-    for (int pos = threadIdx.x * 8; pos < p.len; pos += 8192) {
-      float v[8];
-      load8<TYPE>((const T *)x, pos, p.len, v);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) top = max(top, magnitude(v[e]));
-    }
-    top = block_max<1024>(top, red);
-    const RowScale r = row_scale(top);
-    if (threadIdx.x == 0) p.T[row] = r.scale;
-    for (int pos = threadIdx.x * 8; pos < p.lenp; pos += 8192) {
-      float v[8];
-      uint32_t b[8];
-      load8<TYPE>((const T *)x, pos, p.len, v);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) b[e] = round_byte(v[e], r.inv);
-      v2i o = {pack_bytes(b[0], b[1], b[2], b[3]), pack_bytes(b[4], b[5], b[6], b[7])};
-      if (r.inv == 0.0f) o = v2i{0, 0};
-      *(v2i *)(p.Q + (int64_t)row * p.lenp + pos) = o;
-    }
-  }
-}
-
-// A 16 x 32 by 32 x 16 product (16 x 16 x 16 steps of 4 in float32) of fragments
-// of 8 values a lane: row or column lane % 16, k 8 (lane / 16) + e. In float32 the
-// order of k within the 32 is another, the same on both sides.
+// A 16 x 32 by 32 x 16 product of fragments of 8 values a lane: row or column lane %
+// 16, k 8 (lane / 16) + e (in float32 eight products of depth 4).
 template <int TYPE>
 struct Frag;
 template <>
@@ -224,6 +162,118 @@ __device__ __forceinline__ v4f mfma16(const Frag<TYPE> &a, const Frag<TYPE> &b, 
     return c;
   }
 }
+// 8 elements of a row from `pos`, zero past `len`; int8 rows too.
+template <int TYPE, bool I8>
+struct RowPiece {
+  typename std::conditional<I8, v2i, Raw8<TYPE>>::type w;
+  __device__ __forceinline__ void load(const void *row, int pos, int len) {
+    if constexpr (I8) {
+      typedef v2i V __attribute__((aligned(1)));
+      const uint8_t *q = (const uint8_t *)row;
+      if (pos + 8 <= len) {
+        w = *(const V *)(q + pos);
+      } else {
+        w = v2i{0, 0};
+#pragma unroll
+        for (int e = 0; e < 7; ++e)
+          if (pos + e < len) w[e >> 2] |= (int)((uint32_t)q[pos + e] << (8 * (e & 3)));
+      }
+    } else {
+      w = raw8<TYPE>((const typename Elem<TYPE>::T *)row, pos, len);
+    }
+  }
+  __device__ __forceinline__ float value(int e) const {
+    if constexpr (I8) return (float)(int8_t)((uint32_t)w[e >> 2] >> (8 * (e & 3)));
+    else return raw_value<TYPE>(w, e);
+  }
+  __device__ __forceinline__ Frag<TYPE> frag() const {
+    Frag<TYPE> f;
+    if constexpr (!I8 && TYPE != kF32) {
+      f.v = __builtin_bit_cast(decltype(f.v), w.w);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f.v[e] = (typename Elem<TYPE>::T)value(e);
+    }
+    return f;
+  }
+};
+
+// What a row's sums are multiplied by: a NaN for an adapter that is not there.
+template <bool I8>
+__device__ __forceinline__ float shrink_factor(const ShrinkArgs &p, int row, int a) {
+  if (a >= p.L) return __uint_as_float(0x7fc00000u);
+  return I8 ? p.scale * p.t[row] : p.scale;
+}
+
+// Up to 64 rows, each with an adapter of its own maybe: 16 ranks of a row to a
+// workgroup, whose 16 waves take 32 columns in turn (a fragment, 8 columns of a
+// rank a lane) and join through LDS. The first of a row's workgroups rounds it too,
+// where the int8 product needs that done: the row is in its cache, and a launch
+// less. Bound by the latency of its few loads and, with many adapters, by reading
+// them.
+template <int TYPE, bool I8>
+__global__ __launch_bounds__(1024) void shrink_rows_kernel(ShrinkPair pair) {
+  __shared__ uint32_t tops[16];
+  __shared__ float red[16][16];
+  const ShrinkArgs &p = pair.of[blockIdx.z];
+  typedef typename Elem<TYPE>::T T;
+  constexpr int U = TYPE == kF32 ? 4 : 8;
+  const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4;
+  const int a = p.which ? p.which[row] : 0;
+  const void *x = I8 ? (const void *)((const int8_t *)p.X + row * p.ldx) : (const void *)((const T *)p.X + row * p.ldx);
+  float s = 0.0f;
+  if (a >= 0 && a < p.L) {
+    const T *w = (const T *)p.P + ((int64_t)a * (p.Rp / 16) + blockIdx.y) * 16 * p.lenp + lane * 8;
+    for (int k0 = wave * 32; k0 < p.lenp; k0 += U * 512) {
+      RowPiece<TYPE, I8> v[U];
+      Frag<TYPE> b[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int k = k0 + u * 512;
+        b[u] = load_frag<TYPE>(w + (int64_t)min(k, p.lenp - 32) * 16);
+        v[u].load(x, k + 8 * g, p.len);   // zero past the row's end
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s = fmaf(v[u].value(e), (float)b[u].v[e], s);
+    }
+    s += __shfl_xor(s, 16);
+    s += __shfl_xor(s, 32);
+  }
+  if (lane < 16) red[wave][lane] = s;
+  __syncthreads();
+  if (tid < 16) {
+    s = 0.0f;
+#pragma unroll
+    for (int v = 0; v < 16; ++v) s += red[v][tid];
+    p.U[(int64_t)row * p.Rp + blockIdx.y * 16 + tid] = a < 0 ? 0.0f : s * shrink_factor<I8>(p, row, a);
+  }
+  if constexpr (!I8) {
+    if (!p.Q || blockIdx.y) return;
+    uint32_t top = 0;
+    for (int pos = tid * 8; pos < p.len; pos += 8192) {
+      float v[8];
+      load8<TYPE>((const T *)x, pos, p.len, v);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) top = max(top, magnitude(v[e]));
+    }
+    top = block_max<1024>(top, tops);
+    const RowScale r = row_scale(top);
+    if (tid == 0) p.T[row] = r.scale;
+    for (int pos = tid * 8; pos < p.lenp; pos += 8192) {
+      float v[8];
+      uint32_t b[8];
+      load8<TYPE>((const T *)x, pos, p.len, v);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) b[e] = round_byte(v[e], r.inv);
+      v2i o = {pack_bytes(b[0], b[1], b[2], b[3]), pack_bytes(b[4], b[5], b[6], b[7])};
+      if (r.inv == 0.0f) o = v2i{0, 0};
+      *(v2i *)(p.Q + (int64_t)row * p.lenp + pos) = o;
+    }
+  }
+}
+
 // The adapters of 16 rows, one after another: f(adapter, its rows as bits). a: that
 // of row lane % 16, negative for none. All rows are multiplied by each and only its
 // own are taken: a row is never touched by what another's adapter holds.
@@ -254,31 +304,27 @@ __global__ __launch_bounds__(1024) void shrink_tiles_kernel(ShrinkPair pair) {
   int a = p.which ? p.which[row] : 0;
   if (a >= p.L) a = -1;
   const void *x = I8 ? (const void *)((const int8_t *)p.X + row * p.ldx) : (const void *)((const T *)p.X + row * p.ldx);
-  const T *w = (const T *)p.P + (int64_t)(rank0 + c) * p.lenp + 8 * g;
+  const T *w = (const T *)p.P + (int64_t)rank0 * p.lenp + lane * 8;
   const int64_t step = (int64_t)p.Rp * p.lenp;
   v4f acc[NR];
 #pragma unroll
   for (int n = 0; n < NR; ++n) acc[n] = v4f{0, 0, 0, 0};
   for (int k0 = wave * U * 32; k0 < p.lenp; k0 += WAVES * U * 32) {
-    Frag<TYPE> xa[U];
+    RowPiece<TYPE, I8> xa[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      float v[8];
-      load_row8<TYPE, I8>(x, k0 + u * 32 + 8 * g, p.len, v);
-      xa[u] = to_frag<TYPE>(v);
-    }
+    for (int u = 0; u < U; ++u) xa[u].load(x, k0 + u * 32 + 8 * g, p.len);
     each_adapter(a, [&](int cur, uint32_t rows) {
       Frag<TYPE> b[NR][U];
 #pragma unroll
       for (int n = 0; n < NR; ++n)
 #pragma unroll
         for (int u = 0; u < U; ++u)
-          b[n][u] = load_frag<TYPE>(w + cur * step + (int64_t)n * 16 * p.lenp + min(k0 + u * 32, p.lenp - 32));
+          b[n][u] = load_frag<TYPE>(w + cur * step + ((int64_t)n * p.lenp + min(k0 + u * 32, p.lenp - 32)) * 16);
 #pragma unroll
       for (int n = 0; n < NR; ++n) {
         v4f part = {0, 0, 0, 0};
 #pragma unroll
-        for (int u = 0; u < U; ++u) part = mfma16<TYPE>(xa[u], b[n][u], part);
+        for (int u = 0; u < U; ++u) part = mfma16<TYPE>(xa[u].frag(), b[n][u], part);
 #pragma unroll
         for (int e = 0; e < 4; ++e)
           if (rows >> (4 * g + e) & 1) acc[n][e] += part[e];
@@ -320,16 +366,39 @@ __device__ __forceinline__ int adapter_of(const LowRank &l, int row) {
   return l.which ? min(l.which[row], l.L - 1) : 0;
 }
 
+// Where ranks r .. r + 7 of a column lie: 8 of them, or two fours.
+template <int TYPE>
+__device__ __forceinline__ const typename Elem<TYPE>::T *rank_at(const LowRank &l, int a, int64_t col, int r) {
+  typedef typename Elem<TYPE>::T T;
+  const T *v = (const T *)l.V + (a * l.colsp + (col & ~(int64_t)15)) * l.Rp + (TYPE == kF32 ? 4 : 8) * (col & 15);
+  return v + (TYPE == kF32 ? (r >> 4) * 256 + (r >> 2 & 3) * 64 : (r >> 5) * 512 + (r >> 3 & 3) * 128);
+}
+template <int TYPE>
+__device__ __forceinline__ Frag<TYPE> rank_frag(const typename Elem<TYPE>::T *p) {
+  Frag<TYPE> f;
+  if constexpr (TYPE == kF32) {
+    const v4f a = *(const v4f *)p, b = *(const v4f *)(p + 64);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      f.v[e] = a[e];
+      f.v[4 + e] = b[e];
+    }
+  } else {
+    f = load_frag<TYPE>(p);
+  }
+  return f;
+}
+
 // One element of it, 8 ranks at a time.
 template <int TYPE>
 __device__ __forceinline__ float low_rank_element(const LowRank &l, int row, int64_t col) {
   const int a = adapter_of(l, row);
   if (a < 0) return 0.0f;
   const float *u = l.U + (int64_t)row * l.Rp;
-  const typename Elem<TYPE>::T *v = (const typename Elem<TYPE>::T *)l.V + (a * l.colsp + col) * l.Rp;
   float s = 0.0f;
+#pragma unroll 2
   for (int r = 0; r < l.Rp; r += 8) {
-    const Frag<TYPE> b = load_frag<TYPE>(v + r);
+    const Frag<TYPE> b = rank_frag<TYPE>(rank_at<TYPE>(l, a, col, r));
     const v4f x = *(const v4f *)(u + r), y = *(const v4f *)(u + r + 4);
 #pragma unroll
     for (int e = 0; e < 4; ++e) s = fmaf(x[e], (float)b.v[e], s);
@@ -344,14 +413,14 @@ __device__ __forceinline__ float low_rank_element(const LowRank &l, int row, int
 template <int TYPE, int E>
 __device__ __forceinline__ void low_rank_elements(const LowRank &l, const int (&row)[E], const int (&col)[E], float (&s)[E]) {
   const float *u[E];
-  const typename Elem<TYPE>::T *v[E];
+  int at[E];
   bool in[E];
 #pragma unroll
   for (int i = 0; i < E; ++i) {
     const int a = row[i] < 0 ? -1 : adapter_of(l, row[i]);
     in[i] = a >= 0;
     u[i] = l.U + (int64_t)max(row[i], 0) * l.Rp;
-    v[i] = (const typename Elem<TYPE>::T *)l.V + (max(a, 0) * l.colsp + (row[i] < 0 ? 0 : col[i])) * l.Rp;
+    at[i] = max(a, 0);
     s[i] = 0.0f;
   }
   for (int r = 0; r < l.Rp; r += 8) {
@@ -359,7 +428,7 @@ __device__ __forceinline__ void low_rank_elements(const LowRank &l, const int (&
     v4f x[E], y[E];
 #pragma unroll
     for (int i = 0; i < E; ++i) {
-      b[i] = load_frag<TYPE>(v[i] + r);
+      b[i] = rank_frag<TYPE>(rank_at<TYPE>(l, at[i], row[i] < 0 ? 0 : col[i], r));
       x[i] = *(const v4f *)(u[i] + r);
       y[i] = *(const v4f *)(u[i] + r + 4);
     }
@@ -380,104 +449,150 @@ __device__ __forceinline__ float low_rank_element(const LowRank &l, int type, in
   return type == VT_TYPE_F16 ? low_rank_element<kF16>(l, row, col) : low_rank_element<kBF16>(l, row, col);
 }
 
+// t[i] += a . b[i] for four blocks beside each other, and with LO += lo . b[i]. In
+// inline assembly with the sums in VGPRs: the kernels that do this keep all of
+// their accumulators in AGPRs, where the compiler puts a builtin's too, and
+// would spill. Its operands may have been written by the instruction before (two
+// wait states), and its results are read by the instruction behind: an 8-pass
+// product's by 11 wait states, a 16-pass one's by 19.
+template <int TYPE, bool LO>
+__device__ __forceinline__ void four_products(v4f (&t)[4], const Frag<TYPE> &a, const Frag<TYPE> &lo, const Frag<TYPE> (&b)[4]) {
+#define VT_FOUR(op, A)                                                                            \
+  op " %0, %" A ", %6, %0\n\t" op " %1, %" A ", %7, %1\n\t" op " %2, %" A ", %8, %2\n\t" op " %3, %" A ", %9, %3\n\t"
+#define VT_ASM(text) \
+  asm volatile("s_nop 1\n\t" text "s_nop 15\n\ts_nop 7" \
+               : "+v"(t[0]), "+v"(t[1]), "+v"(t[2]), "+v"(t[3]) \
+               : "v"(a.v), "v"(lo.v), "v"(b[0].v), "v"(b[1].v), "v"(b[2].v), "v"(b[3].v))
+  if constexpr (TYPE == kF16) {
+    if constexpr (LO) VT_ASM(VT_FOUR("v_mfma_f32_16x16x32_f16", "4") VT_FOUR("v_mfma_f32_16x16x32_f16", "5"));
+    else VT_ASM(VT_FOUR("v_mfma_f32_16x16x32_f16", "4"));
+  } else if constexpr (TYPE == kBF16) {
+    if constexpr (LO) VT_ASM(VT_FOUR("v_mfma_f32_16x16x32_bf16", "4") VT_FOUR("v_mfma_f32_16x16x32_bf16", "5"));
+    else VT_ASM(VT_FOUR("v_mfma_f32_16x16x32_bf16", "4"));
+  }
+#undef VT_ASM
+#undef VT_FOUR
+}
+// The same in float32, of depth 4.
+__device__ __forceinline__ void four_products(v4f (&t)[4], float a, float b0, float b1, float b2, float b3) {
+  asm volatile("s_nop 1\n\t"
+               "v_mfma_f32_16x16x4_f32 %0, %4, %5, %0\n\tv_mfma_f32_16x16x4_f32 %1, %4, %6, %1\n\t"
+               "v_mfma_f32_16x16x4_f32 %2, %4, %7, %2\n\tv_mfma_f32_16x16x4_f32 %3, %4, %8, %3\n\ts_nop 15\n\ts_nop 7"
+               : "+v"(t[0]), "+v"(t[1]), "+v"(t[2]), "+v"(t[3])
+               : "v"(a), "v"(b0), "v"(b1), "v"(b2), "v"(b3));
+}
+
 // Blocks of 16 x 16 in the accumulators' layout: d[ni] element e is row row0 +
 // 4 (lane / 16) + e, column col0 + 16 ni + lane % 16. Columns below colsp, any rows;
 // a: adapter_of row row0 + lane % 16.
-// 16-bit adapters: 16 ranks are one 32-deep product, of u in two halves (16 bits
-// of it in bfloat16, 22 in float16; u is then as exact as the 16-bit y that it is
-// added to needs, 2^-8 of a step) against the same 16 values. float16 halves are of
-// u times a power of two for each row, so that none overflows or is lost.
-// All loads of 16 S ranks are under way together: there is one wave to a SIMD
-// here, and nothing else hides them.
+// 16-bit adapters: u enters in two halves (16 bits of it in bfloat16, 22 in
+// float16; it is then as exact as the 16-bit y that it is added to needs, 2^-8 of
+// a step), 32 ranks at a time, or 16 with both halves in one product. float16
+// halves are of u times a power of two for each row and 32 ranks, so that none
+// overflows or is lost. The loads of 64 ranks are under way together: there is one
+// wave to a SIMD here, and nothing else hides them.
 template <int TYPE, int NI>
 __device__ __forceinline__ void low_rank16(const LowRank &l, int a, int row0, int col0, int lane, v4f (&d)[NI]) {
+  static_assert(NI % 4 == 0, "four blocks at a time");
   typedef typename Elem<TYPE>::T T;
-  constexpr int S = NI <= 4 && TYPE != kF32 ? 4 : 2;
   const int g = lane >> 4, c = lane & 15, row = min(row0 + c, l.rows - 1);
-  const float *u = l.U + (int64_t)row * l.Rp + (TYPE == kF32 ? 4 * g : 8 * (g & 1));
+  const float *u = l.U + (int64_t)row * l.Rp;
 #pragma unroll
   for (int ni = 0; ni < NI; ++ni) d[ni] = v4f{0, 0, 0, 0};
   each_adapter(a, [&](int cur, uint32_t rows) {
-    const T *v = (const T *)l.V + (cur * l.colsp + col0 + c) * l.Rp + (TYPE == kF32 ? 4 * g : 8 * (g & 1));
-    v4f t[NI];
+    const T *v = (const T *)l.V + (cur * l.colsp + col0) * l.Rp;
+    auto add = [&](const v4f (&t)[4], int q, const v4f &un) {
 #pragma unroll
-    for (int ni = 0; ni < NI; ++ni) t[ni] = v4f{0, 0, 0, 0};
-    auto ranks = [&](auto count, int r) __attribute__((always_inline)) {
+      for (int e = 0; e < 4; ++e) {
+        const bool mine = rows >> (4 * g + e) & 1;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float x = TYPE == kF16 ? fmaf(t[i][e], un[e], d[4 * q + i][e]) : d[4 * q + i][e] + t[i][e];
+          d[4 * q + i][e] = mine ? x : d[4 * q + i][e];
+        }
+      }
+    };
+    // N groups of ranks from r
+    auto ranks = [&](auto count, auto small, int r) __attribute__((always_inline)) {
       constexpr int N = decltype(count)::value;
+      constexpr bool SMALL = decltype(small)::value;   // 16 ranks in all
       if constexpr (TYPE == kF32) {
         v4f x[N], b[N][NI];
 #pragma unroll
         for (int s = 0; s < N; ++s) {
-          x[s] = *(const v4f *)(u + r + 16 * s);
+          x[s] = *(const v4f *)(u + r + 16 * s + 4 * g);
 #pragma unroll
-          for (int ni = 0; ni < NI; ++ni) b[s][ni] = *(const v4f *)(v + (int64_t)ni * 16 * l.Rp + r + 16 * s);
+          for (int ni = 0; ni < NI; ++ni) b[s][ni] = *(const v4f *)(v + ni * 16 * l.Rp + (r + 16 * s) * 16 + lane * 4);
         }
 #pragma unroll
-        for (int s = 0; s < N; ++s)
+        for (int q = 0; q < NI / 4; ++q) {
+          v4f t[4] = {{0, 0, 0, 0}, {0, 0, 0, 0}, {0, 0, 0, 0}, {0, 0, 0, 0}};
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
+          for (int s = 0; s < N; ++s)
 #pragma unroll
-            for (int ni = 0; ni < NI; ++ni) t[ni] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[s][e], b[s][ni][e], t[ni], 0, 0, 0);
+            for (int e = 0; e < 4; ++e)
+              four_products(t, x[s][e], b[s][4 * q][e], b[s][4 * q + 1][e], b[s][4 * q + 2][e], b[s][4 * q + 3][e]);
+          add(t, q, v4f{1, 1, 1, 1});
+        }
       } else {
         v4f x[N][2];
         Frag<TYPE> b[N][NI];
 #pragma unroll
         for (int s = 0; s < N; ++s) {
-          x[s][0] = *(const v4f *)(u + r + 16 * s);
-          x[s][1] = *(const v4f *)(u + r + 16 * s + 4);
+          const float *at = u + r + 32 * s + 8 * (SMALL ? g & 1 : g);
+          x[s][0] = *(const v4f *)at;
+          x[s][1] = *(const v4f *)(at + 4);
 #pragma unroll
-          for (int ni = 0; ni < NI; ++ni) b[s][ni] = load_frag<TYPE>(v + (int64_t)ni * 16 * l.Rp + r + 16 * s);
+          for (int ni = 0; ni < NI; ++ni)
+            b[s][ni] = load_frag<TYPE>(v + ni * 16 * l.Rp + (r + 32 * s) * 16 + (SMALL ? lane & 31 : lane) * 8);
         }
 #pragma unroll
         for (int s = 0; s < N; ++s) {
-          float f[8];
+          float f[8], h[8];
           uint32_t top = 0;
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
             f[e] = x[s][e >> 2][e & 3];
             top = max(top, magnitude(f[e]));
           }
-          float back = 1.0f;
+          v4f un = {1, 1, 1, 1};
           if constexpr (TYPE == kF16) {
             top = max(top, (uint32_t)__shfl_xor((int)top, 16));
-            const float norm = normaliser(__uint_as_float(top));
-            back = 1.0f / norm;
+            if constexpr (!SMALL) top = max(top, (uint32_t)__shfl_xor((int)top, 32));
+            const float norm = normaliser(__uint_as_float(top)), back = 1.0f / norm;
 #pragma unroll
             for (int e = 0; e < 8; ++e) f[e] *= norm;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) un[e] = __shfl(back, 4 * g + e);
           }
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            const float hi = (float)(T)f[e];
+            h[e] = (float)(T)f[e];
             // (inf - inf of an infinite u would make a NaN of its low half)
-            f[e] = g < 2 ? hi : magnitude(hi) < kInfBits ? f[e] - hi : 0.0f;
+            f[e] = magnitude(h[e]) < kInfBits ? f[e] - h[e] : 0.0f;
+            if (SMALL) h[e] = g < 2 ? h[e] : f[e];
           }
-          const Frag<TYPE> h = to_frag<TYPE>(f);
-          if constexpr (TYPE == kF16) {
-            v4f un;
+          const Frag<TYPE> hi = to_frag<TYPE>(h), lo = to_frag<TYPE>(f);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) un[e] = __shfl(back, 4 * g + e);
-#pragma unroll
-            for (int ni = 0; ni < NI; ++ni) {
-              const v4f p = mfma16<TYPE>(h, b[s][ni], v4f{0, 0, 0, 0});
-#pragma unroll
-              for (int e = 0; e < 4; ++e) t[ni][e] = fmaf(p[e], un[e], t[ni][e]);
-            }
-          } else {
-#pragma unroll
-            for (int ni = 0; ni < NI; ++ni) t[ni] = mfma16<TYPE>(h, b[s][ni], t[ni]);
+          for (int q = 0; q < NI / 4; ++q) {
+            v4f t[4] = {{0, 0, 0, 0}, {0, 0, 0, 0}, {0, 0, 0, 0}, {0, 0, 0, 0}};
+            const Frag<TYPE> four[4] = {b[s][4 * q], b[s][4 * q + 1], b[s][4 * q + 2], b[s][4 * q + 3]};
+            four_products<TYPE, !SMALL>(t, hi, lo, four);
+            add(t, q, un);
           }
         }
       }
     };
-    int r = 0;
-    for (; r + 16 * S <= l.Rp; r += 16 * S) ranks(std::integral_constant<int, S>(), r);
-    for (; r < l.Rp; r += 16) ranks(std::integral_constant<int, 1>(), r);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const bool mine = rows >> (4 * g + e) & 1;
-#pragma unroll
-      for (int ni = 0; ni < NI; ++ni) d[ni][e] = mine ? t[ni][e] : d[ni][e];
+    using One = std::integral_constant<int, 1>;
+    using Two = std::integral_constant<int, 2>;
+    if (TYPE != kF32 && l.Rp == 16) {
+      ranks(One(), std::true_type(), 0);
+      return;
     }
+    constexpr int G = TYPE == kF32 ? 16 : 32;
+    int r = 0;
+    for (; r + 2 * G <= l.Rp; r += 2 * G) ranks(Two(), std::false_type(), r);
+    if (r < l.Rp) ranks(One(), std::false_type(), r);
   });
 }
 
@@ -739,23 +854,28 @@ __global__ __launch_bounds__(256) void outer_kernel(OuterPair pair) {
     }
     constexpr int U = TYPE == kF32 ? 4 : 8;
     for (int i0 = wave * 4 * U; i0 < n; i0 += 16 * U) {
-      float h[U], z[U][8];
+      // all loads under way: rows past the last are the last again, times zero and of zeros
+      float h[U];
+      Raw8<TYPE> z[U];
+      bool in[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const int i = i0 + 4 * u + g;
-        h[u] = 0.0f;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) z[u][e] = 0.0f;
-        if (i < n) {
-          const int row = p.which ? list[i] : r0 + i;
-          h[u] = p.H[(int64_t)row * p.Rp + rank0 + c];
-          load8<TYPE>((const T *)p.Z + row * p.ldz, col, p.cols, z[u]);
-        }
+        in[u] = i < n;
+        const int at = min(i, n - 1), row = p.which ? list[at] : r0 + at;
+        h[u] = p.H[(int64_t)row * p.Rp + rank0 + c];
+        z[u] = raw8<TYPE>((const T *)p.Z + row * p.ldz, col, p.cols);
       }
 #pragma unroll
-      for (int u = 0; u < U; ++u)
+      for (int u = 0; u < U; ++u) {
+        if (i0 + 4 * u >= n) break;
+        const float hu = in[u] ? h[u] : 0.0f;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) acc[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(h[u], z[u][j], acc[j], 0, 0, 0);
+        for (int j = 0; j < 8; ++j) {
+          const float x = raw_value<TYPE>(z[u], j);
+          acc[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(hu, in[u] ? x : 0.0f, acc[j], 0, 0, 0);
+        }
+      }
     }
     if (p.which) __syncthreads();   // the list is the next rows'
   }

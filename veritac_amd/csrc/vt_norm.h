@@ -14,24 +14,58 @@
 
 namespace {
 
-// 8 elements of a row from `pos`, zero past `len`, as 16-byte vectors at any
-// alignment where all 8 are there.
+// 8 elements of a row as they lie in memory, and their values. Apart, since a
+// value's conversion in a branch around its load waits for that load there.
 template <int TYPE>
-__device__ __forceinline__ void load8(const typename Elem<TYPE>::T *row, int64_t pos, int64_t len, float (&v)[8]) {
+struct Raw8 {
+  v4i w[TYPE == kF32 ? 2 : 1];
+};
+
+// From `pos`, zero past `len`, as 16-byte vectors at any alignment where all 8 are
+// there.
+template <int TYPE>
+__device__ __forceinline__ Raw8<TYPE> raw8(const typename Elem<TYPE>::T *row, int64_t pos, int64_t len) {
   typedef typename Elem<TYPE>::T T;
-  constexpr int PER = 16 / sizeof(T);
+  constexpr int N = TYPE == kF32 ? 2 : 1;
+  Raw8<TYPE> r;
   if (pos + 8 <= len) {
-    typedef T VT __attribute__((ext_vector_type(PER), aligned(sizeof(T))));
 #pragma unroll
-    for (int i = 0; i < 8 / PER; ++i) {
-      const VT x = *(const VT *)(row + pos + i * PER);
-#pragma unroll
-      for (int e = 0; e < PER; ++e) v[i * PER + e] = (float)x[e];
-    }
+    for (int i = 0; i < N; ++i) r.w[i] = *(const v4i_any *)(row + pos + i * (8 / N));
   } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = pos + e < len ? (float)row[pos + e] : 0.0f;
+    for (int i = 0; i < N; ++i) r.w[i] = v4i{0, 0, 0, 0};
+    typedef typename std::conditional<TYPE == kF32, uint32_t, uint16_t>::type Bits;
+    const Bits *b = (const Bits *)row;
+#pragma unroll
+    for (int e = 0; e < 7; ++e)
+      if (pos + e < len) {
+        if constexpr (TYPE == kF32) r.w[e >> 2][e & 3] = (int)b[pos + e];
+        else r.w[0][e >> 1] |= (int)((uint32_t)b[pos + e] << (16 * (e & 1)));
+      }
   }
+  return r;
+}
+
+template <int TYPE>
+__device__ __forceinline__ float raw_value(const Raw8<TYPE> &r, int e) {
+  if constexpr (TYPE == kF32) {
+    const int b = r.w[e >> 2][e & 3];
+    return __int_as_float(b);
+  } else {
+    const uint32_t b = (uint32_t)r.w[0][e >> 1] >> (16 * (e & 1)) & 0xffffu;
+    return from16(b, TYPE);
+  }
+}
+
+template <int TYPE>
+__device__ __forceinline__ void raw_values(const Raw8<TYPE> &r, float (&v)[8]) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = raw_value<TYPE>(r, e);
+}
+
+template <int TYPE>
+__device__ __forceinline__ void load8(const typename Elem<TYPE>::T *row, int64_t pos, int64_t len, float (&v)[8]) {
+  raw_values<TYPE>(raw8<TYPE>(row, pos, len), v);
 }
 
 template <int TYPE>

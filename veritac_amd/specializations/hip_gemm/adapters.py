@@ -143,7 +143,8 @@ def _fits(A, W, device):
 
 
 def _u(m, rank, device):
-    return _torch().empty((m, (rank + 15) // 16 * 16), dtype=_torch().float32, device=device)
+    pitch = 16 if rank <= 16 else (rank + 31) // 32 * 32
+    return _torch().empty((m, pitch), dtype=_torch().float32, device=device)
 
 
 def _forward(x, W, A, which, out):
