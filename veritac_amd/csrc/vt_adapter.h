@@ -182,6 +182,9 @@ struct RowPiece {
       w = raw8<TYPE>((const typename Elem<TYPE>::T *)row, pos, len);
     }
   }
+  __device__ __forceinline__ void settle() {
+    if constexpr (!I8) w.settle();
+  }
   __device__ __forceinline__ float value(int e) const {
     if constexpr (I8) return (float)(int8_t)((uint32_t)w[e >> 2] >> (8 * (e & 3)));
     else return raw_value<TYPE>(w, e);
@@ -234,9 +237,11 @@ __global__ __launch_bounds__(1024) void shrink_rows_kernel(ShrinkPair pair) {
         v[u].load(x, k + 8 * g, p.len);   // zero past the row's end
       }
 #pragma unroll
-      for (int u = 0; u < U; ++u)
+      for (int u = 0; u < U; ++u) {
+        v[u].settle();
 #pragma unroll
         for (int e = 0; e < 8; ++e) s = fmaf(v[u].value(e), (float)b[u].v[e], s);
+      }
     }
     s += __shfl_xor(s, 16);
     s += __shfl_xor(s, 32);
@@ -313,6 +318,7 @@ __global__ __launch_bounds__(1024) void shrink_tiles_kernel(ShrinkPair pair) {
     RowPiece<TYPE, I8> xa[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) xa[u].load(x, k0 + u * 32 + 8 * g, p.len);
+    bool settled = false;
     each_adapter(a, [&](int cur, uint32_t rows) {
       Frag<TYPE> b[NR][U];
 #pragma unroll
@@ -320,6 +326,11 @@ __global__ __launch_bounds__(1024) void shrink_tiles_kernel(ShrinkPair pair) {
 #pragma unroll
         for (int u = 0; u < U; ++u)
           b[n][u] = load_frag<TYPE>(w + cur * step + ((int64_t)n * p.lenp + min(k0 + u * 32, p.lenp - 32)) * 16);
+      if (!settled) {   // behind the adapter's loads
+#pragma unroll
+        for (int u = 0; u < U; ++u) xa[u].settle();
+        settled = true;
+      }
 #pragma unroll
       for (int n = 0; n < NR; ++n) {
         v4f part = {0, 0, 0, 0};
@@ -483,25 +494,104 @@ __device__ __forceinline__ void four_products(v4f (&t)[4], float a, float b0, fl
 }
 
 // Blocks of 16 x 16 in the accumulators' layout: d[ni] element e is row row0 +
-// 4 (lane / 16) + e, column col0 + 16 ni + lane % 16. Columns below colsp, any rows;
-// a: adapter_of row row0 + lane % 16.
+// 4 (lane / 16) + e, column col0 + 16 ni + lane % 16 (below colsp), for one strip of 16
+// rows after another.
 // 16-bit adapters: u enters in two halves (16 bits of it in bfloat16, 22 in
 // float16; it is then as exact as the 16-bit y that it is added to needs, 2^-8 of
 // a step), 32 ranks at a time, or 16 with both halves in one product. float16
 // halves are of u times a power of two for each row and 32 ranks, so that none
-// overflows or is lost. The loads of 64 ranks are under way together: there is one
-// wave to a SIMD here, and nothing else hides them.
+// overflows or is lost.
+// One wave to a SIMD runs this, so nothing hides its loads, and they would wait for
+// the strip's stores (all count in vmcnt, in order): a strip's u is loaded a strip
+// ahead, and the adapter's first groups of ranks (two, or one of wide tiles) stay in registers from strip to
+// strip (2000 x 4096 -> 4096, rank 64: 75 us with every load at its use, 56 with
+// those of a strip together, 35 without adapters).
 template <int TYPE, int NI>
-__device__ __forceinline__ void low_rank16(const LowRank &l, int a, int row0, int col0, int lane, v4f (&d)[NI]) {
+struct LowRankStrips {
   static_assert(NI % 4 == 0, "four blocks at a time");
   typedef typename Elem<TYPE>::T T;
-  const int g = lane >> 4, c = lane & 15, row = min(row0 + c, l.rows - 1);
-  const float *u = l.U + (int64_t)row * l.Rp;
+  static constexpr int G = TYPE == kF32 ? 16 : 32, HELD = NI <= 4 ? 2 : 1, UV = TYPE == kF32 ? 1 : 2;
+  struct Part {   // an adapter's 16 columns by G ranks
+    typename std::conditional<TYPE == kF32, v4f, Frag<TYPE>>::type v;
+  };
+  struct Ahead {
+    int a;
+    v4f u[HELD][UV];
+  };
+  const LowRank &l;
+  const int col0, lane, g, c, groups;
+  const bool small;   // 16 ranks in all
+  int held = -1;
+  Part b[HELD][NI];
+
+  __device__ __forceinline__ LowRankStrips(const LowRank &low, int col, int ln)
+      : l(low), col0(col), lane(ln), g(ln >> 4), c(ln & 15), groups(max(low.Rp / G, 1)), small(TYPE != kF32 && low.Rp == 16) {}
+
+  __device__ __forceinline__ void load_u(int row0, int group, v4f (&u)[UV]) const {
+    const float *at = l.U + (int64_t)min(row0 + c, l.rows - 1) * l.Rp + group * G + (TYPE == kF32 ? 4 : 8) * (small ? g & 1 : g);
 #pragma unroll
-  for (int ni = 0; ni < NI; ++ni) d[ni] = v4f{0, 0, 0, 0};
-  each_adapter(a, [&](int cur, uint32_t rows) {
-    const T *v = (const T *)l.V + (cur * l.colsp + col0) * l.Rp;
-    auto add = [&](const v4f (&t)[4], int q, const v4f &un) {
+    for (int i = 0; i < UV; ++i) u[i] = *(const v4f *)(at + 4 * i);
+  }
+  __device__ __forceinline__ void load_b(int a, int group, Part (&p)[NI]) const {
+    const T *v = (const T *)l.V + (a * l.colsp + col0) * l.Rp + group * G * 16 + (TYPE == kF32 ? lane * 4 : (small ? lane & 31 : lane) * 8);
+#pragma unroll
+    for (int ni = 0; ni < NI; ++ni) {
+      if constexpr (TYPE == kF32) p[ni].v = *(const v4f *)(v + ni * 16 * l.Rp);
+      else p[ni].v = load_frag<TYPE>(v + ni * 16 * l.Rp);
+    }
+  }
+  // a: adapter_of row row0 + lane % 16
+  __device__ __forceinline__ Ahead ahead(int a, int row0) const {
+    Ahead r;
+    r.a = a;
+#pragma unroll
+    for (int i = 0; i < HELD; ++i) load_u(row0, min(i, groups - 1), r.u[i]);
+    return r;
+  }
+  // One group of ranks of the rows in `rows`.
+  __device__ __forceinline__ void group_products(const v4f (&u)[UV], const Part (&p)[NI], uint32_t rows, v4f (&d)[NI]) const {
+    v4f un = {1, 1, 1, 1};
+    Frag<TYPE> hi, lo;
+    if constexpr (TYPE != kF32) {
+      float f[8], h[8];
+      uint32_t top = 0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        f[e] = u[e >> 2][e & 3];
+        top = max(top, magnitude(f[e]));
+      }
+      if constexpr (TYPE == kF16) {
+        top = max(top, (uint32_t)__shfl_xor((int)top, 16));
+        top = max(top, (uint32_t)__shfl_xor((int)top, 32));
+        const float norm = normaliser(__uint_as_float(top)), back = 1.0f / norm;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] *= norm;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) un[e] = __shfl(back, 4 * g + e);
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        h[e] = (float)(T)f[e];
+        // (inf - inf of an infinite u would make a NaN of its low half)
+        f[e] = magnitude(h[e]) < kInfBits ? f[e] - h[e] : 0.0f;
+        // 16 ranks: the product's other 16 are the low halves
+        h[e] = small && g >= 2 ? f[e] : h[e];
+        f[e] = small ? 0.0f : f[e];
+      }
+      hi = to_frag<TYPE>(h);
+      lo = to_frag<TYPE>(f);
+    }
+#pragma unroll
+    for (int q = 0; q < NI / 4; ++q) {
+      v4f t[4] = {{0, 0, 0, 0}, {0, 0, 0, 0}, {0, 0, 0, 0}, {0, 0, 0, 0}};
+      if constexpr (TYPE == kF32) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          four_products(t, u[0][e], p[4 * q].v[e], p[4 * q + 1].v[e], p[4 * q + 2].v[e], p[4 * q + 3].v[e]);
+      } else {
+        const Frag<TYPE> four[4] = {p[4 * q].v, p[4 * q + 1].v, p[4 * q + 2].v, p[4 * q + 3].v};
+        four_products<TYPE, true>(t, hi, lo, four);
+      }
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const bool mine = rows >> (4 * g + e) & 1;
@@ -511,90 +601,34 @@ __device__ __forceinline__ void low_rank16(const LowRank &l, int a, int row0, in
           d[4 * q + i][e] = mine ? x : d[4 * q + i][e];
         }
       }
-    };
-    // N groups of ranks from r
-    auto ranks = [&](auto count, auto small, int r) __attribute__((always_inline)) {
-      constexpr int N = decltype(count)::value;
-      constexpr bool SMALL = decltype(small)::value;   // 16 ranks in all
-      if constexpr (TYPE == kF32) {
-        v4f x[N], b[N][NI];
-#pragma unroll
-        for (int s = 0; s < N; ++s) {
-          x[s] = *(const v4f *)(u + r + 16 * s + 4 * g);
-#pragma unroll
-          for (int ni = 0; ni < NI; ++ni) b[s][ni] = *(const v4f *)(v + ni * 16 * l.Rp + (r + 16 * s) * 16 + lane * 4);
-        }
-#pragma unroll
-        for (int q = 0; q < NI / 4; ++q) {
-          v4f t[4] = {{0, 0, 0, 0}, {0, 0, 0, 0}, {0, 0, 0, 0}, {0, 0, 0, 0}};
-#pragma unroll
-          for (int s = 0; s < N; ++s)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              four_products(t, x[s][e], b[s][4 * q][e], b[s][4 * q + 1][e], b[s][4 * q + 2][e], b[s][4 * q + 3][e]);
-          add(t, q, v4f{1, 1, 1, 1});
-        }
-      } else {
-        v4f x[N][2];
-        Frag<TYPE> b[N][NI];
-#pragma unroll
-        for (int s = 0; s < N; ++s) {
-          const float *at = u + r + 32 * s + 8 * (SMALL ? g & 1 : g);
-          x[s][0] = *(const v4f *)at;
-          x[s][1] = *(const v4f *)(at + 4);
-#pragma unroll
-          for (int ni = 0; ni < NI; ++ni)
-            b[s][ni] = load_frag<TYPE>(v + ni * 16 * l.Rp + (r + 32 * s) * 16 + (SMALL ? lane & 31 : lane) * 8);
-        }
-#pragma unroll
-        for (int s = 0; s < N; ++s) {
-          float f[8], h[8];
-          uint32_t top = 0;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            f[e] = x[s][e >> 2][e & 3];
-            top = max(top, magnitude(f[e]));
-          }
-          v4f un = {1, 1, 1, 1};
-          if constexpr (TYPE == kF16) {
-            top = max(top, (uint32_t)__shfl_xor((int)top, 16));
-            if constexpr (!SMALL) top = max(top, (uint32_t)__shfl_xor((int)top, 32));
-            const float norm = normaliser(__uint_as_float(top)), back = 1.0f / norm;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) f[e] *= norm;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) un[e] = __shfl(back, 4 * g + e);
-          }
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            h[e] = (float)(T)f[e];
-            // (inf - inf of an infinite u would make a NaN of its low half)
-            f[e] = magnitude(h[e]) < kInfBits ? f[e] - h[e] : 0.0f;
-            if (SMALL) h[e] = g < 2 ? h[e] : f[e];
-          }
-          const Frag<TYPE> hi = to_frag<TYPE>(h), lo = to_frag<TYPE>(f);
-#pragma unroll
-          for (int q = 0; q < NI / 4; ++q) {
-            v4f t[4] = {{0, 0, 0, 0}, {0, 0, 0, 0}, {0, 0, 0, 0}, {0, 0, 0, 0}};
-            const Frag<TYPE> four[4] = {b[s][4 * q], b[s][4 * q + 1], b[s][4 * q + 2], b[s][4 * q + 3]};
-            four_products<TYPE, !SMALL>(t, hi, lo, four);
-            add(t, q, un);
-          }
-        }
-      }
-    };
-    using One = std::integral_constant<int, 1>;
-    using Two = std::integral_constant<int, 2>;
-    if (TYPE != kF32 && l.Rp == 16) {
-      ranks(One(), std::true_type(), 0);
-      return;
     }
-    constexpr int G = TYPE == kF32 ? 16 : 32;
-    int r = 0;
-    for (; r + 2 * G <= l.Rp; r += 2 * G) ranks(Two(), std::false_type(), r);
-    if (r < l.Rp) ranks(One(), std::false_type(), r);
-  });
-}
+  }
+  __device__ __forceinline__ void run(const Ahead &w, int row0, v4f (&d)[NI]) {
+#pragma unroll
+    for (int ni = 0; ni < NI; ++ni) d[ni] = v4f{0, 0, 0, 0};
+    each_adapter(w.a, [&](int cur, uint32_t rows) {
+      if (cur != held) {
+        load_b(cur, 0, b[0]);
+        if constexpr (HELD > 1) {
+          if (groups > 1) load_b(cur, 1, b[1]);
+        }
+        held = cur;
+      }
+      group_products(w.u[0], b[0], rows, d);
+      if constexpr (HELD > 1) {
+        if (groups > 1) group_products(w.u[1], b[1], rows, d);
+      }
+#pragma unroll 1
+      for (int i = HELD; i < groups; ++i) {
+        v4f u[UV];
+        Part p[NI];
+        load_u(row0, i, u);
+        load_b(cur, i, p);
+        group_products(u, p, rows, d);
+      }
+    });
+  }
+};
 
 // The adapters of a wave's 128 rows from row0: lane l holds rows l and 64 + l.
 struct RowAdapters {
@@ -633,11 +667,18 @@ struct AdaptedTile : ScaledTile<kLinear, TYPE == kF32 ? 4 : 2> {
       b[ni] = this->meta[this->Np + col0 + ni * 16 + c];
     }
     const RowAdapters ra = row_adapters(low, row0, lane);
+    LowRankStrips<TYPE, NI> strips(low, col0, lane);
+    auto next = strips.ahead(adapter_at(ra, 0, lane), row0);
+    v4f next_t = *(const v4f_any *)(this->t + row0 + 4 * g);
 #pragma unroll 1
     for (int mi = 0; mi < MI; ++mi) {
-      const v4f tr = *(const v4f_any *)(this->t + row0 + mi * 16 + 4 * g);
+      const auto now = next;
+      const v4f tr = next_t;
+      const int after = min(mi + 1, MI - 1) * 16;
+      next = strips.ahead(adapter_at(ra, after, lane), row0 + after);
+      next_t = *(const v4f_any *)(this->t + row0 + after + 4 * g);
       v4f d[NI];
-      low_rank16<TYPE, NI>(low, adapter_at(ra, mi * 16, lane), row0 + mi * 16, col0, lane, d);
+      strips.run(now, row0 + mi * 16, d);
       // chunk k of strip row r at k ^ (4 (r / 4 % 4)): an instruction's writes fall on distinct banks
       each([&](auto strip) __attribute__((always_inline)) {
         constexpr int i = decltype(strip)::value;
@@ -673,14 +714,19 @@ struct AdaptedTile : ScaledTile<kLinear, TYPE == kF32 ? 4 : 2> {
     const int g = lane >> 5, c = lane & 31;
     LDS_AS float *f = (LDS_AS float *)lds;   // [32][64]
     const RowAdapters ra = row_adapters(low, row0, lane);
+    LowRankStrips<TYPE, 4> strips(low, col0, lane);
+    auto next = strips.ahead(adapter_at(ra, 0, lane), row0);
     each([&](auto strip) __attribute__((always_inline)) {
       constexpr int mi = decltype(strip)::value;
       const int first = row0 + mi * 32;
       if (first >= this->M) return;
-#pragma unroll
+#pragma unroll 1
       for (int h = 0; h < 2; ++h) {
         v4f d[4];
-        low_rank16<TYPE, 4>(low, adapter_at(ra, mi * 32 + 16 * h, lane), first + 16 * h, col0, lane, d);
+        const auto now = next;
+        const int after = min(mi * 32 + 16 * h + 16, MI * 32 - 16);
+        next = strips.ahead(adapter_at(ra, after, lane), row0 + after);
+        strips.run(now, first + 16 * h, d);
 #pragma unroll
         for (int ni = 0; ni < 4; ++ni)
 #pragma unroll
@@ -740,23 +786,32 @@ struct AdaptedGrad : ScaledTile<kGrad> {
     const int g = lane >> 4, c = lane & 15;
     const float one[2] = {1.0f, 1.0f};
     const RowAdapters ra = row_adapters(low, row0, lane);
+    // columns past the last are not stored, and read from before it
+    LowRankStrips<TYPE, NI> low_strips(low, min(col0, (int)low.colsp - NI * 16), lane);
+    auto next = low_strips.ahead(adapter_at(ra, 0, lane), row0);
     this->template strips<MI / G, 16 * G, NI * 16>(
         [&](auto strip) __attribute__((always_inline)) {
-#pragma unroll
+          constexpr int first = decltype(strip)::value * G;
+#pragma unroll 1
           for (int i = 0; i < G; ++i) {
-            constexpr int first = decltype(strip)::value * G;
-            const int rel = (first + i) * 16;
+            const int rel = (first + i) * 16, after = min(rel + 16, MI * 16 - 16);
+            const auto now = next;
+            next = low_strips.ahead(adapter_at(ra, after, lane), row0 + after);
             v4f d[NI];
-            // columns past the last are not stored, and read from before it
-            low_rank16<TYPE, NI>(low, adapter_at(ra, rel, lane), row0 + rel, min(col0, (int)low.colsp - NI * 16), lane, d);
+            low_strips.run(now, row0 + rel, d);
+            v4f unit;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float unit = __shfl(rel >= 64 ? early[1] : early[0], (rel + 4 * g + e) & 63);
+            for (int e = 0; e < 4; ++e) unit[e] = __shfl(rel >= 64 ? early[1] : early[0], (rel + 4 * g + e) & 63);
+            each([&](auto block) __attribute__((always_inline)) {
+              constexpr int k = decltype(block)::value;
+              if (i != k) return;
 #pragma unroll
-              for (int ni = 0; ni < NI; ++ni)
-                *(LDS_AS float *)(lds + (16 * i + 4 * g + e) * (64 * NI) + ((((ni ^ g) << 2) + (c >> 2)) << 4) + (c & 3) * 4) =
-                    acc[first + i][ni][e] * unit + d[ni][e];
-            }
+              for (int e = 0; e < 4; ++e)
+#pragma unroll
+                for (int ni = 0; ni < NI; ++ni)
+                  *(LDS_AS float *)(lds + (16 * k + 4 * g + e) * (64 * NI) + ((((ni ^ g) << 2) + (c >> 2)) << 4) + (c & 3) * 4) =
+                      acc[first + k][ni][e] * unit[e] + d[ni][e];
+            }, std::make_integer_sequence<int, G>());
           }
         },
         [](int row) { return ((row >> 2) & 3) << 2; }, row0, col0, M, lane, lds, one);
@@ -809,7 +864,7 @@ struct OuterPair {
 // and product j takes column j of every lane's. The rows of other adapters are
 // left out by a list of this one's rows, made in order 1024 rows at a time.
 template <int TYPE>
-__global__ __launch_bounds__(256) void outer_kernel(OuterPair pair) {
+__global__ __launch_bounds__(256, 4) void outer_kernel(OuterPair pair) {
   typedef typename Elem<TYPE>::T T;
   constexpr int ROWS = 1024;
   const int which_of = (int)blockIdx.x >= pair.x0, block = blockIdx.x - (which_of ? pair.x0 : 0);
@@ -852,7 +907,7 @@ __global__ __launch_bounds__(256) void outer_kernel(OuterPair pair) {
       n = total;
       __syncthreads();
     }
-    constexpr int U = TYPE == kF32 ? 4 : 8;
+    constexpr int U = 4;
     for (int i0 = wave * 4 * U; i0 < n; i0 += 16 * U) {
       // all loads under way: rows past the last are the last again, times zero and of zeros
       float h[U];
@@ -869,6 +924,7 @@ __global__ __launch_bounds__(256) void outer_kernel(OuterPair pair) {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         if (i0 + 4 * u >= n) break;
+        z[u].settle();
         const float hu = in[u] ? h[u] : 0.0f;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {

@@ -15,23 +15,55 @@
 namespace {
 
 // 8 elements of a row as they lie in memory, and their values. Apart, since a
-// value's conversion in a branch around its load waits for that load there.
+// value's conversion in a branch around its load waits for that load there. `late`:
+// by how many elements they begin before the piece, whose end is past the row's:
+// a row's last piece is read as the row's last 8 elements and moved, without a
+// branch (element loads of it, each waited for, took 3 us of an odd row's 8).
 template <int TYPE>
 struct Raw8 {
   v4i w[TYPE == kF32 ? 2 : 1];
+  int late;
+
+  __device__ __forceinline__ void settle() {
+    if (!__any(late)) return;
+    if constexpr (TYPE == kF32) {
+#pragma unroll
+      for (int b = 4; b; b >>= 1)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int from = e + b < 8 ? w[(e + b) >> 2 & 1][(e + b) & 3] : 0, is = w[e >> 2][e & 3];
+          w[e >> 2][e & 3] = (late & b) ? from : is;
+        }
+      if (late >= 8) w[0] = w[1] = v4i{0, 0, 0, 0};
+    } else {
+      uint64_t lo = (uint32_t)w[0][0] | (uint64_t)(uint32_t)w[0][1] << 32, hi = (uint32_t)w[0][2] | (uint64_t)(uint32_t)w[0][3] << 32;
+      if (late & 4) {
+        lo = hi;
+        hi = 0;
+      }
+      const int s = 16 * (late & 3);
+      lo = s ? lo >> s | hi << (64 - s) : lo;
+      hi >>= s;
+      if (late >= 8) lo = hi = 0;
+      w[0] = v4i{(int)(uint32_t)lo, (int)(lo >> 32), (int)(uint32_t)hi, (int)(hi >> 32)};
+    }
+    late = 0;
+  }
 };
 
-// From `pos`, zero past `len`, as 16-byte vectors at any alignment where all 8 are
-// there.
+// From `pos`, zero past `len`, as 16-byte vectors at any alignment; rows of fewer
+// than 8 by elements.
 template <int TYPE>
 __device__ __forceinline__ Raw8<TYPE> raw8(const typename Elem<TYPE>::T *row, int64_t pos, int64_t len) {
-  typedef typename Elem<TYPE>::T T;
   constexpr int N = TYPE == kF32 ? 2 : 1;
   Raw8<TYPE> r;
-  if (pos + 8 <= len) {
+  if (len >= 8) {
+    const int64_t at = min(pos, len - 8);
+    r.late = (int)min(pos - at, (int64_t)8);
 #pragma unroll
-    for (int i = 0; i < N; ++i) r.w[i] = *(const v4i_any *)(row + pos + i * (8 / N));
+    for (int i = 0; i < N; ++i) r.w[i] = *(const v4i_any *)(row + at + i * (8 / N));
   } else {
+    r.late = 0;
 #pragma unroll
     for (int i = 0; i < N; ++i) r.w[i] = v4i{0, 0, 0, 0};
     typedef typename std::conditional<TYPE == kF32, uint32_t, uint16_t>::type Bits;
@@ -46,6 +78,7 @@ __device__ __forceinline__ Raw8<TYPE> raw8(const typename Elem<TYPE>::T *row, in
   return r;
 }
 
+// Of a settled piece.
 template <int TYPE>
 __device__ __forceinline__ float raw_value(const Raw8<TYPE> &r, int e) {
   if constexpr (TYPE == kF32) {
@@ -58,7 +91,8 @@ __device__ __forceinline__ float raw_value(const Raw8<TYPE> &r, int e) {
 }
 
 template <int TYPE>
-__device__ __forceinline__ void raw_values(const Raw8<TYPE> &r, float (&v)[8]) {
+__device__ __forceinline__ void raw_values(Raw8<TYPE> r, float (&v)[8]) {
+  r.settle();
 #pragma unroll
   for (int e = 0; e < 8; ++e) v[e] = raw_value<TYPE>(r, e);
 }
