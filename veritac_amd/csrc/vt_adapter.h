@@ -57,12 +57,20 @@ __global__ __launch_bounds__(256) void adapter_pack_kernel(AdapterPackArgs p) {
   const int len = up ? p.N : p.K, lenp = up ? p.Np : p.Kp, a = blockIdx.y, j0 = blockIdx.x * 64;
   if (j0 >= lenp) return;
   const T *src = (const T *)(up ? p.B : p.A) + (int64_t)a * p.R * len;
-  for (int i = threadIdx.x; i < 64 * p.Rp; i += 256) {
-    // down is [R][K], up [N][R]
-    const int j = up ? i / p.Rp : i & 63, r = up ? i % p.Rp : i >> 6;
-    T v = T(0);
-    if (j0 + j < len && r < p.R) v = up ? src[(int64_t)(j0 + j) * p.R + r] : src[(int64_t)r * len + j0 + j];
-    tile[j][r] = v;
+  const int tid = threadIdx.x;
+  for (int r0 = 0; r0 < p.Rp; r0 += 16) {
+    // down is [R][K], up [N][R]; 4 elements a thread under way together
+    T v[4];
+    int j[4], r[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      j[q] = up ? (tid >> 4) + 16 * q : tid & 63;
+      r[q] = r0 + (up ? tid & 15 : (tid >> 6) + 4 * q);
+      v[q] = T(0);
+      if (j0 + j[q] < len && r[q] < p.R) v[q] = up ? src[(int64_t)(j0 + j[q]) * p.R + r[q]] : src[(int64_t)r[q] * len + j0 + j[q]];
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q) tile[j[q]][r[q]] = v[q];
   }
   __syncthreads();
   constexpr int E = sizeof(T) == 4 ? 4 : 8;
@@ -74,14 +82,18 @@ __global__ __launch_bounds__(256) void adapter_pack_kernel(AdapterPackArgs p) {
     uint8_t *to = second ? p.second[back] : p.first[back];
     if (!to) continue;
     T *dst = (T *)to + (int64_t)a * p.Rp * lenp;
-    for (int i = threadIdx.x; i < 64 * p.Rp; i += 256) {
-      if (second) {
-        // 4 blocks of 16 columns, contiguous
-        const int nb = i / (16 * p.Rp), w = i % (16 * p.Rp), f = w % (16 * G);
-        const int r = w / (16 * G) * G + f / (16 * E) * E + f % E, c = f / E % 16;
-        dst[(int64_t)j0 * p.Rp + i] = tile[nb * 16 + c][r];
-      } else {
-        // 2 fragments of 32 columns for each 16 ranks
+    if (second) {
+      // 4 blocks of 16 columns, contiguous
+      const int shift = G == 16 ? 4 : 5;
+#pragma unroll 1
+      for (int nb = 0; nb < 4; ++nb)
+        for (int w = tid; w < 16 * p.Rp; w += 256) {
+          const int f = w & ((16 << shift) - 1), c = f / E % 16, r = (w >> (4 + shift) << shift) + f / (16 * E) * E + f % E;
+          dst[(int64_t)(j0 + nb * 16) * p.Rp + w] = tile[nb * 16 + c][r];
+        }
+    } else {
+      // 2 fragments of 32 columns for each 16 ranks
+      for (int i = tid; i < 64 * p.Rp; i += 256) {
         const int rb = i / 1024, w = i % 1024, f = w % 512;
         const int r = rb * 16 + f / 8 % 16, j = w / 512 * 32 + f / 128 * 8 + f % 8;
         dst[((int64_t)rb * (lenp / 32) + j0 / 32) * 512 + w] = tile[j][r];
@@ -420,17 +432,20 @@ __device__ __forceinline__ float low_rank_element(const LowRank &l, int row, int
 }
 
 // E elements of it at once, so that their loads are under way together; those with
-// a row below 0 are left out.
-template <int TYPE, int E>
-__device__ __forceinline__ void low_rank_elements(const LowRank &l, const int (&row)[E], const int (&col)[E], float (&s)[E]) {
-  const float *u[E];
+// a row below 0 are left out. U: LowRank's u, or a copy of it in LDS.
+template <int TYPE, int E, class FLOATS>
+__device__ __forceinline__ void low_rank_elements(const LowRank &l, FLOATS U, const int (&row)[E], const int (&col)[E], float (&s)[E]) {
+  typedef const v4f *Global;
+  typedef const LDS_AS v4f *Local;
+  typedef typename std::conditional<std::is_same<FLOATS, const float *>::value, Global, Local>::type Four;
+  FLOATS u[E];
   int at[E];
   bool in[E];
 #pragma unroll
   for (int i = 0; i < E; ++i) {
     const int a = row[i] < 0 ? -1 : adapter_of(l, row[i]);
     in[i] = a >= 0;
-    u[i] = l.U + (int64_t)max(row[i], 0) * l.Rp;
+    u[i] = U + (int64_t)max(row[i], 0) * l.Rp;
     at[i] = max(a, 0);
     s[i] = 0.0f;
   }
@@ -440,8 +455,8 @@ __device__ __forceinline__ void low_rank_elements(const LowRank &l, const int (&
 #pragma unroll
     for (int i = 0; i < E; ++i) {
       b[i] = rank_frag<TYPE>(rank_at<TYPE>(l, at[i], row[i] < 0 ? 0 : col[i], r));
-      x[i] = *(const v4f *)(u[i] + r);
-      y[i] = *(const v4f *)(u[i] + r + 4);
+      x[i] = *(Four)(u[i] + r);
+      y[i] = *(Four)(u[i] + r + 4);
     }
 #pragma unroll
     for (int i = 0; i < E; ++i) {
@@ -756,12 +771,20 @@ struct AdaptedTile : ScaledTile<kLinear, TYPE == kF32 ? 4 : 2> {
     }, std::make_integer_sequence<int, MI>());
   }
 
+  // u of all rows (64 at the most) into LDS: its 16 columns' lanes read it again and
+  // again.
+  template <int THREADS>
+  __device__ __forceinline__ void stage(float *lds, int tid) const {
+    for (int i = tid * 4; i < this->M * low.Rp; i += THREADS * 4) *(LDS_AS v4f *)((LDS_AS float *)lds + i) = *(const v4f *)(low.U + i);
+    lds_barrier();
+  }
   // The adapters' part of E elements, before the sums are there.
   template <int E>
-  __device__ __forceinline__ void ahead(const int (&row)[E], const int (&col)[E], float (&d)[E]) const {
-    if (this->type == VT_TYPE_F32) low_rank_elements<kF32>(low, row, col, d);
-    else if (this->type == VT_TYPE_F16) low_rank_elements<kF16>(low, row, col, d);
-    else low_rank_elements<kBF16>(low, row, col, d);
+  __device__ __forceinline__ void ahead(const int (&row)[E], const int (&col)[E], float (&d)[E], float *lds) const {
+    const LDS_AS float *u = (const LDS_AS float *)lds;
+    if (this->type == VT_TYPE_F32) low_rank_elements<kF32>(low, u, row, col, d);
+    else if (this->type == VT_TYPE_F16) low_rank_elements<kF16>(low, u, row, col, d);
+    else low_rank_elements<kBF16>(low, u, row, col, d);
   }
   __device__ __forceinline__ void element(int32_t a0, int32_t, int row, int pc, int j, float t_row) const {
     if (j < this->N) element_with(a0, row, pc, j, t_row, low_rank_element(low, this->type, row, j));
@@ -835,7 +858,12 @@ __global__ __launch_bounds__(256) void adapted_finish_kernel(const int32_t *S, i
 
 // dx from partial sums, with the adapters' part.
 __global__ __launch_bounds__(256) void adapted_dx_sum_kernel(GradSumArgs p, LowRank low) {
-  sum_grad_slices(p, [&](int row, int col) { return low_rank_element(low, p.type, row, col); });
+  sum_grad_slices(p, [&](int row, int col, float (&x)[4]) {
+    const int rows[4] = {row, row, row, row}, cols[4] = {col, col + 1, col + 2, col + 3};   // below colsp, whole fours
+    if (p.type == VT_TYPE_F32) low_rank_elements<kF32>(low, low.U, rows, cols, x);
+    else if (p.type == VT_TYPE_F16) low_rank_elements<kF16>(low, low.U, rows, cols, x);
+    else low_rank_elements<kBF16>(low, low.U, rows, cols, x);
+  });
 }
 
 // ---------------------------------------------------------------------------

@@ -1089,11 +1089,13 @@ __device__ __forceinline__ void skinny_rows(const ScaledSkinnyArgs &p, const O &
   // first weights'.
   constexpr bool AHEAD = !std::is_same<O, ScaledOut>::value;
   constexpr int EPT = (NBW * 256 + 511) / 512;   // elements of a row block
+  __shared__ __attribute__((aligned(16))) float ahead_lds[AHEAD ? 16 * MB * 128 : 4];
   float more[MB][EPT];
   auto look_ahead = [&]() {
     if constexpr (AHEAD) {
       if ((MB == 1 && p.fin) || p.ws) return;
       __builtin_amdgcn_sched_barrier(0);
+      o.template stage<512>(ahead_lds, tid);
       int row[MB * EPT], col[MB * EPT];
       float d[MB * EPT];
 #pragma unroll
@@ -1103,7 +1105,7 @@ __device__ __forceinline__ void skinny_rows(const ScaledSkinnyArgs &p, const O &
         col[i] = (nb0 + n) * 16 + c;
         if (t >= NBW * 256 || row[i] >= M || col[i] >= o.N || c < col_lo(n) || c >= col_hi(n)) row[i] = -1;
       }
-      o.ahead(row, col, d);
+      o.ahead(row, col, d, ahead_lds);
 #pragma unroll
       for (int i = 0; i < MB * EPT; ++i) more[i / EPT][i % EPT] = d[i];
       __builtin_amdgcn_sched_barrier(0);
@@ -1544,7 +1546,7 @@ struct GradSumArgs {
   int M, K, Kp, slices, type;
 };
 
-// `more`: what else an element (row, column) holds.
+// `more`: what else 4 elements of a row, from a column on, hold.
 template <class MORE>
 __device__ __forceinline__ void sum_grad_slices(const GradSumArgs &p, MORE &&more) {
   const int64_t row = blockIdx.x;
@@ -1552,6 +1554,8 @@ __device__ __forceinline__ void sum_grad_slices(const GradSumArgs &p, MORE &&mor
   if (col >= p.K) return;
   const float *w = p.ws + row * p.Kp + col;
   const int64_t step = (int64_t)p.M * p.Kp;
+  float x[4];
+  more((int)row, col, x);   // its loads are under way together with the slices'
   v4f v = {0, 0, 0, 0};
   for (int i = 0; i < p.slices; i += 8) {   // 8 loads in flight; the order of the sums does not depend on them
     v4f part[8];
@@ -1566,14 +1570,14 @@ __device__ __forceinline__ void sum_grad_slices(const GradSumArgs &p, MORE &&mor
 #pragma unroll
   for (int e = 0; e < 4; ++e)
     if (col + e < p.K) {
-      const float x = v[e] + more((int)row, col + e);
-      if (p.type == VT_TYPE_F32) ((float *)p.X)[at + e] = x;
-      else ((uint16_t *)p.X)[at + e] = (uint16_t)pack16(x, 0.0f, p.type);
+      const float y = v[e] + x[e];
+      if (p.type == VT_TYPE_F32) ((float *)p.X)[at + e] = y;
+      else ((uint16_t *)p.X)[at + e] = (uint16_t)pack16(y, 0.0f, p.type);
     }
 }
 
 __global__ __launch_bounds__(256) void grad_sum_kernel(GradSumArgs p) {
-  sum_grad_slices(p, [](int, int) { return 0.0f; });
+  sum_grad_slices(p, [](int, int, float (&x)[4]) { x[0] = x[1] = x[2] = x[3] = 0.0f; });
 }
 
 // ---------------------------------------------------------------------------
