@@ -9,7 +9,7 @@ U32 = ref.U32
 CASES = [(1, 64, 1), (1, 1, 2), (5, 120, 1203), (16, 4096, 700), (17, 128, 5000), (64, 333, 9001), (3, 0, 10), (100, 0, 70),
          (65, 64, 64), (65, 128, 1000), (66, 130, 129), (100, 333, 5003), (200, 127, 63), (300, 999, 1001), (256, 256, 256),
          (700, 1024, 3000), (1000, 512, 8000), (600, 2048, 4999), (2050, 400, 13000), (1030, 1030, 16500), (513, 64, 700),
-         (130, 3000, 40)]
+         (130, 3000, 40), (875, 451, 15691), (2541, 768, 6285), (4872, 408, 2945)]
 
 
 class Loss:

@@ -663,6 +663,12 @@ __device__ __forceinline__ int adapter_at(const RowAdapters &r, int rel, int lan
 // A linear layer's outputs with adapters. TYPE: of adapters and outputs.
 template <int TYPE>
 struct AdaptedTile : ScaledTile<kLinear, TYPE == kF32 ? 4 : 2> {
+  // A wave's 128 x 128 sums and its next fragments leave too few registers for the
+  // low-rank products, and what they spill waits for the stores: 4096 x 4096 -> 14336
+  // with rank 16 / 64 / 128 took 346 / 391 / 465 us on 256 x 256 tiles and takes 292 /
+  // 321 / 414 on 256 x 128 (219 without adapters); 8192^3 614 / 711 / 887 and 661 /
+  // 738 / 946 (484).
+  static constexpr bool kWide = false;
   LowRank low;
   static constexpr int OE = TYPE == kF32 ? 4 : 2;
 
@@ -673,6 +679,7 @@ struct AdaptedTile : ScaledTile<kLinear, TYPE == kF32 ? 4 : 2> {
   // same in both.
   template <int MI, int NI, bool EDGE>
   __device__ __forceinline__ void tile16(const v4i (&acc)[MI][NI], int row0, int col0, int, int, int lane, LDS_AS int8_t *lds) const {
+    static_assert(NI == 4, "64 columns");
     constexpr int W = NI * 16, LPR = W / 8, RPI = 64 / LPR, IT = 16 / RPI;
     const int g = lane >> 4, c = lane & 15, j8 = 8 * (lane % LPR), lr = lane / LPR;
     float s[NI], b[NI];
@@ -1128,7 +1135,7 @@ int adapted_rows(const ScaledCall &c, const LowRank &low, const Rows *ready, Scr
   if (skinny) return launch_skinny<kLinear>(nullptr, 0, 0, c.K, rows, c.Bp, o, scr);
   hipStream_t s = (hipStream_t)scr.stream;
   if (Kp == 0) return AdaptedSkinny::finish(nullptr, 0, o, s);
-  const TilePlan plan = tile_plan(false, c.M, Np, Kp, scr.st->num_cus);
+  const TilePlan plan = tile_plan(false, c.M, Np, Kp, scr.st->num_cus, true, AdaptedTile<kF32>::kWide);
   if (plan.ks > 1) {
     const int32_t *sums = nullptr;
     if (int rc = sliced_sums(plan, rows, c.Bp, c.M, Np, Kp, scr, &sums)) return rc;

@@ -95,7 +95,7 @@ __device__ __forceinline__ v2f join_parts(v2f a, v2f b) {
 // Forward: a tile's logits -> one (maximum, sum) for each of its rows and each
 // wave's columns, and the logits of targets among them.
 struct LseTile : ScaledOut {
-  static constexpr bool kScaled = true;
+  static constexpr bool kScaled = true, kWide = true;
   v2f *part;        // [parts][M]
   float *mine;      // [M]
   Targets targets;
@@ -195,6 +195,7 @@ struct LseTile : ScaledOut {
 // times the rows' normalisers, and with LOW what float16 leaves of them.
 template <bool LOW>
 struct LossTermsTile : ScaledTile<kGradTerms, 2, LOW> {
+  static constexpr bool kWide = true;
   const RowState *state;
   const float *dloss, *count;   // count null: not a mean
   float *norm_out;

@@ -1714,8 +1714,8 @@ struct TilePlan {
   int64_t tiles;
 };
 
-// `slice`: whether K may be split.
-TilePlan tile_plan(bool terms, int64_t M, int64_t Np, int64_t Kp, int cus, bool slice = true) {
+// `slice`: whether K may be split; `wide`: whether 256 x 256 tiles may be taken.
+TilePlan tile_plan(bool terms, int64_t M, int64_t Np, int64_t Kp, int cus, bool slice = true, bool wide = true) {
   const double slices = Kp / 64.0, more = terms ? 3.0 : 0.0;
   TilePlan best = {};
   double least = 0;
@@ -1738,7 +1738,7 @@ TilePlan tile_plan(bool terms, int64_t M, int64_t Np, int64_t Kp, int cus, bool 
     }
   };
   if (M >= 256 && Np >= 256 && Kp % 256 == 0) {
-    offer(256, 256, 1, true);
+    if (wide) offer(256, 256, 1, true);
     offer(256, 128, 1, true);
   }
   if (Kp > 128) offer(128, 128, 1, false);   // their kernel is built for more than one pair of slices
@@ -1778,7 +1778,7 @@ int sliced_sums(const TilePlan &plan, const Rows &rows, const int8_t *Bp, int64_
 }
 
 // The product on a plan without K slices, whose sums OUT takes on kernels of its
-// own type.
+// own type (OUT::kWide: also on 256 x 256 tiles).
 template <class OUT>
 int launch_tiles(const TilePlan &plan, const Rows &rows, const int8_t *Bp, int64_t Kp, const OUT &out, Scratch &scr) {
   hipStream_t s = (hipStream_t)scr.stream;
@@ -1787,8 +1787,10 @@ int launch_tiles(const TilePlan &plan, const Rows &rows, const int8_t *Bp, int64
   const dim3 grid((unsigned)plan.tiles);
   if (plan.persistent) {
     const dim3 wgs((unsigned)std::min<int64_t>(plan.tiles, scr.st->num_cus));
-    if (plan.bn == 256) hipLaunchKernelGGL((out_dma16_kernel<OUT, 256>), wgs, dim3(256), 0, s, a, out);
-    else hipLaunchKernelGGL((out_dma16_kernel<OUT, 128>), wgs, dim3(256), 0, s, a, out);
+    if constexpr (OUT::kWide) {
+      if (plan.bn == 256) hipLaunchKernelGGL((out_dma16_kernel<OUT, 256>), wgs, dim3(256), 0, s, a, out);
+    }
+    if (plan.bn == 128) hipLaunchKernelGGL((out_dma16_kernel<OUT, 128>), wgs, dim3(256), 0, s, a, out);
   } else if (plan.bm == 64) {
     if (Kp <= 128) hipLaunchKernelGGL((gemm_mfma_kernel<64, 128, 1, false, true, false, true, OUT>), grid, dim3(256), 0, s, a, out);
     else hipLaunchKernelGGL((gemm_mfma_kernel<64, 128, 1, false, false, false, true, OUT>), grid, dim3(256), 0, s, a, out);

@@ -109,10 +109,10 @@ def _pack(down, up, scaling):
 def pack_adapters(down, up, *, scaling=1.0, stream=None):
     """Adapters down [L, r, k] and up [L, n, r], laid out once for `adapted`. Not
     differentiable: train with (down, up, scaling) itself."""
-    _pair(down, up)
-    scaling = _scaling(scaling)
     for t in (down, up):
         scaled._constant("pack_adapters", t, "give adapted (down, up, scaling)")
+    _pair(down, up)
+    scaling = _scaling(scaling)
     return scaled._enqueued(down, stream, lambda: _pack(down, up, scaling))
 
 
@@ -186,8 +186,9 @@ def adapted(x, W, adapters, which=None, *, out=None, stream=None):
         down = up = None
         scaling = adapters.scaling
     else:
+        wants = scaled._wants_grad(x)
         down, up, scaling = _triple(adapters)
-        if any([scaled._wants_grad(t) for t in (x, down, up)]):     # each, for its refusal
+        if any([wants] + [scaled._wants_grad(t) for t in (down, up)]):      # each, for its refusal
             if out is not None or stream is not None:
                 raise HipGemmError("a differentiable call takes neither out nor stream")
             if isinstance(x, scaled.QuantRows):
@@ -241,9 +242,10 @@ def adapted_grad(dy, x, W, adapters, which=None, *, stream=None):
     """(dx, ddown, dup): the gradients of `adapted` in x (its int8 product's
     straight through the rounding), down and up, for adapters (down, up) or (down,
     up, scaling) and the x of the forward pass."""
-    down, up, scaling = _triple(adapters)
-    for t in (dy, x, down, up):
+    tensors = adapters[:2] if isinstance(adapters, (tuple, list)) else ()
+    for t in (dy, x, *tensors):
         scaled._constant("adapted_grad", t, "there is no second derivative")
+    down, up, scaling = _triple(adapters)
     return scaled._enqueued(dy, stream, lambda: _adapted_grad(dy, x, W, down, up, scaling, which, None, (True,) * 3))
 
 
