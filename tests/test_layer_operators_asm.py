@@ -1,11 +1,44 @@
 """Compiled code of the loss' and adapters' kernels whose k loops are inline assembly (test_scaled_asm.py says what
 such a loop may hold), and of the low-rank products written as inline assembly themselves."""
+import os
 import re
+import subprocess
 
 import pytest
 
-from test_dma_asm import asm, kernel_body  # noqa: F401  (the fixture compiles the sources once)
-from test_scaled_asm import instructions, m0_belongs_to_dmas, names, operands, registers
+from test_scaled_asm import m0_belongs_to_dmas, operands, registers
+from veritac_amd import _lib
+
+BIN = "/opt/rocm/llvm/bin/"
+
+
+@pytest.fixture(scope="module")
+def asm(tmp_path_factory):
+    """The built library's kernels as {name: instructions} (disassembled: a second compilation takes minutes)."""
+    folder = tmp_path_factory.mktemp("code")
+    fat, code = str(folder / "fat"), str(folder / "code.o")
+    subprocess.run([BIN + "llvm-objcopy", "--dump-section", ".hip_fatbin=" + fat, _lib.library_path(), os.devnull], check=True)
+    listed = subprocess.run([BIN + "clang-offload-bundler", "--list", "--type=o", "--input=" + fat], check=True, capture_output=True, text=True)
+    target = next(t for t in listed.stdout.split() if "gfx950" in t)
+    subprocess.run([BIN + "clang-offload-bundler", "--unbundle", "--type=o", "--input=" + fat, "--targets=" + target, "--output=" + code], check=True)
+    text = subprocess.run([BIN + "llvm-objdump", "-d", "--no-show-raw-insn", "--no-leading-addr", code], check=True, capture_output=True,
+                          text=True).stdout
+    kernels, now = {}, None
+    for line in text.splitlines():
+        m = re.match(r"(?:[0-9a-f]+ )?<(\S+)>:", line)
+        if m:
+            now = kernels.setdefault(m.group(1), [])
+        elif now is not None and line.strip():
+            now.append(re.sub(r"\s+", " ", line.split("//")[0]).strip())
+    return kernels
+
+
+def names(asm, kernel):
+    return sorted(n for n in asm if re.match(r"_Z\S*%s" % kernel, n) and not n.endswith(".kd"))
+
+
+def instructions(asm, name):
+    return asm[name]
 
 TILES = 3 + 2 * 3      # adapted outputs of three types on one tile; the loss and its terms, in one and two halves, on two
 

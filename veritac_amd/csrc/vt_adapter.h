@@ -389,52 +389,19 @@ __device__ __forceinline__ int adapter_of(const LowRank &l, int row) {
   return l.which ? min(l.which[row], l.L - 1) : 0;
 }
 
-// Where ranks r .. r + 7 of a column lie: 8 of them, or two fours.
-template <int TYPE>
-__device__ __forceinline__ const typename Elem<TYPE>::T *rank_at(const LowRank &l, int a, int64_t col, int r) {
-  typedef typename Elem<TYPE>::T T;
-  const T *v = (const T *)l.V + (a * l.colsp + (col & ~(int64_t)15)) * l.Rp + (TYPE == kF32 ? 4 : 8) * (col & 15);
-  return v + (TYPE == kF32 ? (r >> 4) * 256 + (r >> 2 & 3) * 64 : (r >> 5) * 512 + (r >> 3 & 3) * 128);
-}
-template <int TYPE>
-__device__ __forceinline__ Frag<TYPE> rank_frag(const typename Elem<TYPE>::T *p) {
-  Frag<TYPE> f;
-  if constexpr (TYPE == kF32) {
-    const v4f a = *(const v4f *)p, b = *(const v4f *)(p + 64);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      f.v[e] = a[e];
-      f.v[4 + e] = b[e];
-    }
-  } else {
-    f = load_frag<TYPE>(p);
-  }
-  return f;
+// Where ranks r .. r + 7 of a column lie (8 of them, or in float32 two fours), in
+// elements.
+__device__ __forceinline__ int64_t rank_at(const LowRank &l, bool wide, int a, int64_t col, int r) {
+  return (a * l.colsp + (col & ~(int64_t)15)) * l.Rp + (wide ? 4 : 8) * (col & 15) +
+         (wide ? (r >> 4) * 256 + (r >> 2 & 3) * 64 : (r >> 5) * 512 + (r >> 3 & 3) * 128);
 }
 
-// One element of it, 8 ranks at a time.
-template <int TYPE>
-__device__ __forceinline__ float low_rank_element(const LowRank &l, int row, int64_t col) {
-  const int a = adapter_of(l, row);
-  if (a < 0) return 0.0f;
-  const float *u = l.U + (int64_t)row * l.Rp;
-  float s = 0.0f;
-#pragma unroll 2
-  for (int r = 0; r < l.Rp; r += 8) {
-    const Frag<TYPE> b = rank_frag<TYPE>(rank_at<TYPE>(l, a, col, r));
-    const v4f x = *(const v4f *)(u + r), y = *(const v4f *)(u + r + 4);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) s = fmaf(x[e], (float)b.v[e], s);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) s = fmaf(y[e], (float)b.v[4 + e], s);
-  }
-  return s;
-}
-
-// E elements of it at once, so that their loads are under way together; those with
-// a row below 0 are left out. U: LowRank's u, or a copy of it in LDS.
-template <int TYPE, int E, class FLOATS>
-__device__ __forceinline__ void low_rank_elements(const LowRank &l, FLOATS U, const int (&row)[E], const int (&col)[E], float (&s)[E]) {
+// E elements of it at once, 8 ranks at a time, so that their loads are under way
+// together; those with a row below 0 are left out. U: LowRank's u, or a copy of it
+// in LDS. WIDE: float32 adapters, else `type`.
+template <bool WIDE, int E, class FLOATS>
+__device__ __forceinline__ void low_rank_elements(const LowRank &l, int type, FLOATS U, const int (&row)[E], const int (&col)[E],
+                                                  float (&s)[E]) {
   typedef const v4f *Global;
   typedef const LDS_AS v4f *Local;
   typedef typename std::conditional<std::is_same<FLOATS, const float *>::value, Global, Local>::type Four;
@@ -450,29 +417,44 @@ __device__ __forceinline__ void low_rank_elements(const LowRank &l, FLOATS U, co
     s[i] = 0.0f;
   }
   for (int r = 0; r < l.Rp; r += 8) {
-    Frag<TYPE> b[E];
+    v4i b[E][WIDE ? 2 : 1];
     v4f x[E], y[E];
 #pragma unroll
     for (int i = 0; i < E; ++i) {
-      b[i] = rank_frag<TYPE>(rank_at<TYPE>(l, at[i], row[i] < 0 ? 0 : col[i], r));
+      const int64_t w = rank_at(l, WIDE, at[i], row[i] < 0 ? 0 : col[i], r);
+      if constexpr (WIDE) {
+        b[i][0] = *(const v4i *)((const float *)l.V + w);
+        b[i][1] = *(const v4i *)((const float *)l.V + w + 64);
+      } else {
+        b[i][0] = *(const v4i *)((const uint16_t *)l.V + w);
+      }
       x[i] = *(Four)(u[i] + r);
       y[i] = *(Four)(u[i] + r + 4);
     }
 #pragma unroll
     for (int i = 0; i < E; ++i) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s[i] = fmaf(x[i][e], (float)b[i].v[e], s[i]);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) s[i] = fmaf(y[i][e], (float)b[i].v[4 + e], s[i]);
+      for (int e = 0; e < 8; ++e) {
+        float v;
+        if constexpr (WIDE) {
+          const int bits = b[i][e >> 2][e & 3];
+          v = __int_as_float(bits);
+        } else {
+          v = from16((uint32_t)b[i][0][e >> 1] >> (16 * (e & 1)) & 0xffffu, type);
+        }
+        s[i] = fmaf(e < 4 ? x[i][e & 3] : y[i][e & 3], v, s[i]);
+      }
     }
   }
 #pragma unroll
   for (int i = 0; i < E; ++i) s[i] = in[i] ? s[i] : 0.0f;
 }
 
-__device__ __forceinline__ float low_rank_element(const LowRank &l, int type, int row, int64_t col) {
-  if (type == VT_TYPE_F32) return low_rank_element<kF32>(l, row, col);
-  return type == VT_TYPE_F16 ? low_rank_element<kF16>(l, row, col) : low_rank_element<kBF16>(l, row, col);
+template <int E, class FLOATS>
+__device__ __forceinline__ void low_rank_any(const LowRank &l, int type, FLOATS U, const int (&row)[E], const int (&col)[E],
+                                                  float (&s)[E]) {
+  if (type == VT_TYPE_F32) low_rank_elements<true>(l, type, U, row, col, s);
+  else low_rank_elements<false>(l, type, U, row, col, s);
 }
 
 // t[i] += a . b[i] for four blocks beside each other, and with LO += lo . b[i]. In
@@ -788,13 +770,14 @@ struct AdaptedTile : ScaledTile<kLinear, TYPE == kF32 ? 4 : 2> {
   // The adapters' part of E elements, before the sums are there.
   template <int E>
   __device__ __forceinline__ void ahead(const int (&row)[E], const int (&col)[E], float (&d)[E], float *lds) const {
-    const LDS_AS float *u = (const LDS_AS float *)lds;
-    if (this->type == VT_TYPE_F32) low_rank_elements<kF32>(low, u, row, col, d);
-    else if (this->type == VT_TYPE_F16) low_rank_elements<kF16>(low, u, row, col, d);
-    else low_rank_elements<kBF16>(low, u, row, col, d);
+    low_rank_any(low, this->type, (const LDS_AS float *)lds, row, col, d);
   }
   __device__ __forceinline__ void element(int32_t a0, int32_t, int row, int pc, int j, float t_row) const {
-    if (j < this->N) element_with(a0, row, pc, j, t_row, low_rank_element(low, this->type, row, j));
+    if (j >= this->N) return;
+    const int rows[1] = {row}, cols[1] = {j};
+    float d[1];
+    low_rank_any(low, this->type, low.U, rows, cols, d);
+    element_with(a0, row, pc, j, t_row, d[0]);
   }
   __device__ __forceinline__ void element_with(int32_t a0, int row, int pc, int j, float t_row, float d) const {
     if (j >= this->N) return;
@@ -867,9 +850,7 @@ __global__ __launch_bounds__(256) void adapted_finish_kernel(const int32_t *S, i
 __global__ __launch_bounds__(256) void adapted_dx_sum_kernel(GradSumArgs p, LowRank low) {
   sum_grad_slices(p, [&](int row, int col, float (&x)[4]) {
     const int rows[4] = {row, row, row, row}, cols[4] = {col, col + 1, col + 2, col + 3};   // below colsp, whole fours
-    if (p.type == VT_TYPE_F32) low_rank_elements<kF32>(low, low.U, rows, cols, x);
-    else if (p.type == VT_TYPE_F16) low_rank_elements<kF16>(low, low.U, rows, cols, x);
-    else low_rank_elements<kBF16>(low, low.U, rows, cols, x);
+    low_rank_any(low, p.type, low.U, rows, cols, x);
   });
 }
 

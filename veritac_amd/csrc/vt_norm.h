@@ -625,6 +625,7 @@ int vt_norm_grad(const void *dY, int64_t ldd, const void *H, int64_t ldh, const 
   g_err.clear();
   const char *who = "vt_norm_grad";
   if (int rc = check_norm_sizes(who, M, K, type, gain_type, eps)) return rc;
+  if (K > (int64_t)65535 * 2048) return fail(VT_EUNSUPPORTED, "%s: rows of more than 65535 times 2048 (K=%lld)", who, (long long)K);
   if (K == 0 || (M == 0 && !dgain)) return VT_OK;
   if (!gain || (M > 0 && (!dY || !H || !dX))) return fail(VT_EINVAL, "%s: an operand is null", who);
   const int64_t e = elem_size(type), ge = elem_size(gain_type);

@@ -52,6 +52,9 @@ class Adapters:
     def device(self):
         return self.data.device
 
+    def _tensors(self):
+        return (self.data,)
+
     def __repr__(self):
         return "Adapters(%d of rank %d, k=%d, n=%d, %s, device=%s)" % (
             self.count, self.rank, self.k, self.n, self.dtype, self.device)

@@ -188,7 +188,7 @@ def _tensors(result):
     if isinstance(result, ScaledWeight):
         return result.data, result.meta
     if not isinstance(result, tuple):
-        return (result,)
+        return result._tensors() if hasattr(result, "_tensors") else (result,)
     return tuple(t for r in result if r is not None for t in _tensors(r))
 
 
