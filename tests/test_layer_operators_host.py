@@ -142,7 +142,8 @@ def test_forward_mode_is_refused(name):
     ("norm_rows", lambda x: norms.norm_rows(x, G)), ("norm_rows", lambda x: norms.norm_rows(X, G, residual=x)),
     ("norm_rows", lambda x: norms.norm_rows(X, x[0])), ("norm_grad", lambda x: norms.norm_grad(x, X, G)),
     ("norm_grad", lambda x: norms.norm_grad(X, X, G, dh=x)), ("pack_adapters", None),
-    ("adapted_grad", lambda x: adapters.adapted_grad(x[:, :32], X, weight(), (DOWN, UP)))], ids=str)
+    ("adapted_grad", lambda x: adapters.adapted_grad(x[:, :32], X, weight(), (DOWN, UP)))],
+    ids=["rows", "residual", "gain", "dy", "dh", "down", "adapted_grad"])
 def test_gradients_are_not_left_out(name, call):
     v = torch.zeros(3, 64, requires_grad=True)
     if call is None:

