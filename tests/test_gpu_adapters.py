@@ -108,6 +108,30 @@ def test_a_row_is_not_touched_by_others(dev, m, kind):
     assert dd[[0, 3]].isfinite().all() and du[[0, 3]].isfinite().all()
 
 
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("m,k,rank", [(65, 1, 3), (70, 7, 16), (129, 130, 20), (100, 999, 64), (333, 4100, 64), (66, 14336, 128),
+                                      (3100, 520, 64), (1600, 264, 128)])
+def test_rounded_beside_u(dev, m, k, rank, kind):
+    """The rows that u's kernel rounds are linear's: with adapters that add nothing, the outputs are the same."""
+    say("rounded beside u", m, k, rank, kind)
+    g = torch.Generator().manual_seed(m + k)
+    dtype, n, count = KINDS[kind], 40, 3
+    x = torch.randn(m, k + 3, generator=g).mul(torch.rand(m, 1, generator=g) * 4).to(dtype)
+    x[1], x[2, 0], x[3, k - 1], x[4] = 0, float("nan"), float("-inf"), torch.finfo(dtype).tiny / 4
+    x[5, : k - 1] = 0
+    rng = np.random.default_rng(k)
+    W = packed(dev, *weights(rng, k, n, -128), None)
+    down = torch.randn(count, rank, k, generator=g).to(dtype).to(dev)
+    up = torch.zeros(count, n, rank, dtype=dtype, device=dev)
+    which = torch.randint(-1, count, (m,), generator=g, dtype=torch.int32)
+    which[16:32] = -1
+    for at in (0, 1, 3):
+        rows = x.to(dev)[:, at:at + k]
+        want = scaled.linear(rows, W)
+        for w in (which.to(dev), None):
+            torch.testing.assert_close(adapters.adapted(rows, W, (down, up), w), want, rtol=0, atol=0, equal_nan=True)
+
+
 @pytest.mark.parametrize("m", [30, 200])
 def test_u_beyond_float16(dev, m):
     """float16 adapters whose u leaves float16's range, at either end."""
