@@ -101,3 +101,10 @@ def test_low_rank_products_wait_for_themselves(asm, kernel, count):
             for k in range(i - 3, i):
                 if k in low:
                     assert operands(code[k])[0] != ops[0], code[k:i + 1]
+
+
+def test_u_and_the_adapters_gradients_do_not_spill(asm):
+    """Workgroups of 16 waves have 128 registers a lane: their loads in flight are chosen to fit."""
+    kernels = names(asm, "shrink_tiles_kernel") + names(asm, "shrink_rows_kernel") + names(asm, "outer_kernel")
+    assert len(kernels) >= 20
+    assert not [n for n in kernels if any(t.startswith("scratch_") for t in instructions(asm, n))]

@@ -316,7 +316,7 @@ __device__ __forceinline__ void each_adapter(int a, F &&f) {
 template <int TYPE, bool I8, int NR>
 __global__ __launch_bounds__(1024) void shrink_tiles_kernel(ShrinkPair pair) {
   typedef typename Elem<TYPE>::T T;
-  constexpr int WAVES = 16, U = TYPE == kF32 ? 2 : 4;
+  constexpr int WAVES = 16, U = TYPE == kF32 || NR > 2 ? 2 : 4;   // what 128 registers hold
   __shared__ float red[WAVES][16][16 * NR + 1];
   const ShrinkArgs &p = pair.of[blockIdx.z];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, c = lane & 15;
