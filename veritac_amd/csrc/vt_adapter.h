@@ -885,7 +885,8 @@ struct OuterPair {
 // Its waves take 4 rows at a time in turn, as 4-deep float32 products (nothing is
 // rounded on the way, whatever the type): lane l holds 8 columns of row l / 16,
 // and product j takes column j of every lane's. The rows of other adapters are
-// left out by a list of this one's rows, made in order 1024 rows at a time.
+// left out by a list of this one's rows, made in order 1024 rows at a time; without
+// an index all rows are the first adapter's, and the others' sums are empty.
 template <int TYPE>
 __global__ __launch_bounds__(256, 4) void outer_kernel(OuterPair pair) {
   typedef typename Elem<TYPE>::T T;
@@ -900,7 +901,7 @@ __global__ __launch_bounds__(256, 4) void outer_kernel(OuterPair pair) {
   const int tile = block % tiles, rank0 = block / tiles % ranks * 16;
   const int a = blockIdx.y, split = blockIdx.z;
   const int col = tile * 128 + 8 * c;
-  const int beg = (int)((int64_t)p.M * split / p.splits), end = (int)((int64_t)p.M * (split + 1) / p.splits);
+  const int beg = (int)((int64_t)p.M * split / p.splits), end = p.which || !a ? (int)((int64_t)p.M * (split + 1) / p.splits) : beg;
   v4f acc[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) acc[j] = v4f{0, 0, 0, 0};
