@@ -287,7 +287,7 @@ struct NormGradArgs {
   const void *D, *H, *G, *E;   // dy, h, the gain and the residual's own gradient (or null)
   void *X;                     // dx
   float *part;                 // [groups][K] partial sums of the gain's gradient, null: not wanted
-  float *stats;                // NC = 0: two floats a row
+  float *stats;                // rows longer than kNormGradRow: their RowStats, three floats a row
   int64_t ldd, ldh, lde, ldx, M, K;
   float eps;
   int gain32;
@@ -358,38 +358,40 @@ __global__ __launch_bounds__(THREADS) void norm_grad_kernel(NormGradArgs p) {
   }
 }
 
-// Rows too long for a workgroup's registers: first what dx needs of each row,
+// Rows too long for a workgroup's registers: first what dx needs of each row, a
+// workgroup rows w, w + grid, .. (one a row would be beyond a launch from 2^22 on),
 template <int TYPE>
 __global__ __launch_bounds__(1024) void norm_stats_kernel(NormGradArgs p) {
   __shared__ uint64_t red[16];
   typedef typename Elem<TYPE>::T T;
-  const int64_t row = blockIdx.x;
-  float squares, dot;
-  auto all = [&](float f) {
-    squares = dot = 0.0f;
-    for (int64_t pos = threadIdx.x * 8; pos < p.K; pos += 8192) {
-      float d[8], h[8], g[8];
-      load8<TYPE>((const T *)p.D + row * p.ldd, pos, p.K, d);
-      load8<TYPE>((const T *)p.H + row * p.ldh, pos, p.K, h);
-      load_gain<TYPE>(p.G, p.gain32, pos, p.K, g);
+  for (int64_t row = blockIdx.x; row < p.M; row += gridDim.x) {
+    float squares, dot;
+    auto all = [&](float f) {
+      squares = dot = 0.0f;
+      for (int64_t pos = threadIdx.x * 8; pos < p.K; pos += 8192) {
+        float d[8], h[8], g[8];
+        load8<TYPE>((const T *)p.D + row * p.ldd, pos, p.K, d);
+        load8<TYPE>((const T *)p.H + row * p.ldh, pos, p.K, h);
+        load_gain<TYPE>(p.G, p.gain32, pos, p.K, g);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float a = h[e] * f;
-        squares = fmaf(a, a, squares);
-        dot = fmaf(d[e] * g[e], a, dot);
+        for (int e = 0; e < 8; ++e) {
+          const float a = h[e] * f;
+          squares = fmaf(a, a, squares);
+          dot = fmaf(d[e] * g[e], a, dot);
+        }
       }
+      block_two<1024>(squares, dot, add_f, add_f, red);
+    };
+    all(1.0f);
+    const float f = row_factor(squares, p.eps);
+    if (f != 1.0f) all(f);
+    if (threadIdx.x == 0) {
+      const float inv = inverse_rms(squares, f, (float)p.K, p.eps);
+      float *s = p.stats + row * 3;
+      s[0] = f;
+      s[1] = inv;
+      s[2] = dot / (float)p.K * inv * inv;
     }
-    block_two<1024>(squares, dot, add_f, add_f, red);
-  };
-  all(1.0f);
-  const float f = row_factor(squares, p.eps);
-  if (f != 1.0f) all(f);
-  if (threadIdx.x == 0) {
-    const float inv = inverse_rms(squares, f, (float)p.K, p.eps);
-    float *s = p.stats + row * 3;
-    s[0] = f;
-    s[1] = inv;
-    s[2] = dot / (float)p.K * inv * inv;
   }
 }
 
@@ -539,7 +541,7 @@ int launch_norm_grad(NormGradArgs a, void *dgain, int gain_type, Scratch &scr) {
   else if (threads == 512) hipLaunchKernelGGL((norm_grad_kernel<TYPE, 512, 1>), grid, dim3(512), 0, s, a);
   else if (threads == 1024) hipLaunchKernelGGL((norm_grad_kernel<TYPE, 1024, 1>), grid, dim3(1024), 0, s, a);
   else {
-    hipLaunchKernelGGL((norm_stats_kernel<TYPE>), dim3((unsigned)a.M), dim3(1024), 0, s, a);
+    hipLaunchKernelGGL((norm_stats_kernel<TYPE>), dim3((unsigned)resident(a.M, 1024, cus)), dim3(1024), 0, s, a);
     VT_HIP_CHECK(hipGetLastError());
     hipLaunchKernelGGL((norm_apply_kernel<TYPE>), dim3((unsigned)groups, (unsigned)((a.K + 2047) / 2048)), dim3(256), 0, s, a);
   }
