@@ -376,6 +376,7 @@ def gemm_packed_raw(A_ptr, Bp_ptr, D_ptr, C_ptr, M, N, K, lda, ldd, ldc, batch=1
 # VT_TYPE_* and VT_ACT_* of the scaled operators
 TYPE_F32, TYPE_F16, TYPE_BF16, TYPE_I8, TYPE_I8_PADDED = 1, 2, 3, 4, 5
 ACT_IDS = {"silu": 0, "gelu": 1}
+SCALED_MAX_ROWS = (1 << 24) - 1     # M of a call
 # VT_TARGET_* and VT_REDUCE_* of the loss
 TARGET_I32, TARGET_I64 = 1, 2
 REDUCE_IDS = {"none": 0, "mean": 1, "sum": 2}

@@ -99,14 +99,15 @@ class QuantRows:
         return self.data.device
 
     def dequantize(self, dtype=None):
-        """The rows as float32 [..., k], or rounded to float16 or bfloat16."""
+        """The rows as float32 [..., k], or rounded to float16 or bfloat16;
+        differentiable in `scale`."""
         torch = _torch()
         dtype = torch.float32 if dtype is None else dtype
         if dtype not in _types():
             raise HipGemmError("dtype must be float32, float16 or bfloat16 (got %s)" % (dtype,))
         data, k = self.data, self.k
         device = data.device
-        if device.type != "cuda":
+        if device.type != "cuda" or not self._plain():
             return (data[:, :k].float() * self.scale[:, None]).reshape(self.shape).to(dtype)
         y = data.new_empty(self.shape, dtype=dtype)
         with _on(device):
@@ -114,6 +115,16 @@ class QuantRows:
                 data.data_ptr(), _pitch(data), self.scale.data_ptr(), y.data_ptr(), _types()[dtype], max(k, 1),
                 data.shape[0], k, _current_stream(device)), "vt_dequant_rows")
         return y
+
+    def _plain(self):
+        """Whether vt_dequant_rows takes these rows: no derivative, no rows that share
+        memory, sizes of the operators'."""
+        torch = _torch()
+        data, scale, k = self.data, self.scale, self.k
+        kinds = torch.Tensor, torch.nn.Parameter     # not one that stands for another
+        return type(data) in kinds and type(scale) in kinds \
+            and not (scale.requires_grad and torch.is_grad_enabled()) and not _has_tangent(scale) \
+            and _pitch(data) >= k and data.shape[0] <= _lib.SCALED_MAX_ROWS and k < 1 << 30
 
     def __repr__(self):
         return "QuantRows(m=%d, k=%d, device=%s)" % (self.data.shape[0], self.k, self.device)
@@ -404,15 +415,19 @@ def _forward(x, W, pair, act, out_dtype, out):
 _forward_ad = None      # torch.autograd.forward_ad, from the first call on
 
 
-def _wants_grad(x):
+def _has_tangent(x):
     global _forward_ad
+    if _forward_ad is None:
+        _forward_ad = _torch().autograd.forward_ad
+    # outside of its levels nothing has one (asking for it takes 0.3 us)
+    return getattr(_forward_ad, "_current_level", 0) >= 0 and _forward_ad.unpack_dual(x).tangent is not None
+
+
+def _wants_grad(x):
     requires = getattr(x, "requires_grad", None)
     if requires is None:        # not a tensor
         return False
-    if _forward_ad is None:
-        _forward_ad = _torch().autograd.forward_ad
-    # outside of its levels nothing has a tangent (asking for one takes 0.3 us)
-    if getattr(_forward_ad, "_current_level", 0) >= 0 and _forward_ad.unpack_dual(x).tangent is not None:
+    if _has_tangent(x):
         raise HipGemmError("the scaled operators have no forward-mode derivative")
     return requires and _torch().is_grad_enabled()
 
