@@ -71,7 +71,7 @@ class FeedForward:
                 rows, h = rows
         elif residual is not None:
             raise HipGemmError("a residual needs the block's norm")
-        u = scaled.gated(rows, self.gate_up, act=self.act, out_dtype=x.dtype)
+        u = scaled.gated(rows, self.gate_up, act=self.act, out_dtype=None if rows is x else x.dtype)
         if self.adapters is not None:
             y = low_rank.adapted(u, self.down, self.adapters, which)
         elif which is not None:
