@@ -182,12 +182,25 @@ def _enqueued(on, stream, call, record=True, held=()):
         return result
 
 
+_current_device = None      # torch's function for the current device's index, once a runtime is there
+
+
+def _away(device):
+    """Whether another device than `device` is current: the library launches on the
+    one that is."""
+    global _current_device
+    if _current_device is None:
+        torch = _torch()
+        if not torch.cuda.is_initialized():
+            return False
+        _current_device = torch._C._cuda_getDevice
+    index = device.index
+    return index is not None and _current_device() != index
+
+
 def _on(device):
-    """A context with `device` current: the library launches on the device that is."""
-    torch = _torch()
-    if device.index is None or torch._C._cuda_getDevice() == device.index:
-        return _HERE
-    return torch.cuda.device(device)
+    """A context with `device` current."""
+    return _torch().cuda.device(device) if _away(device) else _HERE
 
 
 _HERE = contextlib.nullcontext()
@@ -248,12 +261,12 @@ def _pack(w0, s0, w1, s1, bias):
     size, floats = _lib.scaled_size(k, n, w1 is not None)
     data = torch.empty(size, dtype=torch.int8, device=w0.device)
     meta = torch.empty(floats, dtype=torch.float32, device=w0.device)   # written whole (and not read if n = 0)
-    lib = _lib.load_library()
-    _lib.check(lib.vt_scaled_pack(
-        w0.data_ptr(), None if w1 is None else w1.data_ptr(), _pitch(w0),
-        0 if w1 is None else _pitch(w1), s0.data_ptr(), None if s1 is None else s1.data_ptr(),
-        None if bias is None else bias.data_ptr(), k, n, data.data_ptr(), meta.data_ptr(),
-        _current_stream(w0.device)), "vt_scaled_pack")
+    with _on(w0.device):
+        _lib.check(_lib.load_library().vt_scaled_pack(
+            w0.data_ptr(), None if w1 is None else w1.data_ptr(), _pitch(w0),
+            0 if w1 is None else _pitch(w1), s0.data_ptr(), None if s1 is None else s1.data_ptr(),
+            None if bias is None else bias.data_ptr(), k, n, data.data_ptr(), meta.data_ptr(),
+            _current_stream(w0.device)), "vt_scaled_pack")
     return ScaledWeight(data, meta, k, n, w1 is not None)
 
 
@@ -330,9 +343,10 @@ def _quantize(x):
     pitch = _lib.quant_pitch(k)
     data = torch.empty((m, pitch), dtype=torch.int8, device=x.device)
     scale = torch.empty(m, dtype=torch.float32, device=x.device)
-    lib = _lib.load_library()
-    _lib.check(lib.vt_quant_rows(x2.data_ptr(), _types()[x.dtype], _pitch(x2), data.data_ptr(), pitch,
-                                 scale.data_ptr(), m, k, _current_stream(x.device)), "vt_quant_rows")
+    with _on(x.device):
+        _lib.check(_lib.load_library().vt_quant_rows(
+            x2.data_ptr(), _types()[x.dtype], _pitch(x2), data.data_ptr(), pitch, scale.data_ptr(), m, k,
+            _current_stream(x.device)), "vt_quant_rows")
     return QuantRows._made(data, scale, k, tuple(lead) + (k,))
 
 
@@ -395,6 +409,10 @@ def _forward(x, W, pair, act, out_dtype, out):
             out_dtype = x.dtype if out is None else out.dtype
     m = data.shape[0]
     device = data.device
+    # as _on, in less of an 8 us call
+    if (_current_device is None or _current_device() != device.index) and _away(device):
+        with _torch().cuda.device(device):
+            return _forward(x, W, pair, act, out_dtype, out)
     o2, ret, allocated = _output("output", out, m, W.n, lead, out_dtype, device, data)
     stream = _current_stream(device)
     lib = _lib.load_library()
@@ -488,10 +506,10 @@ def _linear_grad(dy, W, out):
     m = d.shape[0]
     o2, ret, _ = _output("gradient", out, m, W.k, lead, dy.dtype, d.device, d)
     ldx = o2.stride(-2) if o2.dim() == 2 and m > 1 and W.k else max(W.k, 1)
-    lib = _lib.load_library()
-    _lib.check(lib.vt_scaled_linear_grad(d.data_ptr(), _types()[dy.dtype], _pitch(d), m, W.k,
-                                         W.data.data_ptr(), W.meta.data_ptr(), W.n, o2.data_ptr(),
-                                         ldx, _current_stream(d.device)), "vt_scaled_linear_grad")
+    with _on(d.device):
+        _lib.check(_lib.load_library().vt_scaled_linear_grad(
+            d.data_ptr(), _types()[dy.dtype], _pitch(d), m, W.k, W.data.data_ptr(), W.meta.data_ptr(), W.n,
+            o2.data_ptr(), ldx, _current_stream(d.device)), "vt_scaled_linear_grad")
     return ret
 
 
@@ -517,12 +535,12 @@ def _gated_grad(dh, rows, W, a, out):
                            % (m, d.shape[1], rows.data.shape[0], W.n))
     o2, ret, _ = _output("gradient", out, m, W.k, lead, dh.dtype, d.device, d)
     ldx = o2.stride(-2) if o2.dim() == 2 and m > 1 and W.k else max(W.k, 1)
-    lib = _lib.load_library()
-    _lib.check(lib.vt_scaled_gated_grad(
-        d.data_ptr(), _types()[dh.dtype], _pitch(d), rows.data.data_ptr(),
-        _lib.TYPE_I8_PADDED if rows.padded else _lib.TYPE_I8, _pitch(rows.data),
-        rows.scale.data_ptr(), m, W.k, W.data.data_ptr(), W.meta.data_ptr(), W.n, a, o2.data_ptr(),
-        ldx, _current_stream(d.device)), "vt_scaled_gated_grad")
+    with _on(d.device):
+        _lib.check(_lib.load_library().vt_scaled_gated_grad(
+            d.data_ptr(), _types()[dh.dtype], _pitch(d), rows.data.data_ptr(),
+            _lib.TYPE_I8_PADDED if rows.padded else _lib.TYPE_I8, _pitch(rows.data),
+            rows.scale.data_ptr(), m, W.k, W.data.data_ptr(), W.meta.data_ptr(), W.n, a, o2.data_ptr(),
+            ldx, _current_stream(d.device)), "vt_scaled_gated_grad")
     return ret
 
 
