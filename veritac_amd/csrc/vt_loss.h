@@ -632,7 +632,9 @@ int vt_cross_entropy(const void *X, int32_t x_type, int64_t ldx, const float *T,
     int64_t step;
     const bool logits = through_logits(M, Kp);
     if (logits) {
-      step = std::max<int64_t>(1, std::min(M, kScaledBytes / (N * 4 + (N / kLogitChunk + 1) * 8 + 8)));
+      // rows are logit_parts_kernel's second side
+      const int64_t most = std::min<int64_t>(M, 65535);
+      step = std::max<int64_t>(1, std::min(most, kScaledBytes / (N * 4 + (N / kLogitChunk + 1) * 8 + 8)));
     } else {
       // parts of 64 columns at the least
       int64_t row_bytes = (Np + 127) / 128 * 2 * 8 + 4;
