@@ -159,15 +159,33 @@ __device__ __forceinline__ uint32_t max_u(uint32_t a, uint32_t b) { return max(a
 
 // The power of two that a row is scaled by: 1, unless the squares' sum has left
 // float32's range at the top, or is so small beside an eps of next to nothing
-// that squares were lost at the bottom.
+// that squares were lost at the bottom. 2^100 keeps the mean of one least value's
+// square (2^-149) over the longest row a normal number, and eps f^2 below 2^120;
+// a larger eps leaves room for 2^80.
 __device__ __forceinline__ float row_factor(float squares, float eps) {
   if (magnitude(squares) >= kInfBits) return 0x1p-80f;
-  return squares < 0x1p-80f && eps < 0x1p-60f ? 0x1p80f : 1.0f;
+  if (squares >= 0x1p-80f || eps >= 0x1p-60f) return 1.0f;
+  return eps < 0x1p-80f ? 0x1p100f : 0x1p80f;
 }
 
 // 1 / sqrt(mean + eps) of a row scaled by f, over f: n = (h f) * this.
 __device__ __forceinline__ float inverse_rms(float squares, float f, float k, float eps) {
   return 1.0f / sqrtf(squares / k + eps * f * f);
+}
+
+// dot / k inv^2, of a row scaled by f. The dot product of a row that was too small
+// would vanish in the division.
+__device__ __forceinline__ float mean_dot(float dot, float k, float inv, float f) {
+  return f > 1.0f ? dot * inv / k * inv : dot / k * inv * inv;
+}
+
+// inv f as one factor, or as two where float32 has no normal number for it.
+struct Unit {
+  float a, b;
+};
+__device__ __forceinline__ Unit row_unit(float inv, float f) {
+  const float r = inv * f;
+  return r >= 0x1p-126f && magnitude(r) < kInfBits ? Unit{r, 1.0f} : Unit{inv, f};
 }
 
 struct NormArgs {
@@ -339,14 +357,15 @@ __global__ __launch_bounds__(THREADS) void norm_grad_kernel(NormGradArgs p) {
     all(1.0f);
     const float f = row_factor(squares, p.eps);
     if (f != 1.0f) all(f);
-    const float inv = inverse_rms(squares, f, (float)p.K, p.eps), c = dot / (float)p.K * inv * inv;
+    const float inv = inverse_rms(squares, f, (float)p.K, p.eps), c = mean_dot(dot, (float)p.K, inv, f);
+    const Unit unit = row_unit(inv, f);
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const float a = h[i][e] * f;
         sum[i][e] = fmaf(d[i][e], a * inv, sum[i][e]);
-        const float y = (d[i][e] * g[i][e] - a * c) * (inv * f);
+        const float y = (d[i][e] * g[i][e] - a * c) * unit.a * unit.b;
         x[i][e] = p.E ? x[i][e] + y : y;
       }
       store8<TYPE>((T *)p.X + row * p.ldx, pos_of(i), p.K, x[i]);
@@ -390,7 +409,7 @@ __global__ __launch_bounds__(1024) void norm_stats_kernel(NormGradArgs p) {
       float *s = p.stats + row * 3;
       s[0] = f;
       s[1] = inv;
-      s[2] = dot / (float)p.K * inv * inv;
+      s[2] = mean_dot(dot, (float)p.K, inv, f);
     }
   }
 }
@@ -407,6 +426,7 @@ __global__ __launch_bounds__(256) void norm_apply_kernel(NormGradArgs p) {
   for (int64_t row = blockIdx.x; row < p.M; row += gridDim.x) {
     const float *s = p.stats + row * 3;
     const float f = s[0], inv = s[1], c = s[2];
+    const Unit unit = row_unit(inv, f);
     float d[8], h[8], x[8];
     load8<TYPE>((const T *)p.D + row * p.ldd, pos, p.K, d);
     load8<TYPE>((const T *)p.H + row * p.ldh, pos, p.K, h);
@@ -415,7 +435,7 @@ __global__ __launch_bounds__(256) void norm_apply_kernel(NormGradArgs p) {
     for (int e = 0; e < 8; ++e) {
       const float a = h[e] * f;
       sum[e] = fmaf(d[e], a * inv, sum[e]);
-      const float y = (d[e] * g[e] - a * c) * (inv * f);
+      const float y = (d[e] * g[e] - a * c) * unit.a * unit.b;
       x[e] = p.E ? x[e] + y : y;
     }
     store8<TYPE>((T *)p.X + row * p.ldx, pos, p.K, x);
