@@ -419,7 +419,7 @@ __global__ __launch_bounds__(256) void logit_parts_kernel(LogitArgs p) {
 struct LossRowsArgs {
   const v2f *part;
   const float *mine;
-  const float *top_scale;   // the weights' largest |s|
+  const float *top_scale;   // the weights' largest |s|, in kTopParts parts
   Targets targets;
   float *loss;
   RowState *state;
@@ -453,7 +453,10 @@ __global__ __launch_bounds__(1024) void loss_rows_kernel(LossRowsArgs p) {
     // |p - [target]| is at most 1 - p of the target, of which the logits' own rounding
     // leaves no bits below 2^-22 of their size
     const float least = 0x1p-22f * fminf(fmaxf(fabsf(ms[0]), 1.0f), 0x1p20f);
-    st.norm = loss == loss ? normaliser(fmaxf(-expm1f(-loss), least) * *p.top_scale) : loss;
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < kTopParts; ++i) top = max(top, magnitude(p.top_scale[i]));
+    st.norm = loss == loss ? normaliser(fmaxf(-expm1f(-loss), least) * __uint_as_float(top)) : loss;
   }
   p.loss[row] = loss;
   p.state[row] = st;
