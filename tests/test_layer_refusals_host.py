@@ -29,3 +29,17 @@ ROWS = {"int8 rows": lambda: scaled.QuantRows(torch.zeros(3, D, dtype=torch.int8
 def test_a_block_refuses_rows_that_are_no_floating_tensor(rows, normed):
     with pytest.raises(HipGemmError):
         block(**(dict(norm=torch.ones(D)) if normed else {}))(ROWS[rows]())
+
+
+def test_missing_rows_are_refused_where_nothing_is_put_out():
+    """u and h are made from the rows also without columns of the outputs or of dx."""
+    lib, a = _lib.load_library(), [(1 + i) << 30 for i in range(12)]
+    f32, i8 = _lib.TYPE_F32, _lib.TYPE_I8
+
+    def adapted(x, kind, t):
+        return lib.vt_adapted_linear(x, kind, 64, t, 4, 64, a[1], a[2], 0, a[3], 8, 2, 1.0, a[4], a[5], a[6], f32, 1, None)
+
+    def grad(dy):
+        return lib.vt_adapted_grad(dy, f32, 32, None, 1, 4, 0, a[1], a[2], 32, None, a[3], 8, 2, 1.0, a[4], a[5], a[6], a[7], 1, None, a[8], None)
+    for rc in (adapted(None, f32, None), adapted(a[0], i8, None), adapted(None, i8, a[7]), grad(None)):
+        assert rc == _lib.VT_EINVAL, (rc, _lib.last_error())

@@ -1246,6 +1246,8 @@ int vt_adapted_linear(const void *X, int32_t x_type, int64_t ldx, const float *T
   const AdapterLayout l = adapter_layout(K, N, R, L);
   const int64_t e = elem_size(type), size = l.first(false) + l.second(false);
   if (!U || (size > 0 && !P)) return fail(VT_EINVAL, "%s: adapters or U are null", who);
+  // u is made without outputs too
+  if ((K > 0 && !X) || (i8 && !T)) return fail(VT_EINVAL, "%s: input is null, or int8 rows without scales", who);
   const Operand o[] = {{"X", X, M, ldx, x_type == VT_TYPE_I8_PADDED ? l.Kp : K, elem_size(x_type), false},
                        {"T", T, 1, M, M, 4, false}, {"weights", Bp, 1, 0, l.Kp * l.Np, 1, false},
                        {"scales", meta, 1, 0, scaled_meta(l.Np), 4, false}, {"adapters", P, 1, size, size, e, false, 16 / e},
@@ -1292,8 +1294,8 @@ int vt_adapted_grad(const void *dY, int32_t type, int64_t ldd, const void *X, in
   const AdapterLayout l = adapter_layout(K, N, R, L);
   const int64_t e = elem_size(type), size = l.first(true) + l.second(true);
   const bool again = P && dUp;   // u has to be made again
-  if (M > 0 && (!H || (size > 0 && !back) || (dUp && !U) || ((dDown || again) && K > 0 && !X)))
-    return fail(VT_EINVAL, "%s: adapters, X, U or H are null", who);
+  if (M > 0 && (!H || (N > 0 && !dY) || (size > 0 && !back) || (dUp && !U) || ((dDown || again) && K > 0 && !X)))
+    return fail(VT_EINVAL, "%s: adapters, dY, X, U or H are null", who);
   const Operand o[] = {{"dY", dY, M, ldd, N, e, false}, {"X", X, M, ldx, K, e, false}, {"weights", Bp, 1, 0, l.Kp * l.Np, 1, false},
                        {"scales", meta, 1, 0, scaled_meta(l.Np), 4, false}, {"adapters", P, 1, size, size, e, false, 16 / e},
                        {"adapters", back, 1, size, size, e, false, 16 / e}, {"which", which, 1, M, M, 4, false},
