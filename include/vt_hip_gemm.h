@@ -644,9 +644,10 @@ int vt_cross_entropy_grad(const int8_t *Q, int32_t q_type, int64_t ldq, const fl
  * [L][N][R] -> P, what vt_adapted_linear reads, and back, what vt_adapted_grad
  * does, both 16-byte aligned (null: not wanted).
  *
- * vt_adapted_linear: U [M][Rp] float32, 16-byte aligned, is written (Y null: U
- * alone); Rp is 16, or from a rank of 17 on R rounded up to 32. vt_adapted_grad: H like U is written; dX, dDown and
- * dUp may be null where they are not wanted, and X and U without dDown and dUp.
+ * vt_adapted_linear: U [M][Rp] float32, 16-byte aligned, is written; Rp is 16, or
+ * from a rank of 17 on R rounded up to 32. vt_adapted_grad: H like U is written;
+ * dX, dDown and dUp may be null where they are not wanted, and X and U without
+ * dDown and dUp.
  * U is the forward pass' (P null), or made again from X and P. Otherwise as
  * vt_scaled_linear and its gradient.
  */

@@ -43,3 +43,9 @@ def test_missing_rows_are_refused_where_nothing_is_put_out():
         return lib.vt_adapted_grad(dy, f32, 32, None, 1, 4, 0, a[1], a[2], 32, None, a[3], 8, 2, 1.0, a[4], a[5], a[6], a[7], 1, None, a[8], None)
     for rc in (adapted(None, f32, None), adapted(a[0], i8, None), adapted(None, i8, a[7]), grad(None)):
         assert rc == _lib.VT_EINVAL, (rc, _lib.last_error())
+
+
+def test_outputs_are_not_left_out():
+    lib, a = _lib.load_library(), [(1 + i) << 30 for i in range(12)]
+    rc = lib.vt_adapted_linear(a[0], _lib.TYPE_F32, 64, None, 4, 64, a[1], a[2], 32, a[3], 8, 2, 1.0, a[4], a[5], None, _lib.TYPE_F32, 32, None)
+    assert rc == _lib.VT_EINVAL, (rc, _lib.last_error())

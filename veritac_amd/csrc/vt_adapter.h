@@ -462,27 +462,22 @@ __device__ __forceinline__ void low_rank_any(const LowRank &l, int type, FLOATS 
   else low_rank_elements<false>(l, type, U, row, col, s);
 }
 
-// t[i] += a . b[i] for four blocks beside each other, and with LO += lo . b[i]. In
+// t[i] += a . b[i] + lo . b[i] for four blocks beside each other. In
 // inline assembly with the sums in VGPRs: the kernels that do this keep all of
 // their accumulators in AGPRs, where the compiler puts a builtin's too, and
 // would spill. Its operands may have been written by the instruction before (two
 // wait states), and its results are read by the instruction behind: an 8-pass
 // product's by 11 wait states, a 16-pass one's by 19.
-template <int TYPE, bool LO>
+template <int TYPE>
 __device__ __forceinline__ void four_products(v4f (&t)[4], const Frag<TYPE> &a, const Frag<TYPE> &lo, const Frag<TYPE> (&b)[4]) {
 #define VT_FOUR(op, A)                                                                            \
   op " %0, %" A ", %6, %0\n\t" op " %1, %" A ", %7, %1\n\t" op " %2, %" A ", %8, %2\n\t" op " %3, %" A ", %9, %3\n\t"
-#define VT_ASM(text) \
-  asm volatile("s_nop 1\n\t" text "s_nop 15\n\ts_nop 7" \
+#define VT_ASM(op) \
+  asm volatile("s_nop 1\n\t" VT_FOUR(op, "4") VT_FOUR(op, "5") "s_nop 15\n\ts_nop 7" \
                : "+v"(t[0]), "+v"(t[1]), "+v"(t[2]), "+v"(t[3]) \
                : "v"(a.v), "v"(lo.v), "v"(b[0].v), "v"(b[1].v), "v"(b[2].v), "v"(b[3].v))
-  if constexpr (TYPE == kF16) {
-    if constexpr (LO) VT_ASM(VT_FOUR("v_mfma_f32_16x16x32_f16", "4") VT_FOUR("v_mfma_f32_16x16x32_f16", "5"));
-    else VT_ASM(VT_FOUR("v_mfma_f32_16x16x32_f16", "4"));
-  } else if constexpr (TYPE == kBF16) {
-    if constexpr (LO) VT_ASM(VT_FOUR("v_mfma_f32_16x16x32_bf16", "4") VT_FOUR("v_mfma_f32_16x16x32_bf16", "5"));
-    else VT_ASM(VT_FOUR("v_mfma_f32_16x16x32_bf16", "4"));
-  }
+  if constexpr (TYPE == kF16) VT_ASM("v_mfma_f32_16x16x32_f16");
+  else VT_ASM("v_mfma_f32_16x16x32_bf16");
 #undef VT_ASM
 #undef VT_FOUR
 }
@@ -592,7 +587,7 @@ struct LowRankStrips {
           four_products(t, u[0][e], p[4 * q].v[e], p[4 * q + 1].v[e], p[4 * q + 2].v[e], p[4 * q + 3].v[e]);
       } else {
         const Frag<TYPE> four[4] = {p[4 * q].v, p[4 * q + 1].v, p[4 * q + 2].v, p[4 * q + 3].v};
-        four_products<TYPE, true>(t, hi, lo, four);
+        four_products<TYPE>(t, hi, lo, four);
       }
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -1232,14 +1227,8 @@ int vt_adapted_linear(const void *X, int32_t x_type, int64_t ldx, const float *T
   const AdapterCall ad = {who, type, L, R, K, N};
   if (int rc = check_adapters(ad)) return rc;
   const int64_t Rp = rank_pad(R);
-  ScaledCall checked = c;
-  if (!Y) {   // u alone
-    checked.Y = U;
-    checked.y_type = VT_TYPE_F32;
-    checked.ldy = checked.yc = Rp;
-  }
   bool empty = false;
-  if (int rc = check_scaled(checked, &empty)) return rc;
+  if (int rc = check_scaled(c, &empty)) return rc;
   const bool i8 = !float_type(x_type);
   if (!i8 && x_type != type) return fail(VT_EINVAL, "%s: floating rows have the adapters' type", who);
   if (M == 0) return VT_OK;
@@ -1256,7 +1245,7 @@ int vt_adapted_linear(const void *X, int32_t x_type, int64_t ldx, const float *T
   const LowRank low = {U, (const int8_t *)P + l.first(false) * e, which, l.Np, (int)L, (int)Rp, (int)M};
   ShrinkPair pair = {};
   pair.of[0] = ShrinkArgs{X, T, P, which, U, ldx, scale, (int)M, (int)K, (int)l.Kp, (int)L, (int)Rp, nullptr, nullptr};
-  const bool out = Y && !empty;
+  const bool out = !empty;
   // few rows are one part
   const int64_t step = rows_in_place(X, x_type, ldx, K) ? M : rows_at_once(M, l.Kp + 4);
   for (int64_t r = 0; r < M && (out || r == 0); r += step) {
