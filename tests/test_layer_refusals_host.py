@@ -6,7 +6,7 @@ torch = pytest.importorskip("torch")
 
 from veritac_amd import _lib
 from veritac_amd._lib import HipGemmError
-from veritac_amd.specializations.hip_gemm import feed_forward, scaled
+from veritac_amd.specializations.hip_gemm import adapters, feed_forward, scaled
 
 D, N = 64, 96
 
@@ -49,3 +49,19 @@ def test_outputs_are_not_left_out():
     lib, a = _lib.load_library(), [(1 + i) << 30 for i in range(12)]
     rc = lib.vt_adapted_linear(a[0], _lib.TYPE_F32, 64, None, 4, 64, a[1], a[2], 32, a[3], 8, 2, 1.0, a[4], a[5], None, _lib.TYPE_F32, 32, None)
     assert rc == _lib.VT_EINVAL, (rc, _lib.last_error())
+
+
+FITS = dict(dtype=torch.float16, count=2, rank=4, k=64, n=96, scaling=0.5)
+
+
+def held(**kw):
+    size = _lib.adapter_size(64, 96, 4, 2, _lib.TYPE_F16)
+    return adapters.Adapters(torch.zeros(size, dtype=torch.uint8), **{**FITS, **kw})
+
+
+@pytest.mark.parametrize("kw", [dict(count="2"), dict(count=2.0), dict(count=None), dict(rank=4.0), dict(rank=True), dict(k="64"), dict(n=None),
+                                dict(n=1 << 70), dict(n=(1 << 64) + 96), dict(k=-64), dict(rank=0), dict(count=0), dict(dtype=torch.int8), dict(dtype="f16")], ids=str)
+def test_adapters_are_of_whole_sizes(kw):
+    assert held().count == 2
+    with pytest.raises(HipGemmError):
+        held(**kw)

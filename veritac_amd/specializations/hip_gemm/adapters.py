@@ -26,7 +26,7 @@ import math
 from ... import _lib
 from ..._lib import HipGemmError
 from . import scaled
-from .scaled import _current_stream, _gpu, _on, _pitch, _rows, _torch, _types
+from .scaled import _current_stream, _gpu, _is_int, _on, _pitch, _rows, _torch, _types
 
 MAX_RANK = 128
 
@@ -41,6 +41,9 @@ class Adapters:
         torch = _torch()
         if dtype not in _types():
             raise HipGemmError("adapters must be float32, float16 or bfloat16 (got %s)" % (dtype,))
+        for name, v in (("count", count), ("rank", rank), ("k", k), ("n", n)):
+            if not _is_int(v) or not 0 <= v < 1 << 31:      # as far as any size of the library's goes
+                raise HipGemmError("%s must be a whole number of 0 .. 2^31 - 1 (got %r)" % (name, v))
         size = _lib.adapter_size(k, n, rank, count, _types()[dtype])
         if not isinstance(data, torch.Tensor) or data.dtype != torch.uint8 or data.shape != (size,) \
                 or not data.is_contiguous():
