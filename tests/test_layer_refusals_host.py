@@ -65,3 +65,13 @@ def test_adapters_are_of_whole_sizes(kw):
     assert held().count == 2
     with pytest.raises(HipGemmError):
         held(**kw)
+
+
+@pytest.mark.parametrize("scaling", [1e39, -1e39, 10**400, float("inf"), float("nan"), "1", True, None],
+                         ids=["above", "below", "huge", "inf", "nan", "text", "truth", "none"])
+def test_scalings_are_float32_numbers(scaling):
+    assert held(scaling=-3e38).scaling == -3e38
+    with pytest.raises(HipGemmError):
+        held(scaling=scaling)
+    with pytest.raises(HipGemmError):
+        feed_forward.FeedForward(weight(D, N, True), weight(N, D, False), adapters=(torch.zeros(2, 4, N), torch.zeros(2, D, 4), scaling))

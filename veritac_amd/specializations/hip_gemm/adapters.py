@@ -21,8 +21,6 @@ once on a stream can be captured there.
 """
 from __future__ import annotations
 
-import math
-
 from ... import _lib
 from ..._lib import HipGemmError
 from . import scaled
@@ -64,8 +62,8 @@ class Adapters:
 
 
 def _scaling(scaling):
-    if isinstance(scaling, bool) or not isinstance(scaling, (int, float)) or not math.isfinite(scaling):
-        raise HipGemmError("scaling must be a finite number (got %r)" % (scaling,))
+    if isinstance(scaling, bool) or not isinstance(scaling, (int, float)) or not abs(scaling) <= 3.4028234e38:
+        raise HipGemmError("scaling must be a number of float32's range (got %.60r)" % (scaling,))
     return float(scaling)
 
 
