@@ -1,4 +1,4 @@
-"""Gradients of more long rows than their statistics have workgroups (needs a gfx950 GPU), against 64 bits."""
+"""Gradients of many long rows (needs a gfx950 GPU) against 64 bits, and of more than their statistics have workgroups."""
 import pytest
 
 torch = pytest.importorskip("torch")
@@ -21,3 +21,15 @@ def test_gradients_of_many_long_rows(dev, m, k):
     x64, xb, g64, gb = norm_ref.norm_grad(d.double().numpy(), h.double().numpy(), gain.double().numpy(), 1e-6, e.double().numpy())
     close(dx, x64, xb, "dx")
     close(dg, g64, gb, "dgain")
+
+
+def test_more_long_rows_than_workgroups(dev):
+    """2^20 workgroups: the rows behind them, and the first, are those of a call of their own (17 GB an operand)."""
+    say("2^20 long rows")
+    m, k, part = (1 << 20) + 70, 8200, 300
+    h = torch.empty(m, k, dtype=torch.bfloat16, device=dev).normal_()
+    gain = torch.rand(k, device=dev) + 0.5
+    dx, _ = norms.norm_grad(h, h, gain, gain_grad=False)
+    for s in (slice(0, part), slice(m - part, m)):
+        assert torch.equal(dx[s], norms.norm_grad(h[s], h[s], gain, gain_grad=False)[0])
+    assert dx[m - part:].any()

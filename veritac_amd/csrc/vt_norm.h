@@ -173,19 +173,23 @@ __device__ __forceinline__ float inverse_rms(float squares, float f, float k, fl
   return 1.0f / sqrtf(squares / k + eps * f * f);
 }
 
-// dot / k inv^2, of a row scaled by f. The dot product of a row that was too small
-// would vanish in the division.
-__device__ __forceinline__ float mean_dot(float dot, float k, float inv, float f) {
-  return f > 1.0f ? dot * inv / k * inv : dot / k * inv * inv;
-}
-
-// inv f as one factor, or as two where float32 has no normal number for it.
-struct Unit {
-  float a, b;
+// What dx needs of a row scaled by f besides it: dx = ((z - h f c) a b) + dh.
+struct RowUse {
+  float c, a, b;
 };
-__device__ __forceinline__ Unit row_unit(float inv, float f) {
-  const float r = inv * f;
-  return r >= 0x1p-126f && magnitude(r) < kInfBits ? Unit{r, 1.0f} : Unit{inv, f};
+// c = dot / k inv^2 and inv f = a b. A row that was too small (f > 1) has a dot
+// product that would vanish in the division, and float32 may have no normal number
+// for inv f: two factors then, of which b is 1 in any other row.
+__device__ __forceinline__ RowUse row_use(float dot, float k, float inv, float f) {
+  RowUse r = {dot / k * inv * inv, inv * f, 1.0f};
+  if (f != 1.0f) {
+    if (f > 1.0f) r.c = dot * inv / k * inv;
+    if (!(r.a >= 0x1p-126f && magnitude(r.a) < kInfBits)) {
+      r.a = inv;
+      r.b = f;
+    }
+  }
+  return r;
 }
 
 struct NormArgs {
@@ -305,15 +309,10 @@ struct NormGradArgs {
   const void *D, *H, *G, *E;   // dy, h, the gain and the residual's own gradient (or null)
   void *X;                     // dx
   float *part;                 // [groups][K] partial sums of the gain's gradient, null: not wanted
-  float *stats;                // rows longer than kNormGradRow: their RowStats, three floats a row
+  float *stats;                // rows longer than kNormGradRow: four floats a row: f, inv, and c and b of RowUse
   int64_t ldd, ldh, lde, ldx, M, K;
   float eps;
   int gain32;
-};
-
-// What dx needs of a row scaled by f: dx = inv f (z - h f c) + dh, n = h f inv.
-struct RowStats {
-  float f, inv, c;
 };
 
 // A workgroup takes rows w, w + grid, .. whole, and keeps its part of the gain's
@@ -357,17 +356,23 @@ __global__ __launch_bounds__(THREADS) void norm_grad_kernel(NormGradArgs p) {
     all(1.0f);
     const float f = row_factor(squares, p.eps);
     if (f != 1.0f) all(f);
-    const float inv = inverse_rms(squares, f, (float)p.K, p.eps), c = mean_dot(dot, (float)p.K, inv, f);
-    const Unit unit = row_unit(inv, f);
+    const float inv = inverse_rms(squares, f, (float)p.K, p.eps);
+    const RowUse use = row_use(dot, (float)p.K, inv, f);
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
+      float y[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const float a = h[i][e] * f;
         sum[i][e] = fmaf(d[i][e], a * inv, sum[i][e]);
-        const float y = (d[i][e] * g[i][e] - a * c) * unit.a * unit.b;
-        x[i][e] = p.E ? x[i][e] + y : y;
+        y[e] = (d[i][e] * g[i][e] - a * use.c) * use.a;
       }
+      if (use.b != 1.0f) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] *= use.b;
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[i][e] = p.E ? x[i][e] + y[e] : y[e];
       store8<TYPE>((T *)p.X + row * p.ldx, pos_of(i), p.K, x[i]);
     }
   }
@@ -378,7 +383,8 @@ __global__ __launch_bounds__(THREADS) void norm_grad_kernel(NormGradArgs p) {
 }
 
 // Rows too long for a workgroup's registers: first what dx needs of each row, a
-// workgroup rows w, w + grid, .. (one a row would be beyond a launch from 2^22 on),
+// workgroup each up to 2^20 (as many as CUs hold, which take rows in turn, are 2 %
+// slower over 4096 x 16384; a launch has less than 2^22),
 template <int TYPE>
 __global__ __launch_bounds__(1024) void norm_stats_kernel(NormGradArgs p) {
   __shared__ uint64_t red[16];
@@ -406,10 +412,12 @@ __global__ __launch_bounds__(1024) void norm_stats_kernel(NormGradArgs p) {
     if (f != 1.0f) all(f);
     if (threadIdx.x == 0) {
       const float inv = inverse_rms(squares, f, (float)p.K, p.eps);
-      float *s = p.stats + row * 3;
+      float *s = p.stats + row * 4;
+      const RowUse use = row_use(dot, (float)p.K, inv, f);
       s[0] = f;
       s[1] = inv;
-      s[2] = mean_dot(dot, (float)p.K, inv, f);
+      s[2] = use.c;
+      s[3] = use.b;
     }
   }
 }
@@ -424,9 +432,8 @@ __global__ __launch_bounds__(256) void norm_apply_kernel(NormGradArgs p) {
 #pragma unroll
   for (int e = 0; e < 8; ++e) sum[e] = 0.0f;
   for (int64_t row = blockIdx.x; row < p.M; row += gridDim.x) {
-    const float *s = p.stats + row * 3;
-    const float f = s[0], inv = s[1], c = s[2];
-    const Unit unit = row_unit(inv, f);
+    const v4f s = *(const v4f *)(p.stats + row * 4);
+    const float f = s[0], inv = s[1], c = s[2], b = s[3], a1 = b == 1.0f ? inv * f : inv;
     float d[8], h[8], x[8];
     load8<TYPE>((const T *)p.D + row * p.ldd, pos, p.K, d);
     load8<TYPE>((const T *)p.H + row * p.ldh, pos, p.K, h);
@@ -435,9 +442,14 @@ __global__ __launch_bounds__(256) void norm_apply_kernel(NormGradArgs p) {
     for (int e = 0; e < 8; ++e) {
       const float a = h[e] * f;
       sum[e] = fmaf(d[e], a * inv, sum[e]);
-      const float y = (d[e] * g[e] - a * c) * unit.a * unit.b;
-      x[e] = p.E ? x[e] + y : y;
+      d[e] = (d[e] * g[e] - a * c) * a1;
     }
+    if (b != 1.0f) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) d[e] *= b;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = p.E ? x[e] + d[e] : d[e];
     store8<TYPE>((T *)p.X + row * p.ldx, pos, p.K, x);
   }
   if (p.part) store8<kF32>(p.part + blockIdx.x * p.K, pos, p.K, sum);
@@ -549,7 +561,7 @@ int launch_norm_grad(NormGradArgs a, void *dgain, int gain_type, Scratch &scr) {
   void *w = nullptr;
   if (dgain || a.K > kNormGradRow) {
     const size_t part = dgain ? ((size_t)groups * a.K * sizeof(float) + 255) / 256 * 256 : 0;
-    const size_t stats = a.K > kNormGradRow ? (size_t)a.M * 3 * sizeof(float) : 0;
+    const size_t stats = a.K > kNormGradRow ? (size_t)a.M * 4 * sizeof(float) : 0;
     if (int rc = scr.take(kPartials, part + stats, &w)) return rc;
     a.part = dgain ? (float *)w : nullptr;
     a.stats = (float *)((int8_t *)w + part);
@@ -561,7 +573,7 @@ int launch_norm_grad(NormGradArgs a, void *dgain, int gain_type, Scratch &scr) {
   else if (threads == 512) hipLaunchKernelGGL((norm_grad_kernel<TYPE, 512, 1>), grid, dim3(512), 0, s, a);
   else if (threads == 1024) hipLaunchKernelGGL((norm_grad_kernel<TYPE, 1024, 1>), grid, dim3(1024), 0, s, a);
   else {
-    hipLaunchKernelGGL((norm_stats_kernel<TYPE>), dim3((unsigned)resident(a.M, 1024, cus)), dim3(1024), 0, s, a);
+    hipLaunchKernelGGL((norm_stats_kernel<TYPE>), dim3((unsigned)std::min<int64_t>(a.M, 1 << 20)), dim3(1024), 0, s, a);
     VT_HIP_CHECK(hipGetLastError());
     hipLaunchKernelGGL((norm_apply_kernel<TYPE>), dim3((unsigned)groups, (unsigned)((a.K + 2047) / 2048)), dim3(256), 0, s, a);
   }
