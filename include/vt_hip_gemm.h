@@ -558,7 +558,8 @@ int vt_scaled_gated_grad(const void *dH, int32_t type, int64_t ldd, const int8_t
  * Y [M][ldy] of vt_quant_pitch(K) bytes, 16-byte aligned. gain [K] is float32 or
  * of the type. eps >= 0. Squares are summed in float32; a row whose squares leave
  * its range is scaled by a power of two first. A row that holds NaN or an
- * infinity gives NaN where 32-bit arithmetic does, and int8 rows of scale NaN.
+ * infinity gives NaN where 32-bit arithmetic does, and int8 rows of scale NaN;
+ * one whose h gain, scaled so, stays below 2^-120 gives int8 rows of zeros.
  *
  * vt_norm_grad: dY and H as above, and (or null) the gradient dH of h from
  * elsewhere -> dX, the gradient of x and of r, and (or null) dgain [K] of the

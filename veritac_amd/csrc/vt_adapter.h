@@ -646,10 +646,13 @@ __device__ __forceinline__ int adapter_at(const RowAdapters &r, int rel, int lan
 template <int TYPE>
 struct AdaptedTile : ScaledTile<kLinear, TYPE == kF32 ? 4 : 2> {
   // A wave's 128 x 128 sums and its next fragments leave too few registers for the
-  // low-rank products, and what they spill waits for the stores: 4096 x 4096 -> 14336
-  // with rank 16 / 64 / 128 took 346 / 391 / 465 us on 256 x 256 tiles and takes 292 /
-  // 321 / 414 on 256 x 128 (219 without adapters); 8192^3 614 / 711 / 887 and 661 /
-  // 738 / 946 (484).
+  // low-rank products, and what they spill waits for the stores. Whole calls with
+  // rank 16 / 64 / 128, u's kernel in both as it was then (its widest form spilled):
+  // 4096 x 4096 -> 14336 took 346 / 391 / 465 us on 256 x 256 tiles and 292 / 321 / 414
+  // on 256 x 128 (219 without adapters); at 8192^3, whose longer K carries that
+  // epilogue, 614 / 711 / 887 and 661 / 738 / 946 (484). One rule for any K: the 4 -
+  // 7 % that 256 x 256 tiles had there are given up for the 11 - 18 % elsewhere. With
+  // today's u the kept form takes 288 / 301 / 377 and 662 / 635 / 736.
   static constexpr bool kWide = false;
   LowRank low;
   static constexpr int OE = TYPE == kF32 ? 4 : 2;

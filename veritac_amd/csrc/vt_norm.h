@@ -317,7 +317,7 @@ struct NormGradArgs {
 
 // A workgroup takes rows w, w + grid, .. whole, and keeps its part of the gain's
 // gradient in registers over them: dy, h and dh are read once. 4096 x 4096 bfloat16
-// in 25 - 28 us (134 MB, 4.8 - 5.4 TB/s; 31 with each load's conversion in the branch
+// in 25 - 29 us (134 MB, 4.6 - 5.4 TB/s; 31 with each load's conversion in the branch
 // around it), 333 x 1001 float32 in 5.8.
 template <int TYPE, int THREADS, int NC>
 __global__ __launch_bounds__(THREADS) void norm_grad_kernel(NormGradArgs p) {
