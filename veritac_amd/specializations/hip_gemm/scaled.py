@@ -107,7 +107,7 @@ class QuantRows:
             raise HipGemmError("dtype must be float32, float16 or bfloat16 (got %s)" % (dtype,))
         data, k = self.data, self.k
         device = data.device
-        if device.type != "cuda" or not self._plain():
+        if device.type != "cuda" or not self._for_kernel():
             return (data[:, :k].float() * self.scale[:, None]).reshape(self.shape).to(dtype)
         y = data.new_empty(self.shape, dtype=dtype)
         with _on(device):
@@ -116,7 +116,7 @@ class QuantRows:
                 data.shape[0], k, _current_stream(device)), "vt_dequant_rows")
         return y
 
-    def _plain(self):
+    def _for_kernel(self):
         """Whether vt_dequant_rows takes these rows: no derivative, no rows that share
         memory, sizes of the operators'."""
         torch = _torch()
